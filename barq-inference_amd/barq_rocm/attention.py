@@ -48,13 +48,17 @@ def transpose_heads(be: Backend, x, seq_len, n_heads, head_dim, mem=L.MEM_DEVICE
 
 class KVCache:
     """KVCache (context.rs:245-340) in device memory, preallocated for
-    max_size positions per layer and kv head."""
+    max_size positions per layer and kv head; type F32, or Q4_0 for rows held
+    in 4 bits."""
 
-    def __init__(self, be: Backend, max_size: int, n_layers: int, n_head_kv: int, head_dim: int):
+    def __init__(self, be: Backend, max_size: int, n_layers: int, n_head_kv: int, head_dim: int, type: int = L.F32):
         self.be = be
+        self.c = None
         c = ctypes.c_void_p()
-        L.check(be._lib.barq_rocm_kv_cache_create(be.h, max_size, n_layers, n_head_kv, head_dim, ctypes.byref(c)))
+        L.check(be._lib.barq_rocm_kv_cache_create_typed(be.h, max_size, n_layers, n_head_kv, head_dim, type,
+                                                        ctypes.byref(c)))
         self.c = c
+        self.type = type
         self.max_size, self.n_layers, self.n_head_kv, self.head_dim = max_size, n_layers, n_head_kv, head_dim
 
     def close(self):
@@ -119,10 +123,27 @@ class KVCache:
         L.check(self.be._lib.barq_rocm_kv_cache_head(self.c, layer, head, ctypes.byref(k), ctypes.byref(v)))
         return k.value, v.value
 
+    def read(self, layer, first, n, mem=L.MEM_DEVICE, sync=True):
+        """Positions first .. first + n - 1 of the layer as f32: (k, v), each
+        [n_head_kv, n, head_dim], whatever the cache holds them as."""
+        shape = (self.n_head_kv, n, self.head_dim)
+        if mem == L.MEM_HOST:
+            k, v = np.empty(shape, np.float32), np.empty(shape, np.float32)
+        else:
+            import torch
+            k, v = (torch.empty(shape, dtype=torch.float32, device=f"cuda:{self.be.device}") for _ in "kv")
+        L.check(self.be._lib.barq_rocm_kv_cache_read(self.be.h, self.c, layer, first, n, _ptr(k), _ptr(v), mem))
+        if sync and mem == L.MEM_DEVICE:
+            self.be.sync()
+        return k, v
+
     def get_head(self, layer, head):
         """(K, V) of a head as numpy [layer_len, head_dim], copied to the host
         after the backend's stream has finished."""
         n = self.layer_len(layer)
+        if self.type != L.F32:
+            k, v = self.read(layer, 0, n, mem=L.MEM_HOST)
+            return k[head], v[head]
         self.be.sync()
         out = []
         for p in self.head_ptrs(layer, head):

@@ -8,27 +8,14 @@
 
 #include <hip/hip_runtime.h>
 
+#include <exception>
 #include <vector>
 
 #include "api_internal.hpp"
+#include "kv_cache.hpp"
 #include "launch.hpp"
 
 using namespace barq_api;
-
-// Device KV cache: K and V each [n_layers][n_head_kv][max_size][head_dim] f32
-// in one allocation; per-layer lengths on the host (the reference's per-layer
-// vectors grow independently; size() follows layer 0).
-struct barq_rocm_kv_cache {
-    int device = 0;
-    size_t max_size = 0, n_layers = 0, n_head_kv = 0, head_dim = 0;
-    float* k = nullptr;
-    float* v = nullptr;
-    std::vector<size_t> len;
-    size_t size = 0;
-
-    size_t head_stride() const { return max_size * head_dim; }
-    size_t layer_stride() const { return n_head_kv * head_stride(); }
-};
 
 namespace {
 
@@ -102,32 +89,60 @@ int barq_rocm_transpose_heads(barq_rocm_handle* h, const float* x, size_t seq_le
 
 int barq_rocm_kv_cache_create(barq_rocm_handle* h, size_t max_size, size_t n_layers, size_t n_head_kv,
                               size_t head_dim, barq_rocm_kv_cache** out) {
+    return barq_rocm_kv_cache_create_typed(h, max_size, n_layers, n_head_kv, head_dim, BARQ_TYPE_F32, out);
+}
+
+int barq_rocm_kv_cache_create_typed(barq_rocm_handle* h, size_t max_size, size_t n_layers, size_t n_head_kv,
+                                    size_t head_dim, int type, barq_rocm_kv_cache** out) {
     if (!out) return fail(BARQ_E_INVALID, "kv_cache_create: null output pointer");
     *out = nullptr;
     BARQ_CHECK(check_handle(h));
+    if (type != BARQ_TYPE_F32 && type != BARQ_TYPE_Q4_0)
+        return fail(BARQ_E_UNSUPPORTED, "kv_cache_create: type %d (BARQ_TYPE_F32 or BARQ_TYPE_Q4_0)", type);
     if (max_size == 0 || n_layers == 0 || n_head_kv == 0 || head_dim == 0)
         return fail(BARQ_E_DIM, "kv_cache_create: max_size, n_layers, n_head_kv and head_dim must be positive");
     BARQ_CHECK(check_int_range(max_size, "kv_cache_create: max_size"));
-    const size_t elems = n_layers * n_head_kv * max_size * head_dim;
-    if (elems / n_layers / n_head_kv / max_size != head_dim) return fail(BARQ_E_DIM, "kv_cache_create: size overflow");
+    if (type == BARQ_TYPE_Q4_0 && !barq::q4_head_dim(head_dim))
+        return fail(BARQ_E_UNSUPPORTED, "kv_cache_create: a Q4_0 cache takes head_dim 64, 128 or 256, not %zu", head_dim);
+    size_t elems = n_layers, bytes = 0;
+    // (the last factor: both f32 tensors; a 4-bit cache of fewer than 8 positions is a whole tile)
+    for (const size_t f : {n_head_kv, max_size + barq::KV_TILE, head_dim, sizeof(float) * 2})
+        if (__builtin_mul_overflow(elems, f, &elems)) return fail(BARQ_E_DIM, "kv_cache_create: size overflow");
     DeviceGuard g(h);
-    auto* c = new barq_rocm_kv_cache();
+    barq_rocm_kv_cache* c = nullptr;
+    try {
+        c = new barq_rocm_kv_cache();
+        c->len.assign(n_layers, 0);
+    } catch (const std::exception&) {
+        delete c;
+        return fail(BARQ_E_ALLOC, "kv_cache_create: out of host memory");
+    }
     c->device = h->device;
+    c->type = type;
     c->max_size = max_size;
     c->n_layers = n_layers;
     c->n_head_kv = n_head_kv;
     c->head_dim = head_dim;
-    c->len.assign(n_layers, 0);
-    hipError_t e = hipMalloc(&c->k, elems * sizeof(float));
-    if (e == hipSuccess) e = hipMalloc(&c->v, elems * sizeof(float));
+    hipError_t e;
+    if (type == BARQ_TYPE_Q4_0) {
+        bytes = 2 * (c->code_bytes() + c->scale_bytes());
+        e = hipMalloc(&c->q4, bytes);
+    } else {
+        bytes = 2 * n_layers * c->layer_stride() * sizeof(float);
+        e = hipMalloc(&c->k, bytes / 2);
+        if (e == hipSuccess) e = hipMalloc(&c->v, bytes / 2);
+    }
     if (e != hipSuccess) {
+        (void)hipGetLastError();
         if (c->k) (void)hipFree(c->k);
         delete c;
-        return fail(BARQ_E_ALLOC, "kv_cache_create: 2 x %zu bytes: %s", elems * sizeof(float), hipGetErrorString(e));
+        return fail(BARQ_E_ALLOC, "kv_cache_create: %zu bytes: %s", bytes, hipGetErrorString(e));
     }
     *out = c;
     return ok();
 }
+
+int barq_rocm_kv_cache_type(const barq_rocm_kv_cache* c) { return c ? c->type : -1; }
 
 int barq_rocm_kv_cache_destroy(barq_rocm_kv_cache* c) {
     if (!c) return ok();
@@ -135,6 +150,7 @@ int barq_rocm_kv_cache_destroy(barq_rocm_kv_cache* c) {
     (void)hipDeviceSynchronize();
     if (c->k) (void)hipFree(c->k);
     if (c->v) (void)hipFree(c->v);
+    if (c->q4) (void)hipFree(c->q4);
     delete c;
     return ok();
 }
@@ -150,6 +166,8 @@ int barq_rocm_kv_cache_head(const barq_rocm_kv_cache* c, size_t layer, size_t he
     if (layer >= c->n_layers || head >= c->n_head_kv)
         return fail(BARQ_E_INVALID, "kv_cache_head: layer %zu / head %zu out of range (%zu layers, %zu heads)", layer,
                     head, c->n_layers, c->n_head_kv);
+    if (c->type != BARQ_TYPE_F32)
+        return fail(BARQ_E_UNSUPPORTED, "kv_cache_head: the cache holds no f32 rows (kv_cache_read decodes them)");
     const size_t off = layer * c->layer_stride() + head * c->head_stride();
     if (k) *k = c->k + off;
     if (v) *v = c->v + off;
@@ -173,11 +191,31 @@ int barq_rocm_kv_cache_append(barq_rocm_handle* h, barq_rocm_kv_cache* c, size_t
         return fail(BARQ_E_DIM, "kv_cache_append: head_dim %zu, cache has %zu", head_dim, c->head_dim);
     if (n_tokens == 0) return ok();
     if (!k || !v) return fail(BARQ_E_INVALID, "kv_cache_append: null buffer");
-    if (c->len[layer] + n_tokens > c->max_size)
+    if (n_tokens > c->max_size - c->len[layer])
         return fail(BARQ_E_INVALID, "kv_cache_append: layer %zu holds %zu of %zu positions, %zu more do not fit", layer,
                     c->len[layer], c->max_size, n_tokens);
     if (h->device != c->device) return fail(BARQ_E_INVALID, "kv_cache_append: cache is on another device");
     DeviceGuard g(h);
+    if (c->type == BARQ_TYPE_Q4_0) {
+        const size_t n = c->n_head_kv * n_tokens * head_dim;
+        BARQ_CHECK(check_int_range(n, "kv_cache_append: elements"));
+        if (!aligned(k, 4) || !aligned(v, 4)) return fail(BARQ_E_INVALID, "kv_cache_append: rows must be 4-byte aligned");
+        if (mem == BARQ_MEM_HOST) {
+            Arena a;
+            const size_t ok_ = a.add(n * 4), ov = a.add(n * 4);
+            BARQ_CHECK(ensure_ws(h, a.used));
+            BARQ_HIP(hipMemcpyAsync(at<float>(h, ok_), k, n * 4, hipMemcpyHostToDevice, h->stream));
+            BARQ_HIP(hipMemcpyAsync(at<float>(h, ov), v, n * 4, hipMemcpyHostToDevice, h->stream));
+            k = at<float>(h, ok_);
+            v = at<float>(h, ov);
+        }
+        BARQ_CHECK(launched(barq::q4_append_launch(c->view(layer), k, v, n_tokens * head_dim, head_dim, c->n_head_kv,
+                                                   head_dim, c->len[layer], n_tokens, h->stream), "kv_cache_append"));
+        if (mem == BARQ_MEM_HOST) BARQ_HIP(hipStreamSynchronize(h->stream));
+        c->len[layer] += n_tokens;
+        if (layer == 0) c->size += n_tokens;
+        return ok();
+    }
     const size_t row = n_tokens * head_dim * sizeof(float);
     const size_t dst_off = layer * c->layer_stride() + c->len[layer] * head_dim;
     const hipMemcpyKind kind = mem == BARQ_MEM_DEVICE ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
@@ -210,7 +248,7 @@ int append_rope_any(barq_rocm_handle* h, barq_rocm_kv_cache* c, size_t layer, co
     if (!k_proj || !v_proj || !inv_freq) return fail(BARQ_E_INVALID, "%s: null buffer", who);
     // an out-of-range layer appends nothing (the reference returns silently); q is still rotated
     const bool append = layer < c->n_layers;
-    if (append && c->len[layer] + n_tokens > c->max_size)
+    if (append && n_tokens > c->max_size - c->len[layer])
         return fail(BARQ_E_INVALID, "%s: layer %zu holds %zu of %zu positions, %zu more do not fit", who, layer,
                     c->len[layer], c->max_size, n_tokens);
     if (!append && !q_proj) return ok();
@@ -239,7 +277,11 @@ int append_rope_any(barq_rocm_handle* h, barq_rocm_kv_cache* c, size_t layer, co
             qo = at<float>(h, oqo);
         }
     }
-    if (!q_proj) {
+    if (append && c->type == BARQ_TYPE_Q4_0) {
+        BARQ_CHECK(launched(barq::q4_append_rope_launch(layout, c->view(layer), qp, n_head, qo, kp, vp, c->n_head_kv, hd,
+                                                        c->len[layer], n_tokens, start_pos, freq_scale, fp, h->stream),
+                            who));
+    } else if (!q_proj) {
         BARQ_CHECK(launched(barq::rope_launch(layout, kp, c->k + dst_off, n_tokens, c->n_head_kv, hd, start_pos,
                                               freq_scale, fp, c->head_stride(), h->stream), "kv_cache_append_rope (k)"));
         BARQ_CHECK(launched(barq::transpose_heads_launch(vp, c->v + dst_off, n_tokens, c->n_head_kv, hd,
@@ -305,6 +347,7 @@ int barq_rocm_qkv_append_rope(barq_rocm_handle* h, barq_rocm_kv_cache* c, size_t
                     c->len[layer], c->max_size);
     const size_t rows[3] = {nq, nkv, nkv};
     if (mem == BARQ_MEM_DEVICE && act_type == BARQ_TYPE_Q8_K && layout == BARQ_ROPE_INTERLEAVED && append &&
+        c->type == BARQ_TYPE_F32 &&
         aligned(x, 4) && aligned(q_out, 4) && barq::qkv_rope_supported(w_types, w, nq, nkv, k, hd)) {
         DeviceGuard g(h);
         const size_t dst_off = layer * c->layer_stride() + c->len[layer] * hd;
@@ -368,7 +411,9 @@ int attention_any(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache*
     if (q_len > 65535) return fail(BARQ_E_DIM, "attention: q_len %zu above 65535", q_len);
     DeviceGuard g(h);
     const size_t nq = n_head * q_len * head_dim;
-    const size_t wsp = barq::attention_workspace(n_head, head_dim, q_len, kv_len, n_head_kv);
+    const bool q4 = c->type == BARQ_TYPE_Q4_0;
+    const size_t wsp = q4 ? barq::attention_q4_workspace(n_head, n_head_kv, head_dim, q_len, kv_len)
+                          : barq::attention_workspace(n_head, head_dim, q_len, kv_len, n_head_kv);
     Arena a;
     const size_t nq8 = out_q8 ? q_len * (n_head * head_dim / 256) * 292 : 0;
     const size_t op = a.add(wsp ? wsp : 4);
@@ -390,7 +435,7 @@ int attention_any(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache*
         args.out = at<float>(h, oo);
         if (out_q8) args.out_q8 = at<uint8_t>(h, oq8);
     }
-    args.k = c->k;
+    args.k = c->k;   // (null in a 4-bit cache)
     args.v = c->v;
     args.layer_off = layer * c->layer_stride();
     args.head_stride = c->head_stride();
@@ -401,8 +446,9 @@ int attention_any(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache*
     args.kv_len = kv_len;
     args.start_pos = start_pos;
     args.part = at<float>(h, op);
-    BARQ_CHECK(launched(barq::attention_launch(args, h->stream), "attention"));
-    if (out_q8 && !barq::attention_q8_direct(args))
+    BARQ_CHECK(launched(q4 ? barq::attention_q4_launch(args, c->view(layer), h->stream)
+                           : barq::attention_launch(args, h->stream), "attention"));
+    if (out_q8 && !(q4 ? barq::attention_q4_q8_direct(args) : barq::attention_q8_direct(args)))
         BARQ_CHECK(launched(barq::quantize_q8_k_launch(args.out, q_len, n_head * head_dim, args.out_q8, h->stream),
                             "attention_q8k (quantize)"));
     if (mem == BARQ_MEM_HOST) {

@@ -571,6 +571,27 @@ bool attention_q8_direct(const AttnArgs& a) {
     return ns > 1;
 }
 
+template <int HD>
+static hipError_t attn_combine_t(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s) {
+    if (out_q8)
+        hipLaunchKernelGGL(attn_combine_q8k_kernel<HD>, dim3((unsigned)(a.n_head * HD / 256), (unsigned)a.q_len),
+                           dim3(1024), 0, s, a.part, ns, (int)a.n_head, out_q8);
+    else
+        hipLaunchKernelGGL(attn_combine_kernel<HD>, dim3((unsigned)a.n_head, (unsigned)a.q_len), dim3(1024), 0, s,
+                           a.part, ns, (int)a.n_head, a.out);
+    return hipGetLastError();
+}
+
+// a.part's ns partial states per row and head into out_q8, or without it into a.out
+hipError_t attention_combine_launch(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s) {
+    switch (a.head_dim) {
+    case 64: return attn_combine_t<64>(a, ns, out_q8, s);
+    case 128: return attn_combine_t<128>(a, ns, out_q8, s);
+    case 256: return attn_combine_t<256>(a, ns, out_q8, s);
+    default: return hipErrorInvalidValue;
+    }
+}
+
 template <int HD, int G>
 static hipError_t attn_launch_t(const AttnArgs& a, int ns, int chunk, int groups, hipStream_t s) {
     const float scale = (1.0f / sqrtf((float)HD)) * LOG2E;
@@ -579,13 +600,7 @@ static hipError_t attn_launch_t(const AttnArgs& a, int ns, int chunk, int groups
                        (long long)a.start_pos, chunk, scale, a.part, a.out);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || ns == 1) return e;
-    if (a.out_q8 && attention_q8_direct(a))
-        hipLaunchKernelGGL(attn_combine_q8k_kernel<HD>, dim3((unsigned)(a.n_head * HD / 256), (unsigned)a.q_len),
-                           dim3(1024), 0, s, a.part, ns, (int)a.n_head, a.out_q8);
-    else
-        hipLaunchKernelGGL(attn_combine_kernel<HD>, dim3((unsigned)a.n_head, (unsigned)a.q_len), dim3(1024), 0, s,
-                           a.part, ns, (int)a.n_head, a.out);
-    return hipGetLastError();
+    return attn_combine_t<HD>(a, ns, a.out_q8 && attention_q8_direct(a) ? a.out_q8 : nullptr, s);
 }
 
 template <int HD>

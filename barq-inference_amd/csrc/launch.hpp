@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include "kv_q4.hpp"
+
 namespace barq {
 
 // dequant.hip
@@ -201,6 +203,25 @@ void attention_plan(size_t n_head, size_t n_head_kv, size_t q_len, size_t kv_len
 size_t attention_workspace(size_t n_head, size_t head_dim, size_t q_len, size_t kv_len, size_t n_head_kv);
 hipError_t attention_launch(const AttnArgs& a, hipStream_t s);
 int cu_count_attn();   // CUs of the current device
+
+// merges ns partial states [q_len][n_head][ns][head_dim + 2] of a.part (ns <= 1024)
+hipError_t attention_combine_launch(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s);
+
+// kv_q4.hip: rows into and out of a 4-bit cache; first: the cache position of row 0
+hipError_t q4_append_launch(const Q4View& dst, const float* k, const float* v, size_t src_head, size_t src_pos,
+                            size_t n_kv, size_t hd, size_t first, size_t n, hipStream_t s);
+// apply_rope on k_proj [n, n_kv * hd] (and, unless null, on q [n, n_q * hd] into q_out) on the way
+hipError_t q4_append_rope_launch(int layout, const Q4View& dst, const float* q, size_t n_q, float* q_out, const float* k,
+                                 const float* v, size_t n_kv, size_t hd, size_t first, size_t n, size_t start_pos,
+                                 float freq_scale, const float* inv_freq, hipStream_t s);
+// k, v [n_kv, n, hd] f32; either may be null
+hipError_t q4_read_launch(const Q4View& w, size_t n_kv, size_t hd, size_t first, size_t n, float* k, float* v,
+                          hipStream_t s);
+
+// attention_q4.hip: attention_launch and its helpers for a 4-bit cache (a.k, a.v, a.layer_off and a.head_stride unused)
+size_t attention_q4_workspace(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);
+bool attention_q4_q8_direct(const AttnArgs& a);
+hipError_t attention_q4_launch(const AttnArgs& a, const Q4View& kv, hipStream_t s);
 
 // attention_prompt.hip: chunks of many query rows on the matrix cores
 bool attn_prompt_path(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);

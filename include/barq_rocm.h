@@ -416,6 +416,24 @@ int barq_rocm_kv_cache_append_rope(barq_rocm_handle* h, barq_rocm_kv_cache* c, s
                                    const float* k_proj, const float* v_proj, size_t n_tokens,
                                    size_t start_pos, float freq_scale, const float* inv_freq, int layout,
                                    int mem);
+/* A cache that holds its rows as `type` (kv_cache_create: BARQ_TYPE_F32).
+ * BARQ_TYPE_Q4_0: 32 dims share an f16 scale d, each element is a 4-bit code
+ * and reads as (code - 8) * d: 0.5625 bytes an element against 4 (the
+ * reference's 8-bit counterpart is quant/src/q8_kv.rs).  head_dim 64, 128 or
+ * 256.  Every call below and above takes either type: appends quantize, the
+ * attention calls decode.  d = t / -8 in f16 with t the block's first element
+ * of the largest |x|, limited to +-8188 (|x| beyond 65504 saturates); the code
+ * is the nearest one under d, the larger on a border.  A block with a NaN or
+ * an infinity reads as NaN.  kv_cache_head fails with BARQ_E_UNSUPPORTED on such a cache;
+ * device rows to append and read need 4-byte alignment only.
+ * type = the cache's (-1 for a null cache).
+ * read = rows first .. first + n - 1 of the layer as f32, k and v
+ * [n_head_kv, n, head_dim]; either may be NULL. */
+int barq_rocm_kv_cache_create_typed(barq_rocm_handle* h, size_t max_size, size_t n_layers, size_t n_head_kv,
+                                    size_t head_dim, int type, barq_rocm_kv_cache** out);
+int barq_rocm_kv_cache_type(const barq_rocm_kv_cache* c);
+int barq_rocm_kv_cache_read(barq_rocm_handle* h, const barq_rocm_kv_cache* c, size_t layer, size_t first, size_t n,
+                            float* k, float* v, int mem);
 /* append_rope_q = the three steps of self_attention between the projections
  * and compute_attention (transformer.rs:222-245: apply_rope on q, apply_rope
  * on k and transpose_heads on v, then KVCache::append) in one launch:
