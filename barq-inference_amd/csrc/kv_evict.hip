@@ -1,0 +1,349 @@
+// Eviction from the KV cache: which positions each kv head keeps, and moving
+// their rows together.
+//
+//   kept(h) = the newest `recent` positions and, of the others, the keep -
+//   recent with the largest mass (equal masses: the earlier position), in the order
+//   of their positions
+//
+// Selection: a workgroup per kv head looks for the want-th largest key (the
+// mass as an unsigned integer of the same order) 8 bits at a time from the
+// top, each time with a histogram of the keys that share the bits found so far, then numbers
+// the kept positions by a running count.  The histogram has a column for each
+// LDS bank: masses share their leading bits, and 64 lanes adding to one counter
+// would take turns.  Up to 64 keys a thread stay in registers over the five
+// passes; longer heads are read again by each (from the L2).
+//
+// The rows then move in one launch, bound by memory: f32 rows as they are;
+// of a 4-bit cache, whose tiles hold 8 positions of V in one dword per dim, a
+// thread builds the dwords of a tile's dims from those of its 8 sources.
+#include "common.hpp"
+#include "kv_q4.hpp"
+#include "launch.hpp"
+
+namespace barq {
+
+constexpr int EV_NT = 1024;
+constexpr int EV_CHUNK = 4 * EV_NT;   // keys of a pass over the workgroup, four in a row per thread
+
+struct EvictArgs {
+    const float* mass_in;
+    float* mass_out;     // may be mass_in or null
+    size_t stride;
+    int n, m, recent;    // positions, kept ones, the newest among them
+    int32_t* kept;       // [heads][m]
+};
+
+// The order of f32 values as unsigned integers; NaN as -infinity, -0 as 0.
+__device__ __forceinline__ uint32_t ev_key(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x != x ? -INFINITY : x + 0.0f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// Sum of the lanes before this one, and of all (64 lanes).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t& total) {
+    const int l = threadIdx.x & 63;
+    uint32_t s = v;
+    #pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const uint32_t o = (uint32_t)__shfl_up((int)s, d);
+        s += l >= d ? o : 0u;
+    }
+    total = (uint32_t)__builtin_amdgcn_readlane((int)s, 63);
+    return s - v;
+}
+
+// R: chunks whose masses stay in registers (n <= R * EV_CHUNK), or 0.
+template <int R>
+__global__ __launch_bounds__(EV_NT)
+void evict_select_kernel(EvictArgs a) {
+    __shared__ uint32_t hist[256][32];
+    __shared__ uint32_t part[EV_NT / 64];
+    __shared__ uint32_t found[2];   // the digit and what is left to find within it
+    const int t = threadIdx.x, l = t & 63, w = t >> 6, h = blockIdx.x;
+    const float* in = a.mass_in + (size_t)h * a.stride;
+    float* out = a.mass_out ? a.mass_out + (size_t)h * a.stride : nullptr;
+    int32_t* kept = a.kept + (size_t)h * a.m;
+    const int old = a.n - a.recent, want = a.m - a.recent, chunks = (a.n + EV_CHUNK - 1) / EV_CHUNK;
+
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    auto load = [&](int c, float (&x)[4]) {
+        const int j = c * EV_CHUNK + 4 * t;
+        if (j + 4 <= a.n) {
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(in + j);
+            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+        } else {
+            #pragma unroll
+            for (int u = 0; u < 4; u++) x[u] = j + u < a.n ? in[j + u] : 0.0f;
+        }
+    };
+    float reg[R ? R : 1][4];
+    if constexpr (R > 0) {
+        #pragma unroll
+        for (int c = 0; c < R; c++) load(c, reg[c]);
+    }
+    // f(chunk, its four masses): every chunk, in order
+    auto each = [&](auto f) {
+        if constexpr (R > 0) {
+            #pragma unroll
+            for (int c = 0; c < R; c++)
+                if (c < chunks) f(c, reg[c]);
+        } else {
+            float x[4];
+            for (int c = 0; c < chunks; c++) {
+                load(c, x);
+                f(c, x);
+            }
+        }
+    };
+
+    // the want-th largest key among the old positions
+    uint32_t key = 0, ties = 0;   // ties: how many of the keys equal to it are kept
+    const bool some = want > 0 && want < old;
+    if (some) {
+        uint32_t left = (uint32_t)want, mask = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            for (int i = t; i < 256 * 32; i += EV_NT) (&hist[0][0])[i] = 0;
+            __syncthreads();
+            each([&](int c, const float (&x)[4]) {
+                #pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const uint32_t k = ev_key(x[u]);
+                    if (c * EV_CHUNK + 4 * t + u < old && (k & mask) == key)
+                        atomicAdd(&hist[(k >> shift) & 255u][t & 31], 1u);
+                }
+            });
+            __syncthreads();
+            // four threads a digit (whole quads), then the digits above it
+            if (t < 1024) {
+                const int digit = 255 - t / 4;   // wave 0 holds the largest
+                uint32_t s = 0;
+                #pragma unroll
+                for (int i = 0; i < 8; i++) s += hist[digit][(t & 3) * 8 + ((i + t / 4) & 7)];
+                s = (uint32_t)quad_isum((int)s);
+                uint32_t all;
+                const uint32_t before = wave_scan((t & 3) == 0 ? s : 0u, all);
+                if (l == 0) part[w] = all;
+                __syncthreads();
+                uint32_t above = (t & 3) == 0 ? before : 0u;
+                for (int i = 0; i < w; i++) above += part[i];
+                if ((t & 3) == 0 && above < left && left <= above + s) {
+                    found[0] = (uint32_t)digit;
+                    found[1] = left - above;
+                }
+            }
+            __syncthreads();
+            key |= found[0] << shift;
+            left = found[1];
+            mask |= 255u << shift;
+        }
+        ties = left;
+    }
+
+    // numbering: of each position the kept ones before it; larger keys and
+    // keys equal to the last one counted side by side (16 bits each a chunk)
+    uint32_t gt0 = 0, eq0 = 0;
+    each([&](int c, const float (&x)[4]) {
+        uint32_t flags[4], mine = 0;
+        #pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int j = c * EV_CHUNK + 4 * t + u;
+            const uint32_t k = ev_key(x[u]);
+            const bool newest = j >= old && j < a.n;
+            const bool gt = newest || (j < old && (some ? k > key : want > 0));
+            flags[u] = gt ? 1u : some && j < old && k == key ? 0x10000u : 0u;
+            mine += flags[u];
+        }
+        uint32_t all;
+        uint32_t before = wave_scan(mine, all);
+        __syncthreads();   // part is free (and, in place, this chunk's masses are read by all)
+        if (l == 0) part[w] = all;
+        __syncthreads();
+        uint32_t sum = 0;
+        for (int i = 0; i < EV_NT / 64; i++) {
+            const uint32_t p = part[i];
+            before += i < w ? p : 0u;
+            sum += p;
+        }
+        uint32_t gt = gt0 + (before & 0xFFFFu), eq = eq0 + (before >> 16);
+        #pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const bool keep = flags[u] == 1u || (flags[u] && eq < ties);
+            if (keep) {
+                const uint32_t at = gt + (eq < ties ? eq : ties);
+                kept[at] = c * EV_CHUNK + 4 * t + u;
+                if (out) out[at] = x[u];
+            }
+            gt += flags[u] & 0xFFFFu;
+            eq += flags[u] >> 16;
+        }
+        gt0 += sum & 0xFFFFu;
+        eq0 += sum >> 16;
+    });
+    __syncthreads();   // in place: the tail is read
+    if (out)
+        for (int j = a.m + t; j < a.n; j += EV_NT) out[j] = 0.0f;
+}
+
+hipError_t evict_select_launch(const float* mass_in, float* mass_out, size_t stride, size_t n_kv, size_t n, size_t m,
+                               size_t recent, int32_t* kept, hipStream_t s) {
+    EvictArgs a{mass_in, mass_out, stride, (int)n, (int)m, (int)(recent < n ? recent : n), kept};
+    const size_t chunks = (n + EV_CHUNK - 1) / EV_CHUNK;
+    const dim3 grid((unsigned)n_kv), block(EV_NT);
+    if (chunks <= 1) hipLaunchKernelGGL(evict_select_kernel<1>, grid, block, 0, s, a);
+    else if (chunks <= 4) hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, s, a);
+    else if (chunks <= 16) hipLaunchKernelGGL(evict_select_kernel<16>, grid, block, 0, s, a);
+    else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, s, a);
+    return hipGetLastError();
+}
+
+// ---- f32 rows ----------------------------------------------------------------------
+
+// One thread per V of a row: out[h][j] = in[h][kept[h][j]], K and V.
+template <class V>
+__global__ __launch_bounds__(256)
+void gather_rows_kernel(const V* __restrict__ k, const V* __restrict__ v, size_t src_head, V* __restrict__ ko, V* __restrict__ vo,
+                        size_t dst_head, int n_kv, int per_row, int m, const int32_t* __restrict__ kept) {
+    size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const int i = (int)(t % per_row);
+    t /= per_row;
+    const int j = (int)(t % m);
+    t /= m;
+    const int h = (int)(t % n_kv);
+    t /= n_kv;
+    if (t >= 2) return;
+    const size_t from = (size_t)h * src_head + (size_t)kept[(size_t)h * m + j] * per_row + i;
+    (t ? vo : ko)[(size_t)h * dst_head + (size_t)j * per_row + i] = (t ? v : k)[from];
+}
+
+hipError_t gather_rows_launch(const float* k, const float* v, size_t src_head, float* ko, float* vo, size_t dst_head,
+                              size_t n_kv, size_t hd, size_t m, const int32_t* kept, hipStream_t s) {
+    if (hd % 4 == 0) {   // (every row then starts at a multiple of 16 bytes)
+        const size_t n = 2 * n_kv * m * (hd / 4);
+        hipLaunchKernelGGL(gather_rows_kernel<float4>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,
+                           reinterpret_cast<const float4*>(k), reinterpret_cast<const float4*>(v), src_head / 4,
+                           reinterpret_cast<float4*>(ko), reinterpret_cast<float4*>(vo), dst_head / 4, (int)n_kv,
+                           (int)(hd / 4), (int)m, kept);
+    } else {
+        const size_t n = 2 * n_kv * m * hd;
+        hipLaunchKernelGGL(gather_rows_kernel<float>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k, v, src_head,
+                           ko, vo, dst_head, (int)n_kv, (int)hd, (int)m, kept);
+    }
+    return hipGetLastError();
+}
+
+// ---- 4-bit rows ----------------------------------------------------------------------
+
+// Three kinds of workgroups: V codes (a thread per tile and HD / 16 dims),
+// K codes (a thread per 16 bytes of a row), scales (a thread per tile and block, K's and V's).
+template <int HD>
+__global__ __launch_bounds__(256)
+void gather_q4_kernel(Q4View src, Q4View dst, int n_kv, int m, int tiles, const int32_t* __restrict__ kept, unsigned v_blocks,
+                      unsigned k_blocks) {
+    constexpr int NB = HD / 32, CT = HD / 16;
+    if (blockIdx.x < v_blocks) {
+        size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
+        const int i = (int)(t % 16);
+        t /= 16;
+        const int tile = (int)(t % tiles), h = (int)(t / tiles);
+        if (h >= n_kv) return;
+        const int32_t* id = kept + (size_t)h * m;
+        uint32_t w[CT] = {};
+        #pragma unroll
+        for (int e = 0; e < KV_TILE; e++) {
+            if (tile * KV_TILE + e < m) {
+                const int p = id[tile * KV_TILE + e], from = p % KV_TILE;
+                const int down = 4 * (from >> 1) + 16 * (from & 1), up = 4 * (e >> 1) + 16 * (e & 1);
+                const uint4* x = reinterpret_cast<const uint4*>(src.vc + (size_t)h * src.code_head +
+                                                                (size_t)(p / KV_TILE) * (KV_TILE * HD / 2) + i * (CT * 4));
+                #pragma unroll
+                for (int c = 0; c < CT / 4; c++) {
+                    const uint4 q = x[c];
+                    w[4 * c] |= ((q.x >> down) & 15u) << up;
+                    w[4 * c + 1] |= ((q.y >> down) & 15u) << up;
+                    w[4 * c + 2] |= ((q.z >> down) & 15u) << up;
+                    w[4 * c + 3] |= ((q.w >> down) & 15u) << up;
+                }
+            }
+        }
+        uint4* y = reinterpret_cast<uint4*>(dst.vc + (size_t)h * dst.code_head + (size_t)tile * (KV_TILE * HD / 2) + i * (CT * 4));
+        #pragma unroll
+        for (int c = 0; c < CT / 4; c++) y[c] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+    } else if (blockIdx.x < v_blocks + k_blocks) {
+        size_t t = (size_t)(blockIdx.x - v_blocks) * 256 + threadIdx.x;
+        const int i = (int)(t % NB);
+        t /= NB;
+        const int j = (int)(t % m), h = (int)(t / m);
+        if (h >= n_kv) return;
+        const int p = kept[(size_t)h * m + j];
+        reinterpret_cast<uint4*>(dst.kc + (size_t)h * dst.code_head + (size_t)j * (HD / 2))[i] =
+            reinterpret_cast<const uint4*>(src.kc + (size_t)h * src.code_head + (size_t)p * (HD / 2))[i];
+    } else {
+        size_t t = (size_t)(blockIdx.x - v_blocks - k_blocks) * 256 + threadIdx.x;
+        const int b = (int)(t % NB);
+        t /= NB;
+        const bool is_v = t % 2;
+        t /= 2;
+        const int tile = (int)(t % tiles), h = (int)(t / tiles);
+        if (h >= n_kv) return;
+        const uint16_t* x = reinterpret_cast<const uint16_t*>((is_v ? src.vs : src.ks) + (size_t)h * src.scale_head);
+        uint32_t w[4] = {};
+        #pragma unroll
+        for (int e = 0; e < KV_TILE; e++)
+            if (tile * KV_TILE + e < m) {
+                const int p = kept[(size_t)h * m + tile * KV_TILE + e];
+                w[e / 2] |= (uint32_t)x[((size_t)(p / KV_TILE) * NB + b) * KV_TILE + p % KV_TILE] << (16 * (e & 1));
+            }
+        reinterpret_cast<uint4*>((is_v ? dst.vs : dst.ks) + (size_t)h * dst.scale_head)[(size_t)tile * NB + b] =
+            make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+template <int HD>
+static hipError_t gather_q4_t(const Q4View& src, const Q4View& dst, size_t n_kv, size_t m, const int32_t* kept, hipStream_t s) {
+    const size_t tiles = q4_tiles(m);
+    const unsigned vb = (unsigned)((n_kv * tiles * 16 + 255) / 256), kb = (unsigned)((n_kv * m * (HD / 32) + 255) / 256),
+                   sb = (unsigned)((n_kv * tiles * 2 * (HD / 32) + 255) / 256);
+    hipLaunchKernelGGL(gather_q4_kernel<HD>, dim3(vb + kb + sb), dim3(256), 0, s, src, dst, (int)n_kv, (int)m, (int)tiles,
+                       kept, vb, kb);
+    return hipGetLastError();
+}
+
+hipError_t gather_q4_launch(const Q4View& src, const Q4View& dst, size_t n_kv, size_t hd, size_t m, const int32_t* kept,
+                            hipStream_t s) {
+    switch (hd) {
+    case 64: return gather_q4_t<64>(src, dst, n_kv, m, kept, s);
+    case 128: return gather_q4_t<128>(src, dst, n_kv, m, kept, s);
+    case 256: return gather_q4_t<256>(src, dst, n_kv, m, kept, s);
+    default: return hipErrorInvalidValue;
+    }
+}
+
+// ---- back from the staging area ----------------------------------------------------------
+
+template <class V>
+__global__ __launch_bounds__(256)
+void copy_planes_kernel(CopyPlanes p, int heads) {
+    const int plane = blockIdx.z, h = blockIdx.y;
+    const size_t n = p.bytes[plane] / sizeof(V);
+    const V* x = reinterpret_cast<const V*>(p.src[plane] + (size_t)h * p.src_head[plane]);
+    V* y = reinterpret_cast<V*>(p.dst[plane] + (size_t)h * p.dst_head[plane]);
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) y[i] = x[i];
+}
+
+hipError_t copy_planes_launch(const CopyPlanes& p, size_t heads, hipStream_t s) {
+    bool wide = true;
+    size_t most = 0;
+    for (int i = 0; i < p.n; i++) {
+        wide = wide && p.bytes[i] % 16 == 0 && p.src_head[i] % 16 == 0 && p.dst_head[i] % 16 == 0 &&
+               (reinterpret_cast<uintptr_t>(p.src[i]) | reinterpret_cast<uintptr_t>(p.dst[i])) % 16 == 0;
+        most = most > p.bytes[i] ? most : p.bytes[i];
+    }
+    size_t blocks = (most / (wide ? 16 : 4) + 255) / 256;
+    blocks = blocks < 1 ? 1 : blocks > 1024 ? 1024 : blocks;
+    const dim3 grid((unsigned)blocks, (unsigned)heads, (unsigned)p.n);
+    if (wide) hipLaunchKernelGGL(copy_planes_kernel<uint4>, grid, dim3(256), 0, s, p, (int)heads);
+    else hipLaunchKernelGGL(copy_planes_kernel<uint32_t>, grid, dim3(256), 0, s, p, (int)heads);
+    return hipGetLastError();
+}
+
+}  // namespace barq

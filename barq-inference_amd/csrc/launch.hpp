@@ -218,6 +218,24 @@ hipError_t q4_append_rope_launch(int layout, const Q4View& dst, const float* q, 
 hipError_t q4_read_launch(const Q4View& w, size_t n_kv, size_t hd, size_t first, size_t n, float* k, float* v,
                           hipStream_t s);
 
+// kv_evict.hip: kept [n_kv][m] (m = min(keep, n)) from mass_in's rows of n, and the kept masses in
+// mass_out (may be mass_in or null), the rest of its n zero
+hipError_t evict_select_launch(const float* mass_in, float* mass_out, size_t stride, size_t n_kv, size_t n, size_t m,
+                               size_t recent, int32_t* kept, hipStream_t s);
+// rows kept[h][j] of every kv head to rows j (strides: floats between kv heads; source and destination disjoint)
+hipError_t gather_rows_launch(const float* k, const float* v, size_t src_head, float* ko, float* vo, size_t dst_head,
+                              size_t n_kv, size_t hd, size_t m, const int32_t* kept, hipStream_t s);
+hipError_t gather_q4_launch(const Q4View& src, const Q4View& dst, size_t n_kv, size_t hd, size_t m, const int32_t* kept,
+                            hipStream_t s);
+// up to four planes of heads rows each (bytes a multiple of 4, strides in bytes)
+struct CopyPlanes {
+    int n;
+    const uint8_t* src[4];
+    uint8_t* dst[4];
+    size_t src_head[4], dst_head[4], bytes[4];
+};
+hipError_t copy_planes_launch(const CopyPlanes& p, size_t heads, hipStream_t s);
+
 // attention_q4.hip: attention_launch and its helpers for a 4-bit cache (a.k, a.v, a.layer_off and a.head_stride unused)
 size_t attention_q4_workspace(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);
 bool attention_q4_q8_direct(const AttnArgs& a);

@@ -434,6 +434,22 @@ int barq_rocm_kv_cache_create_typed(barq_rocm_handle* h, size_t max_size, size_t
 int barq_rocm_kv_cache_type(const barq_rocm_kv_cache* c);
 int barq_rocm_kv_cache_read(barq_rocm_handle* h, const barq_rocm_kv_cache* c, size_t layer, size_t first, size_t n,
                             float* k, float* v, int mem);
+/* evict = of every kv head of src's layer keep min(keep, len) positions: the
+ * newest `recent` (at most keep) and of the others those with the largest
+ * mass, the earlier one where masses are equal (a NaN counts as -infinity).
+ * They become dst's layer in the order of their positions (dst may be src, or a cache of the same
+ * type, kv heads and head_dim with room for them; what its layer held is
+ * replaced).  mass_in and mass_out are [n_head_kv][mass_stride] with one value per
+ * position, mass_stride >= len (barq_rocm_attention_mass gathers them);
+ * mass_out (may be NULL or mass_in, otherwise disjoint from it) receives the kept
+ * positions' masses and zeros up to src's length, so the positions appended
+ * next start from zero.  kept (may be NULL) is [n_head_kv][min(keep, len)].
+ * Uses the handle's workspace.  RoPE has been applied to the rows, so new ones keep
+ * counting positions from where they were, while attention counts rows of the
+ * cache: its start_pos is then kv_len - q_len. */
+int barq_rocm_kv_cache_evict(barq_rocm_handle* h, const barq_rocm_kv_cache* src, barq_rocm_kv_cache* dst, size_t layer,
+                             const float* mass_in, float* mass_out, size_t mass_stride, size_t keep, size_t recent,
+                             int32_t* kept, int mem);
 /* append_rope_q = the three steps of self_attention between the projections
  * and compute_attention (transformer.rs:222-245: apply_rope on q, apply_rope
  * on k and transpose_heads on v, then KVCache::append) in one launch:
