@@ -67,7 +67,7 @@ EXPORTS = (
     "barq_rocm_kv_cache_head", "barq_rocm_kv_cache_clear", "barq_rocm_kv_cache_destroy", "barq_rocm_attention",
     "barq_rocm_kv_cache_append_rope_q", "barq_rocm_attention_q8k", "barq_rocm_matvec_group",
     "barq_rocm_qkv_append_rope", "barq_rocm_kv_cache_create_typed", "barq_rocm_kv_cache_type", "barq_rocm_kv_cache_read",
-    "barq_rocm_kv_cache_evict", "barq_rocm_matmul_noalloc", "barq_rocm_stream_read",
+    "barq_rocm_kv_cache_evict", "barq_rocm_attention_mass", "barq_rocm_matmul_noalloc", "barq_rocm_stream_read",
 )
 
 # bytes of the fixed per-GPU scratch behind barq_rocm_matmul_noalloc
@@ -155,6 +155,7 @@ def _declare(lib):
         "barq_rocm_kv_cache_type": (_i, [_vp]),
         "barq_rocm_kv_cache_read": (_i, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _i]),
         "barq_rocm_kv_cache_evict": (_i, [_vp, _vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _i]),
+        "barq_rocm_attention_mass": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, _i, _vp, _vp, _vp, _sz, _i]),
         "barq_rocm_kv_cache_size": (_sz, [_vp]),
         "barq_rocm_kv_cache_layer_len": (_sz, [_vp, _sz]),
         "barq_rocm_kv_cache_head": (_i, [_vp, _sz, _sz, ctypes.POINTER(_vp), ctypes.POINTER(_vp)]),

@@ -212,3 +212,25 @@ def compute_attention_q8k(be: Backend, q, cache: KVCache, layer, n_head, n_head_
     if sync and mem == L.MEM_DEVICE:
         be.sync()
     return out
+
+
+def compute_attention_mass(be: Backend, q, cache: KVCache, layer, n_head, n_head_kv, head_dim, q_len, kv_len, start_pos,
+                           mass, mass_out=None, out_type=L.F32, mem=L.MEM_DEVICE, sync=True, out=None):
+    """compute_attention that also adds the positions' softmax weights to mass
+    [n_head_kv, at least kv_len] (None: zeros), into mass_out (by default mass
+    itself).  Returns (out, mass_out); out_type Q8_K gives
+    compute_attention_q8k's rows."""
+    if mass_out is None:
+        mass_out = _empty((n_head_kv, kv_len), q, mem) if mass is None else mass
+    for m in (mass, mass_out):
+        if m is not None and (len(m.shape) != 2 or m.shape[0] != n_head_kv or m.shape[1] != mass_out.shape[1]):
+            raise L.BarqError(L.E_DIM, f"attention_mass: mass must be [{n_head_kv}, positions]")
+    if out is None:
+        out = (_empty((q_len, n_head, head_dim), q, mem) if out_type == L.F32
+               else _empty((q_len, n_head * head_dim // 256 * 292), q, mem, dtype="uint8"))
+    L.check(be._lib.barq_rocm_attention_mass(be.h, _ptr(q), cache.c, layer, n_head, n_head_kv, head_dim, q_len, kv_len,
+                                             start_pos, out_type, _ptr(out), _ptr(mass), _ptr(mass_out),
+                                             mass_out.shape[1], mem))
+    if sync and mem == L.MEM_DEVICE:
+        be.sync()
+    return out, mass_out

@@ -175,11 +175,15 @@ __device__ __forceinline__ float4 kv_ld(__amdgpu_buffer_rsrc_t r, uint32_t off) 
 // Grid: x = split, y = head group (kv head for G > 1; query head for G == 1),
 // z = query row i.  The workgroup covers positions [split * chunk, ...) of
 // the visible prefix [0, min(kv_len, start_pos + i + 1)).
-template <int HD, int G>
+//
+// SC: the scores (log2 units) of the positions a query sees go to scores[i *
+// n_head + h][position] as well, and every split leaves its partial state.
+template <int HD, int G, bool SC = false>
 __global__ __launch_bounds__(ATT_THREADS)
 void attn_kernel(const float* __restrict__ q, const float* __restrict__ kc, const float* __restrict__ vc,
                  size_t layer_off, size_t head_stride, int n_head, int n_head_kv, int q_len, int kv_len,
-                 long long start_pos, int chunk, float score_scale, float* __restrict__ part, float* __restrict__ out) {
+                 long long start_pos, int chunk, float score_scale, float* __restrict__ part, float* __restrict__ out,
+                 float* __restrict__ scores, size_t score_stride) {
     constexpr int LPR = HD / 8;              // lanes per K/V row
     constexpr int R = ATT_THREADS / LPR;     // rows per pass
     static_assert(LPR == 8 || LPR == 16 || LPR == 32, "head_dim 64, 128 or 256");
@@ -258,6 +262,11 @@ void attn_kernel(const float* __restrict__ q, const float* __restrict__ kc, cons
                 // (q . k) / sqrt(hd) * log2(e); rows past the range do not count
                 sc[p] = blk + p * R + r < j1 ? dot * score_scale : -INFINITY;
                 bm = fmaxf(bm, sc[p]);
+                if constexpr (SC) {
+                    const int h = G > 1 ? grp * G + g : grp;
+                    if (c == 0 && blk + p * R + r < j1)
+                        scores[((size_t)i * n_head + h) * score_stride + blk + p * R + r] = sc[p];
+                }
             }
             // No branch on a block without live rows: a branch around the
             // V products lets the compiler's wait insertion assume the V
@@ -357,7 +366,7 @@ void attn_kernel(const float* __restrict__ q, const float* __restrict__ kc, cons
             for (int rr = 0; rr < R; rr++) O = __builtin_fmaf(red_o[rr][g][d], red_ml[rr][g][0], O);
         }
         const int h = G > 1 ? grp * G + g : grp;
-        if (n_split == 1) {
+        if (n_split == 1 && !SC) {
             out[((size_t)i * n_head + h) * HD + d] = O / L;
         } else {
             float* pp = part + (((size_t)i * n_head + h) * n_split + split) * (HD + 2);
@@ -597,7 +606,7 @@ static hipError_t attn_launch_t(const AttnArgs& a, int ns, int chunk, int groups
     const float scale = (1.0f / sqrtf((float)HD)) * LOG2E;
     hipLaunchKernelGGL((attn_kernel<HD, G>), dim3(ns, groups, (unsigned)a.q_len), dim3(ATT_THREADS), 0, s, a.q, a.k,
                        a.v, a.layer_off, a.head_stride, (int)a.n_head, (int)a.n_head_kv, (int)a.q_len, (int)a.kv_len,
-                       (long long)a.start_pos, chunk, scale, a.part, a.out);
+                       (long long)a.start_pos, chunk, scale, a.part, a.out, nullptr, 0);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || ns == 1) return e;
     return attn_combine_t<HD>(a, ns, a.out_q8 && attention_q8_direct(a) ? a.out_q8 : nullptr, s);
@@ -613,6 +622,44 @@ static hipError_t attn_launch_hd(const AttnArgs& a, hipStream_t s) {
     case 4: return attn_launch_t<HD, 4>(a, ns, chunk, (int)a.n_head_kv, s);
     case 8: return attn_launch_t<HD, 8>(a, ns, chunk, (int)a.n_head_kv, s);
     default: return attn_launch_t<HD, 1>(a, ns, chunk, (int)a.n_head, s);
+    }
+}
+
+template <int HD, int G>
+static hipError_t attn_scores_t(const AttnArgs& a, const AttnScores& sc, int ns, int chunk, int groups, hipStream_t s) {
+    const float scale = (1.0f / sqrtf((float)HD)) * LOG2E;
+    hipLaunchKernelGGL((attn_kernel<HD, G, true>), dim3(ns, groups, (unsigned)a.q_len), dim3(ATT_THREADS), 0, s, a.q, a.k,
+                       a.v, a.layer_off, a.head_stride, (int)a.n_head, (int)a.n_head_kv, (int)sc.q_rows, (int)a.kv_len,
+                       (long long)a.start_pos, chunk, scale, a.part, a.out, sc.scores, sc.stride);
+    return hipGetLastError();
+}
+
+template <int HD>
+static hipError_t attn_scores_hd(const AttnArgs& a, const AttnScores& sc, int ns, int chunk, hipStream_t s) {
+    const size_t g = a.n_head % a.n_head_kv == 0 ? a.n_head / a.n_head_kv : 1;
+    switch (g) {
+    case 2: return attn_scores_t<HD, 2>(a, sc, ns, chunk, (int)a.n_head_kv, s);
+    case 4: return attn_scores_t<HD, 4>(a, sc, ns, chunk, (int)a.n_head_kv, s);
+    case 8: return attn_scores_t<HD, 8>(a, sc, ns, chunk, (int)a.n_head_kv, s);
+    default: return attn_scores_t<HD, 1>(a, sc, ns, chunk, (int)a.n_head, s);
+    }
+}
+
+int attention_scores_splits(size_t n_head, size_t n_head_kv, size_t q_len, size_t kv_len) {
+    int ns = 0, chunk = 0;
+    attention_plan(n_head, n_head_kv, q_len, kv_len, &ns, &chunk);
+    return ns;
+}
+
+// The decode kernel for any number of rows (the prompt kernel keeps no scores).
+hipError_t attention_scores_launch(const AttnArgs& a, const AttnScores& sc, hipStream_t s) {
+    int ns = 0, chunk = 0;
+    attention_plan(a.n_head, a.n_head_kv, a.q_len, a.kv_len, &ns, &chunk);
+    switch (a.head_dim) {
+    case 64: return attn_scores_hd<64>(a, sc, ns, chunk, s);
+    case 128: return attn_scores_hd<128>(a, sc, ns, chunk, s);
+    case 256: return attn_scores_hd<256>(a, sc, ns, chunk, s);
+    default: return hipErrorInvalidValue;
     }
 }
 

@@ -55,10 +55,11 @@ struct Q4Args {
     const float* q;        // [n_head, q_len, HD]
     Q4View kv;
     int n_head, n_head_kv, G, q_len, kv_len;
+    int q_rows;            // rows of q per head (the call's are the first q_len)
     long long start_pos;
     int chunk, n_split;    // positions of a split, splits
     float scale;           // 16 log2(e) / sqrt(HD)
-    float* part;           // [q_len][n_head][splits][HD + 2] (more than one split)
+    float* part;           // [q_len][n_head][splits][HD + 2] (SC, or more than one split)
     float* out;            // [q_len, n_head, HD]
     float* scores;         // SC: [q_len * n_head][score_stride], log2 units
     size_t score_stride;
@@ -393,7 +394,7 @@ void attn_q4_kernel(Q4Args a) {
     const int j0 = min(split * a.chunk, visible), j1 = min(visible, j0 + a.chunk), end = min(vis, j1);
 
     Q4Query<HD> q;
-    q.load(a.q + ((size_t)h * a.q_len + i) * HD, a.scale, g, l, wave, reinterpret_cast<bf8v*>(lds));
+    q.load(a.q + ((size_t)h * a.q_rows + i) * HD, a.scale, g, l, wave, reinterpret_cast<bf8v*>(lds));
     float* score_row = nullptr;
     if (SC && r0 + c < rows_n) score_row = a.scores + ((size_t)i * a.n_head + h) * a.score_stride;
     Q4State<HD> st;
@@ -448,7 +449,7 @@ void attn_q4_kernel(Q4Args a) {
         }
         const int ii = (r0 + rr) / a.G, hh = grp * a.G + (r0 + rr - ii * a.G);
         const size_t at = (size_t)ii * a.n_head + hh;
-        if (n_split == 1) {
+        if (n_split == 1 && !SC) {
             a.out[at * HD + d] = O / L;
         } else {
             float* pp = a.part + (at * n_split + split) * (HD + 2);
@@ -499,8 +500,12 @@ bool attention_q4_q8_direct(const AttnArgs& a) {
     return (a.n_head * a.head_dim) % 256 == 0 && q4_plan(a.n_head, a.n_head_kv, a.q_len, a.kv_len).n_split > 1;
 }
 
+int attention_q4_scores_splits(size_t n_head, size_t n_head_kv, size_t q_len, size_t kv_len) {
+    return q4_plan(n_head, n_head_kv, q_len, kv_len).n_split;
+}
+
 template <int HD>
-static hipError_t attn_q4_launch_t(const AttnArgs& a, const Q4View& kv, hipStream_t s) {
+static hipError_t attn_q4_launch_t(const AttnArgs& a, const AttnScores* sc, const Q4View& kv, hipStream_t s) {
     const Q4Plan p = q4_plan(a.n_head, a.n_head_kv, a.q_len, a.kv_len);
     Q4Args k{};
     k.q = a.q;
@@ -510,26 +515,42 @@ static hipError_t attn_q4_launch_t(const AttnArgs& a, const Q4View& kv, hipStrea
     k.G = p.G;
     k.q_len = (int)a.q_len;
     k.kv_len = (int)a.kv_len;
+    k.q_rows = (int)(sc ? sc->q_rows : a.q_len);
     k.start_pos = (long long)a.start_pos;
     k.chunk = p.chunk;
     k.n_split = p.n_split;
     k.scale = 16.0f * 1.44269504088896340736f / sqrtf((float)HD);
     k.part = a.part;
     k.out = a.out;
-    hipLaunchKernelGGL((attn_q4_kernel<HD, false>), dim3((unsigned)p.n_split * (unsigned)p.tiles, p.groups), dim3(64 * Q4A_NW), 0, s, k);
+    const dim3 grid((unsigned)p.n_split * (unsigned)p.tiles, p.groups), block(64 * Q4A_NW);
+    if (sc) {
+        k.scores = sc->scores;
+        k.score_stride = sc->stride;
+        hipLaunchKernelGGL((attn_q4_kernel<HD, true>), grid, block, 0, s, k);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((attn_q4_kernel<HD, false>), grid, block, 0, s, k);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.n_split == 1) return e;
     return attention_combine_launch(a, p.n_split, attention_q4_q8_direct(a) ? a.out_q8 : nullptr, s);
 }
 
-hipError_t attention_q4_launch(const AttnArgs& a, const Q4View& kv, hipStream_t s) {
-    if (a.q_len == 0 || a.n_head == 0) return hipSuccess;
+static hipError_t attn_q4_launch(const AttnArgs& a, const AttnScores* sc, const Q4View& kv, hipStream_t s) {
     switch (a.head_dim) {
-    case 64: return attn_q4_launch_t<64>(a, kv, s);
-    case 128: return attn_q4_launch_t<128>(a, kv, s);
-    case 256: return attn_q4_launch_t<256>(a, kv, s);
+    case 64: return attn_q4_launch_t<64>(a, sc, kv, s);
+    case 128: return attn_q4_launch_t<128>(a, sc, kv, s);
+    case 256: return attn_q4_launch_t<256>(a, sc, kv, s);
     default: return hipErrorInvalidValue;
     }
+}
+
+hipError_t attention_q4_launch(const AttnArgs& a, const Q4View& kv, hipStream_t s) {
+    if (a.q_len == 0 || a.n_head == 0) return hipSuccess;
+    return attn_q4_launch(a, nullptr, kv, s);
+}
+
+hipError_t attention_q4_scores_launch(const AttnArgs& a, const AttnScores& sc, const Q4View& kv, hipStream_t s) {
+    return attn_q4_launch(a, &sc, kv, s);
 }
 
 }  // namespace barq

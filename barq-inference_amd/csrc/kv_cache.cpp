@@ -1,5 +1,6 @@
 // C ABI of what a KV cache offers beyond the reference's (include/barq_rocm.h):
-// reading its rows whatever it holds them as, and dropping positions.
+// reading its rows whatever it holds them as, dropping positions, and
+// the attention that gathers what the dropping goes by.
 #include "../../include/barq_rocm.h"
 
 #include <hip/hip_runtime.h>
@@ -141,6 +142,121 @@ int barq_rocm_kv_cache_evict(barq_rocm_handle* h, const barq_rocm_kv_cache* src,
         BARQ_HIP(hipStreamSynchronize(h->stream));
     }
     return done();
+}
+
+// Scores of one launch at most: a prompt's rows are taken in chunks.
+static constexpr size_t MASS_SCORES = (size_t)64 << 20;
+
+int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache* c, size_t layer, size_t n_head,
+                             size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len, size_t start_pos, int out_type,
+                             void* out, const float* mass_in, float* mass_out, size_t mass_stride, int mem) {
+    const char* who = "attention_mass";
+    BARQ_CHECK(check_mem(mem));
+    BARQ_CHECK(check_handle(h));
+    if (!c) return fail(BARQ_E_INVALID, "%s: null cache", who);
+    if (out_type != BARQ_TYPE_F32 && out_type != BARQ_TYPE_Q8_K)
+        return fail(BARQ_E_UNSUPPORTED, "%s: out_type %d (BARQ_TYPE_F32 or BARQ_TYPE_Q8_K)", who, out_type);
+    if (q_len == 0 || n_head == 0)
+        return fail(BARQ_E_DIM, "%s: no query rows or heads", who);
+    if (!q || !out || !mass_out) return fail(BARQ_E_INVALID, "%s: null buffer", who);
+    if (layer >= c->n_layers) return fail(BARQ_E_INVALID, "%s: layer %zu of %zu", who, layer, c->n_layers);
+    if (n_head_kv != c->n_head_kv || head_dim != c->head_dim)
+        return fail(BARQ_E_DIM, "%s: n_head_kv %zu / head_dim %zu, cache has %zu / %zu", who, n_head_kv, head_dim,
+                    c->n_head_kv, c->head_dim);
+    if (!barq::attention_supported(head_dim))
+        return fail(BARQ_E_UNSUPPORTED, "%s: head_dim %zu (64, 128 or 256 supported)", who, head_dim);
+    const bool q8 = out_type == BARQ_TYPE_Q8_K, q4 = c->type == BARQ_TYPE_Q4_0, host = mem == BARQ_MEM_HOST;
+    if (n_head > 65535 || q_len > 65535 || start_pos > 0x7fffffff - q_len)
+        return fail(BARQ_E_DIM, "%s: n_head %zu and q_len %zu must be at most 65535, start_pos %zu + q_len below 2^31", who,
+                    n_head, q_len, start_pos);
+    if (q8 && (n_head * head_dim) % 256 != 0)
+        return fail(BARQ_E_DIM, "%s: n_head * head_dim = %zu is not a multiple of 256", who, n_head * head_dim);
+    if (kv_len == 0 || kv_len > c->len[layer])
+        return fail(BARQ_E_DIM, "%s: kv_len %zu, layer %zu holds %zu positions", who, kv_len, layer, c->len[layer]);
+    if (mass_stride < kv_len) return fail(BARQ_E_DIM, "%s: mass_stride %zu below kv_len %zu", who, mass_stride, kv_len);
+    if (h->device != c->device) return fail(BARQ_E_INVALID, "%s: cache is on another device", who);
+    if (!host && (!aligned(q, 16) || !aligned(out, 4) || !aligned(mass_in, 4) || !aligned(mass_out, 4)))
+        return fail(BARQ_E_INVALID, "%s: q must be 16-byte aligned, the other buffers 4-byte aligned", who);
+    DeviceGuard g(h);
+    const size_t stride = round_up(kv_len, 32), per_row = n_head * stride * sizeof(float);
+    size_t rows = MASS_SCORES / per_row;
+    rows = rows < 1 ? 1 : rows > q_len ? q_len : rows;
+    const auto splits = [&](size_t n) {
+        return (size_t)(q4 ? barq::attention_q4_scores_splits(n_head, n_head_kv, n, kv_len)
+                           : barq::attention_scores_splits(n_head, n_head_kv, n, kv_len));
+    };
+    const size_t last = q_len % rows;   // the last chunk's rows, if fewer
+    const auto states = [&](size_t n) { return splits(n) * n_head * n * (head_dim + 2) * sizeof(float); };
+    size_t part = states(rows);
+    if (last && states(last) > part) part = states(last);
+    const size_t nq = n_head * q_len * head_dim, out_row = q8 ? n_head * head_dim / 256 * 292 : n_head * head_dim * 4;
+    Arena a;
+    const size_t os = a.add(rows * per_row), op = a.add(part), ost = a.add(barq::attention_mass_stat(n_head, n_head_kv, rows));
+    const size_t oq = host ? a.add(nq * 4) : 0, oo = host ? a.add(q_len * out_row) : 0;
+    const size_t om = host ? a.add(n_head_kv * kv_len * sizeof(float)) : 0;
+    BARQ_CHECK(ensure_ws(h, a.used));
+    const size_t mrow = kv_len * sizeof(float);
+    const float* mi = mass_in;
+    float* mo = mass_out;
+    size_t ms = mass_stride;
+    uint8_t* ob = static_cast<uint8_t*>(out);
+    if (host) {
+        BARQ_HIP(hipMemcpyAsync(at<float>(h, oq), q, nq * 4, hipMemcpyHostToDevice, h->stream));
+        q = at<float>(h, oq);
+        mo = at<float>(h, om);
+        if (mass_in) {
+            BARQ_HIP(hipMemcpy2DAsync(mo, mrow, mass_in, mass_stride * sizeof(float), mrow, n_head_kv, hipMemcpyHostToDevice,
+                                      h->stream));
+            mi = mo;
+        }
+        ms = kv_len;
+        ob = at<uint8_t>(h, oo);
+    }
+    for (size_t i = 0; i < q_len; i += rows) {
+        const size_t n = rows < q_len - i ? rows : q_len - i;
+        barq::AttnArgs args{};
+        args.q = q + i * head_dim;
+        args.k = c->k;   // (null in a 4-bit cache)
+        args.v = c->v;
+        args.layer_off = layer * c->layer_stride();
+        args.head_stride = c->head_stride();
+        args.n_head = n_head;
+        args.n_head_kv = n_head_kv;
+        args.head_dim = head_dim;
+        args.q_len = n;
+        args.kv_len = kv_len;
+        args.start_pos = start_pos + i;
+        args.part = at<float>(h, op);
+        args.out = q8 ? nullptr : reinterpret_cast<float*>(ob + i * out_row);
+        const barq::AttnScores sc{at<float>(h, os), stride, q_len};
+        BARQ_CHECK(launched(q4 ? barq::attention_q4_scores_launch(args, sc, c->view(layer), h->stream)
+                               : barq::attention_scores_launch(args, sc, h->stream), who));
+        const int ns = (int)splits(n);
+        BARQ_CHECK(launched(barq::attention_combine_launch(args, ns, q8 ? ob + i * out_row : nullptr, h->stream), who));
+        barq::MassArgs m{};
+        m.scores = sc.scores;
+        m.score_stride = stride;
+        m.part = args.part;
+        m.ns = ns;
+        m.head_dim = (int)head_dim;
+        m.n_head = (int)n_head;
+        m.n_head_kv = (int)n_head_kv;
+        m.q_len = (int)n;
+        m.kv_len = (int)kv_len;
+        m.start_pos = (long long)(start_pos + i);
+        m.stat = at<float>(h, ost);
+        m.mass_in = i ? mo : mi;
+        m.mass_out = mo;
+        m.mass_stride = ms;
+        BARQ_CHECK(launched(barq::attention_mass_launch(m, h->stream), who));
+    }
+    if (host) {
+        BARQ_HIP(hipMemcpyAsync(out, ob, q_len * out_row, hipMemcpyDeviceToHost, h->stream));
+        BARQ_HIP(hipMemcpy2DAsync(mass_out, mass_stride * sizeof(float), mo, mrow, mrow, n_head_kv, hipMemcpyDeviceToHost,
+                                  h->stream));
+        BARQ_HIP(hipStreamSynchronize(h->stream));
+    }
+    return ok();
 }
 
 }  // extern "C"

@@ -204,6 +204,36 @@ size_t attention_workspace(size_t n_head, size_t head_dim, size_t q_len, size_t 
 hipError_t attention_launch(const AttnArgs& a, hipStream_t s);
 int cu_count_attn();   // CUs of the current device
 
+// Attention that leaves its scores and partial states behind: a.part (ns
+// states per row and head, the splits functions' ns, one at least) and scores
+// [q_len * n_head][stride] in log2 units, positions the row does not see
+// undefined; the caller merges.  q_rows: rows of q per head.
+struct AttnScores {
+    float* scores;
+    size_t stride;   // a multiple of 32, kv_len at least
+    size_t q_rows;
+};
+int attention_scores_splits(size_t n_head, size_t n_head_kv, size_t q_len, size_t kv_len);
+hipError_t attention_scores_launch(const AttnArgs& a, const AttnScores& sc, hipStream_t s);
+int attention_q4_scores_splits(size_t n_head, size_t n_head_kv, size_t q_len, size_t kv_len);
+hipError_t attention_q4_scores_launch(const AttnArgs& a, const AttnScores& sc, const Q4View& kv, hipStream_t s);
+
+// attention_mass.hip: mass_out[hk][j] = mass_in[hk][j] (null: 0) + the softmax weights of position j over the call's
+// rows and the heads of hk, j < kv_len, from what the launches above left (in and out may be the same)
+struct MassArgs {
+    const float* scores;
+    size_t score_stride;
+    const float* part;     // [q_len][n_head][ns][head_dim + 2]
+    int ns, head_dim, n_head, n_head_kv, q_len, kv_len;
+    long long start_pos;
+    float* stat;           // q_len * n_head pairs (attention_mass_stat)
+    const float* mass_in;
+    float* mass_out;
+    size_t mass_stride;
+};
+size_t attention_mass_stat(size_t n_head, size_t n_head_kv, size_t q_len);   // bytes of stat (0: not used)
+hipError_t attention_mass_launch(const MassArgs& a, hipStream_t s);
+
 // merges ns partial states [q_len][n_head][ns][head_dim + 2] of a.part (ns <= 1024)
 hipError_t attention_combine_launch(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s);
 

@@ -507,6 +507,21 @@ int barq_rocm_attention_q8k(barq_rocm_handle* h, const float* q, const barq_rocm
                             size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len,
                             size_t start_pos, void* out_q8k, int mem);
 
+/* attention_mass = barq_rocm_attention (out_type BARQ_TYPE_F32) or _q8k
+ * (BARQ_TYPE_Q8_K) that also gathers how much weight the positions get:
+ * mass_out[hk, j] = mass_in[hk, j] + sum of p_j over the call's queries and
+ * the query heads that read kv head hk, for j < kv_len (a position that no
+ * query sees gets 0).  mass_in (NULL: zeros; may be mass_out) and mass_out are
+ * [n_head_kv][mass_stride], mass_stride >= kv_len; columns from kv_len on are left
+ * as they are.  barq_rocm_kv_cache_evict goes by them.  The output agrees with
+ * barq_rocm_attention's within float rounding (an f32 cache's prompt chunks take
+ * the decode kernel here).  Uses the handle's workspace for the scores, at
+ * most 64 MiB of them or one query's. */
+int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache* c, size_t layer,
+                             size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len,
+                             size_t start_pos, int out_type, void* out, const float* mass_in, float* mass_out,
+                             size_t mass_stride, int mem);
+
 /* ---- measurement ------------------------------------------------------------
  * No counterpart in the reference.  Reads bytes (rounded down to 16) at the
  * device pointer p once, with coalesced non-temporal loads and nothing else:
