@@ -295,19 +295,19 @@ __device__ __forceinline__ void q4_step(Q4Step<HD>& s, int base, int j1, int end
     #pragma unroll
     for (int e = 0; e < 8; e++) least = min(least, __builtin_bit_cast(uint32_t, p[e]) - 1u);
     const bool spread = __any(least < __builtin_bit_cast(uint32_t, Q4A_WINDOW) - 1u);
-    float up = 0x1p15f, inv = w * 0x1p-15f;
+    float inv = w * 0x1p-15f;
     bool more = false;
     do {
         float y[8];
         #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = p[e] * up;
+        for (int e = 0; e < 8; e++) y[e] = p[e] * 0x1p15f;
         if (spread) {
             bool left = false;
             #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const bool later = y[e] < 0x1p15f * Q4A_WINDOW;   // (false for NaN)
+                const bool later = p[e] < Q4A_WINDOW;   // (false for NaN)
                 y[e] = later ? 0.0f : y[e];
-                p[e] = later ? p[e] : 0.0f;
+                p[e] = later ? p[e] * (1.0f / Q4A_WINDOW) : 0.0f;
                 left |= p[e] > 0.0f;
             }
             more = __any(left);
@@ -332,7 +332,6 @@ __device__ __forceinline__ void q4_step(Q4Step<HD>& s, int base, int j1, int end
             #pragma unroll
             for (int r = 0; r < 4; r++) st.o[c][r] = __builtin_fmaf(d[r], inv, st.o[c][r]);
         }
-        up *= 1.0f / Q4A_WINDOW;
         inv *= Q4A_WINDOW;
     } while (more);
 }

@@ -195,6 +195,27 @@ def test_spread_scores_and_values(be):
         assert np.all(np.abs(got[0, h] - ref[0, h]) <= 4e-4 * size + 1e-30)
 
 
+@pytest.mark.parametrize("peak", [60, 140, 1000])
+def test_weights_down_to_the_least(be, peak):
+    """Scores that fall evenly from 0 to -peak (log2) over 64 positions, so
+    that weights of every size down to f32's least, and zeros, meet in a step."""
+    hd, n = 64, 64
+    q = np.zeros((2, 1, hd), F32)
+    q[:, 0, 0] = 1
+    k, v = np.zeros((1, n, hd), F32), rows(13, 1, n, hd)
+    k[0, :, 0] = -np.random.default_rng(1).permutation(n) * peak / n * np.log(2) * np.sqrt(hd)
+    v[0, np.argmax(k[0, :, 0])] = 0
+    c = A.KVCache(be, n, 1, 1, hd, type=B.Q4_0)
+    c.append(0, dev(k), dev(v), n, hd)
+    kq, vq = q4_values(k), q4_values(v)
+    ref, _ = attention(q, kq, vq, n - 1)
+    got = A.compute_attention(be, dev(q), c, 0, 2, 1, hd, 1, n, n - 1).cpu().numpy()
+    s = kq[0, :, 0].astype(np.float64) / np.sqrt(hd)
+    size = np.exp(s - s.max()) @ np.abs(vq[0].astype(np.float64))
+    # one product a score: its three roundings and the exponent's (2^-23 of peak each) and 2^-20 for the rest
+    assert np.all(np.abs(got[0] - ref[0]) <= (4 * peak * 2.0 ** -23 + 2.0 ** -20) * size + 1e-37)
+
+
 def test_refusals(be):
     E = B._lib
     with pytest.raises(B.BarqError) as e:
