@@ -137,18 +137,19 @@ class KVCache:
             self.be.sync()
         return k, v
 
-    def evict(self, layer, mass, keep, recent, dst=None, mass_out=None, mem=L.MEM_DEVICE, sync=True):
+    def evict(self, layer, mass, keep, recent, dst=None, mass_out=None, mem=L.MEM_DEVICE, sync=True, want_kept=True):
         """Keep min(keep, len) positions of every kv head of the layer (in dst,
         by default this cache): the newest `recent` and the heaviest of the
         others by mass [n_head_kv, at least len].  The kept masses and zeros
         behind them go to mass_out (by default mass itself).  Returns (kept
-        positions [n_head_kv, min(keep, len)] int32, mass_out)."""
+        positions [n_head_kv, min(keep, len)] int32, or None without want_kept;
+        mass_out)."""
         dst = self if dst is None else dst
         mass_out = mass if mass_out is None else mass_out
         if len(mass.shape) != 2 or mass.shape[0] != self.n_head_kv or tuple(mass_out.shape) != tuple(mass.shape):
             raise L.BarqError(L.E_DIM, f"evict: mass must be [{self.n_head_kv}, positions]")
         m = min(keep, self.layer_len(layer))
-        kept = _empty((self.n_head_kv, m), mass, mem, dtype="int32")
+        kept = _empty((self.n_head_kv, m), mass, mem, dtype="int32") if want_kept else None
         L.check(self.be._lib.barq_rocm_kv_cache_evict(self.be.h, self.c, dst.c, layer, _ptr(mass), _ptr(mass_out),
                                                        mass.shape[1], keep, recent, _ptr(kept), mem))
         if sync and mem == L.MEM_DEVICE:

@@ -49,6 +49,10 @@ class Backend:
     def set_stream(self, stream_handle: int | None):
         L.check(self._lib.barq_rocm_set_stream(self.h, stream_handle or None))
 
+    def stream(self) -> int:
+        """The hipStream_t that calls are enqueued on."""
+        return self._lib.barq_rocm_get_stream(self.h)
+
     def sync(self):
         L.check(self._lib.barq_rocm_synchronize(self.h))
 

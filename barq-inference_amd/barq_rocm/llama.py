@@ -20,6 +20,11 @@ fused residual-add + RMSNorm quantizer, as a deployment runs it.
       length is the vocabulary's           -> add_rms_norm_quantize, matmul,
                                              barq_rocm_add_bias
 
+The KV cache may hold f32 rows or 4-bit blocks (attention.KVCache's type).
+With a KVBudget the chain gathers each position's attention weight
+(barq_rocm_attention_mass in place of _q8k) and drops the lightest ones when a
+layer has outgrown the budget (barq_rocm_kv_cache_evict).
+
 Weights come from a lookup name -> (type, n_rows, k, device pointer) or
 None: a WeightCache of a GGUF file (WeightCache.find) or any mapping with
 the GGUF tensor names.  Every compute step is a libbarq_rocm call on the
@@ -56,14 +61,32 @@ class LlamaConfig:
                         dtype=np.float32)
 
 
+@dataclass
+class KVBudget:
+    """How many positions a layer keeps: once it holds more than keep + slack
+    after a forward's attention, the newest `recent` and the heaviest others
+    stay, keep in all.  slack spreads the cost of an eviction over that many
+    tokens."""
+    keep: int
+    recent: int
+    slack: int = 0
+
+
 class DeviceLlama:
     """forward(tokens, start_pos) -> logits of the last token, on the device.
 
     get(name) returns (type, n_rows, k, device pointer) or None.  The KV
-    cache is the caller's (attention.KVCache with cfg.n_layer layers)."""
+    cache is the caller's (attention.KVCache with cfg.n_layer layers); clear()
+    it for a new session.  budget: see KVBudget."""
 
-    def __init__(self, be: Backend, cfg: LlamaConfig, get, kv: A.KVCache):
+    def __init__(self, be: Backend, cfg: LlamaConfig, get, kv: A.KVCache, budget: KVBudget | None = None):
         import torch
+        if budget is not None and not (0 <= budget.recent <= budget.keep and budget.keep > 0 and budget.slack >= 0):
+            raise ValueError(f"{budget}: recent may be at most keep, and neither keep 0 nor anything negative")
+        self.budget = budget
+        # the weight each cached position has gathered, per layer
+        self.mass = (None if budget is None else
+                     [torch.zeros((cfg.n_head_kv, kv.max_size), dtype=torch.float32, device="cuda") for _ in range(cfg.n_layer)])
         self.be, self.cfg, self.get, self.kv = be, cfg, get, kv
         self.inv_freq = torch.from_numpy(cfg.inv_freq()).cuda()
         head = get("output.weight") or get("token_embd.weight")
@@ -152,8 +175,11 @@ class DeviceLlama:
                     outs.append(y)
                 kv.append_rope_q(il, outs[0], c.n_head, outs[1], outs[2], seq, start_pos, c.rope_freq_scale,
                                  self.inv_freq, c.rope_layout, q_out=qr)
-            A.compute_attention_q8k(be, qr, kv, il, c.n_head, c.n_head_kv, c.head_dim, seq, start_pos + seq,
-                                    start_pos, sync=False, out=aq)
+            if self.budget is None:
+                A.compute_attention_q8k(be, qr, kv, il, c.n_head, c.n_head_kv, c.head_dim, seq, start_pos + seq,
+                                        start_pos, sync=False, out=aq)
+            else:
+                self._attend_and_evict(il, qr, seq, aq)
             wo = self._need(pre + "attn_output.weight")
             be.matmul_raw(wo[0], wo[3], wo[1], wo[2], L.Q8_K, aq, seq, o, L.MEM_DEVICE)
             be.add_rms_norm_quantize(L.Q8_K, r_in, o, self._norm(pre + "ffn_norm.weight"), c.rms_norm_eps,
@@ -167,6 +193,19 @@ class DeviceLlama:
             # the next layer sums x + ff into res[0] (x is res[1]: no buffer aliases another)
             x, prev = r_mid, ff
         return self.final_output(x[seq - 1:seq], prev[seq - 1:seq])
+
+    def _attend_and_evict(self, il, qr, seq, aq):
+        """The layer's attention over all its cached rows (the last seq are
+        this call's), their masses, and an eviction when they are too many."""
+        import torch
+        be, c, kv, n = self.be, self.cfg, self.kv, self.kv.layer_len(il)
+        if n == seq:   # the layer was empty: a new session
+            with torch.cuda.stream(torch.cuda.ExternalStream(be.stream())):
+                self.mass[il].zero_()
+        A.compute_attention_mass(be, qr, kv, il, c.n_head, c.n_head_kv, c.head_dim, seq, n, n - seq, self.mass[il],
+                                 out_type=L.Q8_K, sync=False, out=aq)
+        if n > self.budget.keep + self.budget.slack:
+            kv.evict(il, self.mass[il], self.budget.keep, self.budget.recent, sync=False, want_kept=False)
 
     def final_output(self, res_last, ff_last):
         """final_output of the last row: output_norm(res + ff) as Q8_K, the
