@@ -515,6 +515,46 @@ void attn_combine_q8k_kernel(const float* __restrict__ part, int n_split, int n_
     }
 }
 
+// The same merge by one wave per 256 output values (256 / HD heads of row i;
+// fewer in a last wave), four values a lane, the states one after another in
+// one pass: for many rows of few states each, which workgroups of 1024 threads
+// would take turns at.  Q8 writes the values' Q8_K block.
+template <int HD, bool Q8>
+__global__ __launch_bounds__(256)
+void attn_merge_kernel(const float* __restrict__ part, int n_split, int n_head, int rows, float* __restrict__ out,
+                       uint8_t* __restrict__ out_q8) {
+    const int nblk = (n_head * HD + 255) / 256;
+    const long long at = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = (int)(at / nblk), b = (int)(at % nblk);
+    if (i >= rows) return;
+    const int l = threadIdx.x & 63;
+    const int h = b * (256 / HD) + 4 * l / HD, d = 4 * l % HD;
+    if (!Q8 && h >= n_head) return;
+    const float* pp = part + ((size_t)i * n_head + h) * n_split * (HD + 2);
+    float M = -INFINITY, L = 0.0f, O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    #pragma unroll 4
+    for (int sp = 0; sp < n_split; sp++, pp += HD + 2) {
+        const float2 ml = *reinterpret_cast<const float2*>(pp);   // 8-byte aligned rows
+        const float2 o0 = *reinterpret_cast<const float2*>(pp + 2 + d), o1 = *reinterpret_cast<const float2*>(pp + 4 + d);
+        const float mn = fmaxf(M, ml.x);
+        // a split that saw no position is (-inf, 0, 0)
+        const float c = M == -INFINITY ? 0.0f : fast_exp2(M - mn), w = ml.x == -INFINITY ? 0.0f : fast_exp2(ml.x - mn);
+        M = mn;
+        L = __builtin_fmaf(ml.y, w, L * c);
+        O[0] = __builtin_fmaf(o0.x, w, O[0] * c);
+        O[1] = __builtin_fmaf(o0.y, w, O[1] * c);
+        O[2] = __builtin_fmaf(o1.x, w, O[2] * c);
+        O[3] = __builtin_fmaf(o1.y, w, O[3] * c);
+    }
+    const float vv[4] = {O[0] / L, O[1] / L, O[2] / L, O[3] / L};
+    if constexpr (!Q8) {
+        typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+        *reinterpret_cast<f32x4u*>(out + ((size_t)i * n_head + h) * HD + d) = f32x4u{vv[0], vv[1], vv[2], vv[3]};
+    } else {
+        q8_k_block(vv, l, out_q8 + ((size_t)i * nblk + b) * Q8_K_BYTES);
+    }
+}
+
 bool attention_supported(size_t head_dim) { return head_dim == 64 || head_dim == 128 || head_dim == 256; }
 
 int cu_count_attn() {
@@ -591,12 +631,29 @@ static hipError_t attn_combine_t(const AttnArgs& a, int ns, uint8_t* out_q8, hip
     return hipGetLastError();
 }
 
+template <int HD>
+static hipError_t attn_merge_t(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s) {
+    // Workgroups per row and head take two or three states as long as thirty
+    // (3.8 us for 32 heads of one row with 64, 26 us for 256 rows with one), waves
+    // 0.1 us a state and run side by side.
+    if (ns > 16 && a.n_head * a.q_len <= 512) return attn_combine_t<HD>(a, ns, out_q8, s);
+    const size_t waves = (a.n_head * HD + 255) / 256 * a.q_len;
+    const dim3 grid((unsigned)((waves + 3) / 4));
+    if (out_q8)
+        hipLaunchKernelGGL((attn_merge_kernel<HD, true>), grid, dim3(256), 0, s, a.part, ns, (int)a.n_head, (int)a.q_len, a.out,
+                           out_q8);
+    else
+        hipLaunchKernelGGL((attn_merge_kernel<HD, false>), grid, dim3(256), 0, s, a.part, ns, (int)a.n_head, (int)a.q_len,
+                           a.out, out_q8);
+    return hipGetLastError();
+}
+
 // a.part's ns partial states per row and head into out_q8, or without it into a.out
 hipError_t attention_combine_launch(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s) {
     switch (a.head_dim) {
-    case 64: return attn_combine_t<64>(a, ns, out_q8, s);
-    case 128: return attn_combine_t<128>(a, ns, out_q8, s);
-    case 256: return attn_combine_t<256>(a, ns, out_q8, s);
+    case 64: return attn_merge_t<64>(a, ns, out_q8, s);
+    case 128: return attn_merge_t<128>(a, ns, out_q8, s);
+    case 256: return attn_merge_t<256>(a, ns, out_q8, s);
     default: return hipErrorInvalidValue;
     }
 }

@@ -63,6 +63,7 @@
 // weights and output follow one another, and two waves share a SIMD.
 #include "attention_prompt_plan.hpp"
 #include "common.hpp"
+#include "f16_split.hpp"
 #include "launch.hpp"
 #include "mfma_common.hpp"
 #include "q8k_block.hpp"
@@ -71,7 +72,6 @@
 
 namespace barq {
 
-typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4n __attribute__((ext_vector_type(4)));
@@ -359,27 +359,6 @@ __device__ __forceinline__ void ap_rows_f32(const uint8_t* lds, uint32_t lds0, c
 
 // ---- split f16 ----------------------------------------------------------------------
 
-// x0, x1 -> packed f16 (hi) and packed f16 of what hi leaves (lo): one packed
-// conversion and two v_fma_mix{lo,hi}_f16.  The empty asm keeps the compiler
-// from converting every value a second time, and minus_one (-1 in a register
-// it knows nothing of) from turning the fma into a conversion and a
-// subtraction.
-__device__ __forceinline__ float ap_minus_one() {
-    float v = -1.0f;
-    asm("" : "+s"(v));
-    return v;
-}
-__device__ __forceinline__ void ap_split(float x0, float x1, float minus_one, uint32_t& hi, uint32_t& lo) {
-    asm("" : "+v"(x0), "+v"(x1));
-    const h2v hv = {(_Float16)x0, (_Float16)x1};
-    hi = __builtin_bit_cast(uint32_t, hv);
-    asm("" : "+v"(hi));
-    const h2v h = __builtin_bit_cast(h2v, hi);
-    const float r0 = __builtin_fmaf((float)h[0], minus_one, x0), r1 = __builtin_fmaf((float)h[1], minus_one, x1);
-    const h2v r = {(_Float16)r0, (_Float16)r1};
-    lo = __builtin_bit_cast(uint32_t, r);
-}
-
 // x0, x1, given times 2^12 -> packed f16 (hi) and 2^12 times what hi leaves
 // (lo; at most 2^15 for |x| up to 2^15): lo's smallest step is then 2^-36 of
 // x's unit instead of 2^-24.  Two
@@ -458,7 +437,7 @@ template <int HD>
 __device__ __forceinline__ void ap_convert(uint8_t* lds, const ApRegs<HD>& r, int n, int t, uint32_t& ve, uint32_t& ke_max, bool& bad) {
     using L = ApLds<HD>;
     uint8_t* st = lds + (n & 1) * L::STAGE;
-    const float mo = ap_minus_one();
+    const float mo = f16_minus_one();
     const int d = t % HD, part = t / HD;
     float mx = 0.0f;   // V: one scale per dim
     {
@@ -479,8 +458,8 @@ __device__ __forceinline__ void ap_convert(uint8_t* lds, const ApRegs<HD>& r, in
     #pragma unroll
     for (int i = 0; i < ApRegs<HD>::NK; i++) {
         uint2 h, lo;
-        ap_split(r.k[i][0] * ks, r.k[i][1] * ks, mo, h.x, lo.x);
-        ap_split(r.k[i][2] * ks, r.k[i][3] * ks, mo, h.y, lo.y);
+        split_f16(r.k[i][0] * ks, r.k[i][1] * ks, mo, h.x, lo.x);
+        split_f16(r.k[i][2] * ks, r.k[i][3] * ks, mo, h.y, lo.y);
         *reinterpret_cast<uint2*>(krow + 8 * L::TPR * i) = h;
         *reinterpret_cast<uint2*>(krow + L::KLO + 8 * L::TPR * i) = lo;
     }
@@ -707,15 +686,15 @@ __device__ __forceinline__ void ap_tile(uint8_t* lds, uint32_t lds0, const ApArg
         const uint32_t qe = ap_exp(qm);
         qm = group_max<32>(qm);
         if (l == 0) reinterpret_cast<float*>(lds + L::QM)[wave] = qm;
-        const float qs = ap_scale<AP_KQ>(qe), mo = ap_minus_one();
+        const float qs = ap_scale<AP_KQ>(qe), mo = f16_minus_one();
         qf = ap_unscale<AP_KQ>(qe) * a.scale;
         #pragma unroll
         for (int s = 0; s < HD / 16; s++) {
             uint32_t h[4], lo[4];
-            ap_split(qv[2 * s].x * qs, qv[2 * s].y * qs, mo, h[0], lo[0]);
-            ap_split(qv[2 * s].z * qs, qv[2 * s].w * qs, mo, h[1], lo[1]);
-            ap_split(qv[2 * s + 1].x * qs, qv[2 * s + 1].y * qs, mo, h[2], lo[2]);
-            ap_split(qv[2 * s + 1].z * qs, qv[2 * s + 1].w * qs, mo, h[3], lo[3]);
+            split_f16(qv[2 * s].x * qs, qv[2 * s].y * qs, mo, h[0], lo[0]);
+            split_f16(qv[2 * s].z * qs, qv[2 * s].w * qs, mo, h[1], lo[1]);
+            split_f16(qv[2 * s + 1].x * qs, qv[2 * s + 1].y * qs, mo, h[2], lo[2]);
+            split_f16(qv[2 * s + 1].z * qs, qv[2 * s + 1].w * qs, mo, h[3], lo[3]);
             qh[s] = __builtin_bit_cast(h8v, u32x4v{h[0], h[1], h[2], h[3]});
             ql[s] = __builtin_bit_cast(h8v, u32x4v{lo[0], lo[1], lo[2], lo[3]});
         }

@@ -1,0 +1,45 @@
+// Attention over a 4-bit KV cache on the host: which kernel a call takes and
+// how its rows and positions are cut into workgroups.
+#pragma once
+#include <stddef.h>
+
+namespace barq {
+
+constexpr int Q4P_NW = 4;               // waves of a workgroup of attn_q4_prompt_kernel
+constexpr int Q4P_ROWS = 16 * Q4P_NW;   // its query rows
+
+constexpr int Q4P_MIN_ROWS = 64;
+
+struct Q4Plan {
+    bool prompt;     // attn_q4_prompt_kernel
+    int G, groups;   // query heads that share a kv head (1 when they do not divide), and how many such groups
+    int tiles;       // workgroups' row tiles
+    int n_split, chunk;   // splits of the positions, positions of one
+};
+
+inline Q4Plan q4_plan(size_t n_head, size_t n_head_kv, size_t hd, size_t q_len, size_t kv_len, size_t cus) {
+    constexpr size_t STEP = 32, TURN = 128;
+    Q4Plan p;
+    const bool even = n_head % n_head_kv == 0;
+    p.G = even ? (int)(n_head / n_head_kv) : 1;
+    p.groups = even ? (int)n_head_kv : (int)n_head;
+    const size_t rows = q_len * p.G;
+    p.prompt = hd <= 128 && rows >= Q4P_MIN_ROWS;
+    const size_t per = p.prompt ? (size_t)Q4P_ROWS : 16, unit = p.prompt ? 4 * STEP : TURN;
+    p.tiles = (int)((rows + per - 1) / per);
+    const size_t wg = (size_t)p.groups * p.tiles, target = cus * (p.prompt || hd > 128 ? 2 : 3);
+    size_t ns = (target + wg - 1) / wg;
+    const size_t most = (kv_len + unit - 1) / unit;
+    if (ns > most) ns = most;
+    if (ns > 1024) ns = 1024;   // the merge's limit
+    // at most 2^20 positions a split (32-bit byte offsets)
+    const size_t least = (kv_len + ((size_t)1 << 20) - 1) >> 20;
+    if (ns < least) ns = least;
+    size_t ch = (kv_len + ns - 1) / ns;
+    ch = (ch + unit - 1) / unit * unit;
+    p.chunk = (int)ch;
+    p.n_split = (int)((kv_len + ch - 1) / ch);
+    return p;
+}
+
+}  // namespace barq

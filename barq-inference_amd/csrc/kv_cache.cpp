@@ -30,9 +30,21 @@ int barq_rocm_kv_cache_read(barq_rocm_handle* h, const barq_rocm_kv_cache* c, si
     const size_t hd = c->head_dim, row = n * hd * sizeof(float), bytes = c->n_head_kv * row;
     if (c->type == BARQ_TYPE_F32) {
         const size_t off = layer * c->layer_stride() + first * hd, pitch = c->head_stride() * sizeof(float);
-        const hipMemcpyKind kind = mem == BARQ_MEM_DEVICE ? hipMemcpyDeviceToDevice : hipMemcpyDeviceToHost;
-        if (k) BARQ_HIP(hipMemcpy2DAsync(k, row, c->k + off, pitch, row, c->n_head_kv, kind, h->stream));
-        if (v) BARQ_HIP(hipMemcpy2DAsync(v, row, c->v + off, pitch, row, c->n_head_kv, kind, h->stream));
+        if (mem == BARQ_MEM_DEVICE) {
+            barq::CopyPlanes p{};
+            for (int i = 0; i < 2; i++)
+                if (float* to = i ? v : k) {
+                    p.src[p.n] = reinterpret_cast<const uint8_t*>((i ? c->v : c->k) + off);
+                    p.dst[p.n] = reinterpret_cast<uint8_t*>(to);
+                    p.src_head[p.n] = pitch;
+                    p.dst_head[p.n] = p.bytes[p.n] = row;
+                    p.n++;
+                }
+            BARQ_CHECK(launched(barq::copy_planes_launch(p, c->n_head_kv, h->stream), "kv_cache_read"));
+            return ok();
+        }
+        if (k) BARQ_HIP(hipMemcpy2DAsync(k, row, c->k + off, pitch, row, c->n_head_kv, hipMemcpyDeviceToHost, h->stream));
+        if (v) BARQ_HIP(hipMemcpy2DAsync(v, row, c->v + off, pitch, row, c->n_head_kv, hipMemcpyDeviceToHost, h->stream));
     } else {
         float *dk = k, *dv = v;
         if (mem == BARQ_MEM_HOST) {
@@ -182,7 +194,7 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
     size_t rows = MASS_SCORES / per_row;
     rows = rows < 1 ? 1 : rows > q_len ? q_len : rows;
     const auto splits = [&](size_t n) {
-        return (size_t)(q4 ? barq::attention_q4_scores_splits(n_head, n_head_kv, n, kv_len)
+        return (size_t)(q4 ? barq::attention_q4_scores_splits(n_head, n_head_kv, head_dim, n, kv_len)
                            : barq::attention_scores_splits(n_head, n_head_kv, n, kv_len));
     };
     const size_t last = q_len % rows;   // the last chunk's rows, if fewer
@@ -192,6 +204,7 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
     const size_t nq = n_head * q_len * head_dim, out_row = q8 ? n_head * head_dim / 256 * 292 : n_head * head_dim * 4;
     Arena a;
     const size_t os = a.add(rows * per_row), op = a.add(part), ost = a.add(barq::attention_mass_stat(n_head, n_head_kv, rows));
+    const size_t osum = a.add(barq::attention_mass_sums(n_head, n_head_kv, rows, stride));
     const size_t oq = host ? a.add(nq * 4) : 0, oo = host ? a.add(q_len * out_row) : 0;
     const size_t om = host ? a.add(n_head_kv * kv_len * sizeof(float)) : 0;
     BARQ_CHECK(ensure_ws(h, a.used));
@@ -245,6 +258,7 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
         m.kv_len = (int)kv_len;
         m.start_pos = (long long)(start_pos + i);
         m.stat = at<float>(h, ost);
+        m.sums = at<float>(h, osum);
         m.mass_in = i ? mo : mi;
         m.mass_out = mo;
         m.mass_stride = ms;

@@ -39,25 +39,44 @@ __device__ __forceinline__ uint32_t ev_key(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sum of the lanes before this one, and of all (64 lanes).
+// Sum of the lanes before this one, and of all (64 lanes): within rows of 16
+// by shifts, then the rows' last lanes to the rows behind them.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t& total) {
-    const int l = threadIdx.x & 63;
-    uint32_t s = v;
+    int s = (int)v;
+    s += __builtin_amdgcn_update_dpp(0, s, 0x111, 0xF, 0xF, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x112, 0xF, 0xF, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x114, 0xF, 0xF, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x118, 0xF, 0xF, true);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x142, 0xA, 0xF, false);
+    s += __builtin_amdgcn_update_dpp(0, s, 0x143, 0xC, 0xF, false);
+    total = (uint32_t)__builtin_amdgcn_readlane(s, 63);
+    return (uint32_t)s - v;
+}
+
+// Sum of part[0 .. w), and of all 16.
+__device__ __forceinline__ uint32_t waves_before(const uint32_t* part, int w, uint32_t& total) {
+    uint32_t before = 0;
+    total = 0;
     #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t o = (uint32_t)__shfl_up((int)s, d);
-        s += l >= d ? o : 0u;
+    for (int i = 0; i < 16; i += 4) {
+        const uint4 p = *reinterpret_cast<const uint4*>(part + i);
+        const uint32_t q[4] = {p.x, p.y, p.z, p.w};
+        #pragma unroll
+        for (int u = 0; u < 4; u++) {
+            before += i + u < w ? q[u] : 0u;
+            total += q[u];
+        }
     }
-    total = (uint32_t)__builtin_amdgcn_readlane((int)s, 63);
-    return s - v;
+    return before;
 }
 
 // R: chunks whose masses stay in registers (n <= R * EV_CHUNK), or 0.
 template <int R>
 __global__ __launch_bounds__(EV_NT)
 void evict_select_kernel(EvictArgs a) {
-    __shared__ uint32_t hist[256][32];
-    __shared__ uint32_t part[EV_NT / 64];
+    __shared__ __align__(16) uint32_t hist[256][32];
+    __shared__ __align__(16) uint32_t part[EV_NT / 64];
+    static_assert(EV_NT == 1024, "16 waves, four threads a digit");
     __shared__ uint32_t found[2];   // the digit and what is left to find within it
     const int t = threadIdx.x, l = t & 63, w = t >> 6, h = blockIdx.x;
     const float* in = a.mass_in + (size_t)h * a.stride;
@@ -102,7 +121,7 @@ void evict_select_kernel(EvictArgs a) {
     if (some) {
         uint32_t left = (uint32_t)want, mask = 0;
         for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = t; i < 256 * 32; i += EV_NT) (&hist[0][0])[i] = 0;
+            for (int i = t; i < 256 * 8; i += EV_NT) reinterpret_cast<uint4*>(&hist[0][0])[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
             each([&](int c, const float (&x)[4]) {
                 #pragma unroll
@@ -114,22 +133,19 @@ void evict_select_kernel(EvictArgs a) {
             });
             __syncthreads();
             // four threads a digit (whole quads), then the digits above it
-            if (t < 1024) {
-                const int digit = 255 - t / 4;   // wave 0 holds the largest
-                uint32_t s = 0;
-                #pragma unroll
-                for (int i = 0; i < 8; i++) s += hist[digit][(t & 3) * 8 + ((i + t / 4) & 7)];
-                s = (uint32_t)quad_isum((int)s);
-                uint32_t all;
-                const uint32_t before = wave_scan((t & 3) == 0 ? s : 0u, all);
-                if (l == 0) part[w] = all;
-                __syncthreads();
-                uint32_t above = (t & 3) == 0 ? before : 0u;
-                for (int i = 0; i < w; i++) above += part[i];
-                if ((t & 3) == 0 && above < left && left <= above + s) {
-                    found[0] = (uint32_t)digit;
-                    found[1] = left - above;
-                }
+            const int digit = 255 - t / 4;   // wave 0 holds the largest
+            uint32_t s = 0;
+            #pragma unroll
+            for (int i = 0; i < 8; i++) s += hist[digit][(t & 3) * 8 + ((i + t / 4) & 7)];
+            s = (uint32_t)quad_isum((int)s);
+            uint32_t all;
+            const uint32_t before = wave_scan((t & 3) == 0 ? s : 0u, all);
+            if (l == 0) part[w] = all;
+            __syncthreads();
+            const uint32_t above = before + waves_before(part, w, all);
+            if ((t & 3) == 0 && above < left && left <= above + s) {
+                found[0] = (uint32_t)digit;
+                found[1] = left - above;
             }
             __syncthreads();
             key |= found[0] << shift;
@@ -158,12 +174,8 @@ void evict_select_kernel(EvictArgs a) {
         __syncthreads();   // part is free (and, in place, this chunk's masses are read by all)
         if (l == 0) part[w] = all;
         __syncthreads();
-        uint32_t sum = 0;
-        for (int i = 0; i < EV_NT / 64; i++) {
-            const uint32_t p = part[i];
-            before += i < w ? p : 0u;
-            sum += p;
-        }
+        uint32_t sum;
+        before += waves_before(part, w, sum);
         uint32_t gt = gt0 + (before & 0xFFFFu), eq = eq0 + (before >> 16);
         #pragma unroll
         for (int u = 0; u < 4; u++) {
@@ -252,7 +264,7 @@ void gather_q4_kernel(Q4View src, Q4View dst, int n_kv, int m, int tiles, const 
         for (int e = 0; e < KV_TILE; e++) {
             if (tile * KV_TILE + e < m) {
                 const int p = id[tile * KV_TILE + e], from = p % KV_TILE;
-                const int down = 4 * (from >> 1) + 16 * (from & 1), up = 4 * (e >> 1) + 16 * (e & 1);
+                const int down = q4_bit(from), up = q4_bit(e);
                 const uint4* x = reinterpret_cast<const uint4*>(src.vc + (size_t)h * src.code_head +
                                                                 (size_t)(p / KV_TILE) * (KV_TILE * HD / 2) + i * (CT * 4));
                 #pragma unroll

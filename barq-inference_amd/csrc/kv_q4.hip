@@ -17,45 +17,70 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // rows 
 
 // ---- the quantizer ---------------------------------------------------------------
 
-// Of (abs bits, value) pairs the larger abs, the lower lane's where equal.
-template <int STEP>   // exchanged with lane ^ STEP (a quad's)
-__device__ __forceinline__ void q4_top(uint32_t& a, float& x, int lane) {
-    constexpr int CTL = STEP == 1 ? 0xB1 : 0x4E;
-    const uint32_t oa = (uint32_t)__builtin_amdgcn_mov_dpp((int)a, CTL, 0xF, 0xF, true);
-    const float ox = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTL, 0xF, 0xF, true));
-    const bool theirs = oa > a || (oa == a && (lane & STEP));
-    a = theirs ? oa : a;
-    x = theirs ? ox : x;
+// The largest and smallest of the quad's elements, and whether all are finite.
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true)));
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true)));
 }
 
 // The block's scale from its 4 lanes' 8 elements each.
 __device__ __forceinline__ _Float16 q4_scale(const float (&x)[8], int lane) {
-    uint32_t a = __builtin_bit_cast(uint32_t, x[0]) & 0x7FFFFFFFu;
-    float t = x[0];
+    float hi = x[0], lo = x[0], z = x[0] * 0.0f;
     #pragma unroll
     for (int e = 1; e < 8; e++) {
-        const uint32_t b = __builtin_bit_cast(uint32_t, x[e]) & 0x7FFFFFFFu;   // orders |x|, NaN above infinity
-        t = b > a ? x[e] : t;
-        a = b > a ? b : a;
+        hi = fmaxf(hi, x[e]);
+        lo = fminf(lo, x[e]);
+        z = __builtin_fmaf(x[e], 0.0f, z);   // NaN after an infinity or a NaN
     }
-    q4_top<1>(a, t, lane);
-    q4_top<2>(a, t, lane);
-    if (a >= 0x7F800000u) return __builtin_bit_cast(_Float16, (uint16_t)0x7E00);
+    hi = quad_max(hi);
+    lo = -quad_max(-lo);
+    const float bad = quad_max(z != z ? 1.0f : 0.0f);
+    float t = hi > -lo ? hi : lo;   // the element of the largest |x|
+    if (__any(hi == -lo && hi != 0.0f)) {
+        // of both signs: the first one counts (lane order within the quad, then element order)
+        int first = 64;
+        #pragma unroll
+        for (int e = 7; e >= 0; e--) first = __builtin_fabsf(x[e]) == hi ? 2 * ((lane & 3) * 8 + e) + (x[e] < 0.0f) : first;
+        int o = __builtin_amdgcn_mov_dpp(first, 0xB1, 0xF, 0xF, true);
+        first = o < first ? o : first;
+        o = __builtin_amdgcn_mov_dpp(first, 0x4E, 0xF, 0xF, true);
+        first = o < first ? o : first;
+        t = hi == -lo ? (first & 1 ? lo : hi) : t;
+    }
+    if (bad != 0.0f) return __builtin_bit_cast(_Float16, (uint16_t)0x7E00);
     const _Float16 d = (_Float16)(t * -0.125f);   // (a power of two: one rounding)
     const float m = (float)d;
     return m > Q4_D_MAX ? (_Float16)Q4_D_MAX : m < -Q4_D_MAX ? (_Float16)-Q4_D_MAX : d;
 }
 
-// The code of x under scale d: floor(x / d + 8.5) within 0 .. 15, exactly.
-// The quotient from f32 can be off by one where x is next to a border; the
-// borders (c - 8.5) d have 16 bits, so comparing with them settles it.
-__device__ __forceinline__ uint32_t q4_code(float x, float ad, float inv, bool neg) {
-    const float xs = neg ? -x : x;
-    const float y = fminf(fmaxf(xs * inv, -9.0f), 8.0f);
-    float c = fminf(fmaxf(floorf(y + 8.5f), 0.0f), 15.0f);
-    if (xs < (c - 8.5f) * ad) c -= 1.0f;
-    else if (xs >= (c - 7.5f) * ad) c += 1.0f;
-    return (uint32_t)(int)fminf(fmaxf(c, 0.0f), 15.0f);
+// The codes of eight elements under scale d: floor(x / d + 8.5) within 0 .. 15,
+// exactly.  In f32 the quotient plus 8.5 is off by less than 2^-18 (three
+// roundings of at most 17); where an element is that near a border, the code's
+// own borders (c - 8.5) d, which have 16 bits, settle it by comparison.
+__device__ __forceinline__ void q4_codes8(const float (&x)[8], float d, uint32_t (&c)[8]) {
+    const float inv = d != 0.0f ? 1.0f / d : 0.0f;   // NaN: as 0, all codes 8
+    const float by = inv == inv ? inv : 0.0f;
+    float f[8], low = 1.0f, high = 0.0f;
+    #pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float y = __builtin_fmaf(x[e], by, 8.5f);
+        f[e] = __builtin_amdgcn_fmed3f(y, 0.0f, 15.0f);
+        c[e] = (uint32_t)f[e];
+        const float r = y - (float)c[e];
+        low = fminf(low, __builtin_fabsf(r));
+        high = fmaxf(high, y < 15.0f ? r : 0.0f);
+    }
+    if (__any(low < 0x1p-16f || high > 1.0f - 0x1p-16f)) {
+        const float ad = __builtin_fabsf(d);
+        #pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float xs = d < 0.0f ? -x[e] : x[e];
+            float k = (float)c[e];
+            if (xs < (k - 8.5f) * ad) k -= 1.0f;
+            else if (xs >= (k - 7.5f) * ad && ad > 0.0f) k += 1.0f;
+            c[e] = (uint32_t)__builtin_amdgcn_fmed3f(k, 0.0f, 15.0f);
+        }
+    }
 }
 
 // ---- append ------------------------------------------------------------------------
@@ -104,10 +129,13 @@ __device__ __forceinline__ void q4_rope8(float (&x)[8], const float* src, int d0
     }
 }
 
+// Grid: x = threads of the tiles, then of q; y = K, V.
 template <int ROPE>
 __global__ __launch_bounds__(256)
 void q4_append_kernel(Q4Append a) {
+    const bool is_v = blockIdx.y != 0;
     if (ROPE != ROPE_NONE && blockIdx.x >= a.kv_blocks) {   // q: one thread per pair, as rope_kernel
+        if (is_v) return;
         const int half = a.hd / 2;
         const size_t t = (size_t)(blockIdx.x - a.kv_blocks) * 256 + threadIdx.x;
         if (t >= (size_t)a.n * a.n_q * half) return;
@@ -128,16 +156,14 @@ void q4_append_kernel(Q4Append a) {
     const int nb = a.hd / 32, lane = threadIdx.x & 63;
     const long long t0 = a.first / KV_TILE, tiles = (a.first + a.n - 1) / KV_TILE + 1 - t0;
     size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const bool live = t < (size_t)2 * a.n_kv * tiles * nb * 4;   // whole quads: every lane of a quad agrees
-    if (!live) return;
+    if (t >= (size_t)a.n_kv * tiles * nb * 4) return;   // (whole quads: every lane of a quad agrees)
     const int kq = (int)(t % 4);
     t /= 4;
     const int b = (int)(t % nb);
     t /= nb;
     const long long tile = t0 + (long long)(t % tiles);
     t /= tiles;
-    const int h = (int)(t % a.n_kv);
-    const bool is_v = t / a.n_kv != 0;
+    const int h = (int)t;
     const int d0 = 32 * b + 8 * kq;
     const float* src = (is_v ? a.v : a.k) + (size_t)h * a.src_head;
     const int e0 = (int)(a.first > tile * KV_TILE ? a.first - tile * KV_TILE : 0);   // the tile's positions in the call
@@ -174,23 +200,24 @@ void q4_append_kernel(Q4Append a) {
     for (int e = 0; e < 8; e++) {
         const _Float16 d = q4_scale(x[e], lane);
         if (e < e0 || e >= e1) continue;
-        const float m = (float)d, ad = fabsf(m);
-        const float inv = 1.0f / ad;
-        uint32_t kw = 0;
-        #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t c = ad > 0.0f ? q4_code(x[e][j], ad, inv, m < 0.0f) : 8u;   // 8 under zero and NaN
-            kw |= (c ^ 8u) << (4 * j);
-            vw[j] |= c << (4 * (e >> 1) + 16 * (e & 1));
+        uint32_t c[8];
+        q4_codes8(x[e], (float)d, c);
+        if (is_v) {
+            #pragma unroll
+            for (int j = 0; j < 8; j++) vw[j] |= c[j] << q4_bit(e);
+        } else {
+            uint32_t kw = 0;
+            #pragma unroll
+            for (int j = 0; j < 8; j++) kw |= c[j] << q4_bit(j);
+            *reinterpret_cast<uint32_t*>(codes + (size_t)(tile * KV_TILE + e) * (a.hd / 2) + 4 * (kq * nb + b)) = kw;
         }
-        if (!is_v) *reinterpret_cast<uint32_t*>(codes + (size_t)(tile * KV_TILE + e) * (a.hd / 2) + 4 * (kq * nb + b)) = kw;
         if (kq == 0) reinterpret_cast<_Float16*>(sc)[e] = d;
     }
     if (is_v) {
         uint32_t* w = reinterpret_cast<uint32_t*>(codes + (size_t)tile * KV_TILE * (a.hd / 2));
         // the tile's earlier positions keep their nibbles
         uint32_t keep = 0;
-        for (int e = 0; e < e0; e++) keep |= 0xFu << (4 * (e >> 1) + 16 * (e & 1));
+        for (int e = 0; e < e0; e++) keep |= 0xFu << q4_bit(e);
         #pragma unroll
         for (int j = 0; j < 8; j++) {
             uint32_t* p = w + ((d0 + j) % 16) * (a.hd / 16) + d0 / 16;
@@ -201,53 +228,52 @@ void q4_append_kernel(Q4Append a) {
 
 // ---- read --------------------------------------------------------------------------
 
+// One thread per 4 dims of a tile (whole rows of 16-byte stores side by
+// side).  Grid: x = threads, y = K, V.
 __global__ __launch_bounds__(256)
 void q4_read_kernel(Q4View w, int n_kv, int hd, long long first, long long n, float* __restrict__ k, float* __restrict__ v) {
-    const int nb = hd / 32;
-    const long long t0 = first / KV_TILE, tiles = (first + n - 1) / KV_TILE + 1 - t0;
-    size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= (size_t)2 * n_kv * tiles * nb * 4) return;
-    const int kq = (int)(t % 4);
-    t /= 4;
-    const int b = (int)(t % nb);
-    t /= nb;
-    const long long tile = t0 + (long long)(t % tiles);
-    t /= tiles;
-    const int h = (int)(t % n_kv);
-    const bool is_v = t / n_kv != 0;
+    const bool is_v = blockIdx.y != 0;
     float* out = is_v ? v : k;
     if (!out) return;
-    const int d0 = 32 * b + 8 * kq;
+    const int nb = hd / 32, quads = hd / 4;
+    const long long t0 = first / KV_TILE, tiles = (first + n - 1) / KV_TILE + 1 - t0;
+    size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
+    const int d0 = 4 * (int)(t % quads);
+    t /= quads;
+    const long long tile = t0 + (long long)(t % tiles);
+    const int h = (int)(t / tiles);
+    if (h >= n_kv) return;
     const uint8_t* codes = (is_v ? w.vc : w.kc) + (size_t)h * w.code_head + (size_t)tile * KV_TILE * (hd / 2);
-    const _Float16* sc = reinterpret_cast<const _Float16*>((is_v ? w.vs : w.ks) + (size_t)h * w.scale_head +
-                                                           ((size_t)tile * nb + b) * (2 * KV_TILE));
-    uint32_t word[8];
+    const uint4 sc = *reinterpret_cast<const uint4*>((is_v ? w.vs : w.ks) + (size_t)h * w.scale_head +
+                                                     ((size_t)tile * nb + d0 / 32) * (2 * KV_TILE));
+    const uint32_t scw[4] = {sc.x, sc.y, sc.z, sc.w};
+    uint32_t word[8];   // V: of the 4 dims; K: of the 8 positions
     #pragma unroll
     for (int j = 0; j < 8; j++)
-        word[j] = is_v ? reinterpret_cast<const uint32_t*>(codes)[((d0 + j) % 16) * (hd / 16) + d0 / 16]
-                       : reinterpret_cast<const uint32_t*>(codes + (size_t)j * (hd / 2))[kq * nb + b];
+        if (!is_v || j < 4)
+            word[j] = is_v ? reinterpret_cast<const uint32_t*>(codes)[((d0 + j) % 16) * (hd / 16) + d0 / 16]
+                           : reinterpret_cast<const uint32_t*>(codes + (size_t)j * (hd / 2))[(d0 / 8 % 4) * nb + d0 / 32];
     #pragma unroll
     for (int e = 0; e < 8; e++) {
         const long long p = tile * KV_TILE + e - first;
         if (p < 0 || p >= n) continue;
-        const float d = (float)sc[e];
-        float y[8];
+        const float d = f16_bits_to_f32((scw[e / 2] >> (16 * (e & 1))) & 0xFFFFu);
+        float y[4];
         #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t c = is_v ? word[j] >> (4 * (e >> 1) + 16 * (e & 1)) : (word[e] >> (4 * j)) ^ 8u;
+        for (int j = 0; j < 4; j++) {
+            const uint32_t c = is_v ? word[j] >> q4_bit(e) : word[e] >> ((d0 & 4) ? q4_bit(4 + j) : q4_bit(j));
             y[j] = (float)((int)(c & 15u) - 8) * d;
         }
-        float* o = out + ((size_t)h * n + p) * hd + d0;
-        *reinterpret_cast<f32x4u*>(o) = f32x4u{y[0], y[1], y[2], y[3]};
-        *reinterpret_cast<f32x4u*>(o + 4) = f32x4u{y[4], y[5], y[6], y[7]};
+        *reinterpret_cast<f32x4u*>(out + ((size_t)h * n + p) * hd + d0) = f32x4u{y[0], y[1], y[2], y[3]};
     }
 }
 
 // ---- launch ------------------------------------------------------------------------
 
-static unsigned q4_grid(size_t n_kv, size_t hd, size_t first, size_t n) {
+// workgroups of K's (or V's) tiles, a thread per `dims` dims of one
+static unsigned q4_grid(size_t n_kv, size_t hd, size_t first, size_t n, size_t dims) {
     const size_t tiles = (first + n - 1) / KV_TILE + 1 - first / KV_TILE;
-    return (unsigned)((2 * n_kv * tiles * (hd / 32) * 4 + 255) / 256);
+    return (unsigned)((n_kv * tiles * (hd / dims) + 255) / 256);
 }
 
 hipError_t q4_append_launch(const Q4View& dst, const float* k, const float* v, size_t src_head, size_t src_pos,
@@ -262,8 +288,8 @@ hipError_t q4_append_launch(const Q4View& dst, const float* k, const float* v, s
     a.hd = (int)hd;
     a.first = (long long)first;
     a.n = (long long)n;
-    a.kv_blocks = q4_grid(n_kv, hd, first, n);
-    hipLaunchKernelGGL(q4_append_kernel<ROPE_NONE>, dim3(a.kv_blocks), dim3(256), 0, s, a);
+    a.kv_blocks = q4_grid(n_kv, hd, first, n, 8);
+    hipLaunchKernelGGL(q4_append_kernel<ROPE_NONE>, dim3(a.kv_blocks, 2), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
@@ -286,18 +312,18 @@ hipError_t q4_append_rope_launch(int layout, const Q4View& dst, const float* q, 
     a.q = q;
     a.q_out = q_out;
     a.n_q = q ? (int)n_q : 0;
-    a.kv_blocks = q4_grid(n_kv, hd, first, n);
+    a.kv_blocks = q4_grid(n_kv, hd, first, n, 8);
     const unsigned grid = a.kv_blocks + (unsigned)((n * a.n_q * (hd / 2) + 255) / 256);
     if (layout == ROPE_INTERLEAVED)
-        hipLaunchKernelGGL(q4_append_kernel<ROPE_INTERLEAVED>, dim3(grid), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(q4_append_kernel<ROPE_INTERLEAVED>, dim3(grid, 2), dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL(q4_append_kernel<ROPE_SPLIT_HALF>, dim3(grid), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(q4_append_kernel<ROPE_SPLIT_HALF>, dim3(grid, 2), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
 hipError_t q4_read_launch(const Q4View& w, size_t n_kv, size_t hd, size_t first, size_t n, float* k, float* v,
                           hipStream_t s) {
-    hipLaunchKernelGGL(q4_read_kernel, dim3(q4_grid(n_kv, hd, first, n)), dim3(256), 0, s, w, (int)n_kv, (int)hd,
+    hipLaunchKernelGGL(q4_read_kernel, dim3(q4_grid(n_kv, hd, first, n, 4), 2), dim3(256), 0, s, w, (int)n_kv, (int)hd,
                        (long long)first, (long long)n, k, v);
     return hipGetLastError();
 }

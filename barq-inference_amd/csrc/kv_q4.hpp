@@ -4,14 +4,14 @@
 // Positions are grouped in tiles of 8.  Per layer and kv head, with HD dims
 // and NB = HD / 32 blocks a row:
 //   K codes   [position][4][NB] dwords: dword (kq, b) holds dims 32 b + 8 kq
-//             .. + 7 of the position, dim e of them in bits 4 e, as code ^ 8
-//             (code - 8 in two's complement, what v_cvt_off_f32_i4 takes): the
-//             8 contraction slots that lane group kq of a 16x16x32 MFMA gives
-//             block b, so a lane loads its part of a row in one piece
+//             .. + 7 of the position, dim e of them in bits 4 (e / 2) + 16 (e %
+//             2): the 8 contraction slots that lane group kq of a 16x16x32
+//             MFMA gives block b, so a lane loads its part of a row in one piece
 //   V codes   [tile][16][HD / 16] dwords: dword (i, c) holds dim 16 c + i of
-//             the tile's 8 positions, position e in bits 4 (e / 2) + 16 (e % 2):
-//             masked by 0x000F000F << 4 j it is positions 2 j and 2 j + 1 as a
-//             packed pair, and V is already transposed for P V
+//             the tile's 8 positions, position e in bits 4 (e / 2) + 16 (e % 2),
+//             so V is already transposed for P V
+//             (a dword masked by 0x000F000F << 4 j holds codes 2 j and 2 j + 1
+//             as a packed pair)
 //   scales    [tile][NB][8] f16, K's and V's alike: a lane's 8 positions of a
 //             block are 16 bytes
 // A position takes HD / 2 + 2 NB bytes of K and as many of V: 144 bytes with
@@ -41,6 +41,9 @@ struct Q4View {
     size_t code_head;  // bytes between kv heads
     size_t scale_head;
 };
+
+// bit of code e of a dword's eight
+__host__ __device__ constexpr int q4_bit(int e) { return 4 * (e >> 1) + 16 * (e & 1); }
 
 inline size_t q4_tiles(size_t positions) { return (positions + KV_TILE - 1) / KV_TILE; }
 // bytes of one kv head's codes / scales (K's, and V's again)

@@ -215,7 +215,7 @@ struct AttnScores {
 };
 int attention_scores_splits(size_t n_head, size_t n_head_kv, size_t q_len, size_t kv_len);
 hipError_t attention_scores_launch(const AttnArgs& a, const AttnScores& sc, hipStream_t s);
-int attention_q4_scores_splits(size_t n_head, size_t n_head_kv, size_t q_len, size_t kv_len);
+int attention_q4_scores_splits(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);
 hipError_t attention_q4_scores_launch(const AttnArgs& a, const AttnScores& sc, const Q4View& kv, hipStream_t s);
 
 // attention_mass.hip: mass_out[hk][j] = mass_in[hk][j] (null: 0) + the softmax weights of position j over the call's
@@ -227,11 +227,13 @@ struct MassArgs {
     int ns, head_dim, n_head, n_head_kv, q_len, kv_len;
     long long start_pos;
     float* stat;           // q_len * n_head pairs (attention_mass_stat)
+    float* sums;           // partial sums (attention_mass_sums)
     const float* mass_in;
     float* mass_out;
     size_t mass_stride;
 };
 size_t attention_mass_stat(size_t n_head, size_t n_head_kv, size_t q_len);   // bytes of stat (0: not used)
+size_t attention_mass_sums(size_t n_head, size_t n_head_kv, size_t q_len, size_t score_stride);
 hipError_t attention_mass_launch(const MassArgs& a, hipStream_t s);
 
 // merges ns partial states [q_len][n_head][ns][head_dim + 2] of a.part (ns <= 1024)

@@ -55,10 +55,13 @@ __device__ __forceinline__ void lds_load16_nt(i32x4v r, void* lds_wave_base, uin
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen nt lds"
                  :: "s"(m0), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
 }
-__device__ __forceinline__ void lds_load4(i32x4v r, void* lds_wave_base, uint32_t voff, uint32_t soff) {
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_addr(lds_wave_base));
+__device__ __forceinline__ void lds_load4_at(i32x4v r, uint32_t lds_wave_addr, uint32_t voff, uint32_t soff) {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_wave_addr);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
                  :: "s"(m0), "v"(voff), "s"(r), "s"(soff) : "memory", "m0");
+}
+__device__ __forceinline__ void lds_load4(i32x4v r, void* lds_wave_base, uint32_t voff, uint32_t soff) {
+    lds_load4_at(r, lds_addr(lds_wave_base), voff, soff);
 }
 __device__ __forceinline__ void lds_load4_nt(i32x4v r, void* lds_wave_base, uint32_t voff, uint32_t soff) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_addr(lds_wave_base));
