@@ -131,7 +131,8 @@ class KVCache:
             k, v = np.empty(shape, np.float32), np.empty(shape, np.float32)
         else:
             import torch
-            k, v = (torch.empty(shape, dtype=torch.float32, device=f"cuda:{self.be.device}") for _ in "kv")
+            dev = torch.device("cuda", self.be.device)
+            k, v = torch.empty(shape, dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.float32, device=dev)
         L.check(self.be._lib.barq_rocm_kv_cache_read(self.be.h, self.c, layer, first, n, _ptr(k), _ptr(v), mem))
         if sync and mem == L.MEM_DEVICE:
             self.be.sync()

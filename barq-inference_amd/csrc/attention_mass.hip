@@ -9,6 +9,9 @@
 // not be read again).  The sums run in a fixed order and need no atomics: a
 // wave takes positions of its own, and where the rows are shared out over
 // workgroups each leaves partial sums that another launch adds.
+#include <type_traits>
+
+#include "attention_combine.hpp"
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -44,41 +47,72 @@ __device__ __forceinline__ int mass_head(const MassArgs& a, int hk) {
     return (int)(((long long)hk * a.n_head + a.n_head_kv - 1) / a.n_head_kv);
 }
 
-// Few rows: a workgroup of four waves takes 64 positions, every wave a fourth
-// of the rows, whose statistics they find themselves.  Grid: x = 64 positions, y = kv head.
-__global__ __launch_bounds__(256)
-void mass_few_kernel(MassArgs a) {
-    __shared__ float2 stat[MASS_INLINE];
-    __shared__ float red[4][64];
-    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hk = blockIdx.y;
-    const int j = blockIdx.x * 64 + l;
+// Few rows, and their merge, in one launch (both need the partial states
+// only): workgroups x < merges merge a row and head (or with Q8 a block of a
+// row); each of the others takes 256 positions of a kv head, a wave 64 of them
+// and a fourth of the rows, whose statistics the workgroup finds itself.
+struct MassLds {
+    float2 stat[MASS_INLINE];
+    float red[4][256];
+};
+template <int HD, bool Q8>
+union FinishLds {
+    MassLds mass;
+    typename std::conditional<Q8, CombineQ8Lds<HD>, CombineLds<HD>>::type merge;
+};
+
+template <int HD, bool Q8>
+__global__ __launch_bounds__(1024)
+void mass_finish_kernel(MassArgs a, int merges, void* __restrict__ out) {
+    __shared__ FinishLds<HD, Q8> lds;
+    if ((int)blockIdx.x < merges) {
+        const int per = Q8 ? a.n_head * HD / 256 : a.n_head, x = (int)blockIdx.x % per, i = (int)blockIdx.x / per;
+        if constexpr (Q8) attn_combine_q8k_block<HD>(a.part, a.ns, a.n_head, x, i, lds.merge, static_cast<uint8_t*>(out));
+        else attn_combine_row<HD>(a.part, a.ns, a.n_head, x, i, lds.merge, static_cast<float*>(out));
+        return;
+    }
+    const int blk = (int)blockIdx.x - merges, hk = blk % a.n_head_kv;
+    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = w / 4;
+    const int j = (blk / a.n_head_kv * 4 + w % 4) * 64 + l;
     const int h0 = mass_head(a, hk), G = mass_head(a, hk + 1) - h0, rows = G * a.q_len;
     // the scores are on their way while the statistics are found
     float s[MASS_INLINE / 4];
     #pragma unroll
     for (int u = 0; u < MASS_INLINE / 4; u++) {
-        const int r = w + 4 * u, i = r < rows ? r / G : 0;
+        const int r = wr + 4 * u, i = r < rows ? r / G : 0;
         // (a position behind the row's last is not seen: its score is undefined)
         const bool seen = r < rows && j < a.kv_len && j <= a.start_pos + i;
         s[u] = seen ? a.scores[((size_t)i * a.n_head + h0 + r - i * G) * a.score_stride + j] : -INFINITY;
     }
-    const float before = a.mass_in && j < a.kv_len ? a.mass_in[(size_t)hk * a.mass_stride + j] : 0.0f;
-    if ((int)threadIdx.x / 16 < rows) {
+    const float before = wr == 0 && a.mass_in && j < a.kv_len ? a.mass_in[(size_t)hk * a.mass_stride + j] : 0.0f;
+    if ((int)threadIdx.x / 16 < rows) {   // (whole rows of 16 lanes)
         const int r = threadIdx.x / 16;
         const float2 st = mass_stat(a, (size_t)(r / G) * a.n_head + h0 + r % G, threadIdx.x & 15);
-        if ((threadIdx.x & 15) == 0) stat[r] = st;
+        if ((threadIdx.x & 15) == 0) lds.mass.stat[r] = st;
     }
     __syncthreads();
     float sum = 0.0f;
     #pragma unroll
     for (int u = 0; u < MASS_INLINE / 4; u++) {
-        const int r = w + 4 * u, i = r < rows ? r / G : 0;
-        if (r < rows && j <= a.start_pos + i) sum += __builtin_amdgcn_exp2f(s[u] - stat[r].x) * stat[r].y;
+        const int r = wr + 4 * u, i = r < rows ? r / G : 0;
+        if (r < rows && j <= a.start_pos + i) sum += __builtin_amdgcn_exp2f(s[u] - lds.mass.stat[r].x) * lds.mass.stat[r].y;
     }
-    red[w][l] = sum;
+    lds.mass.red[wr][64 * (w % 4) + l] = sum;
     __syncthreads();
-    if (w == 0 && j < a.kv_len)
-        a.mass_out[(size_t)hk * a.mass_stride + j] = before + ((red[0][l] + red[1][l]) + (red[2][l] + red[3][l]));
+    if (wr == 0 && j < a.kv_len) {
+        const int q = 64 * w + l;
+        a.mass_out[(size_t)hk * a.mass_stride + j] =
+            before + ((lds.mass.red[0][q] + lds.mass.red[1][q]) + (lds.mass.red[2][q] + lds.mass.red[3][q]));
+    }
+}
+
+template <int HD>
+static hipError_t mass_finish_t(const MassArgs& a, float* out, uint8_t* out_q8, hipStream_t s) {
+    const int merges = (out_q8 ? a.n_head * HD / 256 : a.n_head) * a.q_len;
+    const dim3 grid((unsigned)merges + (unsigned)((a.kv_len + 255) / 256) * (unsigned)a.n_head_kv);
+    if (out_q8) hipLaunchKernelGGL((mass_finish_kernel<HD, true>), grid, dim3(1024), 0, s, a, merges, out_q8);
+    else hipLaunchKernelGGL((mass_finish_kernel<HD, false>), grid, dim3(1024), 0, s, a, merges, out);
+    return hipGetLastError();
 }
 
 // Many rows: a wave takes 256 positions, four in a row per lane, and
@@ -135,16 +169,22 @@ size_t attention_mass_sums(size_t n_head, size_t n_head_kv, size_t q_len, size_t
     return rows <= (size_t)MASS_INLINE ? 0 : (rows + MASS_RUN - 1) / MASS_RUN * n_head_kv * stride * sizeof(float);
 }
 
-hipError_t attention_mass_launch(const MassArgs& a, hipStream_t s) {
+hipError_t attention_mass_launch(const MassArgs& a, const AttnArgs& attn, uint8_t* out_q8, hipStream_t s) {
     const size_t rows = mass_rows(a.n_head, a.n_head_kv, a.q_len);
     const unsigned heads = (unsigned)a.n_head_kv;
     if (rows <= (size_t)MASS_INLINE) {
-        hipLaunchKernelGGL(mass_few_kernel, dim3((unsigned)((a.kv_len + 63) / 64), heads), dim3(256), 0, s, a);
-        return hipGetLastError();
+        switch (a.head_dim) {
+        case 64: return mass_finish_t<64>(a, attn.out, out_q8, s);
+        case 128: return mass_finish_t<128>(a, attn.out, out_q8, s);
+        case 256: return mass_finish_t<256>(a, attn.out, out_q8, s);
+        default: return hipErrorInvalidValue;
+        }
     }
     const unsigned runs = (unsigned)((rows + MASS_RUN - 1) / MASS_RUN);
+    hipError_t e = attention_combine_launch(attn, a.ns, out_q8, s);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(mass_stat_kernel, dim3((unsigned)(((size_t)a.q_len * a.n_head + 15) / 16)), dim3(256), 0, s, a);
-    hipError_t e = hipGetLastError();
+    e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(mass_run_kernel, dim3((unsigned)((a.score_stride + 1023) / 1024), heads, runs), dim3(256), 0, s, a);
     e = hipGetLastError();

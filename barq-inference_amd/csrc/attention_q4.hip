@@ -157,8 +157,8 @@ __device__ __forceinline__ void q4_walk(const Q4Fifo<HD>& fifo, uint8_t* lds, in
     asm volatile("" ::: "memory");
 }
 
-// Grid: x = tile of 16 rows * splits + split, y = group of G heads.  The four
-// waves share out the split's steps.
+// Workgroup x: group of G heads x % groups, then split, then tile of 16 rows.
+// The four waves share out the split's steps.
 template <int HD, bool SC>
 __global__ __launch_bounds__(64 * Q4A_NW, HD <= 128 ? 3 : 2)
 void attn_q4_kernel(Q4Args a) {
@@ -169,8 +169,8 @@ void attn_q4_kernel(Q4Args a) {
     __shared__ int nan_pos[Q4A_NW][NB];
     const int t = threadIdx.x, l = t & 63, c = l & 15, g = l >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int grp = blockIdx.y, rows_n = a.q_len * a.G, n_split = a.n_split;
-    const int r0 = (int)(blockIdx.x / n_split) * Q4A_ROWS, split = (int)(blockIdx.x % n_split);
+    const int grp = (int)(blockIdx.x % a.groups), piece = (int)(blockIdx.x / a.groups), rows_n = a.q_len * a.G, n_split = a.n_split;
+    const int r0 = piece / n_split * Q4A_ROWS, split = piece % n_split;
     const int hk = (int)((long long)(grp * a.G) * a.n_head_kv / a.n_head);
     // the tile's last row bounds the positions
     const int visible = q4_vis(a, r0 + Q4A_ROWS - 1);
@@ -266,6 +266,7 @@ static hipError_t attn_q4_launch_t(const AttnArgs& a, const AttnScores* sc, cons
     k.n_head = (int)a.n_head;
     k.n_head_kv = (int)a.n_head_kv;
     k.G = p.G;
+    k.groups = p.groups;
     k.q_len = (int)a.q_len;
     k.kv_len = (int)a.kv_len;
     k.q_rows = (int)(sc ? sc->q_rows : a.q_len);
@@ -282,9 +283,9 @@ static hipError_t attn_q4_launch_t(const AttnArgs& a, const AttnScores* sc, cons
     }
     hipError_t e;
     if (p.prompt) {
-        e = attn_q4_prompt_launch(k, HD, p.groups, s);
+        e = attn_q4_prompt_launch(k, HD, s);
     } else {
-        const dim3 grid((unsigned)p.n_split * (unsigned)p.tiles, p.groups), block(64 * Q4A_NW);
+        const dim3 grid((unsigned)p.n_split * (unsigned)p.tiles * (unsigned)p.groups), block(64 * Q4A_NW);
         if (sc) hipLaunchKernelGGL((attn_q4_kernel<HD, true>), grid, block, 0, s, k);
         else hipLaunchKernelGGL((attn_q4_kernel<HD, false>), grid, block, 0, s, k);
         e = hipGetLastError();

@@ -51,7 +51,7 @@ constexpr int Q4A_WINDOW = 20;  // log2 of the spread that a step's weights may 
 struct Q4Args {
     const float* q;        // [n_head, q_len, HD]
     Q4View kv;
-    int n_head, n_head_kv, G, q_len, kv_len;
+    int n_head, n_head_kv, G, groups, q_len, kv_len;   // groups of G query heads that share a kv head
     int q_rows;            // rows of q per head (the call's are the first q_len)
     long long start_pos;
     int chunk, n_split;    // positions of a split, splits
@@ -485,6 +485,6 @@ __device__ __forceinline__ void q4_store(const Q4Args& a, const Q4Row& row, int 
 }
 
 // attention_q4_prompt.hip (64 and 128 dims)
-hipError_t attn_q4_prompt_launch(const Q4Args& a, size_t head_dim, int groups, hipStream_t s);
+hipError_t attn_q4_prompt_launch(const Q4Args& a, size_t head_dim, hipStream_t s);
 
 }  // namespace barq

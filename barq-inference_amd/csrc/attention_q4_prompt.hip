@@ -94,8 +94,10 @@ struct Q4Block {
     }
 };
 
-// Grid: x = row tile * splits + split, the tiles from the last one down (it
-// sees the most), y = group of G heads.
+// Workgroup x: group of G heads x % groups, then split, then row tile from the
+// last one down.  The longest tiles of all heads start first (128 us for 2048
+// tokens; 170 with one head's tiles before the next head's), and with eight kv heads an
+// XCD keeps to one of them.
 template <int HD, bool PART, bool SC>
 __global__ __launch_bounds__(64 * Q4P_NW, 3)
 void attn_q4_prompt_kernel(Q4Args a) {
@@ -105,8 +107,8 @@ void attn_q4_prompt_kernel(Q4Args a) {
     __shared__ int nan_at[B::NB];
     const int t = threadIdx.x, l = t & 63, c = l & 15, g = l >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int grp = blockIdx.y, rows_n = a.q_len * a.G;
-    const int tile = a.tiles - 1 - (int)(blockIdx.x / a.n_split), split = (int)(blockIdx.x % a.n_split);
+    const int grp = (int)(blockIdx.x % a.groups), part = (int)(blockIdx.x / a.groups), rows_n = a.q_len * a.G;
+    const int tile = a.tiles - 1 - part / a.n_split, split = part % a.n_split;
     const int hk = (int)((long long)(grp * a.G) * a.n_head_kv / a.n_head);
     const int visible = q4_vis(a, tile * Q4P_ROWS + Q4P_ROWS - 1);
     const int start = split * a.chunk, j0 = min(start, visible), j1 = min(visible, start + a.chunk);
@@ -164,16 +166,16 @@ void attn_q4_prompt_kernel(Q4Args a) {
 }
 
 template <int HD>
-static hipError_t prompt_launch_t(const Q4Args& a, int groups, hipStream_t s) {
-    const dim3 grid((unsigned)a.tiles * (unsigned)a.n_split, groups), block(64 * Q4P_NW);
+static hipError_t prompt_launch_t(const Q4Args& a, hipStream_t s) {
+    const dim3 grid((unsigned)a.tiles * (unsigned)a.n_split * (unsigned)a.groups), block(64 * Q4P_NW);
     if (a.scores) hipLaunchKernelGGL((attn_q4_prompt_kernel<HD, true, true>), grid, block, 0, s, a);
     else if (a.n_split > 1) hipLaunchKernelGGL((attn_q4_prompt_kernel<HD, true, false>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((attn_q4_prompt_kernel<HD, false, false>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
-hipError_t attn_q4_prompt_launch(const Q4Args& a, size_t head_dim, int groups, hipStream_t s) {
-    return head_dim == 64 ? prompt_launch_t<64>(a, groups, s) : prompt_launch_t<128>(a, groups, s);
+hipError_t attn_q4_prompt_launch(const Q4Args& a, size_t head_dim, hipStream_t s) {
+    return head_dim == 64 ? prompt_launch_t<64>(a, s) : prompt_launch_t<128>(a, s);
 }
 
 }  // namespace barq

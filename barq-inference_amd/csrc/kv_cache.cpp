@@ -156,8 +156,9 @@ int barq_rocm_kv_cache_evict(barq_rocm_handle* h, const barq_rocm_kv_cache* src,
     return done();
 }
 
-// Scores of one launch at most: a prompt's rows are taken in chunks.
-static constexpr size_t MASS_SCORES = (size_t)64 << 20;
+// Scores of one launch at most (half of the 256 MB last-level cache, from which
+// they are read again): a longer prompt's rows are taken in chunks.
+static constexpr size_t MASS_SCORES = (size_t)128 << 20;
 
 int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache* c, size_t layer, size_t n_head,
                              size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len, size_t start_pos, int out_type,
@@ -245,7 +246,6 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
         BARQ_CHECK(launched(q4 ? barq::attention_q4_scores_launch(args, sc, c->view(layer), h->stream)
                                : barq::attention_scores_launch(args, sc, h->stream), who));
         const int ns = (int)splits(n);
-        BARQ_CHECK(launched(barq::attention_combine_launch(args, ns, q8 ? ob + i * out_row : nullptr, h->stream), who));
         barq::MassArgs m{};
         m.scores = sc.scores;
         m.score_stride = stride;
@@ -262,7 +262,7 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
         m.mass_in = i ? mo : mi;
         m.mass_out = mo;
         m.mass_stride = ms;
-        BARQ_CHECK(launched(barq::attention_mass_launch(m, h->stream), who));
+        BARQ_CHECK(launched(barq::attention_mass_launch(m, args, q8 ? ob + i * out_row : nullptr, h->stream), who));
     }
     if (host) {
         BARQ_HIP(hipMemcpyAsync(out, ob, q_len * out_row, hipMemcpyDeviceToHost, h->stream));

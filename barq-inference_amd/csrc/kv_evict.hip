@@ -75,7 +75,7 @@ template <int R>
 __global__ __launch_bounds__(EV_NT)
 void evict_select_kernel(EvictArgs a) {
     __shared__ __align__(16) uint32_t hist[256][32];
-    __shared__ __align__(16) uint32_t part[EV_NT / 64];
+    __shared__ __align__(16) uint32_t part[R ? R : 1][EV_NT / 64];
     static_assert(EV_NT == 1024, "16 waves, four threads a digit");
     __shared__ uint32_t found[2];   // the digit and what is left to find within it
     const int t = threadIdx.x, l = t & 63, w = t >> 6, h = blockIdx.x;
@@ -140,9 +140,9 @@ void evict_select_kernel(EvictArgs a) {
             s = (uint32_t)quad_isum((int)s);
             uint32_t all;
             const uint32_t before = wave_scan((t & 3) == 0 ? s : 0u, all);
-            if (l == 0) part[w] = all;
+            if (l == 0) part[0][w] = all;
             __syncthreads();
-            const uint32_t above = before + waves_before(part, w, all);
+            const uint32_t above = before + waves_before(part[0], w, all);
             if ((t & 3) == 0 && above < left && left <= above + s) {
                 found[0] = (uint32_t)digit;
                 found[1] = left - above;
@@ -157,40 +157,65 @@ void evict_select_kernel(EvictArgs a) {
 
     // numbering: of each position the kept ones before it; larger keys and
     // keys equal to the last one counted side by side (16 bits each a chunk)
-    uint32_t gt0 = 0, eq0 = 0;
-    each([&](int c, const float (&x)[4]) {
-        uint32_t flags[4], mine = 0;
+    const auto flag = [&](int j, float x) {
+        const uint32_t k = ev_key(x);
+        const bool gt = (j >= old && j < a.n) || (j < old && (some ? k > key : want > 0));
+        return gt ? 1u : some && j < old && k == key ? 0x10000u : 0u;
+    };
+    const auto put = [&](int c, const float (&x)[4], uint32_t gt, uint32_t eq) {
         #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int j = c * EV_CHUNK + 4 * t + u;
-            const uint32_t k = ev_key(x[u]);
-            const bool newest = j >= old && j < a.n;
-            const bool gt = newest || (j < old && (some ? k > key : want > 0));
-            flags[u] = gt ? 1u : some && j < old && k == key ? 0x10000u : 0u;
-            mine += flags[u];
-        }
-        uint32_t all;
-        uint32_t before = wave_scan(mine, all);
-        __syncthreads();   // part is free (and, in place, this chunk's masses are read by all)
-        if (l == 0) part[w] = all;
-        __syncthreads();
-        uint32_t sum;
-        before += waves_before(part, w, sum);
-        uint32_t gt = gt0 + (before & 0xFFFFu), eq = eq0 + (before >> 16);
-        #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const bool keep = flags[u] == 1u || (flags[u] && eq < ties);
-            if (keep) {
+            const uint32_t f = flag(c * EV_CHUNK + 4 * t + u, x[u]);
+            if (f == 1u || (f && eq < ties)) {
                 const uint32_t at = gt + (eq < ties ? eq : ties);
                 kept[at] = c * EV_CHUNK + 4 * t + u;
                 if (out) out[at] = x[u];
             }
-            gt += flags[u] & 0xFFFFu;
-            eq += flags[u] >> 16;
+            gt += f & 0xFFFFu;
+            eq += f >> 16;
         }
-        gt0 += sum & 0xFFFFu;
-        eq0 += sum >> 16;
-    });
+    };
+    const auto count = [&](int c, const float (&x)[4]) {
+        uint32_t n = 0;
+        #pragma unroll
+        for (int u = 0; u < 4; u++) n += flag(c * EV_CHUNK + 4 * t + u, x[u]);
+        return n;
+    };
+    if constexpr (R > 0) {   // all chunks' counts at once
+        uint32_t before[R];
+        #pragma unroll
+        for (int c = 0; c < R; c++) {
+            uint32_t all;
+            before[c] = wave_scan(count(c, reg[c]), all);
+            if (l == 0) part[c][w] = all;
+        }
+        __syncthreads();   // (and, in place, the masses are read by all)
+        uint32_t gt0 = 0, eq0 = 0;
+        #pragma unroll
+        for (int c = 0; c < R; c++)
+            if (c < chunks) {
+                uint32_t sum;
+                const uint32_t b = before[c] + waves_before(part[c], w, sum);
+                put(c, reg[c], gt0 + (b & 0xFFFFu), eq0 + (b >> 16));
+                gt0 += sum & 0xFFFFu;
+                eq0 += sum >> 16;
+            }
+    } else {
+        uint32_t gt0 = 0, eq0 = 0;
+        float x[4];
+        for (int c = 0; c < chunks; c++) {
+            load(c, x);
+            uint32_t all, sum;
+            uint32_t b = wave_scan(count(c, x), all);
+            __syncthreads();   // part is free (and, in place, this chunk's masses are read by all)
+            if (l == 0) part[0][w] = all;
+            __syncthreads();
+            b += waves_before(part[0], w, sum);
+            put(c, x, gt0 + (b & 0xFFFFu), eq0 + (b >> 16));
+            gt0 += sum & 0xFFFFu;
+            eq0 += sum >> 16;
+        }
+    }
     __syncthreads();   // in place: the tail is read
     if (out)
         for (int j = a.m + t; j < a.n; j += EV_NT) out[j] = 0.0f;

@@ -1,12 +1,11 @@
-// Writing, reading and gathering the rows of a 4-bit KV cache (kv_q4.hpp has
+// Writing and reading the rows of a 4-bit KV cache (kv_q4.hpp has
 // the layout and the quantizer's definition).
 //
-// All three move a few bytes per element once: bound by memory at a prompt's
-// length and by the launch for a token.  A thread owns 8 dims of a block at
-// the 8 positions of a tile, for K and V alike, so K's dwords (8 dims of one
-// position) and V's (8 positions of one dim) both form in its registers; the
-// 4 threads of a block are neighbouring lanes and find its scale with two
-// quad exchanges.
+// Both move a few bytes per element once: bound by memory at a prompt's length
+// and by the launch for a token.  A thread forms whole dwords of codes in its
+// registers (K: 8 dims of one position; V: 8 positions of one dim); the threads
+// of a block of 32 dims are neighbouring lanes, which find its scale by lane
+// exchanges.
 #include "common.hpp"
 #include "kv_q4.hpp"
 #include "launch.hpp"
@@ -17,35 +16,39 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));   // rows 
 
 // ---- the quantizer ---------------------------------------------------------------
 
-// The largest and smallest of the quad's elements, and whether all are finite.
-__device__ __forceinline__ float quad_max(float v) {
+// Over aligned groups of N = 4 or 8 lanes.
+template <int N>
+__device__ __forceinline__ float lanes_max(float v) {
     v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true)));
-    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true)));
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true)));
+    if constexpr (N == 8)
+        v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x141, 0xF, 0xF, true)));
+    return v;
 }
 
-// The block's scale from its 4 lanes' 8 elements each.
-__device__ __forceinline__ _Float16 q4_scale(const float (&x)[8], int lane) {
+// A block's scale from its 32 / D lanes' D elements each.
+template <int D>
+__device__ __forceinline__ _Float16 q4_scale(const float (&x)[D], int lane) {
+    constexpr int N = 32 / D;
     float hi = x[0], lo = x[0], z = x[0] * 0.0f;
     #pragma unroll
-    for (int e = 1; e < 8; e++) {
+    for (int e = 1; e < D; e++) {
         hi = fmaxf(hi, x[e]);
         lo = fminf(lo, x[e]);
         z = __builtin_fmaf(x[e], 0.0f, z);   // NaN after an infinity or a NaN
     }
-    hi = quad_max(hi);
-    lo = -quad_max(-lo);
-    const float bad = quad_max(z != z ? 1.0f : 0.0f);
+    hi = lanes_max<N>(hi);
+    lo = -lanes_max<N>(-lo);
+    const float bad = lanes_max<N>(z != z ? 1.0f : 0.0f);
     float t = hi > -lo ? hi : lo;   // the element of the largest |x|
     if (__any(hi == -lo && hi != 0.0f)) {
-        // of both signs: the first one counts (lane order within the quad, then element order)
-        int first = 64;
+        // of both signs: the first one counts (as the largest of 64 - 2 * place - sign)
+        float first = 0.0f;
         #pragma unroll
-        for (int e = 7; e >= 0; e--) first = __builtin_fabsf(x[e]) == hi ? 2 * ((lane & 3) * 8 + e) + (x[e] < 0.0f) : first;
-        int o = __builtin_amdgcn_mov_dpp(first, 0xB1, 0xF, 0xF, true);
-        first = o < first ? o : first;
-        o = __builtin_amdgcn_mov_dpp(first, 0x4E, 0xF, 0xF, true);
-        first = o < first ? o : first;
-        t = hi == -lo ? (first & 1 ? lo : hi) : t;
+        for (int e = 0; e < D; e++)
+            first = fmaxf(first, __builtin_fabsf(x[e]) == hi ? (float)(65 - 2 * ((lane & (N - 1)) * D + e) - (x[e] < 0.0f)) : 0.0f);
+        first = lanes_max<N>(first);
+        t = hi == -lo ? ((int)first & 1 ? hi : lo) : t;
     }
     if (bad != 0.0f) return __builtin_bit_cast(_Float16, (uint16_t)0x7E00);
     const _Float16 d = (_Float16)(t * -0.125f);   // (a power of two: one rounding)
@@ -53,16 +56,17 @@ __device__ __forceinline__ _Float16 q4_scale(const float (&x)[8], int lane) {
     return m > Q4_D_MAX ? (_Float16)Q4_D_MAX : m < -Q4_D_MAX ? (_Float16)-Q4_D_MAX : d;
 }
 
-// The codes of eight elements under scale d: floor(x / d + 8.5) within 0 .. 15,
+// The codes of D elements under scale d: floor(x / d + 8.5) within 0 .. 15,
 // exactly.  In f32 the quotient plus 8.5 is off by less than 2^-18 (three
 // roundings of at most 17); where an element is that near a border, the code's
 // own borders (c - 8.5) d, which have 16 bits, settle it by comparison.
-__device__ __forceinline__ void q4_codes8(const float (&x)[8], float d, uint32_t (&c)[8]) {
+template <int D>
+__device__ __forceinline__ void q4_codes(const float (&x)[D], float d, uint32_t (&c)[D]) {
     const float inv = d != 0.0f ? 1.0f / d : 0.0f;   // NaN: as 0, all codes 8
     const float by = inv == inv ? inv : 0.0f;
-    float f[8], low = 1.0f, high = 0.0f;
+    float f[D], low = 1.0f, high = 0.0f;
     #pragma unroll
-    for (int e = 0; e < 8; e++) {
+    for (int e = 0; e < D; e++) {
         const float y = __builtin_fmaf(x[e], by, 8.5f);
         f[e] = __builtin_amdgcn_fmed3f(y, 0.0f, 15.0f);
         c[e] = (uint32_t)f[e];
@@ -73,7 +77,7 @@ __device__ __forceinline__ void q4_codes8(const float (&x)[8], float d, uint32_t
     if (__any(low < 0x1p-16f || high > 1.0f - 0x1p-16f)) {
         const float ad = __builtin_fabsf(d);
         #pragma unroll
-        for (int e = 0; e < 8; e++) {
+        for (int e = 0; e < D; e++) {
             const float xs = d < 0.0f ? -x[e] : x[e];
             float k = (float)c[e];
             if (xs < (k - 8.5f) * ad) k -= 1.0f;
@@ -153,76 +157,85 @@ void q4_append_kernel(Q4Append a) {
         dst[i1] = x0 * sn + x1 * cs;
         return;
     }
-    const int nb = a.hd / 32, lane = threadIdx.x & 63;
+    // K: a thread takes 8 dims (a dword) of 4 positions; V: 4 dims of a tile's 8 (a dword each)
+    const int nb = a.hd / 32, lane = threadIdx.x & 63, per_tile = nb * 8;
     const long long t0 = a.first / KV_TILE, tiles = (a.first + a.n - 1) / KV_TILE + 1 - t0;
     size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= (size_t)a.n_kv * tiles * nb * 4) return;   // (whole quads: every lane of a quad agrees)
-    const int kq = (int)(t % 4);
-    t /= 4;
-    const int b = (int)(t % nb);
-    t /= nb;
+    if (t >= (size_t)a.n_kv * tiles * per_tile) return;   // (whole groups of 8 lanes agree)
+    const int u = (int)(t % per_tile);
+    t /= per_tile;
     const long long tile = t0 + (long long)(t % tiles);
-    t /= tiles;
-    const int h = (int)t;
-    const int d0 = 32 * b + 8 * kq;
-    const float* src = (is_v ? a.v : a.k) + (size_t)h * a.src_head;
+    const int h = (int)(t / tiles);
     const int e0 = (int)(a.first > tile * KV_TILE ? a.first - tile * KV_TILE : 0);   // the tile's positions in the call
     const int e1 = (int)(a.first + a.n < (tile + 1) * KV_TILE ? a.first + a.n - tile * KV_TILE : KV_TILE);
-
-    float x[8][8];
+    const float* src = (is_v ? a.v : a.k) + (size_t)h * a.src_head;
+    const auto row = [&](int e) { return src + (size_t)(tile * KV_TILE + e - a.first) * a.src_pos; };
+    uint8_t* codes = (is_v ? a.dst.vc : a.dst.kc) + (size_t)h * a.dst.code_head;
+    const auto scales = [&](int b) {
+        return reinterpret_cast<_Float16*>((is_v ? a.dst.vs : a.dst.ks) + (size_t)h * a.dst.scale_head + ((size_t)tile * nb + b) * (2 * KV_TILE));
+    };
+    if (!is_v) {
+        const int kq = u % 4, b = u / 4 % nb, half = u / 4 / nb, d0 = 32 * b + 8 * kq;
+        float x[4][8];
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int e = 4 * half + i;
+            f32x4u lo = {}, hi = {};
+            if (e >= e0 && e < e1) {
+                lo = *reinterpret_cast<const f32x4u*>(row(e) + d0);
+                hi = *reinterpret_cast<const f32x4u*>(row(e) + d0 + 4);
+            }
+            x[i][0] = lo.x; x[i][1] = lo.y; x[i][2] = lo.z; x[i][3] = lo.w;
+            x[i][4] = hi.x; x[i][5] = hi.y; x[i][6] = hi.z; x[i][7] = hi.w;
+        }
+        if constexpr (ROPE != ROPE_NONE) {
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = 4 * half + i;
+                if (e >= e0 && e < e1)
+                    q4_rope8<ROPE>(x[i], row(e), d0, a.hd, (float)(a.start_pos + tile * KV_TILE + e - a.first) * a.freq_scale, a.inv_freq);
+            }
+        }
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int e = 4 * half + i;
+            const _Float16 d = q4_scale(x[i], lane);
+            if (e < e0 || e >= e1) continue;
+            uint32_t c[8], w = 0;
+            q4_codes(x[i], (float)d, c);
+            #pragma unroll
+            for (int j = 0; j < 8; j++) w |= c[j] << q4_bit(j);
+            *reinterpret_cast<uint32_t*>(codes + (size_t)(tile * KV_TILE + e) * (a.hd / 2) + 4 * (kq * nb + b)) = w;
+            if (kq == 0) scales(b)[e] = d;
+        }
+        return;
+    }
+    const int b = u / 8, d0 = 4 * u;
+    float x[8][4];
     #pragma unroll
     for (int e = 0; e < 8; e++) {
-        if (e >= e0 && e < e1) {
-            const float* p = src + (size_t)(tile * KV_TILE + e - a.first) * a.src_pos + d0;
-            const f32x4u u = *reinterpret_cast<const f32x4u*>(p), w = *reinterpret_cast<const f32x4u*>(p + 4);
-            x[e][0] = u.x; x[e][1] = u.y; x[e][2] = u.z; x[e][3] = u.w;
-            x[e][4] = w.x; x[e][5] = w.y; x[e][6] = w.z; x[e][7] = w.w;
-        } else {
-            #pragma unroll
-            for (int j = 0; j < 8; j++) x[e][j] = 0.0f;
-        }
+        f32x4u v = {};
+        if (e >= e0 && e < e1) v = *reinterpret_cast<const f32x4u*>(row(e) + d0);
+        x[e][0] = v.x; x[e][1] = v.y; x[e][2] = v.z; x[e][3] = v.w;
     }
-    if constexpr (ROPE != ROPE_NONE) {
-        if (!is_v) {
-            #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (e >= e0 && e < e1) {
-                    const long long p = tile * KV_TILE + e - a.first;
-                    q4_rope8<ROPE>(x[e], src + (size_t)p * a.src_pos, d0, a.hd, (float)(a.start_pos + p) * a.freq_scale,
-                                   a.inv_freq);
-                }
-        }
-    }
-    uint8_t* sc = (is_v ? a.dst.vs : a.dst.ks) + (size_t)h * a.dst.scale_head + ((size_t)tile * nb + b) * (2 * KV_TILE);
-    uint8_t* codes = (is_v ? a.dst.vc : a.dst.kc) + (size_t)h * a.dst.code_head;
-    uint32_t vw[8] = {};   // V: one dword per dim
+    uint32_t w[4] = {};
     #pragma unroll
     for (int e = 0; e < 8; e++) {
         const _Float16 d = q4_scale(x[e], lane);
         if (e < e0 || e >= e1) continue;
-        uint32_t c[8];
-        q4_codes8(x[e], (float)d, c);
-        if (is_v) {
-            #pragma unroll
-            for (int j = 0; j < 8; j++) vw[j] |= c[j] << q4_bit(e);
-        } else {
-            uint32_t kw = 0;
-            #pragma unroll
-            for (int j = 0; j < 8; j++) kw |= c[j] << q4_bit(j);
-            *reinterpret_cast<uint32_t*>(codes + (size_t)(tile * KV_TILE + e) * (a.hd / 2) + 4 * (kq * nb + b)) = kw;
-        }
-        if (kq == 0) reinterpret_cast<_Float16*>(sc)[e] = d;
-    }
-    if (is_v) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(codes + (size_t)tile * KV_TILE * (a.hd / 2));
-        // the tile's earlier positions keep their nibbles
-        uint32_t keep = 0;
-        for (int e = 0; e < e0; e++) keep |= 0xFu << q4_bit(e);
+        uint32_t c[4];
+        q4_codes(x[e], (float)d, c);
         #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            uint32_t* p = w + ((d0 + j) % 16) * (a.hd / 16) + d0 / 16;
-            *p = keep ? (*p & keep) | vw[j] : vw[j];
-        }
+        for (int j = 0; j < 4; j++) w[j] |= c[j] << q4_bit(e);
+        if (u % 8 == 0) scales(b)[e] = d;
+    }
+    // the tile's earlier positions keep their nibbles
+    uint32_t keep = 0;
+    for (int e = 0; e < e0; e++) keep |= 0xFu << q4_bit(e);
+    #pragma unroll
+    for (int j = 0; j < 4; j++) {
+        uint32_t* p = reinterpret_cast<uint32_t*>(codes + (size_t)tile * KV_TILE * (a.hd / 2)) + ((d0 + j) % 16) * (a.hd / 16) + d0 / 16;
+        *p = keep ? (*p & keep) | w[j] : w[j];
     }
 }
 
@@ -288,7 +301,7 @@ hipError_t q4_append_launch(const Q4View& dst, const float* k, const float* v, s
     a.hd = (int)hd;
     a.first = (long long)first;
     a.n = (long long)n;
-    a.kv_blocks = q4_grid(n_kv, hd, first, n, 8);
+    a.kv_blocks = q4_grid(n_kv, hd, first, n, 4);
     hipLaunchKernelGGL(q4_append_kernel<ROPE_NONE>, dim3(a.kv_blocks, 2), dim3(256), 0, s, a);
     return hipGetLastError();
 }
@@ -312,7 +325,7 @@ hipError_t q4_append_rope_launch(int layout, const Q4View& dst, const float* q, 
     a.q = q;
     a.q_out = q_out;
     a.n_q = q ? (int)n_q : 0;
-    a.kv_blocks = q4_grid(n_kv, hd, first, n, 8);
+    a.kv_blocks = q4_grid(n_kv, hd, first, n, 4);
     const unsigned grid = a.kv_blocks + (unsigned)((n * a.n_q * (hd / 2) + 255) / 256);
     if (layout == ROPE_INTERLEAVED)
         hipLaunchKernelGGL(q4_append_kernel<ROPE_INTERLEAVED>, dim3(grid, 2), dim3(256), 0, s, a);

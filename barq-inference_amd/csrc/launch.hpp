@@ -219,7 +219,8 @@ int attention_q4_scores_splits(size_t n_head, size_t n_head_kv, size_t head_dim,
 hipError_t attention_q4_scores_launch(const AttnArgs& a, const AttnScores& sc, const Q4View& kv, hipStream_t s);
 
 // attention_mass.hip: mass_out[hk][j] = mass_in[hk][j] (null: 0) + the softmax weights of position j over the call's
-// rows and the heads of hk, j < kv_len, from what the launches above left (in and out may be the same)
+// rows and the heads of hk, j < kv_len, from what the launches above left (in and out may be the same); and the
+// merge of the partial states into attn.out or, if given, out_q8
 struct MassArgs {
     const float* scores;
     size_t score_stride;
@@ -234,7 +235,7 @@ struct MassArgs {
 };
 size_t attention_mass_stat(size_t n_head, size_t n_head_kv, size_t q_len);   // bytes of stat (0: not used)
 size_t attention_mass_sums(size_t n_head, size_t n_head_kv, size_t q_len, size_t score_stride);
-hipError_t attention_mass_launch(const MassArgs& a, hipStream_t s);
+hipError_t attention_mass_launch(const MassArgs& a, const AttnArgs& attn, uint8_t* out_q8, hipStream_t s);
 
 // merges ns partial states [q_len][n_head][ns][head_dim + 2] of a.part (ns <= 1024)
 hipError_t attention_combine_launch(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s);

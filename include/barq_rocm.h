@@ -516,7 +516,7 @@ int barq_rocm_attention_q8k(barq_rocm_handle* h, const float* q, const barq_rocm
  * as they are.  barq_rocm_kv_cache_evict goes by them.  The output agrees with
  * barq_rocm_attention's within float rounding (an f32 cache's prompt chunks take
  * the decode kernel here).  Uses the handle's workspace for the scores, at
- * most 64 MiB of them or one query's. */
+ * most 128 MiB of them or one query's. */
 int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache* c, size_t layer,
                              size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len,
                              size_t start_pos, int out_type, void* out, const float* mass_in, float* mass_out,
