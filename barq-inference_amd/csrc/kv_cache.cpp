@@ -26,6 +26,7 @@ int barq_rocm_kv_cache_read(barq_rocm_handle* h, const barq_rocm_kv_cache* c, si
     if (h->device != c->device) return fail(BARQ_E_INVALID, "kv_cache_read: cache is on another device");
     if (mem == BARQ_MEM_DEVICE && !(aligned(k, 4) && aligned(v, 4)))
         return fail(BARQ_E_INVALID, "kv_cache_read: outputs must be 4-byte aligned");
+    if (c->n_head_kv > 65535) return fail(BARQ_E_DIM, "kv_cache_read: %zu kv heads (at most 65535)", c->n_head_kv);
     DeviceGuard g(h);
     const size_t hd = c->head_dim, row = n * hd * sizeof(float), bytes = c->n_head_kv * row;
     if (c->type == BARQ_TYPE_F32) {

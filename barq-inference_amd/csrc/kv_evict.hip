@@ -6,12 +6,14 @@
 //   of their positions
 //
 // Selection: a workgroup per kv head looks for the want-th largest key (the
-// mass as an unsigned integer of the same order) 8 bits at a time from the
-// top, each time with a histogram of the keys that share the bits found so far, then numbers
-// the kept positions by a running count.  The histogram has a column for each
-// LDS bank: masses share their leading bits, and 64 lanes adding to one counter
-// would take turns.  Up to 64 keys a thread stay in registers over the five
-// passes; longer heads are read again by each (from the L2).
+// mass as an unsigned integer of the same order) 11 bits at a time from the
+// top, each time with a histogram of the keys that share the bits found so
+// far, until all keys that share them are wanted; then it numbers the kept
+// positions by a running count.  The histogram has eight columns, since masses
+// share their leading bits and lanes adding to one counter take turns.  Up to
+// 32 masses a thread stay in registers over the passes; longer heads are read
+// again by each (from the L2).  One workgroup's latencies bound it: 16384
+// positions take hardly longer than 4097.
 //
 // The rows then move in one launch, bound by memory: f32 rows as they are;
 // of a 4-bit cache, whose tiles hold 8 positions of V in one dword per dim, a
@@ -23,6 +25,7 @@
 namespace barq {
 
 constexpr int EV_NT = 1024;
+constexpr int EV_DIGITS = 2 * EV_NT;
 constexpr int EV_CHUNK = 4 * EV_NT;   // keys of a pass over the workgroup, four in a row per thread
 
 struct EvictArgs {
@@ -74,10 +77,10 @@ __device__ __forceinline__ uint32_t waves_before(const uint32_t* part, int w, ui
 template <int R>
 __global__ __launch_bounds__(EV_NT)
 void evict_select_kernel(EvictArgs a) {
-    __shared__ __align__(16) uint32_t hist[256][32];
+    __shared__ __align__(16) uint32_t hist[EV_DIGITS][8];
     __shared__ __align__(16) uint32_t part[R ? R : 1][EV_NT / 64];
-    static_assert(EV_NT == 1024, "16 waves, four threads a digit");
-    __shared__ uint32_t found[2];   // the digit and what is left to find within it
+    static_assert(EV_NT == 1024, "16 waves, two digits a thread");
+    __shared__ uint32_t found[3];   // the digit, what is left to find within it, its keys
     const int t = threadIdx.x, l = t & 63, w = t >> 6, h = blockIdx.x;
     const float* in = a.mass_in + (size_t)h * a.stride;
     float* out = a.mass_out ? a.mass_out + (size_t)h * a.stride : nullptr;
@@ -95,70 +98,92 @@ void evict_select_kernel(EvictArgs a) {
             for (int u = 0; u < 4; u++) x[u] = j + u < a.n ? in[j + u] : 0.0f;
         }
     };
+    constexpr bool KEYS = R > 0 && R <= 4;   // their keys stay in registers too
     float reg[R ? R : 1][4];
+    uint32_t keys[KEYS ? R : 1][4];
     if constexpr (R > 0) {
         #pragma unroll
         for (int c = 0; c < R; c++) load(c, reg[c]);
     }
-    // f(chunk, its four masses): every chunk, in order
+    if constexpr (KEYS) {
+        #pragma unroll
+        for (int c = 0; c < R; c++)
+            #pragma unroll
+            for (int u = 0; u < 4; u++) keys[c][u] = ev_key(reg[c][u]);
+    }
+    // f(chunk, its four masses, their keys): every chunk, in order
     auto each = [&](auto f) {
-        if constexpr (R > 0) {
+        if constexpr (KEYS) {
             #pragma unroll
             for (int c = 0; c < R; c++)
-                if (c < chunks) f(c, reg[c]);
+                if (c < chunks) f(c, reg[c], keys[c]);
+        } else if constexpr (R > 0) {
+            #pragma unroll
+            for (int c = 0; c < R; c++)
+                if (c < chunks) {
+                    const uint32_t k[4] = {ev_key(reg[c][0]), ev_key(reg[c][1]), ev_key(reg[c][2]), ev_key(reg[c][3])};
+                    f(c, reg[c], k);
+                }
         } else {
             float x[4];
             for (int c = 0; c < chunks; c++) {
                 load(c, x);
-                f(c, x);
+                const uint32_t k[4] = {ev_key(x[0]), ev_key(x[1]), ev_key(x[2]), ev_key(x[3])};
+                f(c, x, k);
             }
         }
     };
 
-    // the want-th largest key among the old positions
-    uint32_t key = 0, ties = 0;   // ties: how many of the keys equal to it are kept
+    // the want-th largest key among the old positions, in the bits of mask: all
+    // keys above it there are kept, and `ties` of those equal to it
+    uint32_t key = 0, mask = 0, ties = 0;
     const bool some = want > 0 && want < old;
     if (some) {
-        uint32_t left = (uint32_t)want, mask = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = t; i < 256 * 8; i += EV_NT) reinterpret_cast<uint4*>(&hist[0][0])[i] = make_uint4(0, 0, 0, 0);
+        ties = (uint32_t)want;
+        for (int shift = 21; mask != 0xFFFFFFFFu; shift = shift > 11 ? shift - 11 : 0) {
+            for (int i = t; i < EV_DIGITS * 2; i += EV_NT) reinterpret_cast<uint4*>(&hist[0][0])[i] = make_uint4(0, 0, 0, 0);
             __syncthreads();
-            each([&](int c, const float (&x)[4]) {
+            const uint32_t digits = shift ? 2047u : 1023u;   // 11, 11 and 10 bits
+            each([&](int c, const float (&x)[4], const uint32_t (&k)[4]) {
                 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const uint32_t k = ev_key(x[u]);
-                    if (c * EV_CHUNK + 4 * t + u < old && (k & mask) == key)
-                        atomicAdd(&hist[(k >> shift) & 255u][t & 31], 1u);
-                }
+                for (int u = 0; u < 4; u++)
+                    if (c * EV_CHUNK + 4 * t + u < old && (k[u] & mask) == key) atomicAdd(&hist[(k[u] >> shift) & digits][t & 7], 1u);
             });
             __syncthreads();
-            // four threads a digit (whole quads), then the digits above it
-            const int digit = 255 - t / 4;   // wave 0 holds the largest
-            uint32_t s = 0;
+            // a thread's two digits, and those above them
+            const int digit = EV_DIGITS - 1 - 2 * t;
+            uint32_t s[2];
             #pragma unroll
-            for (int i = 0; i < 8; i++) s += hist[digit][(t & 3) * 8 + ((i + t / 4) & 7)];
-            s = (uint32_t)quad_isum((int)s);
+            for (int i = 0; i < 2; i++) {
+                const uint4 p = *reinterpret_cast<const uint4*>(&hist[digit - i][0]), q = *reinterpret_cast<const uint4*>(&hist[digit - i][4]);
+                s[i] = ((p.x + p.y) + (p.z + p.w)) + ((q.x + q.y) + (q.z + q.w));
+            }
             uint32_t all;
-            const uint32_t before = wave_scan((t & 3) == 0 ? s : 0u, all);
+            const uint32_t before = wave_scan(s[0] + s[1], all);
             if (l == 0) part[0][w] = all;
             __syncthreads();
-            const uint32_t above = before + waves_before(part[0], w, all);
-            if ((t & 3) == 0 && above < left && left <= above + s) {
-                found[0] = (uint32_t)digit;
-                found[1] = left - above;
+            uint32_t above = before + waves_before(part[0], w, all);
+            #pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (above < ties && ties <= above + s[i]) {
+                    found[0] = (uint32_t)(digit - i);
+                    found[1] = ties - above;
+                    found[2] = s[i];
+                }
+                above += s[i];
             }
             __syncthreads();
             key |= found[0] << shift;
-            left = found[1];
-            mask |= 255u << shift;
+            mask |= digits << shift;
+            ties = found[1];
+            if (ties == found[2]) break;   // all that share the bits
         }
-        ties = left;
     }
 
     // numbering: of each position the kept ones before it; larger keys and
     // keys equal to the last one counted side by side (16 bits each a chunk)
     const auto flag = [&](int j, float x) {
-        const uint32_t k = ev_key(x);
+        const uint32_t k = ev_key(x) & mask;
         const bool gt = (j >= old && j < a.n) || (j < old && (some ? k > key : want > 0));
         return gt ? 1u : some && j < old && k == key ? 0x10000u : 0u;
     };
@@ -228,7 +253,7 @@ hipError_t evict_select_launch(const float* mass_in, float* mass_out, size_t str
     const dim3 grid((unsigned)n_kv), block(EV_NT);
     if (chunks <= 1) hipLaunchKernelGGL(evict_select_kernel<1>, grid, block, 0, s, a);
     else if (chunks <= 4) hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, s, a);
-    else if (chunks <= 16) hipLaunchKernelGGL(evict_select_kernel<16>, grid, block, 0, s, a);
+    else if (chunks <= 8) hipLaunchKernelGGL(evict_select_kernel<8>, grid, block, 0, s, a);
     else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, s, a);
     return hipGetLastError();
 }

@@ -66,7 +66,7 @@ def test_evict_in_place(be, type_, kind, n, keep, recent):
     assert c.layer_len(0) == 0 and c.size() == 0
 
 
-@pytest.mark.parametrize("n", [16384, 16385, 70000])
+@pytest.mark.parametrize("n", [16384, 16385, 32768, 70000])
 def test_long_heads(be, n):
     c, (k, v) = fill(be, B.Q4_0, 2, n, 64, layers=1)
     mass = masses("spread", 2, n)
