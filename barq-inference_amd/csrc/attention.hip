@@ -382,18 +382,18 @@ void attn_kernel(const float* __restrict__ q, const float* __restrict__ kc, cons
 // 1024 threads per (h, i).
 template <int HD>
 __global__ __launch_bounds__(1024)
-void attn_combine_kernel(const float* __restrict__ part, int n_split, int n_head, float* __restrict__ out) {
+void attn_combine_kernel(const float* __restrict__ part, int n_split, int n_head, float* __restrict__ out, float2* stat) {
     __shared__ CombineLds<HD> sm;
-    attn_combine_row<HD>(part, n_split, n_head, blockIdx.x, blockIdx.y, sm, out);
+    attn_combine_row<HD>(part, n_split, n_head, blockIdx.x, blockIdx.y, sm, out, stat);
 }
 
 // The same merge with the output row written as Q8_K blocks (the o
 // projection's activation): workgroup (b, i) takes block b of row i.
 template <int HD>
 __global__ __launch_bounds__(1024)
-void attn_combine_q8k_kernel(const float* __restrict__ part, int n_split, int n_head, uint8_t* __restrict__ out) {
+void attn_combine_q8k_kernel(const float* __restrict__ part, int n_split, int n_head, uint8_t* __restrict__ out, float2* stat) {
     __shared__ CombineQ8Lds<HD> sm;
-    attn_combine_q8k_block<HD>(part, n_split, n_head, blockIdx.x, blockIdx.y, sm, out);
+    attn_combine_q8k_block<HD>(part, n_split, n_head, blockIdx.x, blockIdx.y, sm, out, stat);
 }
 
 // The same merge by one wave per 256 output values (256 / HD heads of row i;
@@ -403,7 +403,7 @@ void attn_combine_q8k_kernel(const float* __restrict__ part, int n_split, int n_
 template <int HD, bool Q8>
 __global__ __launch_bounds__(256)
 void attn_merge_kernel(const float* __restrict__ part, int n_split, int n_head, int rows, float* __restrict__ out,
-                       uint8_t* __restrict__ out_q8) {
+                       uint8_t* __restrict__ out_q8, float2* __restrict__ stat) {
     const int nblk = (n_head * HD + 255) / 256;
     const long long at = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = (int)(at / nblk), b = (int)(at % nblk);
@@ -427,6 +427,7 @@ void attn_merge_kernel(const float* __restrict__ part, int n_split, int n_head, 
         O[2] = __builtin_fmaf(o1.x, w, O[2] * c);
         O[3] = __builtin_fmaf(o1.y, w, O[3] * c);
     }
+    if (stat && d == 0) stat[(size_t)i * n_head + h] = make_float2(M, 1.0f / L);
     const float vv[4] = {O[0] / L, O[1] / L, O[2] / L, O[3] / L};
     if constexpr (!Q8) {
         typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -502,39 +503,39 @@ bool attention_q8_direct(const AttnArgs& a) {
 }
 
 template <int HD>
-static hipError_t attn_combine_t(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s) {
+static hipError_t attn_combine_t(const AttnArgs& a, int ns, uint8_t* out_q8, float2* stat, hipStream_t s) {
     if (out_q8)
         hipLaunchKernelGGL(attn_combine_q8k_kernel<HD>, dim3((unsigned)(a.n_head * HD / 256), (unsigned)a.q_len),
-                           dim3(1024), 0, s, a.part, ns, (int)a.n_head, out_q8);
+                           dim3(1024), 0, s, a.part, ns, (int)a.n_head, out_q8, stat);
     else
         hipLaunchKernelGGL(attn_combine_kernel<HD>, dim3((unsigned)a.n_head, (unsigned)a.q_len), dim3(1024), 0, s,
-                           a.part, ns, (int)a.n_head, a.out);
+                           a.part, ns, (int)a.n_head, a.out, stat);
     return hipGetLastError();
 }
 
 template <int HD>
-static hipError_t attn_merge_t(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s) {
+static hipError_t attn_merge_t(const AttnArgs& a, int ns, uint8_t* out_q8, float2* stat, hipStream_t s) {
     // Workgroups per row and head take two or three states as long as thirty
     // (3.8 us for 32 heads of one row with 64, 26 us for 256 rows with one), waves
     // 0.1 us a state and run side by side.
-    if (ns > 16 && a.n_head * a.q_len <= 512) return attn_combine_t<HD>(a, ns, out_q8, s);
+    if (ns > 16 && a.n_head * a.q_len <= 512) return attn_combine_t<HD>(a, ns, out_q8, stat, s);
     const size_t waves = (a.n_head * HD + 255) / 256 * a.q_len;
     const dim3 grid((unsigned)((waves + 3) / 4));
     if (out_q8)
         hipLaunchKernelGGL((attn_merge_kernel<HD, true>), grid, dim3(256), 0, s, a.part, ns, (int)a.n_head, (int)a.q_len, a.out,
-                           out_q8);
+                           out_q8, stat);
     else
         hipLaunchKernelGGL((attn_merge_kernel<HD, false>), grid, dim3(256), 0, s, a.part, ns, (int)a.n_head, (int)a.q_len,
-                           a.out, out_q8);
+                           a.out, out_q8, stat);
     return hipGetLastError();
 }
 
 // a.part's ns partial states per row and head into out_q8, or without it into a.out
-hipError_t attention_combine_launch(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s) {
+hipError_t attention_combine_launch(const AttnArgs& a, int ns, uint8_t* out_q8, float2* stat, hipStream_t s) {
     switch (a.head_dim) {
-    case 64: return attn_merge_t<64>(a, ns, out_q8, s);
-    case 128: return attn_merge_t<128>(a, ns, out_q8, s);
-    case 256: return attn_merge_t<256>(a, ns, out_q8, s);
+    case 64: return attn_merge_t<64>(a, ns, out_q8, stat, s);
+    case 128: return attn_merge_t<128>(a, ns, out_q8, stat, s);
+    case 256: return attn_merge_t<256>(a, ns, out_q8, stat, s);
     default: return hipErrorInvalidValue;
     }
 }
@@ -547,7 +548,7 @@ static hipError_t attn_launch_t(const AttnArgs& a, int ns, int chunk, int groups
                        (long long)a.start_pos, chunk, scale, a.part, a.out, nullptr, 0);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || ns == 1) return e;
-    return attn_combine_t<HD>(a, ns, a.out_q8 && attention_q8_direct(a) ? a.out_q8 : nullptr, s);
+    return attn_combine_t<HD>(a, ns, a.out_q8 && attention_q8_direct(a) ? a.out_q8 : nullptr, nullptr, s);
 }
 
 template <int HD>
@@ -589,7 +590,7 @@ int attention_scores_splits(size_t n_head, size_t n_head_kv, size_t q_len, size_
     return ns;
 }
 
-// The decode kernel for any number of rows (the prompt kernel keeps no scores).
+// The decode kernel for any number of rows.
 hipError_t attention_scores_launch(const AttnArgs& a, const AttnScores& sc, hipStream_t s) {
     int ns = 0, chunk = 0;
     attention_plan(a.n_head, a.n_head_kv, a.q_len, a.kv_len, &ns, &chunk);

@@ -12,7 +12,7 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 constexpr int ATT_MAX_SPLIT = 1024;
 
 // One output head: out value of dim t (t < HD) from the n_split partial
-// states at pp, by NT threads t = 0 .. NT - 1 (all of them call it: it
+// states at pp (and unless null its maximum and 1 / sum to stat), by NT threads t = 0 .. NT - 1 (all of them call it: it
 // synchronises the workgroup).  The split maxima and weights are spread over
 // the threads; the output sums run over SUB = 1024 / HD subsets of the splits
 // (split s in subset s % SUB, in increasing order), then are added in LDS in
@@ -28,7 +28,7 @@ struct CombineLds {
 
 template <int HD, int NT>
 __device__ __forceinline__ float attn_combine_head(const float* __restrict__ pp, int n_split, CombineLds<HD>& sm,
-                                                   int t) {
+                                                   int t, float2* stat = nullptr) {
     constexpr int NWV = NT / 64, SUB = 1024 / HD, K = 1024 / NT, STEP = NT / HD, PRE = 8;
     static_assert(NT % HD == 0 && 1024 % NT == 0, "threads per head");
     const int lane = t & 63, wave = t >> 6;
@@ -88,6 +88,7 @@ __device__ __forceinline__ float attn_combine_head(const float* __restrict__ pp,
     float L = sm.wred[1][0];
     #pragma unroll
     for (int u = 1; u < 1024 / 64; u++) L += sm.wred[1][u];
+    if (stat && t == 0) *stat = make_float2(M, 1.0f / L);
     #pragma unroll
     for (int j = 0; j < K; j++) {
         const int sj = sub + STEP * j;
@@ -114,9 +115,10 @@ __device__ __forceinline__ float attn_combine_head(const float* __restrict__ pp,
 // out[i, h, :] by a workgroup of 1024 threads.
 template <int HD>
 __device__ __forceinline__ void attn_combine_row(const float* __restrict__ part, int n_split, int n_head, int h, int i,
-                                                 CombineLds<HD>& sm, float* __restrict__ out) {
+                                                 CombineLds<HD>& sm, float* __restrict__ out, float2* stat = nullptr) {
     const int t = threadIdx.x;
-    const float v = attn_combine_head<HD, 1024>(part + ((size_t)i * n_head + h) * n_split * (HD + 2), n_split, sm, t);
+    const size_t at = (size_t)i * n_head + h;
+    const float v = attn_combine_head<HD, 1024>(part + at * n_split * (HD + 2), n_split, sm, t, stat ? stat + at : nullptr);
     if (t < HD) out[((size_t)i * n_head + h) * HD + t] = v;
 }
 
@@ -130,10 +132,12 @@ struct CombineQ8Lds {
 };
 template <int HD>
 __device__ __forceinline__ void attn_combine_q8k_block(const float* __restrict__ part, int n_split, int n_head, int b, int i,
-                                                       CombineQ8Lds<HD>& sm, uint8_t* __restrict__ out) {
+                                                       CombineQ8Lds<HD>& sm, uint8_t* __restrict__ out,
+                                                       float2* stat = nullptr) {
     constexpr int NH = 256 / HD, NT = 1024 / NH;
     const int t = threadIdx.x, hh = t / NT, tg = t % NT, h = b * NH + hh;
-    const float v = attn_combine_head<HD, NT>(part + ((size_t)i * n_head + h) * n_split * (HD + 2), n_split, sm.head[hh], tg);
+    const size_t at = (size_t)i * n_head + h;
+    const float v = attn_combine_head<HD, NT>(part + at * n_split * (HD + 2), n_split, sm.head[hh], tg, stat ? stat + at : nullptr);
     if (tg < HD) sm.vals[hh * HD + tg] = v;
     __syncthreads();
     if (t < 64) {

@@ -34,14 +34,6 @@ __device__ __forceinline__ float2 mass_stat(const MassArgs& a, size_t at, int la
     return make_float2(all, 1.0f / L);
 }
 
-__global__ __launch_bounds__(256)
-void mass_stat_kernel(MassArgs a) {
-    const size_t at = (size_t)blockIdx.x * 16 + threadIdx.x / 16;
-    const size_t n = (size_t)a.q_len * a.n_head;
-    const float2 st = mass_stat(a, at < n ? at : n - 1, threadIdx.x & 15);
-    if (at < n && (threadIdx.x & 15) == 0) reinterpret_cast<float2*>(a.stat)[at] = st;
-}
-
 // query heads h with h * n_head_kv / n_head = hk: first, and behind the last
 __device__ __forceinline__ int mass_head(const MassArgs& a, int hk) {
     return (int)(((long long)hk * a.n_head + a.n_head_kv - 1) / a.n_head_kv);
@@ -132,7 +124,7 @@ void mass_run_kernel(MassArgs a) {
     #pragma unroll 4
     for (int r = r0; r < r1; r++) {
         const size_t at = (size_t)i * a.n_head + h0 + g;
-        const float2 st = reinterpret_cast<const float2*>(a.stat)[at];
+        const float2 st = a.stat[at];
         const float4 s = *reinterpret_cast<const float4*>(a.scores + at * a.score_stride + j);   // (whole rows of 32)
         const long long seen = (a.start_pos + i + 1 < a.kv_len ? a.start_pos + i + 1 : a.kv_len) - j;
         const float p[4] = {__builtin_amdgcn_exp2f(s.x - st.x) * st.y, __builtin_amdgcn_exp2f(s.y - st.x) * st.y,
@@ -160,34 +152,28 @@ void mass_sum_kernel(MassArgs a, int runs) {
 
 static size_t mass_rows(size_t n_head, size_t n_head_kv, size_t q_len) { return q_len * ((n_head + n_head_kv - 1) / n_head_kv); }
 
-size_t attention_mass_stat(size_t n_head, size_t n_head_kv, size_t q_len) {
-    return mass_rows(n_head, n_head_kv, q_len) <= (size_t)MASS_INLINE ? 0 : q_len * n_head * sizeof(float2);
+bool attention_mass_few(size_t n_head, size_t n_head_kv, size_t q_len) {
+    return mass_rows(n_head, n_head_kv, q_len) <= (size_t)MASS_INLINE;
 }
 
 size_t attention_mass_sums(size_t n_head, size_t n_head_kv, size_t q_len, size_t stride) {
-    const size_t rows = mass_rows(n_head, n_head_kv, q_len);
-    return rows <= (size_t)MASS_INLINE ? 0 : (rows + MASS_RUN - 1) / MASS_RUN * n_head_kv * stride * sizeof(float);
+    return (mass_rows(n_head, n_head_kv, q_len) + MASS_RUN - 1) / MASS_RUN * n_head_kv * stride * sizeof(float);
 }
 
-hipError_t attention_mass_launch(const MassArgs& a, const AttnArgs& attn, uint8_t* out_q8, hipStream_t s) {
-    const size_t rows = mass_rows(a.n_head, a.n_head_kv, a.q_len);
-    const unsigned heads = (unsigned)a.n_head_kv;
-    if (rows <= (size_t)MASS_INLINE) {
-        switch (a.head_dim) {
-        case 64: return mass_finish_t<64>(a, attn.out, out_q8, s);
-        case 128: return mass_finish_t<128>(a, attn.out, out_q8, s);
-        case 256: return mass_finish_t<256>(a, attn.out, out_q8, s);
-        default: return hipErrorInvalidValue;
-        }
+hipError_t attention_mass_few_launch(const MassArgs& a, const AttnArgs& attn, uint8_t* out_q8, hipStream_t s) {
+    switch (a.head_dim) {
+    case 64: return mass_finish_t<64>(a, attn.out, out_q8, s);
+    case 128: return mass_finish_t<128>(a, attn.out, out_q8, s);
+    case 256: return mass_finish_t<256>(a, attn.out, out_q8, s);
+    default: return hipErrorInvalidValue;
     }
-    const unsigned runs = (unsigned)((rows + MASS_RUN - 1) / MASS_RUN);
-    hipError_t e = attention_combine_launch(attn, a.ns, out_q8, s);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(mass_stat_kernel, dim3((unsigned)(((size_t)a.q_len * a.n_head + 15) / 16)), dim3(256), 0, s, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
+}
+
+hipError_t attention_mass_launch(const MassArgs& a, hipStream_t s) {
+    const unsigned heads = (unsigned)a.n_head_kv;
+    const unsigned runs = (unsigned)((mass_rows(a.n_head, a.n_head_kv, a.q_len) + MASS_RUN - 1) / MASS_RUN);
     hipLaunchKernelGGL(mass_run_kernel, dim3((unsigned)((a.score_stride + 1023) / 1024), heads, runs), dim3(256), 0, s, a);
-    e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(mass_sum_kernel, dim3((unsigned)((a.kv_len + 255) / 256), heads), dim3(256), 0, s, a, (int)runs);
     return hipGetLastError();

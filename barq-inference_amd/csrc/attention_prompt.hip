@@ -82,13 +82,15 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 
 // The merge of a row's pieces: one wave per 256 output values (256 / HD heads
 // of row i; fewer in a last wave), four values per lane; Q8, whose rows are
-// whole blocks, writes the values' Q8_K block (q8_k_block) instead of them.  One pass over
+// whole blocks, writes the values' Q8_K block (q8_k_block) instead of them.  stat, unless
+// null: the rows' maxima and 1 / sums, and every tile has left its states.  One pass over
 // the pieces, each rescaling what was summed before it, so a row waits for
 // memory once per two pieces and not twice per piece.
 template <int HD, bool Q8>
 __global__ __launch_bounds__(256)
 void attn_combine_few_kernel(const float* __restrict__ part, int stride, int chunk, int n_head, int G, int q_len,
-                             int kv_len, long long start_pos, float* __restrict__ out, uint8_t* __restrict__ out_q8) {
+                             int kv_len, long long start_pos, float* __restrict__ out, uint8_t* __restrict__ out_q8,
+                             float2* __restrict__ stat) {
     const int nblk = (n_head * HD + 255) / 256;
     const int b = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = blockIdx.y;
     if (b >= nblk) return;
@@ -98,7 +100,7 @@ void attn_combine_few_kernel(const float* __restrict__ part, int stride, int chu
     // the pieces of the row's tile (attn_prompt_kernel's list)
     const int tile = (i * G + h % G) / AP_ROWS;
     const int n_split = (ap_tile_blocks(tile, G, q_len, kv_len, start_pos) + chunk - 1) / chunk;
-    if (!Q8 && n_split == 1) return;   // stored by the kernel itself
+    if (!Q8 && n_split == 1 && !stat) return;   // stored by the kernel itself
     const float* pp = part + ((size_t)i * n_head + h) * stride * (HD + 2);
     float M = -INFINITY, L = 0.0f, O[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     #pragma unroll 2
@@ -115,6 +117,7 @@ void attn_combine_few_kernel(const float* __restrict__ part, int stride, int chu
         O[2] = __builtin_fmaf(o1.x, w, O[2] * c);
         O[3] = __builtin_fmaf(o1.y, w, O[3] * c);
     }
+    if (stat && d == 0) stat[(size_t)i * n_head + h] = make_float2(M, 1.0f / L);
     const float vv[4] = {O[0] / L, O[1] / L, O[2] / L, O[3] / L};
     if constexpr (!Q8)
         *reinterpret_cast<float4*>(out + ((size_t)i * n_head + h) * HD + d) = make_float4(vv[0], vv[1], vv[2], vv[3]);
@@ -131,12 +134,15 @@ struct ApArgs {
     size_t head_stride;   // floats between kv heads
     int n_head, n_head_kv, G, groups;   // groups of G heads that share a kv head
     int q_len, kv_len;
+    int q_rows;           // rows of q per head (the call's are the first q_len)
     long long start_pos;
     float scale;          // log2(e) / sqrt(HD)
     float* out;           // [q_len, n_head, HD]
     float* part;          // partial states (chunk > 0)
     int chunk, stride;
-    int all_parts;        // tiles of one piece store their state too (the merge quantizes)
+    int all_parts;        // tiles of one piece store their state too (the merge quantizes, or scores are kept)
+    float* scores;        // SC: [q_len * n_head][score_stride], log2 units (unseen positions: anything)
+    size_t score_stride;
 };
 
 // LDS: two stages of a block's split K and V, the V dims' largest values and
@@ -163,7 +169,8 @@ struct ApLds {
     static constexpr int F32_RS = 4 * HD + 16, F32_PIECES = HD / 4 + 1, F32_BLK = 32 * F32_RS;
     static constexpr int TOTAL = VS + 4 * HD;
     static_assert(4 * F32_BLK <= TOTAL, "the f32 stages fit");
-    static_assert(8 / AP_NW * TOTAL <= 163840, "eight waves per CU");
+    static constexpr int PER_CU = HD <= 128 ? 2 : 1;   // workgroups
+    static_assert(PER_CU * TOTAL <= 163840, "their LDS");
     static_assert(AP_NW == 4, "four waves' largest |q|");
     static_assert(PP >= 4 && HD % (4 * TPR) == 0, "whole float4 loads and position groups");
 };
@@ -217,6 +224,12 @@ __device__ __forceinline__ void ap_store_ml(const ApArgs& a, const ApRow& r, int
     p[1] = lsum;
 }
 
+// SC: four scores of the lane's row, in log2 units.
+__device__ __forceinline__ void ap_store_scores(const ApArgs& a, const ApRow& r, int j, float x, float y, float z, float w) {
+    if (r.ok)   // (a row's stride is whole blocks)
+        *reinterpret_cast<float4*>(a.scores + ((size_t)r.i * a.n_head + r.h) * a.score_stride + j) = make_float4(x, y, z, w);
+}
+
 // ---- f32 MFMAs: tiles with values that are not finite ----------------------------
 // v_mfma_f32_32x32x2_f32 on K and V rows copied to LDS as they are.  The dims
 // of a lane: HD / 32 consecutive ones per register (output row i of block b
@@ -239,7 +252,7 @@ __device__ __forceinline__ void ap_f32_issue(uint32_t stage, i32x4v kr, i32x4v v
     }
 }
 
-template <int HD>
+template <int HD, bool SC>
 __device__ __forceinline__ void ap_rows_f32(const uint8_t* lds, uint32_t lds0, const ApArgs& a, int grp, int tile, int piece, int b_lo, int b_hi) {
     using L = ApLds<HD>;
     constexpr int NB = HD / 32;
@@ -252,7 +265,7 @@ __device__ __forceinline__ void ap_rows_f32(const uint8_t* lds, uint32_t lds0, c
     const i32x4v vr = make_rsrc4(a.v + (size_t)hk * a.head_stride, (uint32_t)a.kv_len * (4u * HD));
     ap_f32_issue<HD>(lds0, kr, vr, (uint32_t)b_lo * (128u * HD), wave, l);
     float qv[HD / 2];
-    const float4* qp = reinterpret_cast<const float4*>(a.q + ((size_t)row.h * a.q_len + row.i) * HD + HD / 2 * g);
+    const float4* qp = reinterpret_cast<const float4*>(a.q + ((size_t)row.h * a.q_rows + row.i) * HD + HD / 2 * g);
     #pragma unroll
     for (int u = 0; u < HD / 8; u++) {
         const float4 t = qp[u];
@@ -285,6 +298,11 @@ __device__ __forceinline__ void ap_rows_f32(const uint8_t* lds, uint32_t lds0, c
             const int kv = j0 + 8 * (r >> 2) + 4 * g + (r & 3);
             sc[r] = kv < row.vis ? (sa[r] + sb[r]) * a.scale : -INFINITY;
             bm = fmaxf(bm, sc[r]);
+        }
+        if constexpr (SC) {
+            #pragma unroll
+            for (int q = 0; q < 4; q++)
+                ap_store_scores(a, row, j0 + 8 * q + 4 * g, sc[4 * q], sc[4 * q + 1], sc[4 * q + 2], sc[4 * q + 3]);
         }
         {
             auto hb = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, bm), __builtin_bit_cast(int, bm), false, false);
@@ -347,11 +365,14 @@ __device__ __forceinline__ void ap_rows_f32(const uint8_t* lds, uint32_t lds0, c
     if (!row.ok) return;
     if (piece >= 0 && g == 0) ap_store_ml<HD>(a, row, piece, m, lsum);
     #pragma unroll
-    for (int r = 0; r < 16; r += 4 / NB) {
+    for (int r = 0; r < 16; r += NB < 4 ? 4 / NB : 1) {
         // registers r .. of the NB blocks: four consecutive dims
         const int i = 8 * (r >> 2) + 4 * g + (r & 3);
         float4 v;
-        if constexpr (NB == 4) v = make_float4(o[0][r], o[1][r], o[2][r], o[3][r]);
+        if constexpr (NB == 8) {
+            ap_store4<HD>(a, row, piece, NB * i + 4, make_float4(o[4][r], o[5][r], o[6][r], o[7][r]), lsum);
+            v = make_float4(o[0][r], o[1][r], o[2][r], o[3][r]);
+        } else if constexpr (NB == 4) v = make_float4(o[0][r], o[1][r], o[2][r], o[3][r]);
         else v = make_float4(o[0][r], o[1][r], o[0][r + 1], o[1][r + 1]);
         ap_store4<HD>(a, row, piece, NB * i, v, lsum);
     }
@@ -533,8 +554,8 @@ __device__ __forceinline__ void ap_rescale(const uint8_t* lds, int n, int grown,
 }
 
 // One block from its stage: scores, softmax, O.
-template <int HD>
-__device__ __forceinline__ void ap_compute(const uint8_t* lds, int n, int j0, const h8v (&qh)[HD / 16],
+template <int HD, bool SC>
+__device__ __forceinline__ void ap_compute(const ApArgs& a, const uint8_t* lds, int n, int j0, const h8v (&qh)[HD / 16],
                                            const h8v (&ql)[HD / 16], float qf, int c, int g, const ApRow& row, float& m,
                                            float& lsum, f32x16 (&o)[ApLds<HD>::NB]) {
     using L = ApLds<HD>;
@@ -564,6 +585,15 @@ __device__ __forceinline__ void ap_compute(const uint8_t* lds, int n, int j0, co
         sc[4 * q + 1] = sa[4 * q + 1] * kf.y;
         sc[4 * q + 2] = sa[4 * q + 2] * kf.z;
         sc[4 * q + 3] = sa[4 * q + 3] * kf.w;
+    }
+    if constexpr (SC) {   // (the weights from the scores as they are kept: the sums match)
+        #pragma unroll
+        for (int q = 0; q < 4; q++) {
+            #pragma unroll
+            for (int e = 0; e < 4; e++) sc[4 * q + e] *= qf;
+            ap_store_scores(a, row, j0 + 8 * q + 4 * g, sc[4 * q], sc[4 * q + 1], sc[4 * q + 2], sc[4 * q + 3]);
+        }
+        qf = 1.0f;
     }
     if (j0 + 32 > row.vis_first) {   // some row of the wave does not see the whole block
         #pragma unroll
@@ -644,7 +674,7 @@ __device__ __forceinline__ void ap_compute(const uint8_t* lds, int n, int j0, co
 // One tile, or with chunk > 0 (and more blocks than that) piece `piece` of it: position blocks [piece,
 // piece + 1) * chunk, whose partial state (reference maximum in log2 units,
 // sum, unnormalised output) goes to the merge kernel.
-template <int HD>
+template <int HD, bool SC>
 __device__ __forceinline__ void ap_tile(uint8_t* lds, uint32_t lds0, const ApArgs& a, int grp, int tile, int piece) {
     using L = ApLds<HD>;
     const int t = threadIdx.x, l = t & 63, c = l & 31, g = l >> 5;
@@ -669,7 +699,7 @@ __device__ __forceinline__ void ap_tile(uint8_t* lds, uint32_t lds0, const ApArg
     h8v qh[HD / 16], ql[HD / 16];
     float qf;
     {
-        const float4* qp = reinterpret_cast<const float4*>(a.q + ((size_t)row.h * a.q_len + row.i) * HD + 8 * g);
+        const float4* qp = reinterpret_cast<const float4*>(a.q + ((size_t)row.h * a.q_rows + row.i) * HD + 8 * g);
         float4 qv[HD / 8];
         float qm = 0.0f;
         #pragma unroll
@@ -719,7 +749,7 @@ __device__ __forceinline__ void ap_tile(uint8_t* lds, uint32_t lds0, const ApArg
         if (n + 2 < nb) ap_load<HD>(reg, kr, vr, b_lo + n + 2, t);
         const int j0 = 32 * (b_lo + n);
         ap_rescale<HD>(lds, n, __builtin_amdgcn_readfirstlane(grown), g, o);
-        if (j0 < row.vis_last) ap_compute<HD>(lds, n, j0, qh, ql, qf, c, g, row, m, lsum, o);
+        if (j0 < row.vis_last) ap_compute<HD, SC>(a, lds, n, j0, qh, ql, qf, c, g, row, m, lsum, o);
         if (n + 2 < nb) ap_vmax<HD>(lds, reg, n & 1, t);
     }
     // values too far apart, sums that are not finite: the whole tile again in
@@ -733,7 +763,7 @@ __device__ __forceinline__ void ap_tile(uint8_t* lds, uint32_t lds0, const ApArg
         #pragma unroll
         for (int r = 0; r < 16; r++) z = __builtin_fmaf(o[u][r], 0.0f, z);
     if (__syncthreads_or(bad || (row.ok && z != 0.0f))) {
-        ap_rows_f32<HD>(lds, lds0, a, grp, tile, piece, b_lo, b_hi);
+        ap_rows_f32<HD, SC>(lds, lds0, a, grp, tile, piece, b_lo, b_hi);
         return;
     }
     if (!row.ok) return;
@@ -760,8 +790,8 @@ __device__ __forceinline__ void ap_tile(uint8_t* lds, uint32_t lds0, const ApArg
 // runs from the longest tile down (a free CU takes the longest piece left;
 // with eight kv heads each XCD keeps to one head's K and V): whole tiles, or
 // with chunk > 0 each tile's pieces of chunk blocks.
-template <int HD>
-__global__ __launch_bounds__(64 * AP_NW, 2)
+template <int HD, bool SC>
+__global__ __launch_bounds__(64 * AP_NW, ApLds<HD>::PER_CU)
 void attn_prompt_kernel(ApArgs a) {
     __shared__ __align__(16) uint8_t lds[ApLds<HD>::TOTAL];
     const int grp = blockIdx.x % a.groups;
@@ -777,7 +807,7 @@ void attn_prompt_kernel(ApArgs a) {
         piece = 0;
     }
     if (tile < 0) return;   // past the list (the grid is its length)
-    ap_tile<HD>(lds, lds_addr(lds), a, grp, tile, piece);
+    ap_tile<HD, SC>(lds, lds_addr(lds), a, grp, tile, piece);
 }
 
 // ---- launch ------------------------------------------------------------------
@@ -820,9 +850,41 @@ bool attn_prompt_q8_direct(const AttnArgs& a) {
     return attn_prompt_plan(a.n_head, a.n_head_kv, a.head_dim, a.q_len, a.kv_len).chunk > 0;
 }
 
+// Heads of 256 dims come here with their scores only: a workgroup's LDS is then
+// 143 KiB and its registers are a CU's, so one runs there at a time.  With the
+// masses of an f32 cache, us, decode kernel / this one: 32/8 heads of 256, 1000
+// rows after 1500 3320 / 820, 3 / 4 / 6 / 8 rows after 4000 41 / 60, 53 / 62, 76
+// / 64, 96 / 66, 64 rows from position 0 26 / 42; 14/2 heads, 8 / 16 / 32 rows
+// after 1000 34 / 44, 53 / 49, 83 / 54.  The rule for the smaller heads, at
+// twice the time a block of 128 dims takes, picks the faster in 14 of 18 such calls and is
+// 23 % off at most.  (32/8 heads of 128, 1000 rows after 1500: 1522 / 340.)
+bool attn_prompt_scores_path(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len) {
+    if (head_dim != 256) return attn_prompt_path(n_head, n_head_kv, head_dim, q_len, kv_len);
+    const int min_q = tuning_env(TUNE_ATTN_MFMA_MIN_Q);
+    if (q_len < (min_q > 0 ? (size_t)min_q : 2) || kv_len >= ((size_t)1 << 22)) return false;
+    return min_q > 0 ||
+           ap_rows_time(n_head, n_head_kv, head_dim, q_len, kv_len) >
+               1.1 * (9.4 + attn_prompt_plan(n_head, n_head_kv, head_dim, q_len, kv_len).us);
+}
+
+// Scores are kept beside every tile's states: without pieces, one piece each.
+static void attn_prompt_keep(ApPlan& p, size_t kv_len) {
+    if (p.chunk > 0) return;
+    p.chunk = (int)((kv_len + 31) / 32);
+    p.stride = 1;
+}
+
+size_t attn_prompt_scores_workspace(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len) {
+    ApPlan p = attn_prompt_plan(n_head, n_head_kv, head_dim, q_len, kv_len);
+    attn_prompt_keep(p, kv_len);
+    return (size_t)p.stride * n_head * q_len * (head_dim + 2) * sizeof(float);
+}
+
+// sc and stat: both or neither
 template <int HD>
-static hipError_t attn_prompt_launch_t(const AttnArgs& a, hipStream_t s) {
-    const ApPlan p = attn_prompt_plan(a.n_head, a.n_head_kv, HD, a.q_len, a.kv_len);
+static hipError_t attn_prompt_launch_t(const AttnArgs& a, const AttnScores* sc, float2* stat, hipStream_t s) {
+    ApPlan p = attn_prompt_plan(a.n_head, a.n_head_kv, HD, a.q_len, a.kv_len);
+    if (sc) attn_prompt_keep(p, a.kv_len);
     ApArgs k{};
     k.q = a.q;
     k.k = a.k + a.layer_off;
@@ -834,34 +896,50 @@ static hipError_t attn_prompt_launch_t(const AttnArgs& a, hipStream_t s) {
     k.groups = p.groups;
     k.q_len = (int)a.q_len;
     k.kv_len = (int)a.kv_len;
+    k.q_rows = (int)(sc ? sc->q_rows : a.q_len);
     k.start_pos = (long long)a.start_pos;
     k.scale = (1.0f / sqrtf((float)HD)) * LOG2E;
     k.out = a.out;
     k.part = a.part;
     k.chunk = p.chunk;
     k.stride = p.stride;
-    k.all_parts = a.out_q8 != nullptr;
+    k.all_parts = sc || a.out_q8 != nullptr;
+    if (sc) {
+        k.scores = sc->scores;
+        k.score_stride = sc->stride;
+    }
     unsigned n = (unsigned)p.tiles;
     if (p.chunk > 0) {   // the pieces of every tile at the actual start position
         n = 0;
         for (int t = 0; t < p.tiles; t++)
             n += (unsigned)((ap_tile_blocks(t, p.G, k.q_len, k.kv_len, k.start_pos) + p.chunk - 1) / p.chunk);
     }
-    hipLaunchKernelGGL(attn_prompt_kernel<HD>, dim3(n * (unsigned)p.groups), dim3(64 * AP_NW), 0, s, k);
+    const dim3 grid(n * (unsigned)p.groups), block(64 * AP_NW);
+    if (sc) hipLaunchKernelGGL((attn_prompt_kernel<HD, true>), grid, block, 0, s, k);
+    else if constexpr (HD <= 128) hipLaunchKernelGGL((attn_prompt_kernel<HD, false>), grid, block, 0, s, k);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.chunk == 0) return e;
     const dim3 cg((unsigned)(((a.n_head * HD + 255) / 256 + 3) / 4), (unsigned)a.q_len);
     if (a.out_q8)
         hipLaunchKernelGGL((attn_combine_few_kernel<HD, true>), cg, dim3(256), 0, s, a.part, p.stride, p.chunk,
-                           (int)a.n_head, p.G, (int)a.q_len, (int)a.kv_len, (long long)a.start_pos, a.out, a.out_q8);
+                           (int)a.n_head, p.G, (int)a.q_len, (int)a.kv_len, (long long)a.start_pos, a.out, a.out_q8, stat);
     else
         hipLaunchKernelGGL((attn_combine_few_kernel<HD, false>), cg, dim3(256), 0, s, a.part, p.stride, p.chunk,
-                           (int)a.n_head, p.G, (int)a.q_len, (int)a.kv_len, (long long)a.start_pos, a.out, a.out_q8);
+                           (int)a.n_head, p.G, (int)a.q_len, (int)a.kv_len, (long long)a.start_pos, a.out, a.out_q8, stat);
     return hipGetLastError();
 }
 
 hipError_t attn_prompt_launch(const AttnArgs& a, hipStream_t s) {
-    return a.head_dim == 64 ? attn_prompt_launch_t<64>(a, s) : attn_prompt_launch_t<128>(a, s);
+    return a.head_dim == 64 ? attn_prompt_launch_t<64>(a, nullptr, nullptr, s) : attn_prompt_launch_t<128>(a, nullptr, nullptr, s);
+}
+
+hipError_t attn_prompt_scores_launch(const AttnArgs& a, const AttnScores& sc, float2* stat, hipStream_t s) {
+    switch (a.head_dim) {
+    case 64: return attn_prompt_launch_t<64>(a, &sc, stat, s);
+    case 128: return attn_prompt_launch_t<128>(a, &sc, stat, s);
+    case 256: return attn_prompt_launch_t<256>(a, &sc, stat, s);
+    default: return hipErrorInvalidValue;
+    }
 }
 
 }  // namespace barq

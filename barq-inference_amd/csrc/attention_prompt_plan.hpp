@@ -42,7 +42,8 @@ struct ApPlan {
 // A launch's time, us, if the tiles (runs of equal length, shortest first) are
 // cut into pieces of c position blocks: the last to end of the workgroups,
 // which take pieces in the list's order, longest tile first, two to a CU, and
-// the merge.  A block takes 2.7 us with 128 dims and 1.35 with 64, a piece as
+// the merge.  A block takes 2.7 us with 128 dims and 1.35 with 64 (5.4 with
+// 256, not fitted), a piece as
 // long as 1.4 blocks more for its fixed part (the query rows, the first loads,
 // the partial state), and two pieces that share a CU 1.2 times as long as one;
 // the merge reads a row's pieces one after the other (0.085 us each) and all
@@ -57,7 +58,7 @@ struct ApRun {
 };
 inline double ap_time(const std::vector<ApRun>& runs, size_t groups, size_t head_dim, size_t cus, int c) {
     constexpr double FIXED = 1.4, SHARE = 1.2, MERGE_PIECE = 0.085, MERGE_BYTE = 2.0 / 4.6e6;
-    const double block = head_dim == 128 ? 2.7 : 1.35;
+    const double block = head_dim == 256 ? 5.4 : head_dim == 128 ? 2.7 : 1.35;
     const double inv = 1.0 / (double)c;
     const auto length = [&](const ApRun& r) { return (double)(r.blocks < c ? r.blocks : c) + FIXED; };
     size_t n = 0, merged = 0, blocks = 0;

@@ -291,7 +291,7 @@ static hipError_t attn_q4_launch_t(const AttnArgs& a, const AttnScores* sc, cons
         e = hipGetLastError();
     }
     if (e != hipSuccess || sc || p.n_split == 1) return e;
-    return attention_combine_launch(a, p.n_split, attention_q4_q8_direct(a) ? a.out_q8 : nullptr, s);
+    return attention_combine_launch(a, p.n_split, attention_q4_q8_direct(a) ? a.out_q8 : nullptr, nullptr, s);
 }
 
 static hipError_t attn_q4_launch(const AttnArgs& a, const AttnScores* sc, const Q4View& kv, hipStream_t s) {

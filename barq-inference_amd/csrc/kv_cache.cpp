@@ -200,12 +200,16 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
                            : barq::attention_scores_splits(n_head, n_head_kv, n, kv_len));
     };
     const size_t last = q_len % rows;   // the last chunk's rows, if fewer
-    const auto states = [&](size_t n) { return splits(n) * n_head * n * (head_dim + 2) * sizeof(float); };
+    const auto prompt = [&](size_t n) { return !q4 && barq::attn_prompt_scores_path(n_head, n_head_kv, head_dim, n, kv_len); };
+    const auto states = [&](size_t n) {
+        return prompt(n) ? barq::attn_prompt_scores_workspace(n_head, n_head_kv, head_dim, n, kv_len)
+                         : splits(n) * n_head * n * (head_dim + 2) * sizeof(float);
+    };
     size_t part = states(rows);
     if (last && states(last) > part) part = states(last);
     const size_t nq = n_head * q_len * head_dim, out_row = q8 ? n_head * head_dim / 256 * 292 : n_head * head_dim * 4;
     Arena a;
-    const size_t os = a.add(rows * per_row), op = a.add(part), ost = a.add(barq::attention_mass_stat(n_head, n_head_kv, rows));
+    const size_t os = a.add(rows * per_row), op = a.add(part), ost = a.add(n_head * rows * sizeof(float2));
     const size_t osum = a.add(barq::attention_mass_sums(n_head, n_head_kv, rows, stride));
     const size_t oq = host ? a.add(nq * 4) : 0, oo = host ? a.add(q_len * out_row) : 0;
     const size_t om = host ? a.add(n_head_kv * kv_len * sizeof(float)) : 0;
@@ -244,9 +248,18 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
         args.part = at<float>(h, op);
         args.out = q8 ? nullptr : reinterpret_cast<float*>(ob + i * out_row);
         const barq::AttnScores sc{at<float>(h, os), stride, q_len};
-        BARQ_CHECK(launched(q4 ? barq::attention_q4_scores_launch(args, sc, c->view(layer), h->stream)
-                               : barq::attention_scores_launch(args, sc, h->stream), who));
-        const int ns = (int)splits(n);
+        uint8_t* out_q8 = q8 ? ob + i * out_row : nullptr;
+        float2* stat = at<float2>(h, ost);
+        const bool merged = prompt(n), few = !merged && barq::attention_mass_few(n_head, n_head_kv, n);
+        const int ns = merged ? 0 : (int)splits(n);
+        if (merged) {
+            args.out_q8 = out_q8;
+            BARQ_CHECK(launched(barq::attn_prompt_scores_launch(args, sc, stat, h->stream), who));
+        } else {
+            BARQ_CHECK(launched(q4 ? barq::attention_q4_scores_launch(args, sc, c->view(layer), h->stream)
+                                   : barq::attention_scores_launch(args, sc, h->stream), who));
+            if (!few) BARQ_CHECK(launched(barq::attention_combine_launch(args, ns, out_q8, stat, h->stream), who));
+        }
         barq::MassArgs m{};
         m.scores = sc.scores;
         m.score_stride = stride;
@@ -258,12 +271,13 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
         m.q_len = (int)n;
         m.kv_len = (int)kv_len;
         m.start_pos = (long long)(start_pos + i);
-        m.stat = at<float>(h, ost);
+        m.stat = stat;
         m.sums = at<float>(h, osum);
         m.mass_in = i ? mo : mi;
         m.mass_out = mo;
         m.mass_stride = ms;
-        BARQ_CHECK(launched(barq::attention_mass_launch(m, args, q8 ? ob + i * out_row : nullptr, h->stream), who));
+        BARQ_CHECK(launched(few ? barq::attention_mass_few_launch(m, args, out_q8, h->stream)
+                                : barq::attention_mass_launch(m, h->stream), who));
     }
     if (host) {
         BARQ_HIP(hipMemcpyAsync(out, ob, q_len * out_row, hipMemcpyDeviceToHost, h->stream));

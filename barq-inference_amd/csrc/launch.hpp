@@ -219,26 +219,28 @@ int attention_q4_scores_splits(size_t n_head, size_t n_head_kv, size_t head_dim,
 hipError_t attention_q4_scores_launch(const AttnArgs& a, const AttnScores& sc, const Q4View& kv, hipStream_t s);
 
 // attention_mass.hip: mass_out[hk][j] = mass_in[hk][j] (null: 0) + the softmax weights of position j over the call's
-// rows and the heads of hk, j < kv_len, from what the launches above left (in and out may be the same); and the
-// merge of the partial states into attn.out or, if given, out_q8
+// rows and the heads of hk, j < kv_len, from what the launches above left (in and out may be the same)
 struct MassArgs {
     const float* scores;
     size_t score_stride;
-    const float* part;     // [q_len][n_head][ns][head_dim + 2]
+    const float* part;     // few rows: [q_len][n_head][ns][head_dim + 2]
     int ns, head_dim, n_head, n_head_kv, q_len, kv_len;
     long long start_pos;
-    float* stat;           // q_len * n_head pairs (attention_mass_stat)
+    const float2* stat;    // many rows: maxima and 1 / sums, [q_len][n_head]
     float* sums;           // partial sums (attention_mass_sums)
     const float* mass_in;
     float* mass_out;
     size_t mass_stride;
 };
-size_t attention_mass_stat(size_t n_head, size_t n_head_kv, size_t q_len);   // bytes of stat (0: not used)
-size_t attention_mass_sums(size_t n_head, size_t n_head_kv, size_t q_len, size_t score_stride);
-hipError_t attention_mass_launch(const MassArgs& a, const AttnArgs& attn, uint8_t* out_q8, hipStream_t s);
+bool attention_mass_few(size_t n_head, size_t n_head_kv, size_t q_len);
+size_t attention_mass_sums(size_t n_head, size_t n_head_kv, size_t q_len, size_t score_stride);   // bytes of sums
+// few rows, and the merge of their states into attn.out or, if given, out_q8
+hipError_t attention_mass_few_launch(const MassArgs& a, const AttnArgs& attn, uint8_t* out_q8, hipStream_t s);
+hipError_t attention_mass_launch(const MassArgs& a, hipStream_t s);
 
 // merges ns partial states [q_len][n_head][ns][head_dim + 2] of a.part (ns <= 1024)
-hipError_t attention_combine_launch(const AttnArgs& a, int ns, uint8_t* out_q8, hipStream_t s);
+// (and with stat the rows' maxima and 1 / sums, [q_len][n_head])
+hipError_t attention_combine_launch(const AttnArgs& a, int ns, uint8_t* out_q8, float2* stat, hipStream_t s);
 
 // kv_q4.hip: rows into and out of a 4-bit cache; first: the cache position of row 0
 hipError_t q4_append_launch(const Q4View& dst, const float* k, const float* v, size_t src_head, size_t src_pos,
@@ -279,5 +281,9 @@ bool attn_prompt_path(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q
 size_t attn_prompt_workspace(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);
 bool attn_prompt_q8_direct(const AttnArgs& a);
 hipError_t attn_prompt_launch(const AttnArgs& a, hipStream_t s);
+// the same with the scores kept (AttnScores), and merged (a.out or a.out_q8); stat: the rows' maxima and 1 / sums
+bool attn_prompt_scores_path(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);
+size_t attn_prompt_scores_workspace(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);
+hipError_t attn_prompt_scores_launch(const AttnArgs& a, const AttnScores& sc, float2* stat, hipStream_t s);
 
 }  // namespace barq

@@ -81,12 +81,60 @@ def test_out_and_mass(be, type_, heads, n_kv, hd, n, start):
 
 @pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
 def test_rows_in_chunks(be, type_):
-    """More scores than one launch keeps (64 MiB): 300 rows of 32 heads against 2300 positions."""
-    c, q, k, v = case(be, type_, 32, 8, 64, 300, 2000)
-    ref, added = attention(q, k, v, 2000)
-    out, mass = A.compute_attention_mass(be, dev(q), c, 0, 32, 8, 64, 300, 2300, 2000, None)
-    assert np.max(np.abs(out.cpu().numpy() - ref)) <= 2e-5 * np.max(np.abs(v))
-    assert mass_ok(mass.cpu().numpy(), np.zeros((8, 2300), F32), added)
+    """300 rows of 32 heads against 2300 positions (88 MB of scores), and against 4300: more than one launch keeps
+    (128 MiB), 242 rows of them and 58."""
+    for start in (2000, 4000):
+        total = start + 300
+        c, q, k, v = case(be, type_, 32, 8, 64, 300, start)
+        ref, added = attention(q, k, v, start)
+        out, mass = A.compute_attention_mass(be, dev(q), c, 0, 32, 8, 64, 300, total, start, None)
+        assert np.max(np.abs(out.cpu().numpy() - ref)) <= 2e-5 * np.max(np.abs(v))
+        assert mass_ok(mass.cpu().numpy(), np.zeros((8, total), F32), added)
+
+
+PROMPTS = [(32, 8, 128, 200, 800), (16, 4, 64, 600, 100), (8, 8, 128, 130, 1000), (6, 2, 128, 257, 1500), (12, 4, 128, 500, 0),
+           (20, 1, 64, 33, 3000), (14, 2, 256, 100, 400), (14, 2, 256, 300, 500), (4, 2, 256, 40, 3960), (5, 2, 128, 300, 300)]
+
+
+@pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
+@pytest.mark.parametrize("heads,n_kv,hd,n,start", PROMPTS)
+def test_prompts(be, type_, heads, n_kv, hd, n, start):
+    total = start + n
+    c, q, k, v = case(be, type_, heads, n_kv, hd, n, start)
+    ref, added = attention(q, k, v, start)
+    before = np.abs(rows(4, n_kv, total + 3))
+    out, mass = A.compute_attention_mass(be, dev(q), c, 0, heads, n_kv, hd, n, total, start, dev(before))
+    out, mass = out.cpu().numpy(), mass.cpu().numpy()
+    assert np.max(np.abs(out - ref)) <= 2e-5 * np.max(np.abs(v))
+    assert mass_ok(mass[:, :total], before[:, :total], added) and np.array_equal(mass[:, total:], before[:, total:])
+    if heads * hd % 256 == 0:
+        q8, m1 = A.compute_attention_mass(be, dev(q), c, 0, heads, n_kv, hd, n, total, start, dev(before), out_type=B.Q8_K)
+        assert (q8.flatten() == be.quantize_act(B.Q8_K, dev(out.reshape(n, heads * hd)))).all()
+        assert np.array_equal(m1.cpu().numpy(), mass)
+
+
+@pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompts_of_uneven_rows(be, type_, hd):
+    """Values of very different sizes, rows that see a NaN or an infinity, and rows that do not."""
+    heads, n_kv, n, start = 8, 2, 300, 500
+    q, k, v = rows(5, heads, n, hd), rows(6, n_kv, start + n, hd), rows(7, n_kv, start + n, hd)
+    v[:, ::7] *= F32(2.0 ** -40)
+    k[:, ::11] *= 4
+    for bad in (False, True):
+        if bad:
+            k[1, 700, 3], v[0, 650, 2] = np.nan, np.inf
+        c = A.KVCache(be, start + n, 1, n_kv, hd, type=type_)
+        c.append(0, dev(k), dev(v), start + n, hd)
+        kk, vv = (q4_values(k), q4_values(v)) if type_ == B.Q4_0 else (k, v)
+        ref, added = attention(q, kk, vv, start)
+        out, mass = A.compute_attention_mass(be, dev(q), c, 0, heads, n_kv, hd, n, start + n, start, None)
+        out, mass = out.cpu().numpy(), mass.cpu().numpy()
+        assert np.array_equal(np.isfinite(out), np.isfinite(ref)) and np.array_equal(np.isnan(mass), np.isnan(added))
+        ok = np.isfinite(ref)
+        assert np.max(np.abs(out[ok] - ref[ok])) <= 2e-5 * np.nanmax(np.abs(vv[np.isfinite(vv)]))
+        seen = ~np.isnan(added)
+        assert np.all(np.abs(mass - added)[seen] <= 2.5e-5 * added[seen] + 2.0 ** -23 * added[seen])
 
 
 @pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
