@@ -90,10 +90,10 @@ struct Q4Stage {
 // first position of one goes there, block by block; the rows that see it get
 // NaN at the end.  (0 * NaN would reach rows that do not.)
 template <int HD, bool SC>
-__device__ __forceinline__ void q4_step(const Q4Stage<HD>& s, int base, int j1, const Q4Seen (&seen)[1], const Q4Query<HD> (&q)[1],
-                                        bool exact, const Q4Const& kc, Q4State<HD> (&st)[1], float* const (&score_row)[1],
+__device__ __forceinline__ void q4_step(const Q4Stage<HD>& s, int base, int j1, const Q4Seen& seen, const Q4Query<HD>& q,
+                                        bool exact, const Q4Const& kc, Q4State<HD>& st, float* score_row,
                                         int* nan_at) {
-    float x[1][8];
+    float x[8];
     uint32_t kw[2][HD / 32];
     #pragma unroll
     for (int t = 0; t < 2; t++) s.k_row(t, kw[t]);
@@ -130,7 +130,7 @@ __device__ __forceinline__ void q4_step(const Q4Stage<HD>& s, int base, int j1, 
         }
     }
     uint4 vw;
-    q4_attend<HD, 1, SC>(x, base, at, seen, q, kc, st, score_row, [&](int c, h8v& hi, h8v& lo) {
+    q4_attend<HD, SC>(x, base, at, seen, q, kc, st, score_row, [&](int c, h8v& hi, h8v& lo) {
         if (c % 4 == 0) vw = s.v_dims(c / 4);
         q4_v_frag(c % 4 == 0 ? vw.x : c % 4 == 1 ? vw.y : c % 4 == 2 ? vw.z : vw.w, *s.scale(1, c / 2), kc, hi, lo);
     });
@@ -139,9 +139,9 @@ __device__ __forceinline__ void q4_step(const Q4Stage<HD>& s, int base, int j1, 
 // A wave's steps of positions j0 .. j1: every `turn` positions from the first.
 template <int HD, bool SC>
 __device__ __forceinline__ void q4_walk(const Q4Fifo<HD>& fifo, uint8_t* lds, int j0, int j1, int first, int turn, int l,
-                                        const Q4Seen (&seen)[1], const Q4Query<HD> (&q)[1], bool exact, const Q4Const& kc,
-                                        Q4State<HD> (&st)[1], float* const (&score_row)[1], int* nan_at) {
-    st[0].clear();
+                                        const Q4Seen& seen, const Q4Query<HD>& q, bool exact, const Q4Const& kc,
+                                        Q4State<HD>& st, float* score_row, int* nan_at) {
+    st.clear();
     const int n = j1 - j0;
     if (first >= n) return;
     fifo.issue(0, (uint32_t)first);
@@ -181,32 +181,32 @@ void attn_q4_kernel(Q4Args a) {
     fifo.init(a.kv, hk, start, max(j1, start), l, lds_addr(mine));
     const Q4Const kc;
     const Q4Row row = q4_row(a, grp, r0 + c);
-    const Q4Seen seen[1] = {{min(row.vis, j1), min(q4_vis(a, r0), j1)}};
-    Q4Query<HD> q[1];
-    const bool exact = __any(q[0].load(a.q + ((size_t)row.h * a.q_rows + row.i) * HD, a.scale, g, kc));
-    float* const score_row[1] = {SC && row.ok ? a.scores + ((size_t)row.i * a.n_head + row.h) * a.score_stride : nullptr};
-    Q4State<HD> st[1];
+    const Q4Seen seen{min(row.vis, j1), min(q4_vis(a, r0), j1)};
+    Q4Query<HD> q;
+    const bool exact = __any(q.load(a.q + ((size_t)row.h * a.q_rows + row.i) * HD, a.scale, g, kc));
+    float* const score_row = SC && row.ok ? a.scores + ((size_t)row.i * a.n_head + row.h) * a.score_stride : nullptr;
+    Q4State<HD> st;
     int* nan_at = nullptr;
     for (;;) {
         q4_walk<HD, SC>(fifo, mine, j0, j1, wave * Q4A_STEP, Q4A_NW * Q4A_STEP, l, seen, q, exact, kc, st, score_row, nan_at);
-        if (nan_at || !__any(st[0].not_finite())) break;
+        if (nan_at || !__any(st.not_finite())) break;
         // NaN somewhere: again with V's NaN blocks kept out of the products
         nan_at = nan_pos[wave];
         if (l < NB) nan_at[l] = 0x7FFFFFFF;
     }
     if (nan_at) {
         wait_lgkmcnt0();
-        st[0].put_nan(nan_at, seen[0].end);
+        st.put_nan(nan_at, seen.end);
     }
 
     // the four waves' states
     float (*lo)[Q4A_ROWS][ORS] = reinterpret_cast<float (*)[Q4A_ROWS][ORS]>(lds);
     __syncthreads();
     #pragma unroll
-    for (int u = 0; u < HD / 16; u++) *reinterpret_cast<f32x4*>(&lo[wave][c][16 * u + 4 * g]) = st[0].o[u];
-    const float lsum = groups_sum(st[0].l);
+    for (int u = 0; u < HD / 16; u++) *reinterpret_cast<f32x4*>(&lo[wave][c][16 * u + 4 * g]) = st.o[u];
+    const float lsum = groups_sum(st.l);
     if (g == 0) {
-        lml[wave][c][0] = st[0].m;
+        lml[wave][c][0] = st.m;
         lml[wave][c][1] = lsum;
     }
     __syncthreads();

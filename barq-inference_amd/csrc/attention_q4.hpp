@@ -220,42 +220,39 @@ struct Q4Seen {
     int all;   // every row of its tile sees the positions up to here
 };
 
-// The scores of R tiles' rows (times their scale).  kfrag(t, b, fresh): K codes minus 8 of S tile t,
-// block b, as f16 (fresh: not values it gave before, which would stay in registers between
-// the calls); kscale(b): the group's 8 positions' scales.
-template <int HD, int R, class K, class S>
-__device__ __forceinline__ void q4_scores(float (&x)[R][8], const Q4Query<HD> (&q)[R], bool exact, K kfrag, S kscale) {
+// The scores of the tile's rows (times their scale).  kfrag(t, b, fresh): K
+// codes minus 8 of S tile t, block b, as f16 (fresh: not values it gave before,
+// which would stay in registers between the calls); kscale(b): the group's 8
+// positions' scales.
+template <int HD, class K, class S>
+__device__ __forceinline__ void q4_scores(float (&x)[8], const Q4Query<HD>& q, bool exact, K kfrag, S kscale) {
     #pragma unroll
-    for (int r = 0; r < R; r++)
-        #pragma unroll
-        for (int e = 0; e < 8; e++) x[r][e] = 0.0f;
+    for (int e = 0; e < 8; e++) x[e] = 0.0f;
     if (exact) {
         #pragma unroll
-        for (int b = 0; b < HD / 32; b++)
+        for (int b = 0; b < HD / 32; b++) {
+            bf8v p[3];
+            q.exact(b, p);
+            const h8v d = __builtin_bit_cast(h8v, kscale(b));
             #pragma unroll
-            for (int r = 0; r < R; r++) {
-                bf8v p[3];
-                q[r].exact(b, p);
-                const h8v d = __builtin_bit_cast(h8v, kscale(b));
+            for (int t = 0; t < 2; t++) {
+                const h8v n = kfrag(t, b, true);
+                bf8v k;
                 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const h8v n = kfrag(t, b, true);
-                    bf8v k;
-                    #pragma unroll
-                    for (int e = 0; e < 8; e++) k[e] = (__bf16)(float)n[e];
-                    f32x4 c = {};
-                    #pragma unroll
-                    for (int i = 2; i >= 0; i--) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, p[i], c, 0, 0, 0);
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) x[r][4 * t + e] = __builtin_fmaf(c[e], (float)d[4 * t + e], x[r][4 * t + e]);
-                }
-                __builtin_amdgcn_sched_barrier(0);   // (one block's values at a time)
+                for (int e = 0; e < 8; e++) k[e] = (__bf16)(float)n[e];
+                f32x4 c = {};
+                #pragma unroll
+                for (int i = 2; i >= 0; i--) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, p[i], c, 0, 0, 0);
+                #pragma unroll
+                for (int e = 0; e < 4; e++) x[4 * t + e] = __builtin_fmaf(c[e], (float)d[4 * t + e], x[4 * t + e]);
             }
+            __builtin_amdgcn_sched_barrier(0);   // (one block's values at a time)
+        }
     } else {
         // a block's products run while the next one's codes are fetched (or formed), and the one before is scaled
         h8v k[2][2];
         u32x4v d[2];
-        f32x4 c[2][2][R];
+        f32x4 c[2][2];
         #pragma unroll
         for (int t = 0; t < 2; t++) k[0][t] = kfrag(t, 0, false);
         d[0] = kscale(0);
@@ -265,21 +262,17 @@ __device__ __forceinline__ void q4_scores(float (&x)[R][8], const Q4Query<HD> (&
             if (b < HD / 32) {
                 #pragma unroll
                 for (int t = 0; t < 2; t++)
-                    #pragma unroll
-                    for (int r = 0; r < R; r++) c[cur][t][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[cur][t], q[r].lo[b], f32x4{}, 0, 0, 0);
+                    c[cur][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[cur][t], q.lo[b], f32x4{}, 0, 0, 0);
                 #pragma unroll
                 for (int t = 0; t < 2; t++)
-                    #pragma unroll
-                    for (int r = 0; r < R; r++) c[cur][t][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[cur][t], q[r].hi[b], c[cur][t][r], 0, 0, 0);
+                    c[cur][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[cur][t], q.hi[b], c[cur][t], 0, 0, 0);
             }
             if (b) {
                 const h8v s = __builtin_bit_cast(h8v, d[old]);
                 #pragma unroll
                 for (int t = 0; t < 2; t++)
                     #pragma unroll
-                    for (int r = 0; r < R; r++)
-                        #pragma unroll
-                        for (int e = 0; e < 4; e++) x[r][4 * t + e] = __builtin_fmaf(c[old][t][r][e], (float)s[4 * t + e], x[r][4 * t + e]);
+                    for (int e = 0; e < 4; e++) x[4 * t + e] = __builtin_fmaf(c[old][t][e], (float)s[4 * t + e], x[4 * t + e]);
             }
             if (b + 1 < HD / 32) {
                 #pragma unroll
@@ -293,25 +286,22 @@ __device__ __forceinline__ void q4_scores(float (&x)[R][8], const Q4Query<HD> (&
 
 // O += V times the weights y (at most 2^15, times inv).  vfrag(c, hi, lo): dims 16 c + lane % 16
 // at the group's 8 positions.
-template <int HD, int R, class V>
-__device__ __forceinline__ void q4_pv(const float (&y)[R][8], const float (&inv)[R], const Q4Const& kc, Q4State<HD> (&st)[R], V vfrag) {
-    h8v bh[R], bl[R];
+template <int HD, class V>
+__device__ __forceinline__ void q4_pv(const float (&y)[8], float inv, const Q4Const& kc, Q4State<HD>& st, V vfrag) {
+    h8v bh, bl;
+    u32x4v ph, pl;
     #pragma unroll
-    for (int r = 0; r < R; r++) {
-        u32x4v ph, pl;
-        #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint32_t h, l;
-            split_f16(y[r][2 * j], y[r][2 * j + 1], kc.minus_one, h, l);
-            ph[j] = h;
-            pl[j] = l;
-        }
-        bh[r] = __builtin_bit_cast(h8v, ph);
-        bl[r] = __builtin_bit_cast(h8v, pl);
+    for (int j = 0; j < 4; j++) {
+        uint32_t h, l;
+        split_f16(y[2 * j], y[2 * j + 1], kc.minus_one, h, l);
+        ph[j] = h;
+        pl[j] = l;
     }
+    bh = __builtin_bit_cast(h8v, ph);
+    bl = __builtin_bit_cast(h8v, pl);
     // two dims' products run while the next two's values are fetched (or formed), and the two before join O
     h8v v[2][2][2];
-    f32x4 d[2][2][R];
+    f32x4 d[2][2];
     #pragma unroll
     for (int i = 0; i < 2; i++) vfrag(i, v[0][i][0], v[0][i][1]);
     #pragma unroll
@@ -320,24 +310,19 @@ __device__ __forceinline__ void q4_pv(const float (&y)[R][8], const float (&inv)
         if (u < HD / 32) {
             #pragma unroll
             for (int i = 0; i < 2; i++)
-                #pragma unroll
-                for (int r = 0; r < R; r++) d[cur][i][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[cur][i][1], bh[r], f32x4{}, 0, 0, 0);
+                d[cur][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[cur][i][1], bh, f32x4{}, 0, 0, 0);
             #pragma unroll
             for (int i = 0; i < 2; i++)
-                #pragma unroll
-                for (int r = 0; r < R; r++) d[cur][i][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[cur][i][0], bl[r], d[cur][i][r], 0, 0, 0);
+                d[cur][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[cur][i][0], bl, d[cur][i], 0, 0, 0);
             #pragma unroll
             for (int i = 0; i < 2; i++)
-                #pragma unroll
-                for (int r = 0; r < R; r++) d[cur][i][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[cur][i][0], bh[r], d[cur][i][r], 0, 0, 0);
+                d[cur][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[cur][i][0], bh, d[cur][i], 0, 0, 0);
         }
         if (u)
             #pragma unroll
             for (int i = 0; i < 2; i++)
                 #pragma unroll
-                for (int r = 0; r < R; r++)
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) st[r].o[2 * u - 2 + i][e] = __builtin_fmaf(d[old][i][r][e], inv[r], st[r].o[2 * u - 2 + i][e]);
+                for (int e = 0; e < 4; e++) st.o[2 * u - 2 + i][e] = __builtin_fmaf(d[old][i][e], inv, st.o[2 * u - 2 + i][e]);
         if (u + 1 < HD / 32)
             #pragma unroll
             for (int i = 0; i < 2; i++) vfrag(2 * u + 2 + i, v[old][i][0], v[old][i][1]);
@@ -346,98 +331,86 @@ __device__ __forceinline__ void q4_pv(const float (&y)[R][8], const float (&inv)
 }
 
 // Moves the weights below 2^-20 of 2^15 to `later`, times 2^20; whether there are any.
-template <int R>
-__device__ __forceinline__ bool q4_window(float (&x)[R][8], float (&later)[R][8]) {
+__device__ __forceinline__ bool q4_window(float (&x)[8], float (&later)[8]) {
     bool any = false;
     #pragma unroll
-    for (int r = 0; r < R; r++)
-        #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const bool small = x[r][e] < 0x1p15f / (float)(1 << Q4A_WINDOW);   // (false for NaN)
-            later[r][e] = small ? x[r][e] * (float)(1 << Q4A_WINDOW) : 0.0f;
-            x[r][e] = small ? 0.0f : x[r][e];
-            any |= later[r][e] > 0.0f;
-        }
+    for (int e = 0; e < 8; e++) {
+        const bool small = x[e] < 0x1p15f / (float)(1 << Q4A_WINDOW);   // (false for NaN)
+        later[e] = small ? x[e] * (float)(1 << Q4A_WINDOW) : 0.0f;
+        x[e] = small ? 0.0f : x[e];
+        any |= later[e] > 0.0f;
+    }
     return __any(any);
 }
 
 // Scores to weights to O, for the positions from base (at: this group's first).
-template <int HD, int R, bool SC, class V>
-__device__ __forceinline__ void q4_attend(float (&x)[R][8], int base, int at, const Q4Seen (&seen)[R], const Q4Query<HD> (&q)[R],
-                                          const Q4Const& kc, Q4State<HD> (&st)[R], float* const (&score_row)[R], V vfrag) {
-    float w[R];
-    bool spread = false;
-    #pragma unroll
-    for (int r = 0; r < R; r++) {
-        float bm = -INFINITY, least = INFINITY;
-        if (base + Q4A_STEP <= seen[r].all) {
-            #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                bm = fmaxf(bm, x[r][e]);
-                least = fminf(least, x[r][e]);
-            }
-        } else {
-            #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const bool in = at + e < seen[r].end;
-                least = fminf(least, in ? x[r][e] : INFINITY);
-                x[r][e] = in ? x[r][e] : -INFINITY;
-                bm = fmaxf(bm, x[r][e]);
-            }
-        }
-        float back = q[r].back;
-        if constexpr (SC) {   // (the weights from the scores as they are kept: the sums match)
-            #pragma unroll
-            for (int e = 0; e < 8; e++) x[r][e] *= back;
-            bm *= back;
-            least *= back;
-            back = 1.0f;
-            if (score_row[r]) {   // (a row's stride is whole steps)
-                *reinterpret_cast<f32x4*>(score_row[r] + at) = f32x4{x[r][0], x[r][1], x[r][2], x[r][3]};
-                *reinterpret_cast<f32x4*>(score_row[r] + at + 4) = f32x4{x[r][4], x[r][5], x[r][6], x[r][7]};
-            }
-        }
-        bm = groups_max(bm) * back;
-        // O and l are relative to m, a multiple of 2^-14; it moves when the
-        // maximum has grown by 2^32.  The step's weights are relative to m
-        // plus a whole number, at most 2^15.
-        if (__any(bm > st[r].m + 32.0f)) {
-            const float mn = fmaxf(st[r].m, __builtin_ceilf(bm * 0x1p14f) * 0x1p-14f);
-            const float corr = st[r].m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st[r].m - mn);
-            st[r].m = mn;
-            st[r].l *= corr;
-            #pragma unroll
-            for (int c = 0; c < HD / 16; c++) st[r].o[c] *= corr;
-        }
-        const bool none = bm == -INFINITY;   // a row that sees no position of the step
-        const float k = none ? 0.0f : __builtin_ceilf(bm - st[r].m) - 15.0f;
-        const float ref = none ? 0.0f : st[r].m + k;
-        w[r] = none ? 0.0f : __builtin_amdgcn_exp2f(k);
+template <int HD, bool SC, class V>
+__device__ __forceinline__ void q4_attend(float (&x)[8], int base, int at, const Q4Seen& seen, const Q4Query<HD>& q,
+                                          const Q4Const& kc, Q4State<HD>& st, float* score_row, V vfrag) {
+    float bm = -INFINITY, least = INFINITY;
+    if (base + Q4A_STEP <= seen.all) {
         #pragma unroll
-        for (int e = 0; e < 8; e++) x[r][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r][e], back, -ref));
-        st[r].l = __builtin_fmaf(((x[r][0] + x[r][1]) + (x[r][2] + x[r][3])) + ((x[r][4] + x[r][5]) + (x[r][6] + x[r][7])), w[r], st[r].l);
-        spread |= least * back < ref + (15.0f - Q4A_WINDOW);
+        for (int e = 0; e < 8; e++) {
+            bm = fmaxf(bm, x[e]);
+            least = fminf(least, x[e]);
+        }
+    } else {
+        #pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const bool in = at + e < seen.end;
+            least = fminf(least, in ? x[e] : INFINITY);
+            x[e] = in ? x[e] : -INFINITY;
+            bm = fmaxf(bm, x[e]);
+        }
     }
+    float back = q.back;
+    if constexpr (SC) {   // (the weights from the scores as they are kept: the sums match)
+        #pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= back;
+        bm *= back;
+        least *= back;
+        back = 1.0f;
+        if (score_row) {   // (a row's stride is whole steps)
+            *reinterpret_cast<f32x4*>(score_row + at) = f32x4{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<f32x4*>(score_row + at + 4) = f32x4{x[4], x[5], x[6], x[7]};
+        }
+    }
+    bm = groups_max(bm) * back;
+    // O and l are relative to m, a multiple of 2^-14; it moves when the
+    // maximum has grown by 2^32.  The step's weights are relative to m
+    // plus a whole number, at most 2^15.
+    if (__any(bm > st.m + 32.0f)) {
+        const float mn = fmaxf(st.m, __builtin_ceilf(bm * 0x1p14f) * 0x1p-14f);
+        const float corr = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - mn);
+        st.m = mn;
+        st.l *= corr;
+        #pragma unroll
+        for (int c = 0; c < HD / 16; c++) st.o[c] *= corr;
+    }
+    const bool none = bm == -INFINITY;   // a row that sees no position of the step
+    const float k = none ? 0.0f : __builtin_ceilf(bm - st.m) - 15.0f;
+    const float ref = none ? 0.0f : st.m + k;
+    float w = none ? 0.0f : __builtin_amdgcn_exp2f(k);
+    #pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], back, -ref));
+    st.l = __builtin_fmaf(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])), w, st.l);
+    const bool spread = least * back < ref + (15.0f - Q4A_WINDOW);
     // weights that span more than f16 pairs hold are taken in windows of
     // 2^20, each scaled by itself
-    float later[R][8];
+    float later[8];
     bool more = __any(spread);
     if (more) more = q4_window(x, later);
     for (;;) {
         q4_pv<HD>(x, w, kc, st, vfrag);
         if (!more) break;
+        w *= 1.0f / (float)(1 << Q4A_WINDOW);
         #pragma unroll
-        for (int r = 0; r < R; r++) {
-            w[r] *= 1.0f / (float)(1 << Q4A_WINDOW);
-            #pragma unroll
-            for (int e = 0; e < 8; e++) x[r][e] = later[r][e];
-        }
+        for (int e = 0; e < 8; e++) x[e] = later[e];
         more = q4_window(x, later);
     }
 }
 
-// The lane's row of a row tile (of R tiles' rows from r0; the last row again
-// where there are no more).
+// The lane's row of a row tile (the last row again where there are no more).
 struct Q4Row {
     int i, h;     // query, query head
     bool ok;

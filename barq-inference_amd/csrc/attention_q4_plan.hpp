@@ -8,7 +8,12 @@ namespace barq {
 constexpr int Q4P_NW = 4;               // waves of a workgroup of attn_q4_prompt_kernel
 constexpr int Q4P_ROWS = 16 * Q4P_NW;   // its query rows
 
-constexpr int Q4P_MIN_ROWS = 64;
+// Rows of a kv head from which it is used (64 and 128 dims).  us, attn_q4_kernel
+// / this one, with the merge: 32/8 heads of 128, 16 / 24 / 32 rows (64 / 96 / 128 of a
+// kv head) after 1000 10.9 / 13.5, 13.6 / 14.0, 17.0 / 15.0, after 8000 23 / 23,
+// 26 / 29, 31 / 31, from position 0 7.8 / 6.5 each; of 64, 16 / 24 rows after 1000
+// 8.8 / 10.5, 9.6 / 10.8.
+constexpr int Q4P_MIN_ROWS = 128;
 
 struct Q4Plan {
     bool prompt;     // attn_q4_prompt_kernel

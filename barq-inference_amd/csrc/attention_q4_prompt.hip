@@ -102,7 +102,6 @@ template <int HD, bool PART, bool SC>
 __global__ __launch_bounds__(64 * Q4P_NW, 3)
 void attn_q4_prompt_kernel(Q4Args a) {
     using B = Q4Block<HD>;
-    constexpr int R = 1;
     __shared__ __align__(16) uint8_t lds[2 * B::STAGE];
     __shared__ int nan_at[B::NB];
     const int t = threadIdx.x, l = t & 63, c = l & 15, g = l >> 4;
@@ -112,8 +111,8 @@ void attn_q4_prompt_kernel(Q4Args a) {
     const int hk = (int)((long long)(grp * a.G) * a.n_head_kv / a.n_head);
     const int visible = q4_vis(a, tile * Q4P_ROWS + Q4P_ROWS - 1);
     const int start = split * a.chunk, j0 = min(start, visible), j1 = min(visible, start + a.chunk);
-    const int r0 = tile * Q4P_ROWS + wave * Q4A_ROWS * R;
-    const int mine = r0 < rows_n ? min(j1, q4_vis(a, r0 + Q4A_ROWS * R - 1)) : 0;   // the wave's rows see no more
+    const int r0 = tile * Q4P_ROWS + wave * Q4A_ROWS;
+    const int mine = r0 < rows_n ? min(j1, q4_vis(a, r0 + Q4A_ROWS - 1)) : 0;   // the wave's rows see no more
 
     B blk;
     blk.init(a.kv, hk, start, max(j1, start), l, wave);
@@ -121,22 +120,13 @@ void attn_q4_prompt_kernel(Q4Args a) {
     if (n > 0) blk.load(0);
     if (t < B::NB) nan_at[t] = 0x7FFFFFFF;
     const Q4Const kx;
-    Q4Row row[R];
-    Q4Seen seen[R];
-    Q4Query<HD> q[R];
-    Q4State<HD> st[R];
-    float* score_row[R];
-    bool exact = false;
-    #pragma unroll
-    for (int r = 0; r < R; r++) {
-        row[r] = q4_row(a, grp, r0 + Q4A_ROWS * r + c);
-        seen[r].end = min(row[r].vis, j1);
-        seen[r].all = min(q4_vis(a, r0 + Q4A_ROWS * r), j1);
-        exact |= q[r].load(a.q + ((size_t)row[r].h * a.q_rows + row[r].i) * HD, a.scale, g, kx);
-        score_row[r] = SC && row[r].ok ? a.scores + ((size_t)row[r].i * a.n_head + row[r].h) * a.score_stride : nullptr;
-        st[r].clear();
-    }
-    exact = __any(exact);
+    const Q4Row row = q4_row(a, grp, r0 + c);
+    const Q4Seen seen{min(row.vis, j1), min(q4_vis(a, r0), j1)};
+    Q4Query<HD> q;
+    const bool exact = __any(q.load(a.q + ((size_t)row.h * a.q_rows + row.i) * HD, a.scale, g, kx));
+    float* const score_row = SC && row.ok ? a.scores + ((size_t)row.i * a.n_head + row.h) * a.score_stride : nullptr;
+    Q4State<HD> st;
+    st.clear();
     __syncthreads();   // nan_at
     if (n > 0) blk.convert(lds, j0, j1, kx, nan_at);
     if (n > 1) blk.load(Q4A_STEP);
@@ -147,22 +137,19 @@ void attn_q4_prompt_kernel(Q4Args a) {
         const int base = j0 + b * Q4A_STEP;
         if (base >= mine) continue;
         const uint8_t* s = lds + (b & 1) * B::STAGE;
-        float x[R][8];
+        float x[8];
         q4_scores<HD>(x, q, exact,
                       [&](int t, int b, bool) { return *reinterpret_cast<const h8v*>(s + 1024 * (t * B::NB + b) + 16 * l); },
                       [&](int b) { return *reinterpret_cast<const u32x4v*>(s + B::KS + 16 * (g * B::NB + b)); });
-        q4_attend<HD, R, SC>(x, base, base + 8 * g, seen, q, kx, st, score_row, [&](int c, h8v& hi, h8v& lo) {
+        q4_attend<HD, SC>(x, base, base + 8 * g, seen, q, kx, st, score_row, [&](int c, h8v& hi, h8v& lo) {
             hi = *reinterpret_cast<const h8v*>(s + B::V + 2048 * c + 16 * l);
             lo = *reinterpret_cast<const h8v*>(s + B::V + 2048 * c + 1024 + 16 * l);
         });
     }
     __syncthreads();   // nan_at
-    #pragma unroll
-    for (int r = 0; r < R; r++) {
-        st[r].put_nan(nan_at, seen[r].end);
-        const float lsum = groups_sum(st[r].l);
-        if (row[r].ok) q4_store<HD, PART>(a, row[r], split, g, st[r], lsum);
-    }
+    st.put_nan(nan_at, seen.end);
+    const float lsum = groups_sum(st.l);
+    if (row.ok) q4_store<HD, PART>(a, row, split, g, st, lsum);
 }
 
 template <int HD>

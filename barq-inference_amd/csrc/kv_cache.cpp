@@ -210,7 +210,10 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
     const size_t nq = n_head * q_len * head_dim, out_row = q8 ? n_head * head_dim / 256 * 292 : n_head * head_dim * 4;
     Arena a;
     const size_t os = a.add(rows * per_row), op = a.add(part), ost = a.add(n_head * rows * sizeof(float2));
-    const size_t osum = a.add(barq::attention_mass_sums(n_head, n_head_kv, rows, stride));
+    size_t sums = barq::attention_mass_sums(n_head, n_head_kv, rows, stride);
+    if (last && barq::attention_mass_sums(n_head, n_head_kv, last, stride) > sums)   // (shorter runs may be more)
+        sums = barq::attention_mass_sums(n_head, n_head_kv, last, stride);
+    const size_t osum = a.add(sums);
     const size_t oq = host ? a.add(nq * 4) : 0, oo = host ? a.add(q_len * out_row) : 0;
     const size_t om = host ? a.add(n_head_kv * kv_len * sizeof(float)) : 0;
     BARQ_CHECK(ensure_ws(h, a.used));

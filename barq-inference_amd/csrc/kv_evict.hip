@@ -11,9 +11,10 @@
 // far, until all keys that share them are wanted; then it numbers the kept
 // positions by a running count.  The histogram has eight columns, since masses
 // share their leading bits and lanes adding to one counter take turns.  Up to
-// 32 masses a thread stay in registers over the passes; longer heads are read
-// again by each (from the L2).  One workgroup's latencies bound it: 16384
-// positions take hardly longer than 4097.
+// 16 masses a thread stay in registers over the passes; longer heads are read
+// again by each (from the L2).  One workgroup's latencies bound it (the load, up to three
+// passes of four barriers, the numbering): 14.9 us for 4097 and for 16384 positions of 8
+// heads, 0.7 MB.
 //
 // The rows then move in one launch, bound by memory: f32 rows as they are;
 // of a 4-bit cache, whose tiles hold 8 positions of V in one dword per dim, a
@@ -73,7 +74,7 @@ __device__ __forceinline__ uint32_t waves_before(const uint32_t* part, int w, ui
     return before;
 }
 
-// R: chunks whose masses stay in registers (n <= R * EV_CHUNK), or 0.
+// R: chunks whose masses (and keys) stay in registers (n <= R * EV_CHUNK), or 0.
 template <int R>
 __global__ __launch_bounds__(EV_NT)
 void evict_select_kernel(EvictArgs a) {
@@ -98,14 +99,11 @@ void evict_select_kernel(EvictArgs a) {
             for (int u = 0; u < 4; u++) x[u] = j + u < a.n ? in[j + u] : 0.0f;
         }
     };
-    constexpr bool KEYS = R > 0 && R <= 4;   // their keys stay in registers too
     float reg[R ? R : 1][4];
-    uint32_t keys[KEYS ? R : 1][4];
+    uint32_t keys[R ? R : 1][4];
     if constexpr (R > 0) {
         #pragma unroll
         for (int c = 0; c < R; c++) load(c, reg[c]);
-    }
-    if constexpr (KEYS) {
         #pragma unroll
         for (int c = 0; c < R; c++)
             #pragma unroll
@@ -113,17 +111,10 @@ void evict_select_kernel(EvictArgs a) {
     }
     // f(chunk, its four masses, their keys): every chunk, in order
     auto each = [&](auto f) {
-        if constexpr (KEYS) {
+        if constexpr (R > 0) {
             #pragma unroll
             for (int c = 0; c < R; c++)
                 if (c < chunks) f(c, reg[c], keys[c]);
-        } else if constexpr (R > 0) {
-            #pragma unroll
-            for (int c = 0; c < R; c++)
-                if (c < chunks) {
-                    const uint32_t k[4] = {ev_key(reg[c][0]), ev_key(reg[c][1]), ev_key(reg[c][2]), ev_key(reg[c][3])};
-                    f(c, reg[c], k);
-                }
         } else {
             float x[4];
             for (int c = 0; c < chunks; c++) {
@@ -249,11 +240,11 @@ void evict_select_kernel(EvictArgs a) {
 hipError_t evict_select_launch(const float* mass_in, float* mass_out, size_t stride, size_t n_kv, size_t n, size_t m,
                                size_t recent, int32_t* kept, hipStream_t s) {
     EvictArgs a{mass_in, mass_out, stride, (int)n, (int)m, (int)(recent < n ? recent : n), kept};
-    const size_t chunks = (n + EV_CHUNK - 1) / EV_CHUNK;
     const dim3 grid((unsigned)n_kv), block(EV_NT);
-    if (chunks <= 1) hipLaunchKernelGGL(evict_select_kernel<1>, grid, block, 0, s, a);
-    else if (chunks <= 4) hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, s, a);
-    else if (chunks <= 8) hipLaunchKernelGGL(evict_select_kernel<8>, grid, block, 0, s, a);
+    // in registers / read again, us with the gather of 64 rows: 16384 positions
+    // 18.8 / 20.6, 4097 19.1 / 19.0; 32 masses a thread instead of 16 27.3, and
+    // 28.3 / 23.2 for 16385
+    if (n <= 4 * EV_CHUNK) hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, s, a);
     else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, s, a);
     return hipGetLastError();
 }
