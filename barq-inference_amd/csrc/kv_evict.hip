@@ -9,16 +9,21 @@
 // mass as an unsigned integer of the same order) 11 bits at a time from the
 // top, each time with a histogram of the keys that share the bits found so
 // far, until all keys that share them are wanted; then it numbers the kept
-// positions by a running count.  The histogram has eight columns, since masses
+// positions by a running count.  The histogram has four columns, since masses
 // share their leading bits and lanes adding to one counter take turns.  Up to
-// 16 masses a thread stay in registers over the passes; longer heads are read
-// again by each (from the L2).  One workgroup's latencies bound it (the load, up to three
-// passes of four barriers, the numbering): 14.9 us for 4097 and for 16384 positions of 8
-// heads, 0.7 MB.
+// 16384 masses stay in LDS (and their keys in registers) over the passes, and the kept
+// positions go through a list there, so that they leave by whole lines; longer
+// heads are read again by each pass (from the L2).  One workgroup's latencies bound
+// it, 14.5 us for 16384 positions: the load takes 3500 cycles, a pass 4000 to
+// 6000.  Stores from where a thread finds a position, without the list, took
+// 14400, and the zeros behind the kept masses, one a thread at a time, 4800.
 //
-// The rows then move in one launch, bound by memory: f32 rows as they are;
-// of a 4-bit cache, whose tiles hold 8 positions of V in one dword per dim, a
-// thread builds the dwords of a tile's dims from those of its 8 sources.
+// The rows then move in one launch, bound by memory: f32 rows as they are (2048
+// of 8 heads of 128 dims 6.6 us, 33.6 MB at 5.1 TB/s); of a 4-bit cache, whose
+// tiles hold 8 positions of V in one dword per dim, a thread builds the dwords of
+// a tile's dims from those of its 8 sources, which reads V's codes up to eight
+// times (4096 of 16384 positions 8.1 us, 9.4 MB and the rest of the tiles' lines).  In place they go
+// by way of the workspace (5.4 us back): a row may move onto one that is still to be read.
 #include "common.hpp"
 #include "kv_q4.hpp"
 #include "launch.hpp"
@@ -27,7 +32,9 @@ namespace barq {
 
 constexpr int EV_NT = 1024;
 constexpr int EV_DIGITS = 2 * EV_NT;
+constexpr int EV_COLS = 4;
 constexpr int EV_CHUNK = 4 * EV_NT;   // keys of a pass over the workgroup, four in a row per thread
+constexpr int EV_KEEP = 4 * EV_CHUNK;   // masses that stay in LDS
 
 struct EvictArgs {
     const float* mass_in;
@@ -57,107 +64,109 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v, uint32_t& total) {
     return (uint32_t)s - v;
 }
 
-// Sum of part[0 .. w), and of all 16.
+// Sum of part[0 .. w), and of all 16 (w: the same in every lane).
 __device__ __forceinline__ uint32_t waves_before(const uint32_t* part, int w, uint32_t& total) {
-    uint32_t before = 0;
-    total = 0;
-    #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-        const uint4 p = *reinterpret_cast<const uint4*>(part + i);
-        const uint32_t q[4] = {p.x, p.y, p.z, p.w};
-        #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            before += i + u < w ? q[u] : 0u;
-            total += q[u];
-        }
-    }
-    return before;
+    const int l = threadIdx.x & 63;
+    const uint32_t before = wave_scan(l < EV_NT / 64 ? part[l] : 0u, total);
+    return (uint32_t)__builtin_amdgcn_readlane((int)before, w);
 }
 
-// R: chunks whose masses (and keys) stay in registers (n <= R * EV_CHUNK), or 0.
-template <int R>
+// LDS: the masses stay there, and their keys in registers (n <= EV_KEEP).
+template <bool LDS>
 __global__ __launch_bounds__(EV_NT)
 void evict_select_kernel(EvictArgs a) {
-    __shared__ __align__(16) uint32_t hist[EV_DIGITS][8];
-    __shared__ __align__(16) uint32_t part[R ? R : 1][EV_NT / 64];
-    static_assert(EV_NT == 1024, "16 waves, two digits a thread");
+    static_assert(EV_NT == 1024 && EV_DIGITS == 2 * EV_NT, "16 waves, two digits a thread");
+    __shared__ __align__(16) uint32_t hist[EV_COLS][EV_DIGITS + 8];   // (a digit's columns on distinct banks)
+    __shared__ __align__(16) float4 kept_in[LDS ? EV_KEEP / 4 : 1];
+    __shared__ uint32_t part[EV_NT / 64];
     __shared__ uint32_t found[3];   // the digit, what is left to find within it, its keys
-    const int t = threadIdx.x, l = t & 63, w = t >> 6, h = blockIdx.x;
+    const int t = threadIdx.x, l = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), h = blockIdx.x;
     const float* in = a.mass_in + (size_t)h * a.stride;
     float* out = a.mass_out ? a.mass_out + (size_t)h * a.stride : nullptr;
     int32_t* kept = a.kept + (size_t)h * a.m;
     const int old = a.n - a.recent, want = a.m - a.recent, chunks = (a.n + EV_CHUNK - 1) / EV_CHUNK;
 
+    // masses 4 q .. 4 q + 3, 0 behind the last
     typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-    auto load = [&](int c, float (&x)[4]) {
-        const int j = c * EV_CHUNK + 4 * t;
-        if (j + 4 <= a.n) {
-            const f32x4u v = *reinterpret_cast<const f32x4u*>(in + j);
-            x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    const auto load = [&](int q) {
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (4 * q + 4 <= a.n) {
+            const f32x4u v = *reinterpret_cast<const f32x4u*>(in + 4 * q);
+            x = make_float4(v.x, v.y, v.z, v.w);
         } else {
-            #pragma unroll
-            for (int u = 0; u < 4; u++) x[u] = j + u < a.n ? in[j + u] : 0.0f;
+            if (4 * q < a.n) x.x = in[4 * q];
+            if (4 * q + 1 < a.n) x.y = in[4 * q + 1];
+            if (4 * q + 2 < a.n) x.z = in[4 * q + 2];
         }
+        return x;
     };
-    float reg[R ? R : 1][4];
-    uint32_t keys[R ? R : 1][4];
-    if constexpr (R > 0) {
+    // their place in LDS: threads that read four such in a row each do so from distinct banks
+    const auto place = [](int q) { return q ^ ((q >> 4) & 3); };
+    constexpr int CHUNKS = LDS ? EV_KEEP / EV_CHUNK : 1;
+    uint32_t keys[CHUNKS][4];
+    if constexpr (LDS) {
+        float4 x[CHUNKS];
         #pragma unroll
-        for (int c = 0; c < R; c++) load(c, reg[c]);
+        for (int c = 0; c < CHUNKS; c++) x[c] = load(c * EV_NT + t);   // (all on their way at once)
         #pragma unroll
-        for (int c = 0; c < R; c++)
-            #pragma unroll
-            for (int u = 0; u < 4; u++) keys[c][u] = ev_key(reg[c][u]);
+        for (int c = 0; c < CHUNKS; c++) {
+            kept_in[place(c * EV_NT + t)] = x[c];
+            keys[c][0] = ev_key(x[c].x);
+            keys[c][1] = ev_key(x[c].y);
+            keys[c][2] = ev_key(x[c].z);
+            keys[c][3] = ev_key(x[c].w);
+        }
     }
-    // f(chunk, its four masses, their keys): every chunk, in order
-    auto each = [&](auto f) {
-        if constexpr (R > 0) {
-            #pragma unroll
-            for (int c = 0; c < R; c++)
-                if (c < chunks) f(c, reg[c], keys[c]);
-        } else {
-            float x[4];
-            for (int c = 0; c < chunks; c++) {
-                load(c, x);
-                const uint32_t k[4] = {ev_key(x[0]), ev_key(x[1]), ev_key(x[2]), ev_key(x[3])};
-                f(c, x, k);
-            }
-        }
-    };
 
     // the want-th largest key among the old positions, in the bits of mask: all
     // keys above it there are kept, and `ties` of those equal to it
     uint32_t key = 0, mask = 0, ties = 0;
     const bool some = want > 0 && want < old;
+    // a thread's two digits, 2 t from the top
+    const int digit = EV_DIGITS - 2 - 2 * t;
+    #pragma unroll
+    for (int u = 0; u < EV_COLS; u++) *reinterpret_cast<uint2*>(&hist[u][digit]) = make_uint2(0, 0);
+    __syncthreads();
     if (some) {
         ties = (uint32_t)want;
         for (int shift = 21; mask != 0xFFFFFFFFu; shift = shift > 11 ? shift - 11 : 0) {
-            for (int i = t; i < EV_DIGITS * 2; i += EV_NT) reinterpret_cast<uint4*>(&hist[0][0])[i] = make_uint4(0, 0, 0, 0);
-            __syncthreads();
             const uint32_t digits = shift ? 2047u : 1023u;   // 11, 11 and 10 bits
-            each([&](int c, const float (&x)[4], const uint32_t (&k)[4]) {
+            const auto add = [&](int c, const uint32_t (&k)[4]) {
                 #pragma unroll
                 for (int u = 0; u < 4; u++)
-                    if (c * EV_CHUNK + 4 * t + u < old && (k[u] & mask) == key) atomicAdd(&hist[(k[u] >> shift) & digits][t & 7], 1u);
-            });
+                    if (c * EV_CHUNK + 4 * t + u < old && (k[u] & mask) == key)
+                        atomicAdd(&hist[t % EV_COLS][(k[u] >> shift) & digits], 1u);
+            };
+            if constexpr (LDS) {
+                #pragma unroll
+                for (int c = 0; c < CHUNKS; c++)
+                    if (c < chunks) add(c, keys[c]);
+            } else {
+                for (int c = 0; c < chunks; c++) {
+                    const float4 x = load(c * EV_NT + t);
+                    const uint32_t k[4] = {ev_key(x.x), ev_key(x.y), ev_key(x.z), ev_key(x.w)};
+                    add(c, k);
+                }
+            }
             __syncthreads();
-            // a thread's two digits, and those above them
-            const int digit = EV_DIGITS - 1 - 2 * t;
-            uint32_t s[2];
+            // the thread's two digits, and those above them
+            uint32_t s[2] = {0, 0};
             #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint4 p = *reinterpret_cast<const uint4*>(&hist[digit - i][0]), q = *reinterpret_cast<const uint4*>(&hist[digit - i][4]);
-                s[i] = ((p.x + p.y) + (p.z + p.w)) + ((q.x + q.y) + (q.z + q.w));
+            for (int u = 0; u < EV_COLS; u++) {
+                uint2& p = *reinterpret_cast<uint2*>(&hist[u][digit]);
+                s[0] += p.y;
+                s[1] += p.x;
+                p = make_uint2(0, 0);   // (for the next pass)
             }
             uint32_t all;
             const uint32_t before = wave_scan(s[0] + s[1], all);
-            if (l == 0) part[0][w] = all;
+            if (l == 0) part[w] = all;
             __syncthreads();
-            uint32_t above = before + waves_before(part[0], w, all);
+            uint32_t above = before + waves_before(part, w, all);
             #pragma unroll
             for (int i = 0; i < 2; i++) {
                 if (above < ties && ties <= above + s[i]) {
-                    found[0] = (uint32_t)(digit - i);
+                    found[0] = (uint32_t)(digit + 1 - i);
                     found[1] = ties - above;
                     found[2] = s[i];
                 }
@@ -172,80 +181,107 @@ void evict_select_kernel(EvictArgs a) {
     }
 
     // numbering: of each position the kept ones before it; larger keys and
-    // keys equal to the last one counted side by side (16 bits each a chunk)
+    // keys equal to the last one counted side by side (16 bits each a stretch)
     const auto flag = [&](int j, float x) {
         const uint32_t k = ev_key(x) & mask;
         const bool gt = (j >= old && j < a.n) || (j < old && (some ? k > key : want > 0));
         return gt ? 1u : some && j < old && k == key ? 0x10000u : 0u;
     };
-    const auto put = [&](int c, const float (&x)[4], uint32_t gt, uint32_t eq) {
-        #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const uint32_t f = flag(c * EV_CHUNK + 4 * t + u, x[u]);
-            if (f == 1u || (f && eq < ties)) {
-                const uint32_t at = gt + (eq < ties ? eq : ties);
-                kept[at] = c * EV_CHUNK + 4 * t + u;
-                if (out) out[at] = x[u];
+    if constexpr (LDS) {
+        // a stretch of 4 * chunks positions for each thread, as bits
+        uint32_t gt = 0, eq = 0;
+        for (int c = 0; c < chunks; c++) {
+            const float4 x = kept_in[place(t * chunks + c)];
+            const float v[4] = {x.x, x.y, x.z, x.w};
+            #pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const uint32_t f = flag(4 * (t * chunks + c) + u, v[u]);
+                gt |= (f & 1u) << (4 * c + u);
+                eq |= (f >> 16) << (4 * c + u);
             }
-            gt += f & 0xFFFFu;
-            eq += f >> 16;
         }
-    };
-    const auto count = [&](int c, const float (&x)[4]) {
-        uint32_t n = 0;
-        #pragma unroll
-        for (int u = 0; u < 4; u++) n += flag(c * EV_CHUNK + 4 * t + u, x[u]);
-        return n;
-    };
-    if constexpr (R > 0) {   // all chunks' counts at once
-        uint32_t before[R];
-        #pragma unroll
-        for (int c = 0; c < R; c++) {
-            uint32_t all;
-            before[c] = wave_scan(count(c, reg[c]), all);
-            if (l == 0) part[c][w] = all;
-        }
-        __syncthreads();   // (and, in place, the masses are read by all)
-        uint32_t gt0 = 0, eq0 = 0;
-        #pragma unroll
-        for (int c = 0; c < R; c++)
-            if (c < chunks) {
-                uint32_t sum;
-                const uint32_t b = before[c] + waves_before(part[c], w, sum);
-                put(c, reg[c], gt0 + (b & 0xFFFFu), eq0 + (b >> 16));
-                gt0 += sum & 0xFFFFu;
-                eq0 += sum >> 16;
+        uint32_t all, sum;
+        const uint32_t before = wave_scan(__builtin_popcount(gt) | __builtin_popcount(eq) << 16, all);
+        if (l == 0) part[w] = all;
+        __syncthreads();   // (every mass is in LDS: in place they are overwritten from here on; hist is free)
+        const uint32_t b = before + waves_before(part, w, sum), eq_at = b >> 16;
+        uint32_t at = (b & 0xFFFFu) + (eq_at < ties ? eq_at : ties);
+        // of the equal ones the first ties - eq_at
+        uint32_t bits = gt, left = eq_at < ties ? ties - eq_at : 0;
+        if (left >= (uint32_t)__builtin_popcount(eq)) bits |= eq;
+        else
+            for (; left; left--, eq &= eq - 1) bits |= eq & -eq;
+        uint16_t* list = reinterpret_cast<uint16_t*>(&hist[0][0]);   // the kept positions, in order
+        static_assert(sizeof(hist) >= EV_KEEP * sizeof(uint16_t) && EV_KEEP <= 65536, "room for all");
+        for (; bits; bits &= bits - 1) list[at++] = (uint16_t)(4 * t * chunks + __builtin_ctz(bits));
+        __syncthreads();
+        typedef int i32x4u __attribute__((ext_vector_type(4), aligned(4)));
+        const float* vals = reinterpret_cast<const float*>(kept_in);
+        const auto mass = [&](int j) { return vals[4 * place(j >> 2) + (j & 3)]; };
+        for (int j = 4 * t; j < a.n; j += EV_CHUNK) {
+            int p[4];
+            float x[4];
+            const uint2 four = *reinterpret_cast<const uint2*>(list + j);   // (behind the last: anything)
+            #pragma unroll
+            for (int u = 0; u < 4; u++) {
+                p[u] = (int)((u < 2 ? four.x : four.y) >> (16 * (u & 1)) & 0xFFFFu);
+                x[u] = j + u < a.m ? mass(p[u]) : 0.0f;
             }
+            if (j + 4 <= a.m) *reinterpret_cast<i32x4u*>(kept + j) = i32x4u{p[0], p[1], p[2], p[3]};
+            else
+                #pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (j + u < a.m) kept[j + u] = p[u];
+            if (!out) continue;
+            if (j + 4 <= a.n) *reinterpret_cast<f32x4u*>(out + j) = f32x4u{x[0], x[1], x[2], x[3]};
+            else
+                #pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (j + u < a.n) out[j + u] = x[u];
+        }
     } else {
         uint32_t gt0 = 0, eq0 = 0;
-        float x[4];
         for (int c = 0; c < chunks; c++) {
-            load(c, x);
+            const int q = c * EV_NT + t;
+            const float4 x = load(q);
+            const float v[4] = {x.x, x.y, x.z, x.w};
+            uint32_t f[4], n = 0;
+            #pragma unroll
+            for (int u = 0; u < 4; u++) n += f[u] = flag(4 * q + u, v[u]);
             uint32_t all, sum;
-            uint32_t b = wave_scan(count(c, x), all);
+            uint32_t b = wave_scan(n, all);
             __syncthreads();   // part is free (and, in place, this chunk's masses are read by all)
-            if (l == 0) part[0][w] = all;
+            if (l == 0) part[w] = all;
             __syncthreads();
-            b += waves_before(part[0], w, sum);
-            put(c, x, gt0 + (b & 0xFFFFu), eq0 + (b >> 16));
+            b += waves_before(part, w, sum);
+            uint32_t gt = gt0 + (b & 0xFFFFu), eq = eq0 + (b >> 16);
+            #pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (f[u] == 1u || (f[u] && eq < ties)) {
+                    const uint32_t at = gt + (eq < ties ? eq : ties);
+                    kept[at] = 4 * q + u;
+                    if (out) out[at] = v[u];
+                }
+                gt += f[u] & 0xFFFFu;
+                eq += f[u] >> 16;
+            }
             gt0 += sum & 0xFFFFu;
             eq0 += sum >> 16;
         }
+        __syncthreads();   // in place: the tail is read
+        if (out)
+            for (int j = a.m + t; j < a.n; j += EV_NT) out[j] = 0.0f;
     }
-    __syncthreads();   // in place: the tail is read
-    if (out)
-        for (int j = a.m + t; j < a.n; j += EV_NT) out[j] = 0.0f;
 }
 
 hipError_t evict_select_launch(const float* mass_in, float* mass_out, size_t stride, size_t n_kv, size_t n, size_t m,
                                size_t recent, int32_t* kept, hipStream_t s) {
     EvictArgs a{mass_in, mass_out, stride, (int)n, (int)m, (int)(recent < n ? recent : n), kept};
     const dim3 grid((unsigned)n_kv), block(EV_NT);
-    // in registers / read again, us with the gather of 64 rows: 16384 positions
-    // 18.8 / 20.6, 4097 19.1 / 19.0; 32 masses a thread instead of 16 27.3, and
-    // 28.3 / 23.2 for 16385
-    if (n <= 4 * EV_CHUNK) hipLaunchKernelGGL(evict_select_kernel<4>, grid, block, 0, s, a);
-    else hipLaunchKernelGGL(evict_select_kernel<0>, grid, block, 0, s, a);
+    // kept in LDS / read again, us, 8 heads cut to a quarter: 1000 positions 7.5 /
+    // 6.5, 4097 9.0 / 9.1, 16384 14.5 / 17.7 (16385 19.6, 32768 29.0)
+    if (n > (size_t)EV_CHUNK && n <= (size_t)EV_KEEP) hipLaunchKernelGGL(evict_select_kernel<true>, grid, block, 0, s, a);
+    else hipLaunchKernelGGL(evict_select_kernel<false>, grid, block, 0, s, a);
     return hipGetLastError();
 }
 

@@ -49,7 +49,8 @@ def check(c, layer, k, v, kept):
 @pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
 @pytest.mark.parametrize("kind", ["spread", "ties", "zero", "odd"])
 @pytest.mark.parametrize("n,keep,recent", [(1, 1, 0), (9, 4, 0), (100, 37, 5), (64, 64, 3), (50, 70, 60), (200, 13, 13),
-                                           (4096, 2000, 100), (4097, 1, 0), (5000, 4999, 1)])
+                                           (4096, 2000, 100), (4097, 1, 0), (5000, 4999, 1),
+                                           (12001, 6000, 77), (16383, 16000, 0), (16384, 3, 2)])
 def test_evict_in_place(be, type_, kind, n, keep, recent):
     n_kv, hd = 3, 64
     c, (k, v) = fill(be, type_, n_kv, n, hd)
