@@ -26,6 +26,16 @@ def _empty(shape, like, mem, dtype="float32"):
     return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
 
 
+def _check_mass(who, n_head_kv, *arrays):
+    """f32 rows of one length, [n_head_kv, positions], side by side in memory."""
+    for m in arrays:
+        if len(m.shape) != 2 or m.shape[0] != n_head_kv or m.shape[1] != arrays[0].shape[1]:
+            raise L.BarqError(L.E_DIM, f"{who}: mass must be [{n_head_kv}, positions]")
+        flat = m.flags.c_contiguous if isinstance(m, np.ndarray) else m.is_contiguous()
+        if not flat or not str(m.dtype).endswith("float32"):
+            raise L.BarqError(L.E_INVALID, f"{who}: mass must be contiguous float32")
+
+
 def apply_rope(be: Backend, x, seq_len, n_heads, head_dim, start_pos, rope_freq_scale, rope_inv_freq, layout,
                mem=L.MEM_DEVICE, sync=True):
     """apply_rope (transformer.rs:514-562): x [seq, n_heads*head_dim] -> [n_heads, seq, head_dim]."""
@@ -147,8 +157,7 @@ class KVCache:
         mass_out)."""
         dst = self if dst is None else dst
         mass_out = mass if mass_out is None else mass_out
-        if len(mass.shape) != 2 or mass.shape[0] != self.n_head_kv or tuple(mass_out.shape) != tuple(mass.shape):
-            raise L.BarqError(L.E_DIM, f"evict: mass must be [{self.n_head_kv}, positions]")
+        _check_mass("evict", self.n_head_kv, mass, mass_out)
         m = min(keep, self.layer_len(layer))
         kept = _empty((self.n_head_kv, m), mass, mem, dtype="int32") if want_kept else None
         L.check(self.be._lib.barq_rocm_kv_cache_evict(self.be.h, self.c, dst.c, layer, _ptr(mass), _ptr(mass_out),
@@ -224,9 +233,7 @@ def compute_attention_mass(be: Backend, q, cache: KVCache, layer, n_head, n_head
     compute_attention_q8k's rows."""
     if mass_out is None:
         mass_out = _empty((n_head_kv, kv_len), q, mem) if mass is None else mass
-    for m in (mass, mass_out):
-        if m is not None and (len(m.shape) != 2 or m.shape[0] != n_head_kv or m.shape[1] != mass_out.shape[1]):
-            raise L.BarqError(L.E_DIM, f"attention_mass: mass must be [{n_head_kv}, positions]")
+    _check_mass("attention_mass", n_head_kv, mass_out, *([] if mass is None else [mass]))
     if out is None:
         out = (_empty((q_len, n_head, head_dim), q, mem) if out_type == L.F32
                else _empty((q_len, n_head * head_dim // 256 * 292), q, mem, dtype="uint8"))

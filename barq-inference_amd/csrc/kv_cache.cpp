@@ -87,7 +87,8 @@ int barq_rocm_kv_cache_evict(barq_rocm_handle* h, const barq_rocm_kv_cache* src,
         return fail(BARQ_E_INVALID, "%s: cache is on another device", who);
     if (mem == BARQ_MEM_DEVICE && !(aligned(mass_in, 4) && aligned(mass_out, 4) && aligned(kept, 4)))
         return fail(BARQ_E_INVALID, "%s: buffers must be 4-byte aligned", who);
-    // thread counts and head offsets of the kernels
+    // thread counts, positions (their count rounds up to 4096) and head offsets of the kernels
+    if (n > 0x7ffff000u) return fail(BARQ_E_DIM, "%s: %zu positions (at most 2^31 - 4096)", who, n);
     if (heads > 65535 || 2 * (double)heads * (double)m * (double)hd > 256.0 * 2147483647.0)
         return fail(BARQ_E_DIM, "%s: %zu kv heads x %zu positions x %zu dims", who, heads, m, hd);
     const auto done = [&]() {
@@ -187,6 +188,7 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
         return fail(BARQ_E_DIM, "%s: n_head * head_dim = %zu is not a multiple of 256", who, n_head * head_dim);
     if (kv_len == 0 || kv_len > c->len[layer])
         return fail(BARQ_E_DIM, "%s: kv_len %zu, layer %zu holds %zu positions", who, kv_len, layer, c->len[layer]);
+    if (kv_len > 0x7ffff000u) return fail(BARQ_E_DIM, "%s: kv_len %zu (at most 2^31 - 4096)", who, kv_len);
     if (mass_stride < kv_len) return fail(BARQ_E_DIM, "%s: mass_stride %zu below kv_len %zu", who, mass_stride, kv_len);
     if (h->device != c->device) return fail(BARQ_E_INVALID, "%s: cache is on another device", who);
     if (!host && (!aligned(q, 16) || !aligned(out, 4) || !aligned(mass_in, 4) || !aligned(mass_out, 4)))

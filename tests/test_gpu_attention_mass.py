@@ -169,6 +169,7 @@ def test_refusals(be):
     d, m = dev(q), dev(np.zeros((2, 40), F32))
     for kw, code in (({"kv_len": 41}, B.E_DIM), ({"kv_len": 0}, B.E_DIM), ({"layer": 1}, B.E_INVALID), ({"q_len": 0}, B.E_DIM),
                      ({"n_head_kv": 4}, B.E_DIM), ({"head_dim": 128}, B.E_DIM), ({"out_type": B.Q8_0}, B.E_UNSUPPORTED),
+                     ({"mass": dev(np.zeros((2, 40), np.float64))}, B.E_INVALID), ({"mass": dev(np.zeros((2, 41), F32))[:, 1:]}, B.E_INVALID),
                      ({"mass": dev(np.zeros((2, 39), F32))}, B.E_DIM), ({"mass": dev(np.zeros((1, 40), F32))}, B.E_DIM),
                      ({"q_len": 65536}, B.E_DIM), ({"start_pos": 2 ** 31 - 1}, B.E_DIM), ({"n_head": 6, "out_type": B.Q8_K}, B.E_DIM)):
         a = {"layer": 0, "n_head": 8, "n_head_kv": 2, "head_dim": 64, "q_len": 1, "kv_len": 40, "start_pos": 39, "mass": m,
