@@ -8,6 +8,15 @@
 // one of two LDS stages, lane by lane as the products will read them; one
 // barrier per block.  Loads run one block ahead of that.  NaN scales of V are
 // taken out here, so that they cannot reach rows that do not see them.
+//
+// What bounds it: the softmax and the products follow one another in a wave, and
+// with three workgroups a CU three waves share a SIMD.  2048 tokens of 32/8 heads of
+// 128 dims: 104 to 125 us, 34.4 GFLOP at 275 to 330 TFLOP/s of results, 2.5 f16
+// products each (hi and lo of q, of V and of the weights): 0.7 to 0.8 PFLOP/s on the
+// matrix unit, which a large f16 matrix product runs at 1.09.  With each wave
+// converting for itself 207.  Scores kept, 512 rows after 1536: 82.7, 134 MB of
+// them among that.  256 dims would take a CU's LDS for one workgroup and stay
+// with attn_q4_kernel.
 #include "attention_q4.hpp"
 #include "attention_q4_plan.hpp"
 #include "launch.hpp"
@@ -95,9 +104,9 @@ struct Q4Block {
 };
 
 // Workgroup x: group of G heads x % groups, then split, then row tile from the
-// last one down.  The longest tiles of all heads start first (128 us for 2048
-// tokens; 170 with one head's tiles before the next head's), and with eight kv heads an
-// XCD keeps to one of them.
+// last one down.  The longest tiles of all heads start first (2048 tokens when this was
+// chosen: 128 us, and 170 with one head's tiles before the next head's), and
+// with eight kv heads an XCD keeps to one of them.
 template <int HD, bool PART, bool SC>
 __global__ __launch_bounds__(64 * Q4P_NW, 3)
 void attn_q4_prompt_kernel(Q4Args a) {

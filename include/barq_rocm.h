@@ -514,9 +514,9 @@ int barq_rocm_attention_q8k(barq_rocm_handle* h, const float* q, const barq_rocm
  * query sees gets 0).  mass_in (NULL: zeros; may be mass_out) and mass_out are
  * [n_head_kv][mass_stride], mass_stride >= kv_len; columns from kv_len on are left
  * as they are.  barq_rocm_kv_cache_evict goes by them.  The output agrees with
- * barq_rocm_attention's within float rounding (an f32 cache's prompt chunks take
- * the decode kernel here).  Uses the handle's workspace for the scores, at
- * most 128 MiB of them or one query's. */
+ * barq_rocm_attention's within float rounding (rows may be cut into other
+ * pieces here).  Uses the handle's workspace for the scores, at most 128 MiB of
+ * them or one query's. */
 int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache* c, size_t layer,
                              size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len,
                              size_t start_pos, int out_type, void* out, const float* mass_in, float* mass_out,
