@@ -150,6 +150,33 @@ def test_less_than_the_cache(be, type_):
 
 
 @pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_prompts_of_less_than_the_cache(be, type_, hd):
+    """Positions that no query sees, and queries far behind the last one: whole tiles, and pieces that a tile lacks."""
+    c, q, k, v = case(be, type_, 8, 2, hd, 300, 900)
+    for kv_len, start in ((1200, 10), (77, 200), (1000, 0), (1000, 5000), (1, 3)):
+        ref, added = attention(q, k[:, :kv_len], v[:, :kv_len], start)
+        out, mass = A.compute_attention_mass(be, dev(q), c, 0, 8, 2, hd, 300, kv_len, start, None)
+        assert np.max(np.abs(out.cpu().numpy() - ref)) <= 2e-5 * np.max(np.abs(v))
+        mass = mass.cpu().numpy()
+        assert mass_ok(mass, np.zeros((2, kv_len), F32), added)
+        assert not mass[:, start + 300:].any()   # seen by no query
+
+
+@pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
+@pytest.mark.parametrize("heads,n_kv,n,total", [(16, 16, 1, 20000), (8, 2, 3, 66000)])
+def test_few_rows_of_a_long_cache(be, type_, heads, n_kv, n, total):
+    """More positions than the workgroups that sum the masses take at a time; one row sees fewer than the others."""
+    c, q, k, v = case(be, type_, heads, n_kv, 64, n, total - n, extra=3)
+    ref, added = attention(q, k, v, total - n)
+    before = np.abs(rows(4, n_kv, total + 2))
+    out, mass = A.compute_attention_mass(be, dev(q), c, 0, heads, n_kv, 64, n, total, total - n, dev(before))
+    assert np.max(np.abs(out.cpu().numpy() - ref)) <= 2e-5 * np.max(np.abs(v))
+    mass = mass.cpu().numpy()
+    assert mass_ok(mass[:, :total], before[:, :total], added) and np.array_equal(mass[:, total:], before[:, total:])
+
+
+@pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
 def test_nan_keys_reach_only_rows_that_see_them(be, type_):
     q, k, v = rows(5, 4, 2, 64), rows(6, 2, 60, 64), rows(7, 2, 60, 64)
     k[1, 59, 3], v[0, 59, 2] = np.nan, np.inf

@@ -28,7 +28,7 @@ def inv_freq(hd):
 
 
 @pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
-@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("n", [1, 40, 200])
 def test_a_step_in_a_graph(be, type_, n):
     """append with RoPE, attention with its mass, eviction into another cache."""
     import torch
