@@ -44,8 +44,8 @@ __device__ __forceinline__ int mass_head(const MassArgs& a, int hk) {
 // row); each of the others takes 256 positions of a kv head at a time, a wave 64 of them
 // and a fourth of the rows, whose statistics the workgroup finds itself (once: in a
 // long cache it takes several 256).  One decoded token of 32/8 heads against 4096
-// positions, with the attention: 11.7 us (4-bit) and 13.0 (f32); as many rows'
-// launches took 16.2 and 17.3.
+// positions, with the attention: 11.5 to 12.4 us (4-bit) and 14.2 (f32); the launches
+// for many rows took 16.2 and 17.3.
 struct MassLds {
     float2 stat[MASS_INLINE];
     float red[4][256];

@@ -10,10 +10,9 @@
 // scores' scales and O's sums 64, the softmax and the weights' split the rest)
 // beside 40 MFMAs of 16 cycles, for 4.5 KB of the cache, and a 16-column product
 // serves the G rows alone.  One row of 32/8 heads of 128 dims against 65536
-// positions (75.5 MB): 26.2 us and 3.9 for the merge, 2.9 TB/s, with vector issue
-// 59 % and the matrix unit 18 % busy; 4096 positions 6.4 + 3.9 (first bytes and launches);
-// five rows of 16/16 heads of 256 against 3003 14.8 + 4.0 (one step a wave).
-// Three workgroups a CU (two with 256 dims): the FIFO's LDS, 36 KB each with 128.
+// positions (75.5 MB): 24.7 us and 3.8 for the merge, 3.1 TB/s (vector issue 59 % and
+// the matrix unit 18 % busy, counted at 26.2); 4096 positions 6.5 + 3.8 (first bytes
+// and launches); five rows of 16/16 heads of 256 against 3003 14.9 + 3.8 (one step a wave).
 #include "attention_q4.hpp"
 #include "attention_q4_plan.hpp"
 #include "launch.hpp"

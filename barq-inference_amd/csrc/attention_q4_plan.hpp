@@ -32,8 +32,13 @@ inline Q4Plan q4_plan(size_t n_head, size_t n_head_kv, size_t hd, size_t q_len, 
     p.prompt = hd <= 128 && rows >= Q4P_MIN_ROWS;
     const size_t per = p.prompt ? (size_t)Q4P_ROWS : 16, unit = p.prompt ? 4 * STEP : TURN;
     p.tiles = (int)((rows + per - 1) / per);
-    const size_t wg = (size_t)p.groups * p.tiles, target = cus * (p.prompt || hd > 128 ? 2 : 3);
-    size_t ns = (target + wg - 1) / wg;
+    // About two workgroups a CU, and no splits from one and a half on.  us with
+    // targets of 1 / 1.5 / 2 / 3 a CU: 32/8 heads of 128, one row after 65535 28.4 / 30.0
+    // / 25.6 / 27.5, 10 after 10000 20.3 / 21.2 / 20.1 / 21.6, 64 after 4000 33.4 /
+    // 35.4 / 31.2 / 31.0, 512 after 1536 91 / 71 / 71 / 66, 1000 after 1500 (504
+    // workgroups unsplit) 121 / 121 / 142 / 142; 200 after 800 of 64 23.7 / 19.8 / 19.7 / 21.6
+    const size_t wg = (size_t)p.groups * p.tiles;
+    size_t ns = 2 * wg >= 3 * cus ? 1 : (2 * cus + wg - 1) / wg;
     const size_t most = (kv_len + unit - 1) / unit;
     if (ns > most) ns = most;
     if (ns > 1024) ns = 1024;   // the merge's limit

@@ -11,10 +11,10 @@
 //
 // What bounds it: the softmax and the products follow one another in a wave, and
 // with three workgroups a CU three waves share a SIMD.  2048 tokens of 32/8 heads of
-// 128 dims: 104 to 125 us, 34.4 GFLOP at 275 to 330 TFLOP/s of results, 2.5 f16
+// 128 dims: 104 to 121 us, 34.4 GFLOP at 285 to 330 TFLOP/s of results, 2.5 f16
 // products each (hi and lo of q, of V and of the weights): 0.7 to 0.8 PFLOP/s on the
 // matrix unit, which a large f16 matrix product runs at 1.09.  With each wave
-// converting for itself 207.  Scores kept, 512 rows after 1536: 82.7, 134 MB of
+// converting for itself 207.  Scores kept, 512 rows after 1536: 81.8, 134 MB of
 // them among that.  256 dims would take a CU's LDS for one workgroup and stay
 // with attn_q4_kernel.
 #include "attention_q4.hpp"

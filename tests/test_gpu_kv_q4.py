@@ -5,7 +5,8 @@ Bars:
   - codes and scales (read back as f32): exact.  The quantizer is defined by
     comparisons that are exact in f32, and a value (code - 8) * d has 15 bits.
   - attention against 64 bits on the rows the cache reads as: a score (in
-    log2 units) sums HD products in three parts.  With S the sum of their
+    log2 units) sums HD products in two parts (three of a query whose elements
+    are very uneven).  With S the sum of their
     sizes (about 0.64 * 1.44 * sqrt(HD) = 10 to 15 for normal queries and
     keys), HD roundings or truncations of at most 2^-23 of the partial sum
     add up to sqrt(3 * 32) * 2^-23 * S = 1.7e-5 root mean square over a block's 96
