@@ -156,7 +156,7 @@ __device__ __forceinline__ void q4_walk(const Q4Fifo<HD>& fifo, uint8_t* lds, in
     fifo.issue(0, (uint32_t)first);
     int stage = 0;
     for (int at = first; at < n; at += turn, stage ^= 1) {
-        fifo.issue(stage ^ 1, (uint32_t)(at + turn));   // (past the range: zeros)
+        fifo.issue(stage ^ 1, (uint32_t)q4_ahead(at, turn, n));   // (always as many copies: the wait counts them)
         wait_vmcnt<Q4Fifo<HD>::COPIES>();
         asm volatile("" ::: "memory");
         const Q4Stage<HD> s{lds + stage * Q4Fifo<HD>::STAGE, l & 15, l >> 4};

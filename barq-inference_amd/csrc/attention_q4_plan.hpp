@@ -52,4 +52,11 @@ inline Q4Plan q4_plan(size_t n_head, size_t n_head_kv, size_t hd, size_t q_len, 
     return p;
 }
 
+// What a wave of attn_q4_kernel fetches while it works on the step at `at` (of
+// n positions, a step every `turn`): the next one, or behind the last the end
+// of the range's whole tiles.  There the scalar offset is the descriptor's limit
+// itself, and every address is out of bounds and reads as zero (the bounds
+// check subtracts the scalar offset from the limit; it need not go below zero).
+constexpr int q4_ahead(int at, int turn, int n) { return at + turn < n ? at + turn : (n + 7) / 8 * 8; }
+
 }  // namespace barq
