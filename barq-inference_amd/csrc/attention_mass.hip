@@ -26,7 +26,9 @@ __device__ __forceinline__ float2 mass_stat(const MassArgs& a, size_t at, int la
     for (int s = lane16; s < a.ns; s += 16) {
         const float m = p[(size_t)s * (a.head_dim + 2)], l = p[(size_t)s * (a.head_dim + 2) + 1];
         const float mn = fmaxf(M, m);
+        // (pieces that saw nothing leave -infinity and 0, pieces that saw only NaN -infinity and NaN, which stays in the sum)
         if (mn != -INFINITY) L = L * __builtin_amdgcn_exp2f(M - mn) + l * __builtin_amdgcn_exp2f(m - mn);
+        else L += l;
         M = mn;
     }
     const float all = row16_max(M);

@@ -1,0 +1,51 @@
+"""Edges of attention over the KV cache and of its masses: rows that see only
+NaN in a piece of the cache.
+
+Bars, where a test names no other: those of test_gpu_kv_q4.py and
+test_gpu_attention_mass.py (2e-5 * max |V| for the output; for a position's mass 2.5e-5 of
+what the call adds, and 2^-23 of the total)."""
+import numpy as np
+import pytest
+
+import barq_rocm as B
+from barq_rocm import attention as A
+from kv_ref import attention, q4_values
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+
+
+def dev(a):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def rows(seed, *shape):
+    return np.random.default_rng(seed).standard_normal(shape).astype(F32)
+
+
+def cache(be, type_, k, v):
+    n_kv, n, hd = k.shape
+    c = A.KVCache(be, n, 1, n_kv, hd, type=type_)
+    c.append(0, dev(k), dev(v), n, hd)
+    return (c, q4_values(k), q4_values(v)) if type_ == B.Q4_0 else (c, k, v)
+
+
+@pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
+@pytest.mark.parametrize("total,bad", [(129, 1), (300, 44), (1000, 1), (4097, 1), (4200, 200)])
+@pytest.mark.parametrize("n", [1, 3])
+def test_masses_of_rows_that_see_only_nan_in_a_piece(be, type_, total, bad, n):
+    """The last `bad` keys of one kv head are NaN: the pieces that hold nothing else have no maximum, but their sum
+    is NaN, and so are the weights of every position that the rows see."""
+    heads, n_kv, hd = 32, 8, 128
+    q, k, v = rows(1, heads, n, hd), rows(2, n_kv, total, hd), rows(3, n_kv, total, hd)
+    k[5, total - bad:, 9] = np.nan
+    c, k, v = cache(be, type_, k, v)
+    ref, added = attention(q, k, v, total - n)
+    out, mass = A.compute_attention_mass(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n, None)
+    out, mass = out.cpu().numpy(), mass.cpu().numpy()
+    assert np.isnan(added[5]).all() and np.isfinite(np.delete(added, 5, 0)).all()
+    assert np.array_equal(np.isnan(out), np.isnan(ref)) and np.array_equal(np.isnan(mass), np.isnan(added))
+    ok, seen = np.isfinite(ref), np.isfinite(added)
+    assert np.max(np.abs(out[ok] - ref[ok])) <= 2e-5 * np.max(np.abs(v))
+    assert np.all(np.abs(mass - added)[seen] <= (2.5e-5 + 2.0 ** -23) * added[seen])
