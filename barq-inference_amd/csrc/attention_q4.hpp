@@ -16,10 +16,12 @@
 // A query row is scaled by a power of two so that its largest element is in
 // [2^14, 2^15) and split into two f16 values, off by at most 2^-23 of an element
 // down to 2^-17 of the largest and by 2^-40 of the largest below that.  (A normal
-// query has such an element in one row of 300.)  Where more than a sixteenth
-// of a row's elements are that small, beside a largest one that keys need not
-// share, the wave forms its scores from three bf16 values instead, which hold any f32
-// exactly.  The products are exact, the sums f32, the block's scale joins in
+// query has such an element in one row of 300.)  What that can do to a score is
+// bounded by the keys' largest value, 65504, whatever else the row and the keys hold;
+// where the bound passes 2^-20 in log2 units the wave forms its scores from three
+// bf16 values instead, which hold any f32 exactly: with 128 dims from one such
+// element on beside a largest one of 64 or more, from 32 on beside one of 2 to 4.
+// The products are exact, the sums f32, the block's scale joins in
 // f32 and the row's in the exponent's fma.
 // A V element (code - 8) * d has 15 bits and is exactly hi + lo in f16: all
 // its parts are multiples of 2^-24, the least f16 step, and the quantizer keeps it
@@ -132,7 +134,8 @@ struct Q4Query {
     h8v hi[HD / 32], lo[HD / 32];
     const float* at;     // its dims 0 .. 7 of block 0
     float scale, back;   // what the row is multiplied by; scores times back are in log2 units
-    // true if more than a sixteenth of the elements are small enough to lose bits to the split
+    // true if the split may lose 2^-20 of a score (log2 units): each element below
+    // 2^-2 is off by 2^-25 at most there, its key is at most 8 * Q4_D_MAX < 2^16
     __device__ __forceinline__ bool load(const float* row, float score_scale, int g, const Q4Const& kc) {
         at = row + 8 * g;
         float4 y[HD / 16];
@@ -168,7 +171,7 @@ struct Q4Query {
             hi[b] = __builtin_bit_cast(h8v, h);
             lo[b] = __builtin_bit_cast(h8v, l);
         }
-        return groups_sum(small) > (float)(HD / 16);
+        return groups_sum(small) * back > 0x1p-11f;   // 2^(-20 + 25 - 16)
     }
     // block b in three bf16 values, which hold any f32 exactly
     __device__ __forceinline__ void exact(int b, bf8v (&p)[3]) const {

@@ -6,6 +6,8 @@ import subprocess
 
 import pytest
 
+from test_gpu_kv_edges import PROMPT_CALLS
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "barq-inference_amd", "csrc")
 
@@ -63,3 +65,8 @@ def plan(tmp_path_factory):
 
 def test_fetches_begin_within_the_range(tmp_path):
     subprocess.run([compiled(tmp_path, WALK)], check=True)
+
+
+def test_calls_meant_for_the_prompt_kernel_take_it(plan):
+    calls = sorted(PROMPT_CALLS)
+    assert calls and all(p["prompt"] for p in plan(calls))

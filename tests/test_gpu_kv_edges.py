@@ -1,5 +1,9 @@
 """Edges of attention over the KV cache and of its masses: rows that see only
-NaN in a piece of the cache.
+NaN in a piece of the cache, queries whose elements differ by many powers of two.
+
+Calls that are meant for the matrix prompt kernel of a 4-bit cache are in
+PROMPT_CALLS (heads, kv heads, head_dim, rows, positions); test_attention_q4_plan.py
+checks on the host that they go there.
 
 Bars, where a test names no other: those of test_gpu_kv_q4.py and
 test_gpu_attention_mass.py (2e-5 * max |V| for the output; for a position's mass 2.5e-5 of
@@ -13,6 +17,12 @@ from kv_ref import attention, q4_values
 
 pytestmark = pytest.mark.gpu
 F32 = np.float32
+PROMPT_CALLS = set()
+
+
+def prompt_calls(*calls):
+    PROMPT_CALLS.update(calls)
+    return list(calls)
 
 
 def dev(a):
@@ -49,3 +59,27 @@ def test_masses_of_rows_that_see_only_nan_in_a_piece(be, type_, total, bad, n):
     ok, seen = np.isfinite(ref), np.isfinite(added)
     assert np.max(np.abs(out[ok] - ref[ok])) <= 2e-5 * np.max(np.abs(v))
     assert np.all(np.abs(mass - added)[seen] <= (2.5e-5 + 2.0 ** -23) * added[seen])
+
+
+UNEVEN = [(8, 2, 64, 1, 200), (8, 2, 128, 3, 200), (8, 2, 256, 1, 200), (8, 2, 256, 40, 300)] + prompt_calls(
+    (8, 2, 64, 33, 200), (8, 2, 128, 40, 300))
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,n,total", UNEVEN)
+@pytest.mark.parametrize("big", [3e4, 1e9, -1e25, 1e38])
+def test_few_small_elements_beside_a_large_one(be, heads, n_kv, hd, n, total, big):
+    """Keys that are zero in the large dim: the scores come from the small elements alone."""
+    q, k, v = np.zeros((heads, n, hd), F32), 3 * rows(2, n_kv, total, hd), rows(3, n_kv, total, hd)
+    q[:, :, 7] = big
+    k[:, :, 7] = 0
+    for h in range(heads):   # one of them up to as many as a row of this size may have by chance
+        few = [1, 2, 4, hd // 16][h % 4]
+        q[h][:, 10:10 + few] = rows(h, n, few) + F32(1 / 3)
+    c, k, v = cache(be, B.Q4_0, k, v)
+    assert not k[:, :, 7].any()
+    ref, added = attention(q, k, v, total - n)
+    got = A.compute_attention(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n).cpu().numpy()
+    assert np.max(np.abs(got - ref)) <= 2e-5 * np.max(np.abs(v))
+    out, mass = A.compute_attention_mass(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n, None)
+    assert np.max(np.abs(out.cpu().numpy() - ref)) <= 2e-5 * np.max(np.abs(v))
+    assert np.all(np.abs(mass.cpu().numpy() - added) <= (2.5e-5 + 2.0 ** -23) * added)
