@@ -379,11 +379,11 @@ __device__ __forceinline__ void q4_attend(float (&x)[8], int base, int at, const
         }
     }
     bm = groups_max(bm) * back;
-    // O and l are relative to m, a multiple of 2^-14; it moves when the
-    // maximum has grown by 2^32.  The step's weights are relative to m
-    // plus a whole number, at most 2^15.
+    // O and l are relative to m, a multiple of 2^-14 (which every f32 value from 2^9
+    // on is); it moves when the maximum has grown by 2^32.  The step's weights are
+    // relative to ref, m plus a whole number as f32 rounds it, and at most 2^15.5.
     if (__any(bm > st.m + 32.0f)) {
-        const float mn = fmaxf(st.m, __builtin_ceilf(bm * 0x1p14f) * 0x1p-14f);
+        const float mn = fmaxf(st.m, __builtin_fabsf(bm) < 0x1p9f ? __builtin_ceilf(bm * 0x1p14f) * 0x1p-14f : bm);
         const float corr = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(st.m - mn);
         st.m = mn;
         st.l *= corr;
@@ -391,9 +391,17 @@ __device__ __forceinline__ void q4_attend(float (&x)[8], int base, int at, const
         for (int c = 0; c < HD / 16; c++) st.o[c] *= corr;
     }
     const bool none = bm == -INFINITY;   // a row that sees no position of the step
-    const float k = none ? 0.0f : __builtin_ceilf(bm - st.m) - 15.0f;
-    const float ref = none ? 0.0f : st.m + k;
-    float w = none ? 0.0f : __builtin_amdgcn_exp2f(k);
+    float ref = none ? 0.0f : st.m + (__builtin_ceilf(bm - st.m) - 15.0f);
+    // From scores of 2^21 on their rounding (bm's against the product below, ref's) would let
+    // weights pass 65504: there the scores are rounded first, and ref is bm itself where it came out lower.
+    if (__any(__builtin_fabsf(ref) >= 0x1p21f || bm - ref > 15.5f)) {
+        #pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= back;
+        least *= back;
+        back = 1.0f;
+        ref = bm - ref > 15.5f ? bm : ref;
+    }
+    float w = none ? 0.0f : __builtin_amdgcn_exp2f(ref - st.m);
     #pragma unroll
     for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], back, -ref));
     st.l = __builtin_fmaf(((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])), w, st.l);

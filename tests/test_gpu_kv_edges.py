@@ -1,5 +1,6 @@
 """Edges of attention over the KV cache and of its masses: rows that see only
-NaN in a piece of the cache, queries whose elements differ by many powers of two.
+NaN in a piece of the cache, queries whose elements differ by many powers of two,
+scores up to f32's largest.
 
 Calls that are meant for the matrix prompt kernel of a 4-bit cache are in
 PROMPT_CALLS (heads, kv heads, head_dim, rows, positions); test_attention_q4_plan.py
@@ -83,3 +84,36 @@ def test_few_small_elements_beside_a_large_one(be, heads, n_kv, hd, n, total, bi
     out, mass = A.compute_attention_mass(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n, None)
     assert np.max(np.abs(out.cpu().numpy() - ref)) <= 2e-5 * np.max(np.abs(v))
     assert np.all(np.abs(mass.cpu().numpy() - added) <= (2.5e-5 + 2.0 ** -23) * added)
+
+
+@pytest.mark.parametrize("type_", [B.F32, B.Q4_0])
+@pytest.mark.parametrize("heads,n_kv,hd,n,total", [(8, 2, 64, 1, 300), (8, 2, 128, 2, 700), (8, 2, 256, 1, 300), (8, 2, 256, 40, 300)] +
+                         prompt_calls((8, 2, 64, 40, 300), (8, 2, 128, 64, 500)))
+@pytest.mark.parametrize("size,signs", [(2.0 ** 22, 0), (2.0 ** 24, 0), (2.0 ** 26, 0), (2.0 ** 28, 0), (2.0 ** 30, 0), (1e33, 0), (1e36, 0), (1e36, 1), (1e36, -1)])
+def test_scores_up_to_the_largest(be, type_, heads, n_kv, hd, n, total, size, signs):
+    """Queries so large that a row's weight is all on one position; scores of both signs, or of one.  They come near
+    f32's largest (a sum's parts must stay below it).  Rows whose two largest scores agree to 2^-16 are left out: 24
+    bits may not tell them apart."""
+    q, k, v = rows(1, heads, n, hd) * F32(size), rows(2, n_kv, total, hd), rows(3, n_kv, total, hd)
+    if signs:
+        q, k = np.abs(q) * signs, np.abs(k) + F32(0.01)
+    c, k, v = cache(be, type_, k, v)
+    ref, _ = attention(q, k, v, total - n)
+    apart = np.empty((n, heads), bool)
+    for h in range(heads):
+        s = q[h].astype(np.float64) @ k[h * n_kv // heads].T.astype(np.float64) / np.sqrt(hd)
+        assert (np.abs(q[h]).astype(np.float64) @ np.abs(k[h * n_kv // heads]).T.astype(np.float64)).max() < 3e38
+        for i in range(n):
+            two = np.sort(s[i, :total - n + i + 1])[-2:]
+            apart[i, h] = two[1] - two[0] > 2.0 ** -16 * np.abs(s[i]).max()
+    assert apart.mean() > 0.9
+    got = A.compute_attention(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n).cpu().numpy()
+    out, mass = A.compute_attention_mass(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n, None)
+    for o in (got, out.cpu().numpy()):
+        assert np.isfinite(o).all()
+        # One weight and one V row.  In steps of 2^-23 of the result: the weight's split into two f16 values 1, the
+        # product of both low parts (2^-11 of each) that is left out 2, three products' sums that the matrix unit
+        # does not round to nearest 3, the sums into O and of the weights 1/2 each, the division 1.
+        assert np.max(np.abs(o - ref)[apart]) <= 8 * 2.0 ** -23 * np.max(np.abs(v))
+    mass = mass.cpu().numpy()
+    assert np.isfinite(mass).all() and np.allclose(mass.sum(1), n * heads // n_kv, rtol=1e-5)
