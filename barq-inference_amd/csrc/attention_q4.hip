@@ -183,7 +183,7 @@ void attn_q4_kernel(Q4Args a) {
     const int hk = (int)((long long)(grp * a.G) * a.n_head_kv / a.n_head);
     // the tile's last row bounds the positions
     const int visible = q4_vis(a, r0 + Q4A_ROWS - 1);
-    const int start = split * a.chunk, j0 = min(start, visible), j1 = min(visible, start + a.chunk);
+    const int start = split * a.chunk, j0 = min(start, visible), j1 = q4_range_end(start, a.chunk, visible);
 
     Q4Fifo<HD> fifo;
     uint8_t* mine = lds + wave * Q4Fifo<HD>::BYTES;

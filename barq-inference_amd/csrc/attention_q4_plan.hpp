@@ -42,8 +42,9 @@ inline Q4Plan q4_plan(size_t n_head, size_t n_head_kv, size_t hd, size_t q_len, 
     const size_t most = (kv_len + unit - 1) / unit;
     if (ns > most) ns = most;
     if (ns > 1024) ns = 1024;   // the merge's limit
-    // at most 2^20 positions a split (32-bit byte offsets)
-    const size_t least = (kv_len + ((size_t)1 << 20) - 1) >> 20;
+    // At most 2^21 positions a split (byte offsets in 32 bits: 2^28 of 256 dims), so
+    // that no cache below 2^31 positions takes more than the merge's limit.
+    const size_t least = (kv_len + ((size_t)1 << 21) - 1) >> 21;
     if (ns < least) ns = least;
     size_t ch = (kv_len + ns - 1) / ns;
     ch = (ch + unit - 1) / unit * unit;
@@ -51,6 +52,11 @@ inline Q4Plan q4_plan(size_t n_head, size_t n_head_kv, size_t hd, size_t q_len, 
     p.n_split = (int)((kv_len + ch - 1) / ch);
     return p;
 }
+
+// Where the split that begins at start ends, for a row tile that sees `visible`
+// positions (below start where it sees none of the split).  Without start + chunk,
+// which may pass 2^31 in the last split.
+constexpr int q4_range_end(int start, int chunk, int visible) { return visible - start < chunk ? visible : start + chunk; }
 
 // What a wave of attn_q4_kernel fetches while it works on the step at `at` (of
 // n positions, a step every `turn`): the next one, or behind the last the end

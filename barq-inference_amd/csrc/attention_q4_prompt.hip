@@ -119,7 +119,7 @@ void attn_q4_prompt_kernel(Q4Args a) {
     const int tile = a.tiles - 1 - part / a.n_split, split = part % a.n_split;
     const int hk = (int)((long long)(grp * a.G) * a.n_head_kv / a.n_head);
     const int visible = q4_vis(a, tile * Q4P_ROWS + Q4P_ROWS - 1);
-    const int start = split * a.chunk, j0 = min(start, visible), j1 = min(visible, start + a.chunk);
+    const int start = split * a.chunk, j0 = min(start, visible), j1 = q4_range_end(start, a.chunk, visible);
     const int r0 = tile * Q4P_ROWS + wave * Q4A_ROWS;
     const int mine = r0 < rows_n ? min(j1, q4_vis(a, r0 + Q4A_ROWS - 1)) : 0;   // the wave's rows see no more
 

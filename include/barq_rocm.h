@@ -491,8 +491,9 @@ int barq_rocm_kv_cache_destroy(barq_rocm_kv_cache* c);
  * j < min(kv_len, start_pos + i + 1) with weights softmax((q . K[j]) /
  * sqrt(head_dim)); out[i, h, :] = sum_j p_j V[j, :].  kv_len must be at most
  * the layer's length; head_dim 64, 128 or 256 (else BARQ_E_UNSUPPORTED).
- * n_head_kv and head_dim must be the cache's.  Uses the handle's workspace
- * for the partial results of long sequences. */
+ * n_head_kv and head_dim must be the cache's.  Of a 4-bit cache kv_len is at
+ * most 2^31 - 4096 (else BARQ_E_DIM), as in attention_mass and evict.  Uses the
+ * handle's workspace for the partial results of long sequences. */
 int barq_rocm_attention(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache* c, size_t layer,
                         size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len,
                         size_t start_pos, float* out, int mem);

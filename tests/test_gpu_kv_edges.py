@@ -117,3 +117,22 @@ def test_scores_up_to_the_largest(be, type_, heads, n_kv, hd, n, total, size, si
         assert np.max(np.abs(o - ref)[apart]) <= 8 * 2.0 ** -23 * np.max(np.abs(v))
     mass = mass.cpu().numpy()
     assert np.isfinite(mass).all() and np.allclose(mass.sum(1), n * heads // n_kv, rtol=1e-5)
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,n,total", prompt_calls((4, 1, 64, 6150, 2 ** 20 + 5000)))
+def test_a_million_positions_in_one_piece(be, heads, n_kv, hd, n, total):
+    """Enough rows that the positions stay in one piece, of more than 2^20; a few of the rows against 64 bits."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k, v, q = (torch.randn(*s, device="cuda", generator=g) for s in ((n_kv, total, hd), (n_kv, total, hd), (heads, n, hd)))
+    k[:, 2 ** 20:] *= 2   # what lies behind 2^20 counts
+    c = A.KVCache(be, total, 1, n_kv, hd, type=B.Q4_0)
+    torch.cuda.synchronize()
+    c.append(0, k, v, total, hd)
+    kq, vq = (t.cpu().numpy().astype(np.float64) for t in c.read(0, 0, total))
+    got = A.compute_attention(be, q, c, 0, heads, n_kv, hd, n, total, total - n).cpu().numpy()
+    q = q.cpu().numpy()
+    for i in (0, 3001, n - 1):
+        ref, _ = attention(q[:, i:i + 1], kq[:, :total - n + i + 1], vq[:, :total - n + i + 1], total - n + i)
+        assert np.max(np.abs(got[i] - ref[0])) <= 2e-5 * np.max(np.abs(vq))
+    c.close()
