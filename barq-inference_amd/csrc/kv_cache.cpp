@@ -7,6 +7,7 @@
 
 #include "api_internal.hpp"
 #include "kv_cache.hpp"
+#include "kv_evict_plan.hpp"
 #include "launch.hpp"
 
 using namespace barq_api;
@@ -87,9 +88,10 @@ int barq_rocm_kv_cache_evict(barq_rocm_handle* h, const barq_rocm_kv_cache* src,
         return fail(BARQ_E_INVALID, "%s: cache is on another device", who);
     if (mem == BARQ_MEM_DEVICE && !(aligned(mass_in, 4) && aligned(mass_out, 4) && aligned(kept, 4)))
         return fail(BARQ_E_INVALID, "%s: buffers must be 4-byte aligned", who);
-    // thread counts, positions (their count rounds up to 4096) and head offsets of the kernels
+    // positions (their count rounds up to 4096), heads and threads of the kernels
     if (n > 0x7ffff000u) return fail(BARQ_E_DIM, "%s: %zu positions (at most 2^31 - 4096)", who, n);
-    if (heads > 65535 || 2 * (double)heads * (double)m * (double)hd > 256.0 * 2147483647.0)
+    const bool q4 = src->type == BARQ_TYPE_Q4_0, move = m > 0 && !(src == dst && m == n), stage = move && src == dst;
+    if (heads > 65535 || (move && barq::evict_heads(q4, heads, m, hd) == 0))
         return fail(BARQ_E_DIM, "%s: %zu kv heads x %zu positions x %zu dims", who, heads, m, hd);
     const auto done = [&]() {
         dst->len[layer] = m;
@@ -98,7 +100,6 @@ int barq_rocm_kv_cache_evict(barq_rocm_handle* h, const barq_rocm_kv_cache* src,
     };
     if (n == 0) return done();
     DeviceGuard g(h);
-    const bool q4 = src->type == BARQ_TYPE_Q4_0, move = m > 0 && !(src == dst && m == n), stage = move && src == dst;
     Arena a;
     const size_t oid = a.add(heads * m * sizeof(int32_t));
     const size_t omass = mem == BARQ_MEM_HOST ? a.add(heads * n * sizeof(float)) : 0;

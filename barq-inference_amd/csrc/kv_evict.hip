@@ -25,6 +25,7 @@
 // times (4096 of 16384 positions 8.1 us, 9.4 MB and the rest of the tiles' lines).  In place they go
 // by way of the workspace (5.4 us back): a row may move onto one that is still to be read.
 #include "common.hpp"
+#include "kv_evict_plan.hpp"
 #include "kv_q4.hpp"
 #include "launch.hpp"
 
@@ -306,18 +307,27 @@ void gather_rows_kernel(const V* __restrict__ k, const V* __restrict__ v, size_t
 
 hipError_t gather_rows_launch(const float* k, const float* v, size_t src_head, float* ko, float* vo, size_t dst_head,
                               size_t n_kv, size_t hd, size_t m, const int32_t* kept, hipStream_t s) {
-    if (hd % 4 == 0) {   // (every row then starts at a multiple of 16 bytes)
-        const size_t n = 2 * n_kv * m * (hd / 4);
-        hipLaunchKernelGGL(gather_rows_kernel<float4>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,
-                           reinterpret_cast<const float4*>(k), reinterpret_cast<const float4*>(v), src_head / 4,
-                           reinterpret_cast<float4*>(ko), reinterpret_cast<float4*>(vo), dst_head / 4, (int)n_kv,
-                           (int)(hd / 4), (int)m, kept);
-    } else {
-        const size_t n = 2 * n_kv * m * hd;
-        hipLaunchKernelGGL(gather_rows_kernel<float>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k, v, src_head,
-                           ko, vo, dst_head, (int)n_kv, (int)hd, (int)m, kept);
+    const size_t per = evict_heads(false, n_kv, m, hd);
+    if (per == 0) return hipErrorInvalidValue;
+    for (size_t h = 0; h < n_kv; h += per) {
+        const size_t heads = per < n_kv - h ? per : n_kv - h;
+        const float *k0 = k + h * src_head, *v0 = v + h * src_head;
+        float *k1 = ko + h * dst_head, *v1 = vo + h * dst_head;
+        if (hd % 4 == 0) {   // (every row then starts at a multiple of 16 bytes)
+            const size_t n = 2 * heads * m * (hd / 4);
+            hipLaunchKernelGGL(gather_rows_kernel<float4>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s,
+                               reinterpret_cast<const float4*>(k0), reinterpret_cast<const float4*>(v0), src_head / 4,
+                               reinterpret_cast<float4*>(k1), reinterpret_cast<float4*>(v1), dst_head / 4, (int)heads,
+                               (int)(hd / 4), (int)m, kept + h * m);
+        } else {
+            const size_t n = 2 * heads * m * hd;
+            hipLaunchKernelGGL(gather_rows_kernel<float>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k0, v0, src_head,
+                               k1, v1, dst_head, (int)heads, (int)hd, (int)m, kept + h * m);
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
     }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 // ---- 4-bit rows ----------------------------------------------------------------------
@@ -389,12 +399,25 @@ void gather_q4_kernel(Q4View src, Q4View dst, int n_kv, int m, int tiles, const 
 
 template <int HD>
 static hipError_t gather_q4_t(const Q4View& src, const Q4View& dst, size_t n_kv, size_t m, const int32_t* kept, hipStream_t s) {
-    const size_t tiles = q4_tiles(m);
-    const unsigned vb = (unsigned)((n_kv * tiles * 16 + 255) / 256), kb = (unsigned)((n_kv * m * (HD / 32) + 255) / 256),
-                   sb = (unsigned)((n_kv * tiles * 2 * (HD / 32) + 255) / 256);
-    hipLaunchKernelGGL(gather_q4_kernel<HD>, dim3(vb + kb + sb), dim3(256), 0, s, src, dst, (int)n_kv, (int)m, (int)tiles,
-                       kept, vb, kb);
-    return hipGetLastError();
+    const size_t tiles = q4_tiles(m), per = evict_heads(true, n_kv, m, HD);
+    if (per == 0) return hipErrorInvalidValue;
+    for (size_t h = 0; h < n_kv; h += per) {
+        const size_t heads = per < n_kv - h ? per : n_kv - h;
+        const auto from = [&](Q4View w) {   // its heads from h on
+            w.kc += h * w.code_head;
+            w.vc += h * w.code_head;
+            w.ks += h * w.scale_head;
+            w.vs += h * w.scale_head;
+            return w;
+        };
+        const unsigned vb = (unsigned)((heads * tiles * 16 + 255) / 256), kb = (unsigned)((heads * m * (HD / 32) + 255) / 256),
+                       sb = (unsigned)((heads * tiles * 2 * (HD / 32) + 255) / 256);
+        hipLaunchKernelGGL(gather_q4_kernel<HD>, dim3(vb + kb + sb), dim3(256), 0, s, from(src), from(dst), (int)heads, (int)m,
+                           (int)tiles, kept + h * m, vb, kb);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 hipError_t gather_q4_launch(const Q4View& src, const Q4View& dst, size_t n_kv, size_t hd, size_t m, const int32_t* kept,

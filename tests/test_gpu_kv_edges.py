@@ -14,7 +14,7 @@ import pytest
 
 import barq_rocm as B
 from barq_rocm import attention as A
-from kv_ref import attention, q4_values
+from kv_ref import attention, kept, q4_values
 
 pytestmark = pytest.mark.gpu
 F32 = np.float32
@@ -136,3 +136,32 @@ def test_a_million_positions_in_one_piece(be, heads, n_kv, hd, n, total):
         ref, _ = attention(q[:, i:i + 1], kq[:, :total - n + i + 1], vq[:, :total - n + i + 1], total - n + i)
         assert np.max(np.abs(got[i] - ref[0])) <= 2e-5 * np.max(np.abs(vq))
     c.close()
+
+
+def test_eviction_of_more_rows_than_a_launch_moves():
+    """A launch takes fewer than 2^32 threads, and rows of one dim take one each: the heads go in two launches."""
+    import torch
+    be = B.Backend(0)   # (a workspace of 26 GB goes with it)
+    heads, n, keep = 32768, 65540, 65537
+    c = A.KVCache(be, n, 1, heads, 1)
+    x = torch.randint(0, 1 << 20, (heads, n, 1), device="cuda").float()
+    mass = torch.rand(heads, n, device="cuda")
+    torch.cuda.synchronize()
+    c.append(0, x, x, n, 1)
+    be.sync()
+    few = [0, 1, 20000, heads - 2, heads - 1]
+    before = mass[few].clone()
+    want = torch.from_numpy(kept(before.cpu().numpy(), n, keep, 10)).cuda().long()
+    c.evict(0, mass, keep, 10, want_kept=False)
+    assert c.layer_len(0) == keep
+    assert torch.equal(mass[few][:, :keep], torch.gather(before, 1, want)) and not mass[:, keep:].any()
+    out = torch.empty((heads, keep), device="cuda")
+    for k in (True, False):
+        B._lib.check(be._lib.barq_rocm_kv_cache_read(be.h, c.c, 0, 0, keep, out.data_ptr() if k else None,
+                                                     None if k else out.data_ptr(), B.MEM_DEVICE))
+        be.sync()
+        assert torch.equal(out[few], torch.gather(x[few, :, 0], 1, want))
+    c.close()
+    be.close()
+    del x, out, mass
+    torch.cuda.empty_cache()
