@@ -414,6 +414,8 @@ int attention_any(barq_rocm_handle* h, const float* q, const barq_rocm_kv_cache*
     const bool q4 = c->type == BARQ_TYPE_Q4_0;
     if (q4) BARQ_CHECK(check_int_range(n_head * q_len, "attention: n_head * q_len"));
     if (q4 && kv_len > 0x7ffff000u) return fail(BARQ_E_DIM, "attention: kv_len %zu (at most 2^31 - 4096)", kv_len);
+    if (q4 && !barq::attention_q4_fits(n_head, n_head_kv, head_dim, q_len, kv_len))
+        return fail(BARQ_E_DIM, "attention: %zu heads x %zu rows against %zu positions need too many workgroups", n_head, q_len, kv_len);
     const size_t wsp = q4 ? barq::attention_q4_workspace(n_head, n_head_kv, head_dim, q_len, kv_len)
                           : barq::attention_workspace(n_head, head_dim, q_len, kv_len, n_head_kv);
     Arena a;

@@ -258,6 +258,10 @@ size_t attention_q4_workspace(size_t n_head, size_t n_head_kv, size_t head_dim, 
     return p.n_split > 1 ? (size_t)p.n_split * n_head * q_len * (head_dim + 2) * sizeof(float) : 0;
 }
 
+bool attention_q4_fits(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len) {
+    return q4_fits(q4_plan(n_head, n_head_kv, head_dim, q_len, kv_len), n_head, head_dim, q_len);
+}
+
 bool attention_q4_q8_direct(const AttnArgs& a) {
     return (a.n_head * a.head_dim) % 256 == 0 && q4_plan(a.n_head, a.n_head_kv, a.head_dim, a.q_len, a.kv_len).n_split > 1;
 }

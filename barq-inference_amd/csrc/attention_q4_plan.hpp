@@ -53,6 +53,14 @@ inline Q4Plan q4_plan(size_t n_head, size_t n_head_kv, size_t hd, size_t q_len, 
     return p;
 }
 
+// Whether the call's launches, the merge's among them, stay below 2^32 threads (a
+// larger grid is cut without an error).
+inline bool q4_fits(const Q4Plan& p, size_t n_head, size_t hd, size_t q_len) {
+    const size_t most = ((size_t)1 << 32) - 1;
+    const size_t merge = ((n_head * hd + 255) / 256 * q_len + 3) / 4;   // workgroups
+    return (size_t)p.n_split * p.tiles * p.groups <= most / (64 * Q4P_NW) && (p.n_split == 1 || merge <= most / 256);
+}
+
 // Where the split that begins at start ends, for a row tile that sees `visible`
 // positions (below start where it sees none of the split).  Without start + chunk,
 // which may pass 2^31 in the last split.

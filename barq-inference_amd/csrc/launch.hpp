@@ -273,6 +273,7 @@ hipError_t copy_planes_launch(const CopyPlanes& p, size_t heads, hipStream_t s);
 
 // attention_q4.hip: attention_launch and its helpers for a 4-bit cache (a.k, a.v, a.layer_off and a.head_stride unused)
 size_t attention_q4_workspace(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);
+bool attention_q4_fits(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);   // its grids
 bool attention_q4_q8_direct(const AttnArgs& a);
 hipError_t attention_q4_launch(const AttnArgs& a, const Q4View& kv, hipStream_t s);
 

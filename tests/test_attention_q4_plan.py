@@ -15,12 +15,12 @@ MAIN = r"""
 #include "attention_q4_plan.hpp"
 #include <cstdio>
 using namespace barq;
-// shapes on stdin -> prompt, G, groups, tiles, n_split, chunk
+// shapes on stdin -> prompt, G, groups, tiles, n_split, chunk, fits
 int main() {
     long long nh, nkv, hd, q, kv;
     while (scanf("%lld %lld %lld %lld %lld", &nh, &nkv, &hd, &q, &kv) == 5) {
         const Q4Plan p = q4_plan(nh, nkv, hd, q, kv, 256);
-        printf("%d %d %d %d %d %d\n", (int)p.prompt, p.G, p.groups, p.tiles, p.n_split, p.chunk);
+        printf("%d %d %d %d %d %d %d\n", (int)p.prompt, p.G, p.groups, p.tiles, p.n_split, p.chunk, (int)q4_fits(p, nh, hd, q));
     }
 }
 """
@@ -84,7 +84,7 @@ def plan(tmp_path_factory):
     def run(shapes):
         text = "".join(" ".join(map(str, s)) + "\n" for s in shapes)
         out = subprocess.run([exe], input=text, capture_output=True, text=True, check=True).stdout.splitlines()
-        return [dict(zip(("prompt", "G", "groups", "tiles", "n_split", "chunk"), map(int, o.split()))) for o in out]
+        return [dict(zip(("prompt", "G", "groups", "tiles", "n_split", "chunk", "fits"), map(int, o.split()))) for o in out]
     return run
 
 
@@ -119,3 +119,14 @@ def test_splits_of_every_length(plan, tmp_path):
 def test_a_piece_may_be_longer_than_a_million(plan):
     """(the call of test_gpu_kv_edges.py's test of it)"""
     assert [(p["n_split"], p["chunk"] > 2 ** 20) for p in plan([(4, 1, 64, 6150, 2 ** 20 + 5000)])] == [(1, True)]
+
+
+def test_calls_whose_launches_fit(plan):
+    """Fewer than 2^32 threads each: the kernel's workgroups have 256, the merge's four waves of 256 values."""
+    shapes = [(32, 8, 128, 2048, 2048), (2 ** 24 - 1, 2 ** 24 + 16, 64, 1, 1), (2 ** 24, 2 ** 24 + 16, 64, 1, 1),
+              (16, 1, 64, 65535, LONGEST), (16, 1, 64, 60000, LONGEST), (65535, 1, 64, 1, LONGEST), (32, 8, 128, 65535, 100000)]
+    plans = plan(shapes)
+    for (heads, _, hd, rows, _), p in zip(shapes, plans):
+        grids = [p["n_split"] * p["tiles"] * p["groups"]] + [((heads * hd + 255) // 256 * rows + 3) // 4] * (p["n_split"] > 1)
+        assert p["fits"] == (max(grids) * 256 < 2 ** 32)
+    assert [p["fits"] for p in plans] == [1, 1, 0, 0, 1, 1, 1]

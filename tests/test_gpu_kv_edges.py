@@ -165,3 +165,32 @@ def test_eviction_of_more_rows_than_a_launch_moves():
     be.close()
     del x, out, mass
     torch.cuda.empty_cache()
+
+
+def test_attention_of_more_heads_than_a_launch_has_workgroups_for(be):
+    """2^24 workgroups of 256 threads are refused; one head less is done (a single position: its V row)."""
+    import torch
+    n_kv, hd = 2 ** 24 + 16, 64
+    v = torch.randint(-7, 8, (n_kv, 1, hd), device="cuda", dtype=torch.int8).float()
+    v[:, :, ::32] = -8   # the blocks' scale is 1, and they hold these values
+    q = torch.ones((n_kv, 1, hd), device="cuda")
+    out = torch.full((n_kv, hd), 9.0, device="cuda")
+    c = A.KVCache(be, 8, 1, n_kv, hd, type=B.Q4_0)
+    torch.cuda.synchronize()
+    c.append(0, v, v, 1, hd)
+    for heads in (2 ** 24, 2 ** 24 - 1):
+        args = (be.h, q.data_ptr(), c.c, 0, heads, n_kv, hd, 1, 1, 0, out.data_ptr(), B.MEM_DEVICE)
+        if heads == 2 ** 24:
+            with pytest.raises(B.BarqError) as e:
+                B._lib.check(be._lib.barq_rocm_attention(*args))
+            assert e.value.code == B.E_DIM
+        else:
+            B._lib.check(be._lib.barq_rocm_attention(*args))
+        be.sync()
+        assert torch.all(out[heads:] == 9)
+    at = torch.arange(heads, device="cuda") * n_kv // heads
+    # one weight, which is no power of two, and one row: the steps of 2^-23 counted in test_scores_up_to_the_largest
+    assert torch.all((out[:heads] - v[at, 0]).abs() <= 8 * 2.0 ** -23 * 8)
+    c.close()
+    del v, q, out, at
+    torch.cuda.empty_cache()
