@@ -194,3 +194,74 @@ def test_attention_of_more_heads_than_a_launch_has_workgroups_for(be):
     c.close()
     del v, q, out, at
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,n,total", prompt_calls((8, 2, 64, 33, 233), (8, 2, 64, 70, 270), (8, 2, 128, 33, 233), (8, 2, 128, 70, 270)))
+def test_prompt_queries_of_every_size(be, heads, n_kv, hd, n, total):
+    """Rows with elements of very different sizes, all tiny, all huge, zero."""
+    q, k, v = rows(1, heads, n, hd), rows(2, n_kv, total, hd), rows(3, n_kv, total, hd)
+    q[0] *= 1e-30
+    q[1] *= 2.0 ** -np.arange(hd)
+    q[2] = 0
+    q[3, :, 7] = 1e25
+    k[0, :, 7] = 0
+    q[4] *= 1e-38
+    q[5, :, ::2] = 0
+    c, k, v = cache(be, B.Q4_0, k, v)
+    ref, _ = attention(q, k, v, total - n)
+    got = A.compute_attention(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n).cpu().numpy()
+    assert np.max(np.abs(got - ref)) <= 2e-5 * np.max(np.abs(v))
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,n,total", prompt_calls((4, 2, 64, 64, 200), (4, 2, 64, 100, 200), (4, 2, 128, 70, 200)))
+def test_prompt_nan_rows_reach_only_those_that_see_them(be, heads, n_kv, hd, n, total):
+    k, v, q = rows(7, n_kv, total, hd), rows(8, n_kv, total, hd), rows(9, heads, n, hd)
+    v[0, 190, 3] = np.inf        # one block of kv head 0
+    v[1, 40, 50] = np.nan
+    k[1, 195, 1] = np.nan        # a whole row of scores
+    c, k, v = cache(be, B.Q4_0, k, v)
+    for start in (total - n, total - 20 - n, 0):
+        ref, _ = attention(q, k, v, start)
+        got = A.compute_attention(be, dev(q), c, 0, heads, n_kv, hd, n, total, start).cpu().numpy()
+        assert np.array_equal(np.isnan(got), np.isnan(ref))
+        assert np.max(np.abs(np.nan_to_num(got) - np.nan_to_num(ref))) <= 2e-5 * np.nanmax(np.abs(v))
+
+
+def sizes(q, k, v, start):
+    """sum of p |V|, per row, head and dim: what a relative error of the weights multiplies."""
+    return attention(q, k, np.abs(v), start)[0]
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,n,total", prompt_calls((4, 1, 64, 40, 500), (4, 1, 128, 70, 500)))
+def test_prompt_spread_scores_and_values(be, heads, n_kv, hd, n, total):
+    """A position that takes nearly all the weight of some rows and adds nothing, queries and values of very
+    different sizes."""
+    k, v, q = rows(10, n_kv, total, hd), rows(11, n_kv, total, hd), rows(12, heads, n, hd)
+    v[0, 0] = 0
+    q[0] = q[0, :1]
+    k[0, 0] = 4 * q[0, 0]
+    q[1] *= 1e-20
+    q[2, :, 5] = 1e20
+    k[:, :, 5] = 0
+    v[0, 100:, :32] *= 2.0 ** -20
+    c, k, v = cache(be, B.Q4_0, k, v)
+    ref, _ = attention(q, k, v, total - n)
+    got = A.compute_attention(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n).cpu().numpy()
+    # scores reach 4 |q|^2 / sqrt(hd) * log2(e), about 65 with 128 dims, off by 96 * 2^-24 of it (3.7e-4) at most in log2 units
+    assert np.all(np.abs(got - ref) <= 4e-4 * sizes(q, k, v, total - n) + 1e-30)
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,n,total", prompt_calls((2, 1, 64, 64, 200), (2, 1, 128, 90, 200)))
+@pytest.mark.parametrize("peak", [60, 140, 1000])
+def test_prompt_weights_down_to_the_least(be, heads, n_kv, hd, n, total, peak):
+    """Scores that fall evenly from 0 to -peak (log2) over the positions, shuffled."""
+    q = np.zeros((heads, n, hd), F32)
+    q[:, :, 0] = 1
+    k, v = np.zeros((n_kv, total, hd), F32), rows(13, n_kv, total, hd)
+    k[0, :, 0] = -np.random.default_rng(1).permutation(total) * peak / total * np.log(2) * np.sqrt(hd)
+    v[0, np.argmax(k[0, :, 0])] = 0
+    c, k, v = cache(be, B.Q4_0, k, v)
+    ref, _ = attention(q, k, v, total - n)
+    got = A.compute_attention(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n).cpu().numpy()
+    # one product a score: its three roundings and the exponent's (2^-23 of peak each) and 2^-20 for the rest
+    assert np.all(np.abs(got - ref) <= (4 * peak * 2.0 ** -23 + 2.0 ** -20) * sizes(q, k, v, total - n) + 1e-37)
