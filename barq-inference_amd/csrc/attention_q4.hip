@@ -5,12 +5,12 @@
 // 16 rows a workgroup (one decoded token: its G heads); the positions are split
 // over workgroups and, in steps of 32, over the four waves of one.
 //
-// What bounds it: vector issue.  A step of 128 dims takes about 375 vector
+// What bounds it: vector issue.  A step of 128 dims takes about 380 vector
 // instructions (K's codes to f16 72, V's codes and scales to hi and lo 136, the
 // scores' scales and O's sums 64, the softmax and the weights' split the rest)
 // beside 40 MFMAs of 16 cycles, for 4.5 KB of the cache, and a 16-column product
 // serves the G rows alone.  One row of 32/8 heads of 128 dims against 65536
-// positions (75.5 MB): 24.7 us and 3.8 for the merge, 3.1 TB/s (vector issue 59 % and
+// positions (75.5 MB): 25.0 us and 3.8 for the merge, 3.0 TB/s (vector issue 59 % and
 // the matrix unit 18 % busy, counted at 26.2); 4096 positions 6.5 + 3.8 (first bytes
 // and launches); five rows of 16/16 heads of 256 against 3003 14.9 + 3.8 (one step a wave).
 #include "attention_q4.hpp"

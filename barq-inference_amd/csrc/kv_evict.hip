@@ -18,12 +18,15 @@
 // 6000.  Stores from where a thread finds a position, without the list, took
 // 14400, and the zeros behind the kept masses, one a thread at a time, 4800.
 //
-// The rows then move in one launch, bound by memory: f32 rows as they are (2048
-// of 8 heads of 128 dims 6.6 us, 33.6 MB at 5.1 TB/s); of a 4-bit cache, whose
-// tiles hold 8 positions of V in one dword per dim, a thread builds the dwords of
-// a tile's dims from those of its 8 sources, which reads V's codes up to eight
-// times (4096 of 16384 positions 8.1 us, 9.4 MB and the rest of the tiles' lines).  In place they go
-// by way of the workspace (5.4 us back): a row may move onto one that is still to be read.
+// The rows then move in one launch (more where a launch would pass 2^32 threads), bound by
+// memory: f32 rows as they are (2048 of 8 heads of 128 dims 7.0 us, 33.6 MB at
+// 4.8 TB/s); of a 4-bit cache, whose tiles hold 8 positions of V in one dword per
+// dim, a thread builds the dwords of a tile's dims from those of its 8 sources,
+// which reads V's codes up to eight times (4096 of 16384 positions 7.7 us, 9.4 MB and
+// the rest of the tiles' lines).  In place they go by way of the workspace, since a row may
+// move onto one that is still to be read, and back: the 2048 f32 rows 6.5 us, 4096
+// 4-bit ones 4.6.  A budget's own step, 2112 positions to 2048, takes 7.1 + 4.8
+// + 3.2 us in 4 bits and 7.1 + 7.2 + 6.5 in f32.
 #include "common.hpp"
 #include "kv_evict_plan.hpp"
 #include "kv_q4.hpp"

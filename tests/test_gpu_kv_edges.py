@@ -265,3 +265,17 @@ def test_prompt_weights_down_to_the_least(be, heads, n_kv, hd, n, total, peak):
     got = A.compute_attention(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n).cpu().numpy()
     # one product a score: its three roundings and the exponent's (2^-23 of peak each) and 2^-20 for the rest
     assert np.all(np.abs(got - ref) <= (4 * peak * 2.0 ** -23 + 2.0 ** -20) * sizes(q, k, v, total - n) + 1e-37)
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,n,total", [(4, 2, 64, 1, 1), (4, 2, 128, 1, 300), (4, 2, 256, 30, 200)] +
+                         prompt_calls((8, 2, 64, 40, 200), (8, 2, 128, 64, 500)))
+def test_values_near_f16s_least(be, heads, n_kv, hd, n, total):
+    """V rows of 2^-12 down to 2^-28, some rows of 1.  Beside the weights' errors an output is off by 2^-36 at most:
+    three sums of products a step, each cut at 2^-24, under a largest weight of 2^14 to 2^15."""
+    q, k, v = rows(1, heads, n, hd), rows(2, n_kv, total, hd), rows(3, n_kv, total, hd)
+    v *= np.exp2(np.random.default_rng(4).integers(-28, -12, (n_kv, total, 1))).astype(F32)
+    v[:, 7::50] = rows(5, *v[:, 7::50].shape)
+    c, k, v = cache(be, B.Q4_0, k, v)
+    ref, _ = attention(q, k, v, total - n)
+    got = A.compute_attention(be, dev(q), c, 0, heads, n_kv, hd, n, total, total - n).cpu().numpy()
+    assert np.all(np.abs(got - ref) <= 2 * 2.4e-5 * sizes(q, k, v, total - n) + 2.0 ** -36)
