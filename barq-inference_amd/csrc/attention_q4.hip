@@ -100,7 +100,7 @@ struct Q4Stage {
 // NaN at the end.  (0 * NaN would reach rows that do not.)
 template <int HD, bool SC>
 __device__ __forceinline__ void q4_step(const Q4Stage<HD>& s, int base, int j1, const Q4Seen& seen, const Q4Query<HD>& q,
-                                        bool exact, const Q4Const& kc, Q4State<HD>& st, float* score_row,
+                                        float lost, const Q4Const& kc, Q4State<HD>& st, float* score_row,
                                         int* nan_at) {
     float x[8];
     uint32_t kw[2][HD / 32];
@@ -111,7 +111,7 @@ __device__ __forceinline__ void q4_step(const Q4Stage<HD>& s, int base, int j1, 
         if (fresh) asm volatile("" : "+v"(w));
         return q4_k_frag(w, kc);
     };
-    q4_scores<HD>(x, q, exact, kfrag, [&](int b) { return *s.scale(0, b); });
+    q4_scores<HD>(x, q, lost, kfrag, [&](int b) { return *s.scale(0, b); });
     const int at = base + 8 * s.g;
     if (base + Q4A_STEP > j1) {   // the range's last step: what lies behind it is not the cache's
         u32x4v m;
@@ -148,7 +148,7 @@ __device__ __forceinline__ void q4_step(const Q4Stage<HD>& s, int base, int j1, 
 // A wave's steps of positions j0 .. j1: every `turn` positions from the first.
 template <int HD, bool SC>
 __device__ __forceinline__ void q4_walk(const Q4Fifo<HD>& fifo, uint8_t* lds, int j0, int j1, int first, int turn, int l,
-                                        const Q4Seen& seen, const Q4Query<HD>& q, bool exact, const Q4Const& kc,
+                                        const Q4Seen& seen, const Q4Query<HD>& q, float lost, const Q4Const& kc,
                                         Q4State<HD>& st, float* score_row, int* nan_at) {
     st.clear();
     const int n = j1 - j0;
@@ -160,7 +160,7 @@ __device__ __forceinline__ void q4_walk(const Q4Fifo<HD>& fifo, uint8_t* lds, in
         wait_vmcnt<Q4Fifo<HD>::COPIES>();
         asm volatile("" ::: "memory");
         const Q4Stage<HD> s{lds + stage * Q4Fifo<HD>::STAGE, l & 15, l >> 4};
-        q4_step<HD, SC>(s, j0 + at, j1, seen, q, exact, kc, st, score_row, nan_at);
+        q4_step<HD, SC>(s, j0 + at, j1, seen, q, lost, kc, st, score_row, nan_at);
     }
     wait_vmcnt<0>();   // nothing on its way to LDS any more
     asm volatile("" ::: "memory");
@@ -192,12 +192,12 @@ void attn_q4_kernel(Q4Args a) {
     const Q4Row row = q4_row(a, grp, r0 + c);
     const Q4Seen seen{min(row.vis, j1), min(q4_vis(a, r0), j1)};
     Q4Query<HD> q;
-    const bool exact = __any(q.load(a.q + ((size_t)row.h * a.q_rows + row.i) * HD, a.scale, g, kc));
+    const float lost = uniform(row16_max(q.load(a.q + ((size_t)row.h * a.q_rows + row.i) * HD, a.scale, g, kc)));
     float* const score_row = SC && row.ok ? a.scores + ((size_t)row.i * a.n_head + row.h) * a.score_stride : nullptr;
     Q4State<HD> st;
     int* nan_at = nullptr;
     for (;;) {
-        q4_walk<HD, SC>(fifo, mine, j0, j1, wave * Q4A_STEP, Q4A_NW * Q4A_STEP, l, seen, q, exact, kc, st, score_row, nan_at);
+        q4_walk<HD, SC>(fifo, mine, j0, j1, wave * Q4A_STEP, Q4A_NW * Q4A_STEP, l, seen, q, lost, kc, st, score_row, nan_at);
         if (nan_at || !__any(st.not_finite())) break;
         // NaN somewhere: again with V's NaN blocks kept out of the products
         nan_at = nan_pos[wave];

@@ -17,10 +17,10 @@
 // [2^14, 2^15) and split into two f16 values, off by at most 2^-23 of an element
 // down to 2^-17 of the largest and by 2^-40 of the largest below that.  (A normal
 // query has such an element in one row of 300.)  What that can do to a score is
-// bounded by the keys' largest value, 65504, whatever else the row and the keys hold;
-// where the bound passes 2^-20 in log2 units the wave forms its scores from three
-// bf16 values instead, which hold any f32 exactly: with 128 dims from one such
-// element on beside a largest one of 64 or more, from 32 on beside one of 2 to 4.
+// bounded by the keys' scales; where the bound passes 2^-20 in log2 units the wave
+// forms the step's scores from three bf16 values instead, which hold any f32
+// exactly.  With the largest key there may be (65504) and 128 dims that is from one such
+// element on beside a largest one of 64 or more; with keys up to 64 beside one of 2^16.
 // The products are exact, the sums f32, the block's scale joins in
 // f32 and the row's in the exponent's fma.
 // A V element (code - 8) * d has 15 bits and is exactly hi + lo in f16: all
@@ -131,15 +131,21 @@ __device__ __forceinline__ float groups_sum(float v) {
     return swap32_add(v, v);
 }
 
+// A value that all lanes hold, in a scalar register.
+__device__ __forceinline__ float uniform(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+
 // The lane's part of a query row: hi + lo.
 template <int HD>
 struct Q4Query {
     h8v hi[HD / 32], lo[HD / 32];
     const float* at;     // its dims 0 .. 7 of block 0
     float scale, back;   // what the row is multiplied by; scores times back are in log2 units
-    // true if the split may lose 2^-20 of a score (log2 units): each element below
-    // 2^-2 is off by 2^-25 at most there, its key is at most 8 * Q4_D_MAX < 2^16
-    __device__ __forceinline__ bool load(const float* row, float score_scale, int g, const Q4Const& kc) {
+    // Returns what the split may cost a score (log2 units), in steps of 2^-22 times the
+    // keys' largest scale: each element below 2^-2 is off by 2^-25 at most, its key is
+    // at most 8 scales.
+    __device__ __forceinline__ float load(const float* row, float score_scale, int g, const Q4Const& kc) {
         at = row + 8 * g;
         float4 y[HD / 16];
         float m = 0.0f;
@@ -174,7 +180,7 @@ struct Q4Query {
             hi[b] = __builtin_bit_cast(h8v, h);
             lo[b] = __builtin_bit_cast(h8v, l);
         }
-        return groups_sum(small) * back > 0x1p-11f;   // 2^(-20 + 25 - 16)
+        return groups_sum(small) * back;
     }
     // block b in three bf16 values, which hold any f32 exactly
     __device__ __forceinline__ void exact(int b, bf8v (&p)[3]) const {
@@ -226,14 +232,29 @@ struct Q4Seen {
     int all;   // every row of its tile sees the positions up to here
 };
 
-// The scores of the tile's rows (times their scale).  kfrag(t, b, fresh): K
+// The scores of the tile's rows (times their scale).  lost: the largest of what the
+// rows' load returned, in a scalar register.  kfrag(t, b, fresh): K
 // codes minus 8 of S tile t, block b, as f16 (fresh: not values it gave before,
 // which would stay in registers between the calls); kscale(b): the group's 8
 // positions' scales.
 template <int HD, class K, class S>
-__device__ __forceinline__ void q4_scores(float (&x)[8], const Q4Query<HD>& q, bool exact, K kfrag, S kscale) {
+__device__ __forceinline__ void q4_scores(float (&x)[8], const Q4Query<HD>& q, float lost, K kfrag, S kscale) {
     #pragma unroll
     for (int e = 0; e < 8; e++) x[e] = 0.0f;
+    bool exact = false;
+    if (lost * Q4_D_MAX > 4.0f) {   // 2^(-20 + 22)
+        h2v m = {};
+        #pragma unroll
+        for (int b = 0; b < HD / 32; b++) {
+            const u32x4v d = kscale(b);
+            #pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const uint32_t pair = d[j] & 0x7FFF7FFFu;
+                m = __builtin_elementwise_max(m, __builtin_bit_cast(h2v, pair));   // (a NaN is passed over: its scores are NaN either way)
+            }
+        }
+        exact = __any(fmaxf((float)m[0], (float)m[1]) * lost > 4.0f);
+    }
     if (exact) {
         #pragma unroll
         for (int b = 0; b < HD / 32; b++) {

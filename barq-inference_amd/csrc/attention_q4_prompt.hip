@@ -132,7 +132,7 @@ void attn_q4_prompt_kernel(Q4Args a) {
     const Q4Row row = q4_row(a, grp, r0 + c);
     const Q4Seen seen{min(row.vis, j1), min(q4_vis(a, r0), j1)};
     Q4Query<HD> q;
-    const bool exact = __any(q.load(a.q + ((size_t)row.h * a.q_rows + row.i) * HD, a.scale, g, kx));
+    const float lost = uniform(row16_max(q.load(a.q + ((size_t)row.h * a.q_rows + row.i) * HD, a.scale, g, kx)));
     float* const score_row = SC && row.ok ? a.scores + ((size_t)row.i * a.n_head + row.h) * a.score_stride : nullptr;
     Q4State<HD> st;
     st.clear();
@@ -147,7 +147,7 @@ void attn_q4_prompt_kernel(Q4Args a) {
         if (base >= mine) continue;
         const uint8_t* s = lds + (b & 1) * B::STAGE;
         float x[8];
-        q4_scores<HD>(x, q, exact,
+        q4_scores<HD>(x, q, lost,
                       [&](int t, int b, bool) { return *reinterpret_cast<const h8v*>(s + 1024 * (t * B::NB + b) + 16 * l); },
                       [&](int b) { return *reinterpret_cast<const u32x4v*>(s + B::KS + 16 * (g * B::NB + b)); });
         q4_attend<HD, SC>(x, base, base + 8 * g, seen, q, kx, st, score_row, [&](int c, h8v& hi, h8v& lo) {
