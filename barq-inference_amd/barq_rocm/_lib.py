@@ -68,6 +68,9 @@ EXPORTS = (
     "barq_rocm_kv_cache_append_rope_q", "barq_rocm_attention_q8k", "barq_rocm_matvec_group",
     "barq_rocm_qkv_append_rope", "barq_rocm_kv_cache_create_typed", "barq_rocm_kv_cache_type", "barq_rocm_kv_cache_read",
     "barq_rocm_kv_cache_evict", "barq_rocm_attention_mass", "barq_rocm_matmul_noalloc", "barq_rocm_stream_read",
+    "barq_rocm_rope_frequencies", "barq_rocm_norm_rope", "barq_rocm_paged_cache_create", "barq_rocm_paged_cache_destroy",
+    "barq_rocm_paged_batch_create", "barq_rocm_paged_batch_destroy", "barq_rocm_paged_batch_set", "barq_rocm_paged_append",
+    "barq_rocm_paged_read", "barq_rocm_paged_attention",
 )
 
 # bytes of the fixed per-GPU scratch behind barq_rocm_matmul_noalloc
@@ -75,6 +78,9 @@ NOALLOC_SCRATCH_BYTES = 32 << 20
 
 ROPE_INTERLEAVED = 0
 ROPE_SPLIT_HALF = 1
+
+# how rope_frequencies stretches a context
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = range(4)
 
 
 class BarqError(RuntimeError):
@@ -90,6 +96,12 @@ _sz = ctypes.c_size_t
 _i = ctypes.c_int
 _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
+
+
+class RotaryArg(ctypes.Structure):
+    """barq_rocm_rotary"""
+    _fields_ = [("rot_dim", _sz), ("layout", _i), ("freq_scale", ctypes.c_float), ("magnitude", ctypes.c_float),
+                ("inv_freq", _vp)]
 
 
 def _declare(lib):
@@ -168,6 +180,16 @@ def _declare(lib):
         "barq_rocm_qkv_append_rope": (_i, [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _i, _vp, _vp, _sz, ctypes.c_float, _vp,
                                            _i, _i]),
         "barq_rocm_matmul_noalloc": (_i, [_vp, _i, _vp, _sz, _sz, _i, _vp, _sz, _vp]),
+        "barq_rocm_rope_frequencies": (_i, [_i, _sz] + [ctypes.c_double] * 5 + [_vp, ctypes.POINTER(ctypes.c_float)]),
+        "barq_rocm_norm_rope": (_i, [_vp, _vp, _sz, _sz, _sz, _sz, _vp, ctypes.c_float, ctypes.POINTER(RotaryArg), _vp, _i]),
+        "barq_rocm_paged_cache_create": (_i, [_vp, _sz, _sz, _sz, _sz, _sz, _i, ctypes.POINTER(_vp)]),
+        "barq_rocm_paged_cache_destroy": (_i, [_vp]),
+        "barq_rocm_paged_batch_create": (_i, [_vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, ctypes.POINTER(_vp)]),
+        "barq_rocm_paged_batch_destroy": (_i, [_vp]),
+        "barq_rocm_paged_batch_set": (_i, [_vp, _vp, _sz, _vp, _vp, _vp, _sz]),
+        "barq_rocm_paged_append": (_i, [_vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, ctypes.POINTER(RotaryArg), _i]),
+        "barq_rocm_paged_read": (_i, [_vp, _vp, _sz, _vp, _vp, _i]),
+        "barq_rocm_paged_attention": (_i, [_vp, _vp, _sz, _vp, _i, _vp, _i]),
     }
     for name, (res, args) in P.items():
         fn = getattr(lib, name)

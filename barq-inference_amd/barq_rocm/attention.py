@@ -56,6 +56,48 @@ def transpose_heads(be: Backend, x, seq_len, n_heads, head_dim, mem=L.MEM_DEVICE
     return out
 
 
+class Rotary:
+    """The rotation of a head's first rot_dim dims (barq_rocm_rotary): pair i
+    turns by position * freq_scale * inv_freq[i].  inv_freq lives where the calls'
+    `mem` says."""
+
+    def __init__(self, inv_freq, rot_dim, layout=ROPE_INTERLEAVED, freq_scale=1.0, magnitude=1.0):
+        if tuple(inv_freq.shape) != (rot_dim // 2,) or not str(inv_freq.dtype).endswith("float32"):
+            raise L.BarqError(L.E_DIM, f"Rotary: inv_freq must be {rot_dim // 2} float32 values")
+        self.inv_freq = inv_freq   # (kept alive: the argument below has its address)
+        self.arg = L.RotaryArg(rot_dim, layout, freq_scale, magnitude, _ptr(inv_freq) or None)
+
+    @classmethod
+    def scaled(cls, rot_dim, base, layout=ROPE_INTERLEAVED, scaling=L.ROPE_PLAIN, factor=1.0, trained=0.0, fast=32.0, slow=1.0,
+               mem=L.MEM_DEVICE, device="cuda"):
+        """The frequencies of barq_rocm_rope_frequencies."""
+        f, m = rope_frequencies(scaling, rot_dim, base, factor, trained, fast, slow)
+        if mem == L.MEM_DEVICE:
+            import torch
+            f = torch.from_numpy(f).to(device)
+        return cls(f, rot_dim, layout, magnitude=m)
+
+
+def rope_frequencies(scaling, rot_dim, base, factor=1.0, trained=0.0, fast=32.0, slow=1.0):
+    """barq_rocm_rope_frequencies: (inv_freq [rot_dim / 2] float32, magnitude)."""
+    f, m = np.empty(rot_dim // 2, np.float32), ctypes.c_float()
+    L.check(L.lib().barq_rocm_rope_frequencies(scaling, rot_dim, base, factor, trained, fast, slow, _ptr(f) or None, ctypes.byref(m)))
+    return f, m.value
+
+
+def norm_rope(be: Backend, x, seq_len, n_heads, head_dim, start_pos, rotary=None, norm=None, eps=1e-5, mem=L.MEM_DEVICE,
+              sync=True, out=None):
+    """RMSNorm of each head (with norm) and the rotation, in one pass: x
+    [seq, n_heads*head_dim] -> [n_heads, seq, head_dim]."""
+    if out is None:
+        out = _empty((n_heads, seq_len, head_dim), x, mem)
+    L.check(be._lib.barq_rocm_norm_rope(be.h, _ptr(x), seq_len, n_heads, head_dim, start_pos, _ptr(norm), eps,
+                                        ctypes.byref(rotary.arg) if rotary is not None else None, _ptr(out), mem))
+    if sync and mem == L.MEM_DEVICE:
+        be.sync()
+    return out
+
+
 class KVCache:
     """KVCache (context.rs:245-340) in device memory, preallocated for
     max_size positions per layer and kv head; type F32, or Q4_0 for rows held

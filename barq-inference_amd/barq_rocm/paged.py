@@ -1,0 +1,139 @@
+"""The paged KV cache over the C ABI: a pool of pages, a step's batch of
+sequences, append with norm and rotation, attention.
+
+Device buffers are torch tensors, host buffers numpy arrays (``mem=MEM_HOST``).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+
+from . import _lib as L
+from .attention import _empty
+from .backend import Backend, _ptr
+
+
+def _rows(who, x, heads_dim, n_tokens):
+    """n_tokens rows of f32, side by side in memory."""
+    size = x.size if isinstance(x, np.ndarray) else x.numel()
+    flat = x.flags.c_contiguous if isinstance(x, np.ndarray) else x.is_contiguous()
+    if size != n_tokens * heads_dim:
+        raise L.BarqError(L.E_DIM, f"{who}: {size} values, {n_tokens} tokens of {heads_dim} are wanted")
+    if not flat or not str(x.dtype).endswith("float32"):
+        raise L.BarqError(L.E_INVALID, f"{who}: rows must be contiguous float32")
+
+
+class PagedCache:
+    """n_pages pages of page_size positions for each layer and kv head; type
+    F16 or F32."""
+
+    def __init__(self, be: Backend, n_pages: int, page_size: int, n_layers: int, n_head_kv: int, head_dim: int,
+                 type: int = L.F16):
+        self.be, self.c = be, None
+        c = ctypes.c_void_p()
+        L.check(be._lib.barq_rocm_paged_cache_create(be.h, n_pages, page_size, n_layers, n_head_kv, head_dim, type,
+                                                     ctypes.byref(c)))
+        self.c = c
+        self.n_pages, self.page_size, self.n_layers, self.n_head_kv, self.head_dim, self.type = (
+            n_pages, page_size, n_layers, n_head_kv, head_dim, type)
+
+    def close(self):
+        if self.c:
+            self.be._lib.barq_rocm_paged_cache_destroy(self.c)
+            self.c = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class PagedBatch:
+    """The sequences of one step (see barq_rocm_paged_batch_set) and the calls
+    on their new tokens.  window, n_sink: a query sees its last `window`
+    positions (0: all before it) and the first n_sink."""
+
+    def __init__(self, cache: PagedCache, n_head: int, max_seqs: int, max_tokens: int, max_pages: int, window: int = 0,
+                 n_sink: int = 0):
+        self.be, self.cache, self.b = cache.be, cache, None
+        b = ctypes.c_void_p()
+        L.check(self.be._lib.barq_rocm_paged_batch_create(self.be.h, cache.c, n_head, max_seqs, max_tokens, max_pages, window,
+                                                          n_sink, ctypes.byref(b)))
+        self.b = b
+        self.n_head, self.max_seqs, self.max_tokens, self.max_pages = n_head, max_seqs, max_tokens, max_pages
+        self.n_tokens = 0
+
+    def close(self):
+        if self.b:
+            self.be._lib.barq_rocm_paged_batch_destroy(self.b)
+            self.b = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def set(self, q_lens, kv_lens, pages):
+        """q_lens, kv_lens: one number a sequence; pages: [sequences, pages]
+        int32 (or a list of lists of ids), -1 where there is none."""
+        q = np.ascontiguousarray(q_lens, dtype=np.int32)
+        kv = np.ascontiguousarray(kv_lens, dtype=np.int32)
+        if not isinstance(pages, np.ndarray):
+            width = max((len(p) for p in pages), default=0)
+            table = np.full((len(pages), width), -1, np.int32)
+            for row, ids in zip(table, pages):
+                row[:len(ids)] = ids
+            pages = table
+        pages = np.ascontiguousarray(pages, dtype=np.int32)
+        if q.ndim != 1 or q.shape != kv.shape or pages.ndim != 2 or len(pages) != len(q):
+            raise L.BarqError(L.E_DIM, f"paged_batch_set: q_lens {q.shape}, kv_lens {kv.shape}, pages {pages.shape}")
+        L.check(self.be._lib.barq_rocm_paged_batch_set(self.be.h, self.b, len(q), _ptr(q), _ptr(kv), _ptr(pages), pages.shape[1]))
+        self.n_tokens = int(q.sum())
+
+    def append(self, layer, k, v, q=None, rotary=None, q_norm=None, k_norm=None, eps=1e-5, q_out=None, mem=L.MEM_DEVICE):
+        """k, v [n_tokens, n_head_kv*head_dim] into the layer's pages, k normed by
+        head (with k_norm) and rotated (with rotary); returns q [n_tokens,
+        n_head*head_dim] likewise, as [n_head, n_tokens, head_dim], or None."""
+        c, t = self.cache, self.n_tokens
+        for name, x, heads in (("q", q, self.n_head), ("k", k, c.n_head_kv), ("v", v, c.n_head_kv)):
+            if x is not None:
+                _rows(f"paged_append: {name}", x, heads * c.head_dim, t)
+        if q is not None and q_out is None:
+            q_out = _empty((self.n_head, t, c.head_dim), q, mem)
+        L.check(self.be._lib.barq_rocm_paged_append(self.be.h, self.b, layer, _ptr(q), _ptr(q_out), _ptr(k), _ptr(v), _ptr(q_norm),
+                                                    _ptr(k_norm), eps, ctypes.byref(rotary.arg) if rotary is not None else None,
+                                                    mem))
+        return q_out
+
+    def read(self, layer, mem=L.MEM_DEVICE, sync=True):
+        """The tokens' rows as the cache holds them: (k, v), each [n_tokens,
+        n_head_kv, head_dim] float16 or float32."""
+        c = self.cache
+        shape, dtype = (self.n_tokens, c.n_head_kv, c.head_dim), "float16" if c.type == L.F16 else "float32"
+        if mem == L.MEM_HOST:
+            k, v = np.empty(shape, dtype), np.empty(shape, dtype)
+        else:
+            import torch
+            dev = torch.device("cuda", self.be.device)
+            k, v = (torch.empty(shape, dtype=getattr(torch, dtype), device=dev) for _ in "kv")
+        L.check(self.be._lib.barq_rocm_paged_read(self.be.h, self.b, layer, _ptr(k), _ptr(v), mem))
+        if sync and mem == L.MEM_DEVICE:
+            self.be.sync()
+        return k, v
+
+    def attention(self, layer, q, out_type=L.F32, mem=L.MEM_DEVICE, sync=True, out=None):
+        """q [n_head, n_tokens, head_dim] -> [n_tokens, n_head, head_dim], or with
+        out_type Q8_K the rows' blocks, uint8 [n_tokens, n_head*head_dim/256 * 292]."""
+        c, t = self.cache, self.n_tokens
+        width = self.n_head * c.head_dim
+        _rows("paged_attention: q", q, width, t)
+        if out is None:
+            out = (_empty((t, self.n_head, c.head_dim), q, mem) if out_type == L.F32
+                   else _empty((t, width // 256 * 292), q, mem, dtype="uint8"))
+        L.check(self.be._lib.barq_rocm_paged_attention(self.be.h, self.b, layer, _ptr(q), out_type, _ptr(out), mem))
+        if sync and mem == L.MEM_DEVICE:
+            self.be.sync()
+        return out

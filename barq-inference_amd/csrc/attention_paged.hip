@@ -1,0 +1,445 @@
+// Attention over a paged KV cache for sequences with few rows (new tokens x the
+// query heads of a kv head): the next token, drafted tokens.  attention_paged.hpp
+// has the formulas and numerics.
+//
+// Bound by the reading of K and V.  A workgroup is four waves, each with key steps
+// of its own (every fourth of the item's), so nothing is shared and nothing waits
+// before the end: the pages' layout is the MFMA operands', 16 bytes a lane straight
+// into registers, the next step's in flight while this one is computed.  A step is
+// 32 positions in f16, 16 in f32: 16 KiB of K and V for 128 dims either way.
+#include "attention_paged.hpp"
+#include "q8k_block.hpp"
+
+namespace barq {
+
+namespace {
+
+constexpr int NW = 4;   // waves
+
+// Over the four lane groups (lanes l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float groups_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    v = fmaxf(__builtin_bit_cast(float, (int)a[0]), __builtin_bit_cast(float, (int)a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (int)b[0]), __builtin_bit_cast(float, (int)b[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+    v = swap16_add(v, v);
+    return swap32_add(v, v);
+}
+
+// A lane's part of one step: K of tile t (position 8 (i / 4) + 4 t + i % 4 of the
+// step in f16, i in f32, for lane i of its group), dims E (4 c + g) .. ; V of dim
+// 16 d + i, the group's E positions.
+template <bool H, int HD>
+struct Step {
+    static constexpr int KT = H ? 2 : 1, NC = H ? HD / 32 : HD / 16, NV = HD / 16;
+    u32x4v k[KT][NC], v[NV];
+};
+
+template <bool H, int HD>
+struct Query {
+    static constexpr int NC = H ? HD / 32 : HD / 16;
+    u32x4v hi[NC], lo[H ? NC : 1];   // f32: the values in hi
+    float back;
+    __device__ __forceinline__ void load(const float* row, float scale, int g) {
+        if constexpr (H) {
+            float x[NC][8], m = 0.0f;
+            #pragma unroll
+            for (int c = 0; c < NC; c++)
+                #pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float4 y = *reinterpret_cast<const float4*>(row + 8 * (4 * c + g) + 4 * u);
+                    const float w[4] = {y.x, y.y, y.z, y.w};
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        x[c][4 * u + e] = w[e] * scale;
+                        m = fmaxf(m, __builtin_fabsf(x[c][4 * u + e]));
+                    }
+                }
+            const float up = paged_row_scale(groups_max(m), back);
+            #pragma unroll
+            for (int c = 0; c < NC; c++)
+                #pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    uint32_t h, l;
+                    paged_split(x[c][2 * u] * up, x[c][2 * u + 1] * up, h, l);
+                    hi[c][u] = h;
+                    lo[c][u] = l;
+                }
+        } else {
+            back = 1.0f;
+            #pragma unroll
+            for (int c = 0; c < NC; c++) {
+                const float4 y = *reinterpret_cast<const float4*>(row + 4 * (4 * c + g));
+                const float w[4] = {y.x * scale, y.y * scale, y.z * scale, y.w * scale};
+                #pragma unroll
+                for (int u = 0; u < 4; u++) hi[c][u] = __builtin_bit_cast(uint32_t, w[u]);
+            }
+        }
+    }
+};
+
+// The scores of the lane's positions (log2 units): index 4 t + r is position 8 g + 4 t + r (f16), 4 g + r (f32).
+template <bool H, int HD>
+__device__ __forceinline__ void scores(const Step<H, HD>& st, const Query<H, HD>& q, float (&s)[4 * Step<H, HD>::KT]) {
+    constexpr int KT = Step<H, HD>::KT, NC = Step<H, HD>::NC;
+    #pragma unroll
+    for (int t = 0; t < KT; t++) {
+        f32x4 hi = {}, lo = {};
+        #pragma unroll
+        for (int c = 0; c < NC; c++) {
+            if constexpr (H) {
+                const h8v k = __builtin_bit_cast(h8v, st.k[t][c]);
+                lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(h8v, q.lo[c]), lo, 0, 0, 0);
+                hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(h8v, q.hi[c]), hi, 0, 0, 0);
+            } else {
+                const f32x4 k = __builtin_bit_cast(f32x4, st.k[t][c]), x = __builtin_bit_cast(f32x4, q.hi[c]);
+                #pragma unroll
+                for (int e = 0; e < 4; e++) hi = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], x[e], hi, 0, 0, 0);
+            }
+        }
+        #pragma unroll
+        for (int r = 0; r < 4; r++) s[4 * t + r] = H ? __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) * q.back : hi[r];
+    }
+}
+
+// V^T times the weights (or what stands for them) of the lane's positions, dims 16 d + 4 g + r of the lane's row.
+template <bool H>
+struct Weights {
+    u32x4v hi, lo;
+    float w[H ? 1 : 4];
+    __device__ __forceinline__ void set(const float* p, float minus_one) {
+        if constexpr (H) {
+            #pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t h, l;
+                split_f16(p[2 * j], p[2 * j + 1], minus_one, h, l);
+                hi[j] = h;
+                lo[j] = l;
+            }
+        } else {
+            #pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = p[j];
+        }
+    }
+    __device__ __forceinline__ f32x4 times(u32x4v v) const {
+        f32x4 acc = {};
+        if constexpr (H) {
+            const h8v a = __builtin_bit_cast(h8v, v);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(h8v, lo), acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(h8v, hi), acc, 0, 0, 0);
+        } else {
+            const f32x4 a = __builtin_bit_cast(f32x4, v);
+            #pragma unroll
+            for (int j = 0; j < 4; j++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], w[j], acc, 0, 0, 0);
+        }
+        return acc;
+    }
+};
+
+// NT tiles of 16 rows.
+template <bool H, int HD, int NT>
+__global__ __launch_bounds__(64 * NW, HD == 256 || NT == 2 ? 1 : 2)
+void paged_few_kernel(PagedAttn a, int first, int count) {
+    constexpr int STEP = H ? 32 : 16, E = H ? 8 : 4, KT = H ? 2 : 1, NV = HD / 16, NP = 4 * KT;
+    constexpr int ROW = HD + 4;   // floats of a row in LDS: 16-byte pieces, the four groups in other banks
+    constexpr size_t BLOCK = (size_t)PAGE_BLOCK * HD * (H ? 2 : 4);
+    __shared__ __align__(16) float o_s[NW][16][ROW];
+    __shared__ float m_s[NW][16 * NT], l_s[NW][16 * NT];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+    int n_tokens = a.n_tokens;
+    if (n_tokens < 0) {
+        n_tokens = a.counts->n_tokens;
+        first = NT == 1 ? 0 : a.counts->few16;
+        count = (NT == 1 ? a.counts->few16 : a.counts->few) - first;
+    }
+    const float minus_one = f16_minus_one();
+    const PagedSight sight = {a.window, a.n_sink};
+    const size_t page_bytes = BLOCK << (a.log_page - 4);   // of one kv head
+    for (int w = blockIdx.x; w < count * a.n_kv; w += gridDim.x) {
+        const int hk = w % a.n_kv;
+        const PagedItem it = a.few[first + w / a.n_kv];
+        Query<H, HD> q[NT];
+        int pos[NT];
+        #pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int r = it.row0 + min(16 * n + i, it.rows - 1), tok = r / a.G, head = hk * a.G + r % a.G;
+            pos[n] = it.past + tok;
+            q[n].load(a.q + ((size_t)head * n_tokens + it.q0 + tok) * HD, a.scale, g);
+        }
+        const int p_first = it.past + it.row0 / a.G, p_last = it.past + (it.row0 + it.rows - 1) / a.G;
+        float m[NT], l[NT];
+        f32x4 o[NT][NV];
+        #pragma unroll
+        for (int n = 0; n < NT; n++) {
+            m[n] = -INFINITY;
+            l[n] = 0.0f;
+            #pragma unroll
+            for (int d = 0; d < NV; d++) o[n][d] = f32x4{};
+        }
+        const int32_t* table = a.table + it.table;
+        const int steps = (it.v1 - it.v0 - wave + NW - 1) / NW;   // this wave's (none: 0 or less)
+        const auto base_of = [&](int j) {
+            const int v = it.v0 + wave + NW * j;
+            return (v < it.a ? v : v - it.a + it.b) * STEP;
+        };
+        // lane j holds the pages of the wave's step 64 n + j, of its first 16 positions and (f16) of the others
+        int id0 = -1, id1 = -1;
+        const auto fetch_ids = [&](int j0) {
+            id0 = id1 = -1;
+            const int j = j0 + lane;
+            if (j < steps) {
+                const int at = base_of(j);
+                id0 = table[at >> a.log_page];
+                if (H && at + 16 < it.kv_len) id1 = table[(at + 16) >> a.log_page];
+            }
+        };
+        const auto block_at = [&](const uint8_t* pool, int id, int at) {   // (an absent page: the first one, unseen)
+            return pool + ((size_t)max(id, 0) * a.n_kv + hk) * page_bytes + (size_t)((at & ((1 << a.log_page) - 1)) >> 4) * BLOCK;
+        };
+        Step<H, HD> st[2];
+        int page0[2], page1[2];
+        const auto load = [&](int j, int x) __attribute__((always_inline)) {
+            if (j >= steps) return;
+            if ((j & 63) == 0) fetch_ids(j);
+            const int at = base_of(j), p0 = __builtin_amdgcn_readlane(id0, j & 63), p1 = __builtin_amdgcn_readlane(id1, j & 63);
+            page0[x] = p0;
+            page1[x] = p1;
+            const uint8_t *k0 = block_at(a.k, p0, at), *v0 = block_at(a.v, p0, at);
+            const uint8_t *kb = k0, *vb = v0;
+            if (H) {
+                const uint8_t *k1 = block_at(a.k, p1, at + 16), *v1 = block_at(a.v, p1, at + 16);
+                kb = i < 8 ? k0 : k1;
+                vb = g < 2 ? v0 : v1;
+            }
+            #pragma unroll
+            for (int t = 0; t < KT; t++) {
+                const int slot = H ? (8 * (i >> 2) + 4 * t + (i & 3)) & 15 : i;
+                #pragma unroll
+                for (int c = 0; c < Step<H, HD>::NC; c++)
+                    st[x].k[t][c] = *reinterpret_cast<const u32x4v*>(kb + ((4 * c + g) * 16 + slot) * 16);
+            }
+            #pragma unroll
+            for (int d = 0; d < NV; d++)
+                st[x].v[d] = *reinterpret_cast<const u32x4v*>(vb + ((H ? g & 1 : g) * HD + 16 * d + i) * 16);
+        };
+        const auto compute = [&](int j, int x) __attribute__((always_inline)) {
+            const int base = base_of(j);
+            const bool here0 = page0[x] >= 0, here1 = H ? page1[x] >= 0 : here0;
+            const bool whole = here0 && here1 && sight.all(base, STEP, p_first, p_last);
+            bool seen[NT][NP];
+            bool nan_v = false;
+            if (!whole) {
+                #pragma unroll
+                for (int n = 0; n < NT; n++)
+                    #pragma unroll
+                    for (int e = 0; e < NP; e++)   // (a group's positions lie in one block)
+                        seen[n][e] = (H && g >= 2 ? here1 : here0) && sight.sees(pos[n], base + E * g + e);
+                #pragma unroll
+                for (int d = 0; d < NV; d++)
+                    #pragma unroll
+                    for (int u = 0; u < 4; u++) nan_v |= (H ? f16_bad(st[x].v[d][u]) : f32_bad(st[x].v[d][u])) != 0;
+            }
+            const bool bad = __any(nan_v);
+            #pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float s[NP];
+                scores<H, HD>(st[x], q[n], s);
+                if (!whole) {
+                    #pragma unroll
+                    for (int e = 0; e < NP; e++) s[e] = seen[n][e] ? s[e] : -INFINITY;
+                }
+                float top = s[0];
+                #pragma unroll
+                for (int e = 1; e < NP; e++) top = fmaxf(top, s[e]);
+                top = fmaxf(m[n], groups_max(top));
+                const float ref = top == -INFINITY ? 0.0f : top, shift = H ? ref - 15.0f : ref;
+                const float alpha = paged_exp2(m[n] - ref);
+                m[n] = top;
+                float sum = 0.0f;
+                #pragma unroll
+                for (int e = 0; e < NP; e++) {
+                    s[e] = paged_exp2(s[e] - shift);
+                    sum += s[e];
+                }
+                l[n] = __builtin_fmaf(l[n], alpha, sum);
+                Weights<H> p;
+                p.set(s, minus_one);
+                if (!bad) {
+                    #pragma unroll
+                    for (int d = 0; d < NV; d++) {
+                        const f32x4 y = p.times(st[x].v[d]);
+                        #pragma unroll
+                        for (int r = 0; r < 4; r++) o[n][d][r] = __builtin_fmaf(o[n][d][r], alpha, y[r]);
+                    }
+                } else {
+                    Weights<H> ones;
+                    float z[NP];
+                    #pragma unroll
+                    for (int e = 0; e < NP; e++) z[e] = seen[n][e] ? 1.0f : 0.0f;
+                    ones.set(z, minus_one);
+                    #pragma unroll
+                    for (int d = 0; d < NV; d++) {
+                        u32x4v v = st[x].v[d], is;
+                        #pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const uint32_t b = H ? f16_bad(v[u]) : f32_bad(v[u]);
+                            v[u] &= ~b;
+                            is[u] = b & (H ? 0x3C003C00u : 0x3F800000u);
+                        }
+                        const f32x4 y = p.times(v), nan = ones.times(is);
+                        #pragma unroll
+                        for (int r = 0; r < 4; r++) o[n][d][r] = nan[r] > 0.0f ? NAN : __builtin_fmaf(o[n][d][r], alpha, y[r]);
+                    }
+                }
+            }
+        };
+        load(0, 0);
+        for (int j = 0; j < steps; j += 2) {
+            load(j + 1, 1);
+            compute(j, 0);
+            if (j + 1 >= steps) break;
+            load(j + 2, 0);
+            compute(j + 1, 1);
+        }
+        // the four waves' states, joined
+        #pragma unroll
+        for (int n = 0; n < NT; n++) {
+            l[n] = groups_sum(l[n]);
+            if (g == 0) {
+                m_s[wave][16 * n + i] = m[n];
+                l_s[wave][16 * n + i] = l[n];
+            }
+        }
+        __syncthreads();
+        #pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int at = 16 * n + i;
+            float top = m_s[0][at];
+            #pragma unroll
+            for (int u = 1; u < NW; u++) top = fmaxf(top, m_s[u][at]);
+            const float mine = m[n] == -INFINITY ? 1.0f : paged_exp2(m[n] - top);   // (1: o is zero, or NaN and stays it)
+            #pragma unroll
+            for (int d = 0; d < NV; d++) {
+                f32x4 y;
+                #pragma unroll
+                for (int r = 0; r < 4; r++) y[r] = o[n][d][r] * mine;
+                *reinterpret_cast<f32x4*>(&o_s[wave][i][16 * d + 4 * g]) = y;
+            }
+            __syncthreads();
+            for (int u = threadIdx.x; u < 16 * (HD / 4); u += 64 * NW) {
+                const int row = u / (HD / 4), d = 4 * (u % (HD / 4)), r = 16 * n + row;
+                if (r < it.rows) {
+                    float t = m_s[0][r];
+                    #pragma unroll
+                    for (int x = 1; x < NW; x++) t = fmaxf(t, m_s[x][r]);
+                    float sum = 0.0f;
+                    #pragma unroll
+                    for (int x = 0; x < NW; x++) sum = __builtin_fmaf(l_s[x][r], m_s[x][r] == -INFINITY ? 1.0f : paged_exp2(m_s[x][r] - t), sum);
+                    f32x4 y = *reinterpret_cast<const f32x4*>(&o_s[0][row][d]);
+                    #pragma unroll
+                    for (int x = 1; x < NW; x++) y += *reinterpret_cast<const f32x4*>(&o_s[x][row][d]);
+                    if (it.part < 0) {
+                        const int rr = it.row0 + r, tok = it.q0 + rr / a.G, head = hk * a.G + rr % a.G;
+                        float* out = a.out + ((size_t)tok * a.n_head + head) * HD + d;
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) out[e] = sum == 0.0f ? 0.0f : y[e] / sum;
+                    } else {
+                        const size_t row_at = (size_t)hk * a.part_rows + it.part + r;
+                        *reinterpret_cast<f32x4*>(a.part + row_at * HD + d) = y;
+                        if (d == 0) a.stat[row_at] = make_float2(t, sum);
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+// Joins the partial states of rows that several workgroups share: a wave a row.
+template <int HD>
+__global__ __launch_bounds__(64 * NW)
+void paged_merge_kernel(PagedAttn a) {
+    constexpr int PER = HD / 64, AHEAD = 8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int merges = a.n_tokens < 0 ? a.counts->merges : a.n_merges, hk = blockIdx.y, span = a.merge_span;
+    for (int w = blockIdx.x; w < merges * span; w += gridDim.x) {
+        const PagedMerge mg = a.merges[w / span];
+        const int r = (w % span) * NW + wave;
+        if (r >= mg.rows) continue;
+        const size_t at = (size_t)hk * a.part_rows + mg.part + r;
+        float top = -INFINITY;
+        for (int s = lane; s < mg.n_split; s += 64) top = fmaxf(top, a.stat[at + (size_t)s * mg.rows].x);
+        top = wave_max_all(top);
+        float sum = 0.0f, y[PER];
+        #pragma unroll
+        for (int e = 0; e < PER; e++) y[e] = 0.0f;
+        for (int s0 = 0; s0 < mg.n_split; s0 += AHEAD) {
+            float x[AHEAD][PER];
+            float2 z[AHEAD];
+            #pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                const int s = min(s0 + u, mg.n_split - 1);
+                z[u] = a.stat[at + (size_t)s * mg.rows];
+                #pragma unroll
+                for (int e = 0; e < PER; e++) x[u][e] = a.part[(at + (size_t)s * mg.rows) * HD + lane * PER + e];
+            }
+            #pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                if (s0 + u >= mg.n_split) break;
+                const float f = z[u].x == -INFINITY ? 1.0f : paged_exp2(z[u].x - top);   // (1: zeros, or NaN)
+                sum = __builtin_fmaf(z[u].y, f, sum);
+                #pragma unroll
+                for (int e = 0; e < PER; e++) y[e] = __builtin_fmaf(x[u][e], f, y[e]);
+            }
+        }
+        const int rr = mg.row0 + r, tok = mg.q0 + rr / a.G, head = hk * a.G + rr % a.G;
+        float* out = a.out + ((size_t)tok * a.n_head + head) * HD + lane * PER;
+        #pragma unroll
+        for (int e = 0; e < PER; e++) out[e] = sum == 0.0f ? 0.0f : y[e] / sum;
+    }
+}
+
+// The output rows as Q8_K blocks: a wave a block.
+__global__ __launch_bounds__(64 * NW)
+void paged_q8k_kernel(const float* __restrict__ rows, uint8_t* __restrict__ out, int n_tokens, int blocks, const PagedCounts* counts) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const size_t n = (size_t)(n_tokens < 0 ? counts->n_tokens : n_tokens) * blocks;
+    for (size_t b = (size_t)blockIdx.x * NW + wave; b < n; b += (size_t)gridDim.x * NW) {
+        const float4 v = reinterpret_cast<const float4*>(rows + b * 256)[lane];
+        const float x[4] = {v.x, v.y, v.z, v.w};
+        q8_k_block(x, lane, out + b * Q8_K_BYTES);
+    }
+}
+
+}  // namespace
+
+hipError_t paged_attention_launch(const PagedAttn& a, bool f16, int hd, hipStream_t s) {
+    // A captured call replays with other counts: its grids are fixed, their workgroups go round the items.
+    const bool captured = a.n_tokens < 0;
+    const auto grid = [&](int n) { return dim3(captured ? 1024u : (unsigned)n * (unsigned)a.n_kv); };
+    const int few32 = a.n_few - a.n_few16;
+    #define BARQ_FEW(H, D)                                                                                                      \
+        if (f16 == H && hd == D) {                                                                                              \
+            if (captured || a.n_few16) hipLaunchKernelGGL((paged_few_kernel<H, D, 1>), grid(a.n_few16), dim3(256), 0, s, a, 0, a.n_few16); \
+            if (captured || few32) hipLaunchKernelGGL((paged_few_kernel<H, D, 2>), grid(few32), dim3(256), 0, s, a, a.n_few16, few32);    \
+        }
+    BARQ_FEW(true, 64) BARQ_FEW(true, 128) BARQ_FEW(true, 256)
+    BARQ_FEW(false, 64) BARQ_FEW(false, 128) BARQ_FEW(false, 256)
+    #undef BARQ_FEW
+    if (captured || a.n_merges) {
+        const dim3 g(captured ? 256u : (unsigned)a.n_merges * (unsigned)a.merge_span, (unsigned)a.n_kv);
+        if (hd == 64) hipLaunchKernelGGL(paged_merge_kernel<64>, g, dim3(256), 0, s, a);
+        if (hd == 128) hipLaunchKernelGGL(paged_merge_kernel<128>, g, dim3(256), 0, s, a);
+        if (hd == 256) hipLaunchKernelGGL(paged_merge_kernel<256>, g, dim3(256), 0, s, a);
+    }
+    if (a.out_q8) {
+        const size_t blocks = (size_t)a.n_head * hd / 256, n = (captured ? 256 : (size_t)a.n_tokens) * blocks;
+        hipLaunchKernelGGL(paged_q8k_kernel, dim3((unsigned)((n + NW - 1) / NW < 8192 ? (n + NW - 1) / NW : 8192)), dim3(256), 0, s, a.out,
+                           a.out_q8, a.n_tokens, (int)blocks, a.counts);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace barq

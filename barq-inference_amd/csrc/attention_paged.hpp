@@ -1,0 +1,76 @@
+// What the kernels of attention over a paged cache share (attention_paged.hip:
+// few rows of a sequence, attention_paged_many.hip: many).
+//
+// Row r of a sequence and kv head (new token r / G at position p, query head r % G):
+//   s_j = (q . K[j]) / sqrt(HD)   for j <= p and, with a window, j > p - window or j < first tokens, j's page there
+//   out = sum_j exp(s_j - max) V[j] / sum_j exp(s_j - max), zero where no j is left
+// S^T = K Q^T and O^T += V^T P^T on the matrix cores, so that a query is a lane's
+// column throughout: its maximum, sum and rescaling need no exchange but the one
+// over the lane groups, and P^T is already PV's operand.
+//
+// Numerics over an f16 cache (f32 results of f32 queries).  K and V are exact f16
+// operands.  A query row times scale log2(e) is multiplied by a power of two so
+// that its largest element is in [2^14, 2^15) and split into hi + 2^-11 lo, two
+// f16 values whose products have sums of their own: an element is off by 2^-23
+// of itself down to 2^-29 of the row's largest, by 2^-52 of the largest below that.
+// A weight exp2(s - max + 15), at most 2^15, is split into two f16 values likewise
+// but joined in one sum: it is off by 2^-23 of itself down to 2^-17 of the row's
+// largest weight, by 2^-40 of the largest below that.  That is half of the matrix rate for results
+// that one f16 value a weight would have at 2^-12.  The MFMA's f32 sums are not rounded to
+// nearest, so each step's start from zero and join O in one fma.
+// Over an f32 cache all products are the f32 MFMA's, an eighth of the rate
+// of split f16 with three products but with nothing to bound.
+//
+// V in unseen places: a weight of zero keeps finite values out, not NaN.  Steps
+// that some row does not see all of replace what is not finite by zero, and put
+// NaN where a row does see one.
+#pragma once
+#include "common.hpp"
+#include "f16_split.hpp"
+#include "launch.hpp"
+#include "mfma_common.hpp"
+#include "paged.hpp"
+
+namespace barq {
+
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float paged_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// What a row sees.
+struct PagedSight {
+    int window, n_sink;
+    __device__ __forceinline__ bool sees(int row_pos, int j) const {
+        return j <= row_pos && (!window || j > row_pos - window || j < n_sink);
+    }
+    // all positions base .. base + n - 1 by all rows at positions first .. last
+    __device__ __forceinline__ bool all(int base, int n, int first, int last) const {
+        return base + n - 1 <= first && (!window || base > last - window || base + n <= n_sink);
+    }
+};
+
+// Scale of a query row (a power of two) whose largest |element| is m; 1 / it.
+__device__ __forceinline__ float paged_row_scale(float m, float& back) {
+    // at least 2^-100 and below infinity, so that both are normal f32 values
+    uint32_t e = __builtin_bit_cast(uint32_t, m) >> 23;
+    e = e < 27u ? 27u : e > 254u ? 254u : e;
+    back = __builtin_bit_cast(float, (e - 14u) << 23);
+    return __builtin_bit_cast(float, (254u + 14u - e) << 23);
+}
+
+// x -> f16 hi and f16 of (x - hi) 2^11
+__device__ __forceinline__ void paged_split(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const h2v h = {(_Float16)x0, (_Float16)x1};
+    const h2v l = {(_Float16)((x0 - (float)h[0]) * 2048.0f), (_Float16)((x1 - (float)h[1]) * 2048.0f)};
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, l);
+}
+
+// The f16 halves of a dword that are not finite, as 0xFFFF each.
+__device__ __forceinline__ uint32_t f16_bad(uint32_t x) {
+    return ((((x & 0x7C007C00u) + 0x04000400u) >> 15) & 0x00010001u) * 0xFFFFu;
+}
+__device__ __forceinline__ uint32_t f32_bad(uint32_t x) { return (x & 0x7F800000u) == 0x7F800000u ? 0xFFFFFFFFu : 0u; }
+
+}  // namespace barq

@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include "kv_q4.hpp"
+#include "paged.hpp"
 
 namespace barq {
 
@@ -286,5 +287,60 @@ hipError_t attn_prompt_launch(const AttnArgs& a, hipStream_t s);
 bool attn_prompt_scores_path(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);
 size_t attn_prompt_scores_workspace(size_t n_head, size_t n_head_kv, size_t head_dim, size_t q_len, size_t kv_len);
 hipError_t attn_prompt_scores_launch(const AttnArgs& a, const AttnScores& sc, float2* stat, hipStream_t s);
+
+// ---- the paged cache (paged_append.hip, attention_paged.hip) ----
+// The rotation of a head's first `rot` dims (0: none): see rotary.hpp.
+struct Rotary {
+    const float* inv_freq;
+    int rot, layout;
+    float freq_scale, magnitude;
+};
+struct PagedAppend {
+    const float *q, *k, *v;        // [n_tokens, heads * hd]; q with n_q 0: none
+    const float *q_norm, *k_norm;  // [hd] or null
+    float* q_out;                  // [n_q, n_tokens, hd]
+    uint8_t *k_pool, *v_pool;      // the layer's pages
+    const PagedToken* tokens;
+    const PagedCounts* counts;
+    int n_tokens;                  // -1: counts has them (a captured call)
+    int n_q, n_kv, log_page;
+    float eps;
+    Rotary rotary;
+};
+hipError_t paged_append_launch(const PagedAppend& a, bool f16, size_t hd, hipStream_t s);
+// the tokens' rows in the cache's type, [n_tokens, n_kv, hd]; either output may be null
+hipError_t paged_read_launch(const PagedAppend& a, bool f16, size_t hd, void* k_out, void* v_out, hipStream_t s);
+hipError_t norm_rope_launch(const float* x, float* out, size_t seq, size_t heads, size_t hd, size_t start_pos,
+                            const float* w, float eps, const Rotary& r, hipStream_t s);
+// Up to six pieces (bytes a multiple of 16) from host memory that the device can read.
+struct PagedPieces {
+    int n;
+    const uint8_t* src;
+    uint8_t* dst[6];
+    uint32_t from[6], bytes[6];
+};
+hipError_t paged_upload_launch(const PagedPieces& p, hipStream_t s);
+struct PagedAttn {
+    const float* q;        // [n_head, n_tokens, hd]
+    float* out;            // [n_tokens, n_head, hd]
+    uint8_t* out_q8;       // or null: the rows as Q8_K blocks too
+    const uint8_t* k;      // the layer's pages
+    const uint8_t* v;
+    const int32_t* table;
+    const PagedItem* few;
+    const PagedItem* many;
+    const PagedMerge* merges;
+    const PagedCounts* counts;
+    int n_tokens;          // -1: counts has them (a captured call)
+    int n_few16, n_few, n_many, n_merges;
+    int merge_span;        // workgroups of four rows that a merge takes
+    int n_head, n_kv, G, log_page;
+    int window, n_sink;
+    float scale;           // log2(e) / sqrt(hd)
+    float* part;           // [n_kv][part_rows][hd]
+    float2* stat;          // [n_kv][part_rows]: maximum (log2 units), sum
+    size_t part_rows;
+};
+hipError_t paged_attention_launch(const PagedAttn& a, bool f16, int hd, hipStream_t s);
 
 }  // namespace barq

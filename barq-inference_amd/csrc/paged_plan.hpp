@@ -1,0 +1,175 @@
+// How a step's attention over a paged cache is cut into workgroups (host).
+//
+// A sequence's rows (new tokens x query heads of a kv head) are cut into tiles of
+// 16, 32 (the kernel for few rows) or 128 (for many); a tile's rows see the key
+// positions [0, first tokens) and [window's start, last row's position], counted
+// in the kernel's steps.  Where there are fewer tiles than the card has room for,
+// the tiles' steps are split, evenly over all of them, so that the longest
+// workgroup is about the mean one; what the splits leave is merged.
+#pragma once
+#include <algorithm>
+#include <cstdint>
+#include <cstdio>
+#include <vector>
+
+#include "paged.hpp"
+
+namespace barq {
+
+struct PagedShape {
+    int G = 1, n_kv = 1;          // query heads of a kv head, kv heads
+    int64_t window = 0, n_sink = 0;
+    int few_step = 32, many_step = 64;   // positions of a kernel's step
+    int64_t many_from = 65;       // rows from which a sequence's tiles are the large ones
+    int64_t few_target = 1024, many_target = 512;   // workgroups that fill the card
+    int64_t few_least = 4, many_least = 4;          // steps that a split has at least
+    size_t part_rows = 0;         // partial states there is room for, for each kv head
+};
+
+struct PagedSeq {
+    int64_t q_len, kv_len, table;
+};
+
+struct PagedPlan {
+    std::vector<PagedItem> few, many;
+    std::vector<PagedMerge> merges;
+    int few16 = 0;
+};
+
+struct PagedLimits {
+    size_t max_seqs, max_tokens, max_pages, n_pages, page_size;
+};
+
+enum class PagedFault { none, dim, invalid };
+
+// What is wrong with a step's arrays (said in msg), none if nothing is; then tokens, and entries of the page table.
+// stamp has one value a page, none of them `number`: the pages that take new tokens get it.
+inline PagedFault paged_check(const PagedLimits& lim, size_t n_seqs, const int32_t* q_len, const int32_t* kv_len,
+                              const int32_t* pages, size_t stride, uint32_t* stamp, uint32_t number, size_t& tokens,
+                              size_t& entries, char* msg, size_t room) {
+    constexpr int32_t most = 0x7ffff000;   // positions: a step past the last one stays an int
+    tokens = entries = 0;
+    if (n_seqs > lim.max_seqs) {
+        snprintf(msg, room, "%zu sequences, the batch has room for %zu", n_seqs, lim.max_seqs);
+        return PagedFault::dim;
+    }
+    if (n_seqs && (!q_len || !kv_len || !pages)) {
+        snprintf(msg, room, "null array");
+        return PagedFault::invalid;
+    }
+    for (size_t s = 0; s < n_seqs; s++) {
+        if (q_len[s] < 0 || kv_len[s] < q_len[s] || kv_len[s] > most) {
+            snprintf(msg, room, "sequence %zu: %d new tokens, kv_len %d (with them; at most 2^31 - 4096)", s, q_len[s], kv_len[s]);
+            return PagedFault::dim;
+        }
+        const size_t n = ((size_t)kv_len[s] + lim.page_size - 1) / lim.page_size;
+        if (n > lim.max_pages || n > stride) {
+            snprintf(msg, room, "sequence %zu needs %zu pages: the batch has room for %zu, the table has %zu", s, n, lim.max_pages, stride);
+            return PagedFault::dim;
+        }
+        tokens += (size_t)q_len[s];
+        entries += n;
+        const size_t written = ((size_t)kv_len[s] - (size_t)q_len[s]) / lim.page_size;
+        for (size_t i = 0; i < n; i++) {
+            const int32_t id = pages[s * stride + i];
+            if (id < -1 || (id >= 0 && (size_t)id >= lim.n_pages)) {
+                snprintf(msg, room, "sequence %zu: page %zu is %d, the cache has %zu (-1: none)", s, i, id, lim.n_pages);
+                return PagedFault::invalid;
+            }
+            if (id >= 0 && q_len[s] && i >= written) {
+                if (stamp[id] == number) {
+                    snprintf(msg, room, "sequence %zu: page %d takes new tokens in two places", s, id);
+                    return PagedFault::invalid;
+                }
+                stamp[id] = number;
+            }
+        }
+    }
+    if (tokens > lim.max_tokens) {
+        snprintf(msg, room, "%zu new tokens, the batch has room for %zu", tokens, lim.max_tokens);
+        return PagedFault::dim;
+    }
+    return PagedFault::none;
+}
+
+// The most items and merges that a plan of these limits has.
+inline size_t paged_max_tiles(size_t max_seqs, size_t max_tokens, size_t G) { return (max_tokens * G + 15) / 16 + max_seqs; }
+
+// The kernels' steps for a type and head_dim, and from how many rows the one for many is taken.
+inline void paged_shape_for(PagedShape& sh, bool f16, size_t hd) {
+    (void)hd;
+    sh.few_step = f16 ? 32 : 16;
+    sh.many_from = INT64_MAX;
+}
+
+// Partial states to have room for (of each kv head): 64 MiB of them with 128 dims at most.
+inline size_t paged_part_rows(const PagedShape& sh, size_t max_tokens) {
+    const size_t splits = 2 * (size_t)std::max(sh.few_target, sh.many_target) / sh.n_kv + 2;
+    return std::min(max_tokens * sh.G * splits, std::max<size_t>(131072 / sh.n_kv, 256));
+}
+
+inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, PagedPlan& p) {
+    p.few.clear();
+    p.many.clear();
+    p.merges.clear();
+    int64_t steps[2] = {0, 0}, q0 = 0;
+    for (const PagedSeq& s : seqs) {
+        const int64_t rows = s.q_len * sh.G, past = s.kv_len - s.q_len;
+        const bool many = rows >= sh.many_from;
+        const int64_t tile = many ? 128 : rows <= 16 ? 16 : 32, unit = many ? sh.many_step : sh.few_step;
+        for (int64_t r = 0; r < rows; r += tile) {
+            PagedItem it{};
+            it.q0 = (int32_t)q0;
+            it.past = (int32_t)past;
+            it.kv_len = (int32_t)s.kv_len;
+            it.table = (int32_t)s.table;
+            it.row0 = (int32_t)r;
+            it.rows = (int32_t)std::min(tile, rows - r);
+            const int64_t first = past + r / sh.G, end = past + (r + it.rows - 1) / sh.G + 1;
+            const int64_t low = sh.window ? std::max<int64_t>(first - sh.window + 1, 0) / unit : 0;
+            it.a = (int32_t)std::min((std::min(sh.n_sink, end) + unit - 1) / unit, low);
+            it.b = (int32_t)low;
+            it.v1 = (int32_t)(it.a + (end + unit - 1) / unit - low);
+            it.part = -1;
+            steps[many] += it.v1;
+            (many ? p.many : p.few).push_back(it);
+        }
+        q0 += s.q_len;
+    }
+    size_t part = 0;
+    for (int kind = 0; kind < 2; kind++) {
+        std::vector<PagedItem>& items = kind ? p.many : p.few;
+        const int64_t target = std::max<int64_t>((kind ? sh.many_target : sh.few_target) / sh.n_kv, 1);
+        const int64_t least = kind ? sh.many_least : sh.few_least;
+        if (!items.empty() && (int64_t)items.size() < target) {
+            const int64_t each = std::max((steps[kind] + target - 1) / target, least);
+            std::vector<PagedItem> cut;
+            for (const PagedItem& it : items) {
+                int64_t n = std::max<int64_t>((it.v1 + each - 1) / each, 1);
+                n = std::min<int64_t>(n, (int64_t)((sh.part_rows - part) / (size_t)it.rows));
+                if (n < 2) {
+                    cut.push_back(it);
+                    continue;
+                }
+                p.merges.push_back({it.q0, it.row0, it.rows, (int32_t)part, (int32_t)n, {0, 0, 0}});
+                for (int64_t i = 0; i < n; i++) {
+                    PagedItem c = it;
+                    c.v0 = (int32_t)(it.v1 * i / n);
+                    c.v1 = (int32_t)(it.v1 * (i + 1) / n);
+                    c.part = (int32_t)part;
+                    part += (size_t)it.rows;
+                    cut.push_back(c);
+                }
+            }
+            items.swap(cut);
+        }
+        // the longest first: the last workgroups to start are short ones
+        std::stable_sort(items.begin(), items.end(), [kind](const PagedItem& x, const PagedItem& y) {
+            if (!kind && (x.rows <= 16) != (y.rows <= 16)) return x.rows <= 16;
+            return x.v1 - x.v0 > y.v1 - y.v0;
+        });
+    }
+    p.few16 = (int)(std::find_if(p.few.begin(), p.few.end(), [](const PagedItem& x) { return x.rows > 16; }) - p.few.begin());
+}
+
+}  // namespace barq

@@ -523,6 +523,104 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
                              size_t start_pos, int out_type, void* out, const float* mass_in, float* mass_out,
                              size_t mass_stride, int mem);
 
+/* ---- paged KV cache ---------------------------------------------------------
+ * For servers that answer many sequences at once (the reference keeps the
+ * bookkeeping of such a cache, advanced/src/paged_attention.rs, and its
+ * attention on the CPU).  The pool holds n_pages pages of page_size positions (a power
+ * of two, 16 to 65536) for every layer and kv head, as BARQ_TYPE_F16 or
+ * BARQ_TYPE_F32; head_dim 64, 128 or 256.  Who has which page is the caller's
+ * to keep.  f16 rounds to nearest (ties to even), finite values beyond +-65504
+ * are kept as that; NaN and infinities are kept as NaN in either type.
+ *
+ * A batch describes one step: n_seqs sequences, of each the number of new tokens
+ * q_len (0 is fine), its positions kv_len with the new ones (the last q_len
+ * positions), and its page ids, ceil(kv_len / page_size) of them (pages + s *
+ * pages_stride; host arrays).  -1 is no page: positions on it are seen by no
+ * query, tokens there are not kept and read as zeros.  A page may belong to several
+ * sequences (a shared prefix), but only one may add tokens to it.  The
+ * attention's window (0: none) and number of first tokens that stay visible
+ * (n_sink, with a window) belong to the batch, as its plan goes by them: a query
+ * at position p sees positions j <= p with j > p - window or j < n_sink.  A model whose
+ * layers differ keeps a batch for each kind.  n_head is a multiple of the
+ * cache's kv heads; query head h reads kv head h * n_head_kv / n_head.
+ *
+ * batch_set is enqueued on the handle's stream like the calls below, which all
+ * work on the latest set's tokens, sequence after sequence (n_tokens = the sum of
+ * q_len).  It fails without changing the batch where an array does not fit it, and on
+ * a stream that is being captured.  Calls captured in a graph replay with
+ * whatever batch_set gave since, so n_tokens may change within the batch's limits
+ * (q, out and the other buffers are then those of that many tokens;
+ * rows behind them are left as they are).  A batch has its own scratch memory: calls on one batch must be ordered by the caller,
+ * calls on different batches need not be.  A cache's memory lives until the
+ * cache and all its batches are destroyed. */
+typedef struct barq_rocm_paged_cache barq_rocm_paged_cache;
+typedef struct barq_rocm_paged_batch barq_rocm_paged_batch;
+int barq_rocm_paged_cache_create(barq_rocm_handle* h, size_t n_pages, size_t page_size, size_t n_layers,
+                                 size_t n_head_kv, size_t head_dim, int type, barq_rocm_paged_cache** out);
+int barq_rocm_paged_cache_destroy(barq_rocm_paged_cache* c);
+int barq_rocm_paged_batch_create(barq_rocm_handle* h, barq_rocm_paged_cache* c, size_t n_head, size_t max_seqs,
+                                 size_t max_tokens, size_t max_pages, size_t window, size_t n_sink,
+                                 barq_rocm_paged_batch** out);
+int barq_rocm_paged_batch_destroy(barq_rocm_paged_batch* b);
+int barq_rocm_paged_batch_set(barq_rocm_handle* h, barq_rocm_paged_batch* b, size_t n_seqs, const int32_t* q_len,
+                              const int32_t* kv_len, const int32_t* pages, size_t pages_stride);
+
+/* The rotation of the first rot_dim dims of a head (even, at most head_dim; 0 or
+ * a null pointer: none): pair i turns by position * freq_scale * inv_freq[i],
+ * formed in 64 bits; cos and sin are multiplied by magnitude.  Pairs as for
+ * barq_rocm_rope within the rot_dim dims (interleaved: 2 i and 2 i + 1, split half: i and i +
+ * rot_dim / 2); the dims behind them stay.  inv_freq [rot_dim / 2] lives where the call's `mem` says.
+ * rope_frequencies fills inv_freq and magnitude (host) for contexts of `factor`
+ * times the length that the model was trained on:
+ *   PLAIN   base^(-2 i / rot_dim)
+ *   LINEAR  that / factor (every position is divided by it)
+ *   NTK     PLAIN with base * factor^(rot_dim / (rot_dim - 2)): the fastest pair stays, the slowest is LINEAR's
+ *   YARN    with turns = trained * PLAIN / (2 pi), the turns of a pair in the trained context, and keep = (turns - slow) / (fast - slow)
+ *           within 0 and 1: PLAIN * keep + LINEAR * (1 - keep); magnitude 0.1 ln(factor) + 1
+ *           (Peng et al., "YaRN", 2023; fast 32 and slow 1 there)
+ * magnitude is 1 for the others, which do not read trained, fast and slow (PLAIN nor factor).
+ * The reference's counterpart is advanced/src/rope_scaling.rs:13-160. */
+#define BARQ_ROPE_PLAIN 0
+#define BARQ_ROPE_LINEAR 1
+#define BARQ_ROPE_NTK 2
+#define BARQ_ROPE_YARN 3
+typedef struct {
+    size_t rot_dim;
+    int layout;
+    float freq_scale;
+    float magnitude;
+    const float* inv_freq;
+} barq_rocm_rotary;
+int barq_rocm_rope_frequencies(int scaling, size_t rot_dim, double base, double factor, double trained, double fast,
+                               double slow, float* inv_freq, float* magnitude);
+
+/* norm_rope = RMSNorm of every head (norm [head_dim] or NULL: none; eps as in
+ * barq_rocm_rms_norm) and the rotation, in one pass: x [seq_len, n_heads *
+ * head_dim] -> out [n_heads, seq_len, head_dim], which must not overlap.  For models with
+ * norms of their queries and keys whose session has a cache of its own.
+ * paged_append = the same on q (into q_out [n_head, n_tokens, head_dim]; both NULL: no q)
+ * and k, then k and v (projections [n_tokens, n_head_kv * head_dim]) into the
+ * layer's pages.  A token's position is its place in its sequence.
+ * paged_read = the rows that the cache holds of the batch's tokens, in its type:
+ * [n_tokens, n_head_kv, head_dim] each; either may be NULL.  (A batch with q_len =
+ * kv_len reads whole sequences.)
+ * paged_attention = the attention of the batch's tokens, q [n_head, n_tokens,
+ * head_dim], over their sequences' pages: out [n_tokens, n_head, head_dim] f32
+ * (out_type BARQ_TYPE_F32), or its rows as Q8_K blocks (BARQ_TYPE_Q8_K: n_head * head_dim a
+ * multiple of 256; the bytes barq_rocm_quantize_act writes for them).  A query that sees no position
+ * gives zeros.  Softmax statistics and sums are f32.  Over an f16 cache a query element counts to 2^-23 of itself or 2^-52 of
+ * its row's largest, a weight to 2^-23 of itself or 2^-40 of its row's largest, whichever is more.
+ * Device buffers: q, q_out, k, v, x and norm_rope's out 16-byte aligned, the others 4-byte. */
+int barq_rocm_norm_rope(barq_rocm_handle* h, const float* x, size_t seq_len, size_t n_heads, size_t head_dim,
+                        size_t start_pos, const float* norm, float eps, const barq_rocm_rotary* rotary, float* out,
+                        int mem);
+int barq_rocm_paged_append(barq_rocm_handle* h, barq_rocm_paged_batch* b, size_t layer, const float* q, float* q_out,
+                           const float* k, const float* v, const float* q_norm, const float* k_norm, float eps,
+                           const barq_rocm_rotary* rotary, int mem);
+int barq_rocm_paged_read(barq_rocm_handle* h, const barq_rocm_paged_batch* b, size_t layer, void* k, void* v, int mem);
+int barq_rocm_paged_attention(barq_rocm_handle* h, barq_rocm_paged_batch* b, size_t layer, const float* q, int out_type,
+                              void* out, int mem);
+
 /* ---- measurement ------------------------------------------------------------
  * No counterpart in the reference.  Reads bytes (rounded down to 16) at the
  * device pointer p once, with coalesced non-temporal loads and nothing else:
