@@ -159,7 +159,7 @@ void paged_few_kernel(PagedAttn a, int first, int count) {
     const size_t page_bytes = BLOCK << (a.log_page - 4);   // of one kv head
     for (int w = blockIdx.x; w < count * a.n_kv; w += gridDim.x) {
         const int hk = w % a.n_kv;
-        const PagedItem it = a.few[first + w / a.n_kv];
+        const PagedItem it = paged_item(&a.few[first + w / a.n_kv]);
         Query<H, HD> q[NT];
         int pos[NT];
         #pragma unroll
@@ -428,6 +428,10 @@ hipError_t paged_attention_launch(const PagedAttn& a, bool f16, int hd, hipStrea
     BARQ_FEW(true, 64) BARQ_FEW(true, 128) BARQ_FEW(true, 256)
     BARQ_FEW(false, 64) BARQ_FEW(false, 128) BARQ_FEW(false, 256)
     #undef BARQ_FEW
+    if (captured || a.n_many) {
+        const hipError_t e = paged_many_launch(a, f16, hd, s);
+        if (e != hipSuccess) return e;
+    }
     if (captured || a.n_merges) {
         const dim3 g(captured ? 256u : (unsigned)a.n_merges * (unsigned)a.merge_span, (unsigned)a.n_kv);
         if (hd == 64) hipLaunchKernelGGL(paged_merge_kernel<64>, g, dim3(256), 0, s, a);

@@ -38,6 +38,16 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float paged_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// An item, in scalar registers.
+__device__ __forceinline__ PagedItem paged_item(const PagedItem* p) {
+    PagedItem it;
+    const int* from = reinterpret_cast<const int*>(p);
+    int* to = reinterpret_cast<int*>(&it);
+    #pragma unroll
+    for (int i = 0; i < 11; i++) to[i] = __builtin_amdgcn_readfirstlane(from[i]);
+    return it;
+}
+
 // What a row sees.
 struct PagedSight {
     int window, n_sink;

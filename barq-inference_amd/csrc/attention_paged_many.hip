@@ -1,0 +1,323 @@
+// Attention over a paged KV cache for sequences with many rows (new tokens x the
+// query heads of a kv head): prompts and their chunks.  attention_paged.hpp has the
+// formulas and numerics.
+//
+// Bound by the matrix products: two of f16 for each of an f32 result's.  A workgroup
+// is four waves of 32 rows each, the queries in registers; a step's K and V (64 positions in
+// f16, 32 in f32) come by direct loads into one of two LDS buffers while the other is
+// computed on.  The pages' blocks are the MFMA operands' layout already, so they
+// are copied as they lie and read without bank conflicts: wave w fetches block w.
+#include "attention_paged.hpp"
+
+namespace barq {
+
+namespace {
+
+constexpr int NW = 4;   // waves
+
+__device__ __forceinline__ float halves_max(float v) {
+    auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (int)b[0]), __builtin_bit_cast(float, (int)b[1]));
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// Register r of a lane of half h is position base + at(r, h) of a tile of 32: in f16 16 (r / 8) + 8 h + r % 8 (row i of
+// the MFMA stands for position 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4), in f32 the MFMA's own row 8 (r / 4) + 4 h + r % 4.
+template <bool H>
+__device__ __forceinline__ int tile_pos(int r, int h) { return H ? 16 * (r / 8) + 8 * h + r % 8 : 8 * (r / 4) + 4 * h + r % 4; }
+
+template <bool H, int HD>
+__global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2)
+void paged_many_kernel(PagedAttn a, int count) {
+    constexpr int STEP = H ? 64 : 32, T = STEP / 32, NB = STEP / PAGE_BLOCK, NC = H ? HD / 16 : HD / 8, ND = HD / 32;
+    constexpr int BLOCK = PAGE_BLOCK * HD * (H ? 2 : 4);   // bytes
+    extern __shared__ __align__(16) uint8_t lds[];         // [2][K, V][NB][BLOCK]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
+    int n_tokens = a.n_tokens;
+    if (n_tokens < 0) {
+        n_tokens = a.counts->n_tokens;
+        count = a.counts->many;
+    }
+    const float minus_one = f16_minus_one();
+    const PagedSight sight = {a.window, a.n_sink};
+    const size_t page_bytes = (size_t)BLOCK << (a.log_page - 4);   // of one kv head
+    const uint32_t lds0 = lds_addr(lds);
+    for (int w = blockIdx.x; w < count * a.n_kv; w += gridDim.x) {
+        const int hk = w % a.n_kv;
+        const PagedItem it = paged_item(&a.many[w / a.n_kv]);
+        const int32_t* table = a.table + it.table;
+        const int steps = it.v1 - it.v0;
+        const auto base_of = [&](int j) {
+            const int v = it.v0 + j;
+            return (v < it.a ? v : v - it.a + it.b) * STEP;
+        };
+        // lane j: of step 64 n + j the page of the block that this wave fetches, and which blocks have one
+        int id = -1, has = 0;
+        const auto fetch_ids = [&](int j0) {
+            id = -1, has = 0;
+            if (j0 + lane < steps) {
+                const int at = base_of(j0 + lane);
+                #pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const int p = at + 16 * b < it.kv_len ? table[(at + 16 * b) >> a.log_page] : -1;
+                    has |= p >= 0 ? 1 << b : 0;
+                    if (b == (wave & (NB - 1))) id = p;
+                }
+            }
+        };
+        const auto fetch = [&](int j, int has_all) {
+            // f16: K and V of block `wave`; f32, of two blocks a step: K by waves 0 and 1, V by the others
+            const int blk = wave & (NB - 1), p = __builtin_amdgcn_readlane(id, j & 63), at = base_of(j) + 16 * blk;
+            const size_t off = ((size_t)max(p, 0) * a.n_kv + hk) * page_bytes + (size_t)((at & ((1 << a.log_page) - 1)) >> 4) * BLOCK;
+            #pragma unroll
+            for (int kv = 0; kv < 2; kv++) {
+                if (!H && kv != wave / 2) continue;
+                i32x4v r = make_rsrc4((kv ? a.v : a.k) + off, (has_all >> blk) & 1 ? BLOCK : 0);   // (no page: zeros)
+                #pragma unroll
+                for (int e = 0; e < 4; e++) r[e] = __builtin_amdgcn_readfirstlane(r[e]);
+                const uint32_t to = lds0 + (((j & 1) * 2 + kv) * NB + blk) * BLOCK;
+                #pragma unroll
+                for (int u = 0; u < BLOCK / 1024; u++) lds_load16_at(r, to + 1024 * u, lane * 16, 1024 * u);
+            }
+        };
+        fetch_ids(0);
+        int has_now = __builtin_amdgcn_readlane(has, 0), has_next = 0;
+        fetch(0, has_now);
+        // the wave's rows
+        const int row0 = it.row0 + 32 * wave, end = it.row0 + it.rows, mine = min(row0 + i, end - 1), tok = mine / a.G;
+        const int pos = it.past + tok, p_first = it.past + min(row0, end - 1) / a.G, p_last = it.past + min(row0 + 31, end - 1) / a.G;
+        u32x4v qh[NC], ql[H ? NC : 1];
+        float back = 1.0f;
+        {
+            const float* row = a.q + ((size_t)(hk * a.G + mine % a.G) * n_tokens + it.q0 + tok) * HD;
+            if constexpr (H) {
+                float m = 0.0f;
+                #pragma unroll
+                for (int c = 0; c < 2 * NC; c++) {
+                    const float4 y = *reinterpret_cast<const float4*>(row + 16 * (c / 2) + 8 * h + 4 * (c & 1));
+                    m = fmaxf(fmaxf(fmaxf(m, __builtin_fabsf(y.x * a.scale)), fmaxf(__builtin_fabsf(y.y * a.scale), __builtin_fabsf(y.z * a.scale))),
+                              __builtin_fabsf(y.w * a.scale));
+                }
+                const float up = paged_row_scale(halves_max(m), back);
+                #pragma unroll
+                for (int c = 0; c < NC; c++)
+                    #pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const float4 y = *reinterpret_cast<const float4*>(row + 16 * c + 8 * h + 4 * u);
+                        uint32_t x0, y0, x1, y1;
+                        paged_split(y.x * a.scale * up, y.y * a.scale * up, x0, y0);
+                        paged_split(y.z * a.scale * up, y.w * a.scale * up, x1, y1);
+                        qh[c][2 * u] = x0, qh[c][2 * u + 1] = x1;
+                        ql[c][2 * u] = y0, ql[c][2 * u + 1] = y1;
+                    }
+            } else {
+                #pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const float4 y = *reinterpret_cast<const float4*>(row + 8 * c + 4 * h);
+                    const float x[4] = {y.x * a.scale, y.y * a.scale, y.z * a.scale, y.w * a.scale};
+                    #pragma unroll
+                    for (int u = 0; u < 4; u++) qh[c][u] = __builtin_bit_cast(uint32_t, x[u]);
+                }
+            }
+        }
+        float m = -INFINITY, l = 0.0f;
+        f32x16 o[ND];
+        #pragma unroll
+        for (int d = 0; d < ND; d++) o[d] = f32x16{};
+        for (int j = 0; j < steps; j++) {
+            wait_vmcnt<0>();
+            __syncthreads();   // the step is there for all waves, and none still reads the other buffer
+            if (j + 1 < steps) {
+                if (((j + 1) & 63) == 0) fetch_ids(j + 1);
+                has_next = __builtin_amdgcn_readlane(has, (j + 1) & 63);
+                fetch(j + 1, has_next);
+            }
+            const int base = base_of(j), have = has_now;
+            has_now = has_next;
+            // no row of the wave, or nothing that one sees (first tokens end where the window's steps begin)
+            if (row0 >= end || base > p_last || (a.window && base >= a.n_sink && base + STEP - 1 <= p_first - a.window)) continue;
+            const uint8_t *kt = lds + (size_t)(j & 1) * 2 * NB * BLOCK, *vt = kt + NB * BLOCK;
+            const bool whole = have == (1 << NB) - 1 && sight.all(base, STEP, p_first, p_last);
+            float s[T][16];
+            #pragma unroll
+            for (int t = 0; t < T; t++) {
+                f32x16 hi = {}, lo = {};
+                const int slot = H ? 8 * ((i >> 2) & 1) + 4 * ((i >> 3) & 1) + (i & 3) : i & 15;
+                const uint8_t* kb = kt + (2 * t + (i >> 4)) * BLOCK + slot * 16 + h * 256;
+                #pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const u32x4v k = *reinterpret_cast<const u32x4v*>(kb + c * 512);
+                    if constexpr (H) {
+                        lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, k), __builtin_bit_cast(h8v, ql[c]), lo, 0, 0, 0);
+                        hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, k), __builtin_bit_cast(h8v, qh[c]), hi, 0, 0, 0);
+                    } else {
+                        const f32x4 x = __builtin_bit_cast(f32x4, k), y = __builtin_bit_cast(f32x4, qh[c]);
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) hi = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], hi, 0, 0, 0);
+                    }
+                }
+                #pragma unroll
+                for (int r = 0; r < 16; r++) s[t][r] = H ? __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) : hi[r];
+            }
+            uint32_t seen = 0xFFFFFFFFu;   // bit 16 t + r
+            bool bad = false;
+            if (!whole) {
+                seen = 0;
+                #pragma unroll
+                for (int t = 0; t < T; t++)
+                    #pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int x = 32 * t + tile_pos<H>(r, h);
+                        const bool see = ((have >> (x / 16)) & 1) && sight.sees(pos, base + x);
+                        seen |= see ? 1u << (16 * t + r) : 0u;
+                        s[t][r] = see ? s[t][r] : -INFINITY;
+                    }
+                uint32_t any = 0;
+                for (int u = lane; u < NB * BLOCK / 16; u += 64) {
+                    const u32x4v x = reinterpret_cast<const u32x4v*>(vt)[u];
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) any |= H ? f16_bad(x[e]) : f32_bad(x[e]);
+                }
+                bad = __any(any != 0);
+            }
+            float top = s[0][0];
+            #pragma unroll
+            for (int t = 0; t < T; t++)
+                #pragma unroll
+                for (int r = 0; r < 16; r++) top = fmaxf(top, s[t][r]);
+            top = fmaxf(m, halves_max(top) * back);
+            const float ref = top == -INFINITY ? 0.0f : top, shift = H ? 15.0f - ref : -ref;
+            const float alpha = paged_exp2(m - ref);
+            m = top;
+            float sum = 0.0f;
+            u32x4v ph[T][2], pl[T][2];   // f16
+            #pragma unroll
+            for (int t = 0; t < T; t++) {
+                #pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    s[t][r] = paged_exp2(__builtin_fmaf(s[t][r], back, shift));
+                    sum += s[t][r];
+                }
+                if constexpr (H) {
+                    #pragma unroll
+                    for (int r = 0; r < 16; r += 2) {
+                        uint32_t x, y;
+                        split_f16(s[t][r], s[t][r + 1], minus_one, x, y);
+                        ph[t][r / 8][r % 8 / 2] = x;
+                        pl[t][r / 8][r % 8 / 2] = y;
+                    }
+                }
+            }
+            l = __builtin_fmaf(l, alpha, sum);
+            if (!bad) {
+                #pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    f32x16 y = {};
+                    #pragma unroll
+                    for (int t = 0; t < T; t++) {
+                        if constexpr (H) {
+                            #pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                const h8v v = *reinterpret_cast<const h8v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16);
+                                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(h8v, pl[t][u]), y, 0, 0, 0);
+                                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(h8v, ph[t][u]), y, 0, 0, 0);
+                            }
+                        } else {
+                            #pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const f32x4 v = *reinterpret_cast<const f32x4*>(vt + (2 * t + q / 2) * BLOCK + ((2 * (q & 1) + h) * HD + 32 * d + i) * 16);
+                                #pragma unroll
+                                for (int e = 0; e < 4; e++) y = __builtin_amdgcn_mfma_f32_32x32x2f32(v[e], s[t][4 * q + e], y, 0, 0, 0);
+                            }
+                        }
+                    }
+                    #pragma unroll
+                    for (int r = 0; r < 16; r++) o[d][r] = __builtin_fmaf(o[d][r], alpha, y[r]);
+                }
+            } else {
+                // the same with what is not finite as zero, and the number of such places that a row sees
+                for (int d = 0; d < ND; d++) {
+                    f32x16 y = {}, n = {};
+                    #pragma unroll
+                    for (int t = 0; t < T; t++) {
+                        if constexpr (H) {
+                            #pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16), is, one;
+                                #pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const uint32_t b = f16_bad(v[e]), two = seen >> (16 * t + 8 * u + 2 * e);
+                                    v[e] &= ~b;
+                                    is[e] = b & 0x3C003C00u;
+                                    one[e] = (two & 1 ? 0x3C00u : 0u) | (two & 2 ? 0x3C000000u : 0u);
+                                }
+                                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, is), __builtin_bit_cast(h8v, one), n, 0, 0, 0);
+                                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, v), __builtin_bit_cast(h8v, pl[t][u]), y, 0, 0, 0);
+                                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, v), __builtin_bit_cast(h8v, ph[t][u]), y, 0, 0, 0);
+                            }
+                        } else {
+                            #pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + q / 2) * BLOCK + ((2 * (q & 1) + h) * HD + 32 * d + i) * 16);
+                                #pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const uint32_t b = f32_bad(v[e]), z = v[e] & ~b;
+                                    n = __builtin_amdgcn_mfma_f32_32x32x2f32(b ? 1.0f : 0.0f, (seen >> (16 * t + 4 * q + e)) & 1 ? 1.0f : 0.0f, n, 0, 0, 0);
+                                    y = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, z), s[t][4 * q + e], y, 0, 0, 0);
+                                }
+                            }
+                        }
+                    }
+                    #pragma unroll
+                    for (int dd = 0; dd < ND; dd++)
+                        if (dd == d) {
+                            #pragma unroll
+                            for (int r = 0; r < 16; r++) o[dd][r] = n[r] > 0.0f ? NAN : __builtin_fmaf(o[dd][r], alpha, y[r]);
+                        }
+                }
+            }
+        }
+        const float sum = swap32_add(l, l);
+        if (row0 + i < end) {
+            if (it.part < 0) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                float* out = a.out + ((size_t)(it.q0 + tok) * a.n_head + hk * a.G + mine % a.G) * HD;
+                #pragma unroll
+                for (int d = 0; d < ND; d++)
+                    #pragma unroll
+                    for (int r = 0; r < 16; r++) out[32 * d + 8 * (r / 4) + 4 * h + r % 4] = o[d][r] * inv;
+            } else {
+                const size_t at = (size_t)hk * a.part_rows + it.part + (mine - it.row0);
+                float* out = a.part + at * HD;
+                #pragma unroll
+                for (int d = 0; d < ND; d++)
+                    #pragma unroll
+                    for (int r = 0; r < 16; r++) out[32 * d + 8 * (r / 4) + 4 * h + r % 4] = o[d][r];
+                if (h == 0) a.stat[at] = make_float2(m, sum);
+            }
+        }
+        __syncthreads();   // (a next item's first loads go where this one's last step may be read from)
+    }
+}
+
+template <bool H, int HD>
+hipError_t launch(const PagedAttn& a, hipStream_t s) {
+    constexpr unsigned bytes = 2 * 2 * (H ? 64 : 32) * HD * (H ? 2 : 4);
+    if (bytes > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_many_kernel<H, HD>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != hipSuccess) return e;
+    }
+    const dim3 g(a.n_tokens < 0 ? 1024u : (unsigned)a.n_many * (unsigned)a.n_kv);
+    hipLaunchKernelGGL((paged_many_kernel<H, HD>), g, dim3(64 * NW), bytes, s, a, a.n_many);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t paged_many_launch(const PagedAttn& a, bool f16, int hd, hipStream_t s) {
+    if (f16) return hd == 64 ? launch<true, 64>(a, s) : hd == 128 ? launch<true, 128>(a, s) : launch<true, 256>(a, s);
+    return hd == 64 ? launch<false, 64>(a, s) : hd == 128 ? launch<false, 128>(a, s) : launch<false, 256>(a, s);
+}
+
+}  // namespace barq

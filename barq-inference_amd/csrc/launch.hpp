@@ -342,5 +342,6 @@ struct PagedAttn {
     size_t part_rows;
 };
 hipError_t paged_attention_launch(const PagedAttn& a, bool f16, int hd, hipStream_t s);
+hipError_t paged_many_launch(const PagedAttn& a, bool f16, int hd, hipStream_t s);   // its items of many rows (attention_paged_many.hip)
 
 }  // namespace barq

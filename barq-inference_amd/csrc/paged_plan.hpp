@@ -99,7 +99,8 @@ inline size_t paged_max_tiles(size_t max_seqs, size_t max_tokens, size_t G) { re
 inline void paged_shape_for(PagedShape& sh, bool f16, size_t hd) {
     (void)hd;
     sh.few_step = f16 ? 32 : 16;
-    sh.many_from = INT64_MAX;
+    sh.many_step = f16 ? 64 : 32;
+    sh.many_from = 65;
 }
 
 // Partial states to have room for (of each kv head): 64 MiB of them with 128 dims at most.
