@@ -198,110 +198,113 @@ void paged_few_kernel(PagedAttn a, int first, int count) {
         const auto block_at = [&](const uint8_t* pool, int id, int at) {   // (an absent page: the first one, unseen)
             return pool + ((size_t)max(id, 0) * a.n_kv + hk) * page_bytes + (size_t)((at & ((1 << a.log_page) - 1)) >> 4) * BLOCK;
         };
-        Step<H, HD> st[2];
-        int page0[2], page1[2];
-        const auto load = [&](int j, int x) __attribute__((always_inline)) {
+        // One set of registers: K's are free once the scores are there, V's after P V, and take the next step's at once.
+        Step<H, HD> st;
+        int k_pages = 0;   // bit 0, 1: the first 16 positions of the step in K's registers have a page, the others
+        const auto load = [&](int j, bool keys) __attribute__((always_inline)) {
             if (j >= steps) return;
-            if ((j & 63) == 0) fetch_ids(j);
-            const int at = base_of(j), p0 = __builtin_amdgcn_readlane(id0, j & 63), p1 = __builtin_amdgcn_readlane(id1, j & 63);
-            page0[x] = p0;
-            page1[x] = p1;
-            const uint8_t *k0 = block_at(a.k, p0, at), *v0 = block_at(a.v, p0, at);
-            const uint8_t *kb = k0, *vb = v0;
-            if (H) {
-                const uint8_t *k1 = block_at(a.k, p1, at + 16), *v1 = block_at(a.v, p1, at + 16);
-                kb = i < 8 ? k0 : k1;
-                vb = g < 2 ? v0 : v1;
-            }
-            #pragma unroll
-            for (int t = 0; t < KT; t++) {
-                const int slot = H ? (8 * (i >> 2) + 4 * t + (i & 3)) & 15 : i;
+            const int at = base_of(j), p0 = __builtin_amdgcn_readlane(id0, j & 63), p1 = H ? __builtin_amdgcn_readlane(id1, j & 63) : -1;
+            const uint8_t *pool = keys ? a.k : a.v, *b0 = block_at(pool, p0, at), *b1 = H ? block_at(pool, p1, at + 16) : b0;
+            if (keys) {
+                k_pages = (p0 >= 0 ? 1 : 0) | (p1 >= 0 ? 2 : 0);
+                const uint8_t* b = H && i >= 8 ? b1 : b0;
                 #pragma unroll
-                for (int c = 0; c < Step<H, HD>::NC; c++)
-                    st[x].k[t][c] = *reinterpret_cast<const u32x4v*>(kb + ((4 * c + g) * 16 + slot) * 16);
-            }
-            #pragma unroll
-            for (int d = 0; d < NV; d++)
-                st[x].v[d] = *reinterpret_cast<const u32x4v*>(vb + ((H ? g & 1 : g) * HD + 16 * d + i) * 16);
-        };
-        const auto compute = [&](int j, int x) __attribute__((always_inline)) {
-            const int base = base_of(j);
-            const bool here0 = page0[x] >= 0, here1 = H ? page1[x] >= 0 : here0;
-            const bool whole = here0 && here1 && sight.all(base, STEP, p_first, p_last);
-            bool seen[NT][NP];
-            bool nan_v = false;
-            if (!whole) {
-                #pragma unroll
-                for (int n = 0; n < NT; n++)
+                for (int t = 0; t < KT; t++) {
+                    const int slot = H ? (8 * (i >> 2) + 4 * t + (i & 3)) & 15 : i;
                     #pragma unroll
-                    for (int e = 0; e < NP; e++)   // (a group's positions lie in one block)
-                        seen[n][e] = (H && g >= 2 ? here1 : here0) && sight.sees(pos[n], base + E * g + e);
+                    for (int c = 0; c < Step<H, HD>::NC; c++) st.k[t][c] = *reinterpret_cast<const u32x4v*>(b + ((4 * c + g) * 16 + slot) * 16);
+                }
+            } else {
+                const uint8_t* b = H && g >= 2 ? b1 : b0;
+                #pragma unroll
+                for (int d = 0; d < NV; d++) st.v[d] = *reinterpret_cast<const u32x4v*>(b + ((H ? g & 1 : g) * HD + 16 * d + i) * 16);
+            }
+        };
+        if (steps > 0) fetch_ids(0);
+        load(0, true);
+        load(0, false);
+        for (int j = 0; j < steps; j++) {
+            const int base = base_of(j), have = k_pages;
+            const bool whole = have == (H ? 3 : 1) && sight.all(base, STEP, p_first, p_last);
+            float s[NT][NP];
+            #pragma unroll
+            for (int n = 0; n < NT; n++) scores<H, HD>(st, q[n], s[n]);
+            if (((j + 1) & 63) == 0) fetch_ids(j + 1);
+            load(j + 1, true);
+            uint32_t seen[NT];   // bit e: the lane's row sees the lane's position e
+            bool bad = false;
+            if (!whole) {
+                const bool here = H && g >= 2 ? have & 2 : have & 1;   // (a group's positions lie in one block)
+                #pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    seen[n] = 0;
+                    #pragma unroll
+                    for (int e = 0; e < NP; e++) {
+                        const bool see = here && sight.sees(pos[n], base + E * g + e);
+                        seen[n] |= see ? 1u << e : 0u;
+                        s[n][e] = see ? s[n][e] : -INFINITY;
+                    }
+                }
+                uint32_t any = 0;
                 #pragma unroll
                 for (int d = 0; d < NV; d++)
                     #pragma unroll
-                    for (int u = 0; u < 4; u++) nan_v |= (H ? f16_bad(st[x].v[d][u]) : f32_bad(st[x].v[d][u])) != 0;
+                    for (int u = 0; u < 4; u++) any |= H ? f16_bad(st.v[d][u]) : f32_bad(st.v[d][u]);
+                bad = __any(any != 0);
             }
-            const bool bad = __any(nan_v);
+            float alpha[NT];
+            Weights<H> p[NT];
             #pragma unroll
             for (int n = 0; n < NT; n++) {
-                float s[NP];
-                scores<H, HD>(st[x], q[n], s);
-                if (!whole) {
-                    #pragma unroll
-                    for (int e = 0; e < NP; e++) s[e] = seen[n][e] ? s[e] : -INFINITY;
-                }
-                float top = s[0];
+                float top = s[n][0];
                 #pragma unroll
-                for (int e = 1; e < NP; e++) top = fmaxf(top, s[e]);
+                for (int e = 1; e < NP; e++) top = fmaxf(top, s[n][e]);
                 top = fmaxf(m[n], groups_max(top));
                 const float ref = top == -INFINITY ? 0.0f : top, shift = H ? ref - 15.0f : ref;
-                const float alpha = paged_exp2(m[n] - ref);
+                alpha[n] = paged_exp2(m[n] - ref);
                 m[n] = top;
                 float sum = 0.0f;
                 #pragma unroll
                 for (int e = 0; e < NP; e++) {
-                    s[e] = paged_exp2(s[e] - shift);
-                    sum += s[e];
+                    s[n][e] = paged_exp2(s[n][e] - shift);
+                    sum += s[n][e];
                 }
-                l[n] = __builtin_fmaf(l[n], alpha, sum);
-                Weights<H> p;
-                p.set(s, minus_one);
-                if (!bad) {
+                l[n] = __builtin_fmaf(l[n], alpha[n], sum);
+                p[n].set(s[n], minus_one);
+            }
+            if (!bad) {
+                #pragma unroll
+                for (int d = 0; d < NV; d++)
                     #pragma unroll
-                    for (int d = 0; d < NV; d++) {
-                        const f32x4 y = p.times(st[x].v[d]);
+                    for (int n = 0; n < NT; n++) {
+                        const f32x4 y = p[n].times(st.v[d]);
                         #pragma unroll
-                        for (int r = 0; r < 4; r++) o[n][d][r] = __builtin_fmaf(o[n][d][r], alpha, y[r]);
+                        for (int r = 0; r < 4; r++) o[n][d][r] = __builtin_fmaf(o[n][d][r], alpha[n], y[r]);
                     }
-                } else {
+            } else {
+                #pragma unroll
+                for (int n = 0; n < NT; n++) {
                     Weights<H> ones;
                     float z[NP];
                     #pragma unroll
-                    for (int e = 0; e < NP; e++) z[e] = seen[n][e] ? 1.0f : 0.0f;
+                    for (int e = 0; e < NP; e++) z[e] = (seen[n] >> e) & 1 ? 1.0f : 0.0f;
                     ones.set(z, minus_one);
                     #pragma unroll
                     for (int d = 0; d < NV; d++) {
-                        u32x4v v = st[x].v[d], is;
+                        u32x4v v = st.v[d], is;
                         #pragma unroll
                         for (int u = 0; u < 4; u++) {
                             const uint32_t b = H ? f16_bad(v[u]) : f32_bad(v[u]);
                             v[u] &= ~b;
                             is[u] = b & (H ? 0x3C003C00u : 0x3F800000u);
                         }
-                        const f32x4 y = p.times(v), nan = ones.times(is);
+                        const f32x4 y = p[n].times(v), nan = ones.times(is);
                         #pragma unroll
-                        for (int r = 0; r < 4; r++) o[n][d][r] = nan[r] > 0.0f ? NAN : __builtin_fmaf(o[n][d][r], alpha, y[r]);
+                        for (int r = 0; r < 4; r++) o[n][d][r] = nan[r] > 0.0f ? NAN : __builtin_fmaf(o[n][d][r], alpha[n], y[r]);
                     }
                 }
             }
-        };
-        load(0, 0);
-        for (int j = 0; j < steps; j += 2) {
-            load(j + 1, 1);
-            compute(j, 0);
-            if (j + 1 >= steps) break;
-            load(j + 2, 0);
-            compute(j + 1, 1);
+            load(j + 1, false);
         }
         // the four waves' states, joined
         #pragma unroll
@@ -357,47 +360,80 @@ void paged_few_kernel(PagedAttn a, int first, int count) {
     }
 }
 
-// Joins the partial states of rows that several workgroups share: a wave a row.
+// Joins the partial states of rows that several workgroups share.  Bound by its latencies: all of a wave's loads are
+// in flight together.  Up to 8 states a wave a row, beyond that the four waves of a workgroup share a row's.
 template <int HD>
 __global__ __launch_bounds__(64 * NW)
 void paged_merge_kernel(PagedAttn a) {
     constexpr int PER = HD / 64, AHEAD = 8;
+    __shared__ float part_s[NW][HD];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int merges = a.n_tokens < 0 ? a.counts->merges : a.n_merges, hk = blockIdx.y, span = a.merge_span;
     for (int w = blockIdx.x; w < merges * span; w += gridDim.x) {
         const PagedMerge mg = a.merges[w / span];
-        const int r = (w % span) * NW + wave;
-        if (r >= mg.rows) continue;
-        const size_t at = (size_t)hk * a.part_rows + mg.part + r;
-        float top = -INFINITY;
-        for (int s = lane; s < mg.n_split; s += 64) top = fmaxf(top, a.stat[at + (size_t)s * mg.rows].x);
+        const bool shared = mg.n_split > PAGED_MERGE_WAVE;
+        const int r = shared ? w % span : (w % span) * NW + wave;
+        const int step = shared ? NW : 1, mine = shared ? (mg.n_split - wave + NW - 1) / NW : mg.n_split, s0 = shared ? wave : 0;
+        if (shared ? r >= mg.rows : (w % span) * NW >= mg.rows) continue;
+        const size_t at = (size_t)hk * a.part_rows + mg.part + min(r, mg.rows - 1);
+        const auto states = [&](int k, float (&x)[AHEAD][PER]) __attribute__((always_inline)) {
+            #pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                const float* from = a.part + (at + (size_t)(s0 + step * max(min(k + u, mine - 1), 0)) * mg.rows) * HD + lane * PER;
+                #pragma unroll
+                for (int e = 0; e < PER; e++) x[u][e] = from[e];
+            }
+        };
+        float x[AHEAD][PER], y[PER], top = -INFINITY, sum = 0.0f;
+        states(0, x);
+        float2 z = make_float2(-INFINITY, 0.0f);
+        for (int s = lane; s < mg.n_split; s += 64) {
+            const float2 t = a.stat[at + (size_t)s * mg.rows];
+            if (s < 64) z = t;
+            top = fmaxf(top, t.x);
+        }
         top = wave_max_all(top);
-        float sum = 0.0f, y[PER];
+        const auto factor = [&](float m) { return m == -INFINITY ? 1.0f : paged_exp2(m - top); };   // (1: zeros, or NaN)
+        const float f = factor(z.x);
+        sum = z.y * f;
+        for (int s = lane + 64; s < mg.n_split; s += 64) {
+            const float2 t = a.stat[at + (size_t)s * mg.rows];
+            sum = __builtin_fmaf(t.y, factor(t.x), sum);
+        }
+        sum = wave_sum_all(sum);
         #pragma unroll
         for (int e = 0; e < PER; e++) y[e] = 0.0f;
-        for (int s0 = 0; s0 < mg.n_split; s0 += AHEAD) {
-            float x[AHEAD][PER];
-            float2 z[AHEAD];
+        for (int k = 0; k < mine; k += AHEAD) {
+            if (k) states(k, x);
             #pragma unroll
             for (int u = 0; u < AHEAD; u++) {
-                const int s = min(s0 + u, mg.n_split - 1);
-                z[u] = a.stat[at + (size_t)s * mg.rows];
-                #pragma unroll
-                for (int e = 0; e < PER; e++) x[u][e] = a.part[(at + (size_t)s * mg.rows) * HD + lane * PER + e];
-            }
-            #pragma unroll
-            for (int u = 0; u < AHEAD; u++) {
-                if (s0 + u >= mg.n_split) break;
-                const float f = z[u].x == -INFINITY ? 1.0f : paged_exp2(z[u].x - top);   // (1: zeros, or NaN)
-                sum = __builtin_fmaf(z[u].y, f, sum);
-                #pragma unroll
-                for (int e = 0; e < PER; e++) y[e] = __builtin_fmaf(x[u][e], f, y[e]);
+                const int s = s0 + step * (k + u);
+                if (k + u < mine) {
+                    const float g = s < 64 ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s & 63))
+                                           : factor(a.stat[at + (size_t)s * mg.rows].x);
+                    #pragma unroll
+                    for (int e = 0; e < PER; e++) y[e] = __builtin_fmaf(x[u][e], g, y[e]);
+                }
             }
         }
-        const int rr = mg.row0 + r, tok = mg.q0 + rr / a.G, head = hk * a.G + rr % a.G;
-        float* out = a.out + ((size_t)tok * a.n_head + head) * HD + lane * PER;
-        #pragma unroll
-        for (int e = 0; e < PER; e++) out[e] = sum == 0.0f ? 0.0f : y[e] / sum;
+        if (shared) {
+            __syncthreads();   // (an earlier row's sums have been read)
+            #pragma unroll
+            for (int e = 0; e < PER; e++) part_s[wave][lane * PER + e] = y[e];
+            __syncthreads();
+            #pragma unroll
+            for (int e = 0; e < PER; e++) {
+                y[e] = part_s[0][lane * PER + e];
+                #pragma unroll
+                for (int u = 1; u < NW; u++) y[e] += part_s[u][lane * PER + e];
+            }
+        }
+        if (shared ? wave == 0 : r < mg.rows) {
+            const int rr = mg.row0 + r, tok = mg.q0 + rr / a.G, head = hk * a.G + rr % a.G;
+            float* out = a.out + ((size_t)tok * a.n_head + head) * HD + lane * PER;
+            #pragma unroll
+            for (int e = 0; e < PER; e++) out[e] = sum == 0.0f ? 0.0f : y[e] / sum;
+        }
     }
 }
 
@@ -423,7 +459,8 @@ hipError_t paged_attention_launch(const PagedAttn& a, bool f16, int hd, hipStrea
     #define BARQ_FEW(H, D)                                                                                                      \
         if (f16 == H && hd == D) {                                                                                              \
             if (captured || a.n_few16) hipLaunchKernelGGL((paged_few_kernel<H, D, 1>), grid(a.n_few16), dim3(256), 0, s, a, 0, a.n_few16); \
-            if (captured || few32) hipLaunchKernelGGL((paged_few_kernel<H, D, 2>), grid(few32), dim3(256), 0, s, a, a.n_few16, few32);    \
+            if constexpr (D != 256)                                                                                            \
+                if (captured || few32) hipLaunchKernelGGL((paged_few_kernel<H, D, 2>), grid(few32), dim3(256), 0, s, a, a.n_few16, few32);    \
         }
     BARQ_FEW(true, 64) BARQ_FEW(true, 128) BARQ_FEW(true, 256)
     BARQ_FEW(false, 64) BARQ_FEW(false, 128) BARQ_FEW(false, 256)

@@ -333,7 +333,7 @@ struct PagedAttn {
     const PagedCounts* counts;
     int n_tokens;          // -1: counts has them (a captured call)
     int n_few16, n_few, n_many, n_merges;
-    int merge_span;        // workgroups of four rows that a merge takes
+    int merge_span;        // workgroups of a merge
     int n_head, n_kv, G, log_page;
     int window, n_sink;
     float scale;           // log2(e) / sqrt(hd)

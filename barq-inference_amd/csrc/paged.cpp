@@ -585,11 +585,13 @@ int barq_rocm_paged_attention(barq_rocm_handle* h, barq_rocm_paged_batch* b, siz
     x.n_few = (int)b->plan.few.size();
     x.n_many = (int)b->plan.many.size();
     x.n_merges = (int)b->plan.merges.size();
-    x.merge_span = 32;
+    x.merge_span = 128;
     if (!captured) {
-        int most = 1;
-        for (const barq::PagedMerge& m : b->plan.merges) most = m.rows > most ? m.rows : most;
-        x.merge_span = (most + 3) / 4;
+        x.merge_span = 1;
+        for (const barq::PagedMerge& m : b->plan.merges) {
+            const int n = m.n_split > barq::PAGED_MERGE_WAVE ? m.rows : (m.rows + 3) / 4;
+            x.merge_span = n > x.merge_span ? n : x.merge_span;
+        }
     }
     x.n_head = (int)b->n_head;
     x.n_kv = (int)p.n_head_kv;

@@ -21,6 +21,7 @@
 namespace barq {
 
 constexpr int PAGE_BLOCK = 16;            // positions of a block
+constexpr int PAGED_MERGE_WAVE = 8;       // partial states of a row that one wave joins; more: four of them
 constexpr size_t PAGE_MAX = 1u << 16;     // positions of a page
 
 // One workgroup's share of the attention of a step: rows of one sequence (row r

@@ -20,6 +20,7 @@ struct PagedShape {
     int G = 1, n_kv = 1;          // query heads of a kv head, kv heads
     int64_t window = 0, n_sink = 0;
     int few_step = 32, many_step = 64;   // positions of a kernel's step
+    int few_rows = 32;            // rows of the kernel for few's larger tiles
     int64_t many_from = 65;       // rows from which a sequence's tiles are the large ones
     int64_t few_target = 1024, many_target = 512;   // workgroups that fill the card
     int64_t few_least = 4, many_least = 4;          // steps that a split has at least
@@ -97,10 +98,11 @@ inline size_t paged_max_tiles(size_t max_seqs, size_t max_tokens, size_t G) { re
 
 // The kernels' steps for a type and head_dim, and from how many rows the one for many is taken.
 inline void paged_shape_for(PagedShape& sh, bool f16, size_t hd) {
-    (void)hd;
     sh.few_step = f16 ? 32 : 16;
     sh.many_step = f16 ? 64 : 32;
     sh.many_from = 65;
+    sh.few_rows = hd == 256 ? 16 : 32;   // (two tiles of 256 dims do not fit the registers)
+    sh.many_target = hd == 256 ? 256 : 512;
 }
 
 // Partial states to have room for (of each kv head): 64 MiB of them with 128 dims at most.
@@ -117,7 +119,7 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
     for (const PagedSeq& s : seqs) {
         const int64_t rows = s.q_len * sh.G, past = s.kv_len - s.q_len;
         const bool many = rows >= sh.many_from;
-        const int64_t tile = many ? 128 : rows <= 16 ? 16 : 32, unit = many ? sh.many_step : sh.few_step;
+        const int64_t tile = many ? 128 : std::min<int64_t>(rows <= 16 ? 16 : 32, sh.few_rows), unit = many ? sh.many_step : sh.few_step;
         for (int64_t r = 0; r < rows; r += tile) {
             PagedItem it{};
             it.q0 = (int32_t)q0;
