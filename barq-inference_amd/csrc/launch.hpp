@@ -300,9 +300,9 @@ struct PagedAppend {
     const float *q_norm, *k_norm;  // [hd] or null
     float* q_out;                  // [n_q, n_tokens, hd]
     uint8_t *k_pool, *v_pool;      // the layer's pages
-    const PagedToken* tokens;
+    const PagedGroup* groups;
     const PagedCounts* counts;
-    int n_tokens;                  // -1: counts has them (a captured call)
+    int n_tokens, n_groups;        // -1: counts has them (a captured call)
     int n_q, n_kv, log_page;
     float eps;
     Rotary rotary;

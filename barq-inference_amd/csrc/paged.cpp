@@ -58,7 +58,7 @@ struct barq_rocm_paged_batch {
     // device, of a fixed size: graphs captured with this batch keep the addresses
     uint8_t* mem = nullptr;
     float* rows = nullptr;   // [max_tokens, n_head * head_dim], from the first call for Q8_K rows on
-    size_t counts_at = 0, tokens_at = 0, merges_at = 0, few_at = 0, many_at = 0, table_at = 0, stat_at = 0, part_at = 0;
+    size_t counts_at = 0, groups_at = 0, merges_at = 0, few_at = 0, many_at = 0, table_at = 0, stat_at = 0, part_at = 0;
     size_t items_most = 0, merges_most = 0;
     Stage stage[2];
     int next = 0;
@@ -133,9 +133,10 @@ barq::PagedAppend append_args(const barq_rocm_paged_batch* b, size_t layer, bool
     barq::PagedAppend a{};
     a.k_pool = p.k + layer * p.layer_bytes();
     a.v_pool = p.v + layer * p.layer_bytes();
-    a.tokens = reinterpret_cast<const barq::PagedToken*>(b->mem + b->tokens_at);
+    a.groups = reinterpret_cast<const barq::PagedGroup*>(b->mem + b->groups_at);
     a.counts = b->dev_counts();
     a.n_tokens = captured ? -1 : b->counts.n_tokens;
+    a.n_groups = captured ? -1 : b->counts.groups;
     a.n_kv = (int)p.n_head_kv;
     a.log_page = p.log_page;
     return a;
@@ -315,7 +316,7 @@ int barq_rocm_paged_batch_create(barq_rocm_handle* h, barq_rocm_paged_cache* c, 
     b->merges_most = barq::paged_max_tiles(max_seqs, max_tokens, G);
     Arena a;
     b->counts_at = a.add(sizeof(barq::PagedCounts));
-    b->tokens_at = a.add((max_tokens + 1) * sizeof(barq::PagedToken));
+    b->groups_at = a.add(barq::paged_max_groups(max_seqs, max_tokens) * sizeof(barq::PagedGroup));
     b->merges_at = a.add(b->merges_most * sizeof(barq::PagedMerge));
     b->few_at = a.add(b->items_most * sizeof(barq::PagedItem));
     b->many_at = a.add(b->items_most * sizeof(barq::PagedItem));
@@ -380,6 +381,8 @@ int barq_rocm_paged_batch_set(barq_rocm_handle* h, barq_rocm_paged_batch* b, siz
     if (plan.few.size() > b->items_most || plan.many.size() > b->items_most || plan.merges.size() > b->merges_most)
         return fail(BARQ_E_DIM, "%s: the plan does not fit the batch", who);   // (it does: paged_plan.hpp)
     counts.n_tokens = (int32_t)tokens;
+    for (size_t s = 0; s < n_seqs; s++)
+        if (q_len[s]) counts.groups += (kv_len[s] - 1) / barq::PAGE_BLOCK - (kv_len[s] - q_len[s]) / barq::PAGE_BLOCK + 1;
     counts.few = (int32_t)plan.few.size();
     counts.few16 = plan.few16;
     counts.many = (int32_t)plan.many.size();
@@ -393,7 +396,7 @@ int barq_rocm_paged_batch_set(barq_rocm_handle* h, barq_rocm_paged_batch* b, siz
         used += round_up(bytes, 16);
         return from;
     };
-    const size_t pc = piece(b->counts_at, sizeof counts), pt = piece(b->tokens_at, tokens * sizeof(barq::PagedToken));
+    const size_t pc = piece(b->counts_at, sizeof counts), pt = piece(b->groups_at, (size_t)counts.groups * sizeof(barq::PagedGroup));
     const size_t pm = piece(b->merges_at, plan.merges.size() * sizeof(barq::PagedMerge));
     const size_t pf = piece(b->few_at, plan.few.size() * sizeof(barq::PagedItem));
     const size_t pn = piece(b->many_at, plan.many.size() * sizeof(barq::PagedItem));
@@ -416,14 +419,13 @@ int barq_rocm_paged_batch_set(barq_rocm_handle* h, barq_rocm_paged_batch* b, siz
         st.size = want;
     }
     std::memcpy(st.p + pc, &counts, sizeof counts);
-    auto* tok = reinterpret_cast<barq::PagedToken*>(st.p + pt);
+    auto* group = reinterpret_cast<barq::PagedGroup*>(st.p + pt);
     auto* table = reinterpret_cast<int32_t*>(st.p + pp);
+    int32_t t0 = 0;
     for (size_t s = 0; s < n_seqs; s++) {
         const int32_t* ids = pages + s * pages_stride;
-        for (int32_t j = kv_len[s] - q_len[s]; j < kv_len[s]; j++) {
-            const int32_t id = ids[(size_t)j >> p.log_page];
-            *tok++ = {id < 0 ? -1 : (id << p.log_page) + (j & (int32_t)(p.page_size - 1)), j};
-        }
+        group = barq::paged_groups(t0, q_len[s], kv_len[s], ids, p.log_page, group);
+        t0 += q_len[s];
         const size_t n = ((size_t)kv_len[s] + p.page_size - 1) / p.page_size;
         if (n) std::memcpy(table, ids, n * sizeof(int32_t));
         table += n;

@@ -37,7 +37,8 @@ struct PagedItem {
                      // tokens that stay visible, then the window
     int32_t v0, v1;  // this item's steps
     int32_t part;    // its first row among the partial states, -1: it writes the output itself
-    int32_t pad[5];
+    int32_t tile;    // rows of its tile's kernel: 16, 32, 128
+    int32_t pad[4];
 };
 static_assert(sizeof(PagedItem) == 64, "items are fetched as 64 bytes");
 
@@ -50,14 +51,17 @@ static_assert(sizeof(PagedMerge) == 32, "");
 // What a replayed graph reads anew (a call outside a capture passes it along).
 struct PagedCounts {
     int32_t n_tokens, few, many, merges;
-    int32_t few16;   // items of `few` with at most 16 rows: the first ones
-    int32_t pad[11];
+    int32_t few16;   // items of `few` in tiles of 16 rows: the first ones
+    int32_t groups;
+    int32_t pad[10];
 };
 static_assert(sizeof(PagedCounts) == 64, "");
 
-// The new tokens: their row of the pool (page * page_size + slot, -1: none) and their position.
-struct PagedToken {
-    int32_t row, pos;
+// New tokens t0 .. t0 + n - 1 of a sequence whose positions pos .. pos + n - 1 lie in one block, in the pool's rows
+// row .. row + n - 1 (row: page * page_size + slot; -1: none).
+struct PagedGroup {
+    int32_t t0, n, row, pos;
 };
+static_assert(sizeof(PagedGroup) == 16, "");
 
 }  // namespace barq

@@ -3,14 +3,18 @@
 // one tensor by itself.
 //
 // Bound by the bytes: q is read and written in f32, K and V read in f32 and written
-// in the cache's type.  A workgroup has some heads of one token, so that a pair's
-// cos and sin (64-bit angles) are formed once for all of them; HD / 8 lanes a head.
+// in the cache's type.  A workgroup has up to 16 tokens of one block and some of their
+// heads: HD / 8 lanes a row of q or K, the next rows in flight while these are rotated; of
+// V eight tokens (four in f32) of a dim a lane, which are 16 bytes there.  The pairs' cos and
+// sin (64-bit angles) are formed once for a workgroup's tokens, while its first rows come.
 #include "paged.hpp"
 #include "rotary.hpp"
 
 namespace barq {
 
 namespace {
+
+constexpr size_t TURN_WORKGROUPS = 1024;
 
 // f32 to the cache's f16: nearest, the finite ones kept within its range, the others NaN.
 __device__ __forceinline__ uint32_t cache_f16(float x) {
@@ -29,91 +33,117 @@ __device__ __forceinline__ size_t block_of(int row, int hk, int n_kv, int log_pa
     return (((page * n_kv + hk) << (log_page - 4)) + (slot >> 4)) * (PAGE_BLOCK * HD * (H ? 2 : 4));
 }
 
+// The workgroups' rows: of a group of n tokens and `heads` heads, row r is token r % n of head r / n; workgroup y of `per`
+// has rows y * ROWS + sub + k * per * ROWS.
 template <bool H, int HD>
 __global__ __launch_bounds__(256)
-void paged_append_kernel(PagedAppend a) {
+void paged_append_kernel(PagedAppend a, int per, int per_v) {
     constexpr int LANES = HD / 8, ROWS = 256 / LANES;
-    __shared__ float2 turn[HD / 2];
-    const int n_tokens = a.n_tokens < 0 ? a.counts->n_tokens : a.n_tokens;
-    const int heads = a.n_q + 2 * a.n_kv, sub = threadIdx.x / LANES, d0 = 8 * (threadIdx.x % LANES);
-    for (int t = blockIdx.x; t < n_tokens; t += gridDim.x) {
-        const PagedToken tok = a.tokens[t];
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.rotary.rot / 2; i += 256) turn[i] = rotary_turn(tok.pos, a.rotary, i);
-        __syncthreads();
-        for (int r = blockIdx.y * ROWS + sub; r < heads; r += gridDim.y * ROWS) {
-            float y[8];
-            if (r < a.n_q) {
-                norm_turn8<HD>(a.q + ((size_t)t * a.n_q + r) * HD, d0, a.q_norm, a.eps, a.rotary, turn, y);
-                float4* out = reinterpret_cast<float4*>(a.q_out + ((size_t)r * n_tokens + t) * HD + d0);
-                out[0] = make_float4(y[0], y[1], y[2], y[3]);
-                out[1] = make_float4(y[4], y[5], y[6], y[7]);
-            } else if (r < a.n_q + a.n_kv) {
-                const int hk = r - a.n_q;
-                norm_turn8<HD>(a.k + ((size_t)t * a.n_kv + hk) * HD, d0, a.k_norm, a.eps, a.rotary, turn, y);
-                if (tok.row < 0) continue;
-                uint8_t* b = a.k_pool + block_of<H, HD>(tok.row, hk, a.n_kv, a.log_page);
-                const int slot = tok.row & 15;
-                if constexpr (H) {
-                    uint4 h;
-                    h.x = cache_f16(y[0]) | cache_f16(y[1]) << 16;
-                    h.y = cache_f16(y[2]) | cache_f16(y[3]) << 16;
-                    h.z = cache_f16(y[4]) | cache_f16(y[5]) << 16;
-                    h.w = cache_f16(y[6]) | cache_f16(y[7]) << 16;
-                    *reinterpret_cast<uint4*>(b + ((d0 / 8) * 16 + slot) * 16) = h;
-                } else {
-                    #pragma unroll
-                    for (int u = 0; u < 2; u++)
-                        *reinterpret_cast<uint4*>(b + ((d0 / 4 + u) * 16 + slot) * 16) =
-                            make_uint4(cache_f32(y[4 * u]), cache_f32(y[4 * u + 1]), cache_f32(y[4 * u + 2]), cache_f32(y[4 * u + 3]));
+    __shared__ float2 turn[TURN_TOKENS][HD / 2];
+    const int n_tokens = a.n_tokens < 0 ? a.counts->n_tokens : a.n_tokens, n_groups = a.n_tokens < 0 ? a.counts->groups : a.n_groups;
+    const int sub = threadIdx.x / LANES, d0 = 8 * (threadIdx.x % LANES), heads = a.n_q + a.n_kv;
+    for (int w = blockIdx.x; w < n_groups; w += gridDim.x) {
+        const PagedGroup gr = a.groups[w];
+        if ((int)blockIdx.y < per) {
+            const int rows = heads * gr.n;
+            const auto from = [&](int r) {
+                const int head = r / gr.n, t = gr.t0 + r % gr.n;
+                return head < a.n_q ? a.q + ((size_t)t * a.n_q + head) * HD : a.k + ((size_t)t * a.n_kv + head - a.n_q) * HD;
+            };
+            int r = blockIdx.y * ROWS + sub;
+            TurnRow<HD> x, next;
+            if (r < rows) x.load(from(r), d0);
+            __syncthreads();   // (the table of an earlier group has been read)
+            turn_table<HD>(turn, gr.pos, gr.n, a.rotary);
+            __syncthreads();
+            for (; r < rows; r += per * ROWS) {
+                if (r + per * ROWS < rows) next.load(from(r + per * ROWS), d0);
+                const int head = r / gr.n, t = r % gr.n;
+                x.turn(from(r), d0, head < a.n_q ? a.q_norm : a.k_norm, a.eps, a.rotary, turn[t]);
+                if (head < a.n_q) {
+                    float4* out = reinterpret_cast<float4*>(a.q_out + ((size_t)head * n_tokens + gr.t0 + t) * HD + d0);
+                    out[0] = make_float4(x.x[0], x.x[1], x.x[2], x.x[3]);
+                    out[1] = make_float4(x.x[4], x.x[5], x.x[6], x.x[7]);
+                } else if (gr.row >= 0) {
+                    uint8_t* b = a.k_pool + block_of<H, HD>(gr.row, head - a.n_q, a.n_kv, a.log_page);
+                    const int slot = (gr.row & 15) + t;
+                    if constexpr (H) {
+                        uint4 h;
+                        h.x = cache_f16(x.x[0]) | cache_f16(x.x[1]) << 16;
+                        h.y = cache_f16(x.x[2]) | cache_f16(x.x[3]) << 16;
+                        h.z = cache_f16(x.x[4]) | cache_f16(x.x[5]) << 16;
+                        h.w = cache_f16(x.x[6]) | cache_f16(x.x[7]) << 16;
+                        *reinterpret_cast<uint4*>(b + ((d0 / 8) * 16 + slot) * 16) = h;
+                    } else {
+                        #pragma unroll
+                        for (int u = 0; u < 2; u++)
+                            *reinterpret_cast<uint4*>(b + ((d0 / 4 + u) * 16 + slot) * 16) =
+                                make_uint4(cache_f32(x.x[4 * u]), cache_f32(x.x[4 * u + 1]), cache_f32(x.x[4 * u + 2]), cache_f32(x.x[4 * u + 3]));
+                    }
                 }
-            } else {
-                if (tok.row < 0) continue;
-                const int hk = r - a.n_q - a.n_kv;
-                const float4* src = reinterpret_cast<const float4*>(a.v + ((size_t)t * a.n_kv + hk) * HD + d0);
-                const float4 v0 = src[0], v1 = src[1];
-                const float x[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-                uint8_t* b = a.v_pool + block_of<H, HD>(tok.row, hk, a.n_kv, a.log_page);
-                const int slot = tok.row & 15;
-                #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    if constexpr (H)
-                        reinterpret_cast<uint16_t*>(b)[((slot >> 3) * HD + d0 + e) * 8 + (slot & 7)] = (uint16_t)cache_f16(x[e]);
-                    else
-                        reinterpret_cast<uint32_t*>(b)[((slot >> 2) * HD + d0 + e) * 4 + (slot & 3)] = cache_f32(x[e]);
+                x = next;
+            }
+        } else if (gr.row >= 0) {
+            constexpr int E = H ? 8 : 4, PARTS = PAGE_BLOCK / E;
+            const int slot0 = gr.row & 15, y = blockIdx.y - per;
+            for (int u = y * 256 + threadIdx.x; u < a.n_kv * PARTS * HD; u += per_v * 256) {
+                const int d = u % HD, part = u / HD % PARTS, hk = u / HD / PARTS;
+                // the slots of the part that are the group's
+                const int first = max(slot0, E * part) - E * part, last = min(slot0 + gr.n, E * part + E) - E * part;
+                if (first >= last) continue;
+                const ptrdiff_t next = (ptrdiff_t)a.n_kv * HD;   // (token's row)
+                const float* src = a.v + (gr.t0 + E * part - slot0) * next + hk * HD + d;   // of the part's first slot
+                uint8_t* to = a.v_pool + block_of<H, HD>(gr.row, hk, a.n_kv, a.log_page) + (part * HD + d) * 16;
+                uint32_t x[E];
+                if (last - first == E) {
+                    #pragma unroll
+                    for (int e = 0; e < E; e++) x[e] = __builtin_bit_cast(uint32_t, src[e * next]);
+                    #pragma unroll
+                    for (int e = 0; e < E; e++) x[e] = H ? cache_f16(__builtin_bit_cast(float, x[e])) : cache_f32(__builtin_bit_cast(float, x[e]));
+                    if constexpr (H) *reinterpret_cast<uint4*>(to) = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+                    else *reinterpret_cast<uint4*>(to) = make_uint4(x[0], x[1], x[2], x[3]);
+                } else {
+                    for (int e = first; e < last; e++) {
+                        const float v = src[e * next];
+                        if constexpr (H) reinterpret_cast<uint16_t*>(to)[e] = (uint16_t)cache_f16(v);
+                        else reinterpret_cast<uint32_t*>(to)[e] = cache_f32(v);
+                    }
                 }
             }
         }
     }
 }
 
-// The tokens' rows of K and V as they lie in the cache, [n_tokens, n_kv, HD] of its type (zeros where they have none).
+// The tokens' rows of K and V as they lie in the cache, [n_tokens, n_kv, HD] of its type (zeros where they have none):
+// 16 bytes of a row a lane.
 template <bool H, int HD>
 __global__ __launch_bounds__(256)
 void paged_read_kernel(PagedAppend a, uint8_t* k_out, uint8_t* v_out) {
-    constexpr int E = H ? 8 : 4, LANES = HD / E;   // 16 bytes a lane
-    const int n_tokens = a.n_tokens < 0 ? a.counts->n_tokens : a.n_tokens;
-    const size_t n = (size_t)n_tokens * a.n_kv * LANES;
-    for (size_t w = (size_t)blockIdx.x * 256 + threadIdx.x; w < n; w += (size_t)gridDim.x * 256) {
-        const int c = (int)(w % LANES), hk = (int)(w / LANES % a.n_kv), t = (int)(w / LANES / a.n_kv);
-        const int row = a.tokens[t].row, slot = row & 15;
-        const size_t at = row < 0 ? 0 : block_of<H, HD>(row, hk, a.n_kv, a.log_page);
-        uint4 x = make_uint4(0, 0, 0, 0), y = x;
-        if (row >= 0) {
-            x = *reinterpret_cast<const uint4*>(a.k_pool + at + (c * 16 + slot) * 16);
-            if constexpr (H) {
-                const uint16_t* b = reinterpret_cast<const uint16_t*>(a.v_pool + at) + ((slot >> 3) * HD + 8 * c) * 8 + (slot & 7);
-                y.x = b[0] | (uint32_t)b[8] << 16;
-                y.y = b[16] | (uint32_t)b[24] << 16;
-                y.z = b[32] | (uint32_t)b[40] << 16;
-                y.w = b[48] | (uint32_t)b[56] << 16;
-            } else {
-                const uint32_t* b = reinterpret_cast<const uint32_t*>(a.v_pool + at) + ((slot >> 2) * HD + 4 * c) * 4 + (slot & 3);
-                y = make_uint4(b[0], b[4], b[8], b[12]);
+    constexpr int E = H ? 8 : 4, LANES = HD / E;
+    const int n_groups = a.n_tokens < 0 ? a.counts->groups : a.n_groups;
+    for (int w = blockIdx.x; w < n_groups; w += gridDim.x) {
+        const PagedGroup gr = a.groups[w];
+        for (int u = blockIdx.y * 256 + threadIdx.x; u < gr.n * a.n_kv * LANES; u += gridDim.y * 256) {
+            const int c = u % LANES, hk = u / LANES % a.n_kv, t = u / LANES / a.n_kv, slot = (gr.row & 15) + t;
+            uint4 x = make_uint4(0, 0, 0, 0), y = x;
+            if (gr.row >= 0) {
+                const size_t at = block_of<H, HD>(gr.row, hk, a.n_kv, a.log_page);
+                x = *reinterpret_cast<const uint4*>(a.k_pool + at + (c * 16 + slot) * 16);
+                if constexpr (H) {
+                    const uint16_t* b = reinterpret_cast<const uint16_t*>(a.v_pool + at) + ((slot >> 3) * HD + 8 * c) * 8 + (slot & 7);
+                    y.x = b[0] | (uint32_t)b[8] << 16;
+                    y.y = b[16] | (uint32_t)b[24] << 16;
+                    y.z = b[32] | (uint32_t)b[40] << 16;
+                    y.w = b[48] | (uint32_t)b[56] << 16;
+                } else {
+                    const uint32_t* b = reinterpret_cast<const uint32_t*>(a.v_pool + at) + ((slot >> 2) * HD + 4 * c) * 4 + (slot & 3);
+                    y = make_uint4(b[0], b[4], b[8], b[12]);
+                }
             }
+            const size_t to = ((size_t)(gr.t0 + t) * a.n_kv + hk) * LANES + c;
+            if (k_out) reinterpret_cast<u32x4_a4*>(k_out)[to] = u32x4_a4{x.x, x.y, x.z, x.w};
+            if (v_out) reinterpret_cast<u32x4_a4*>(v_out)[to] = u32x4_a4{y.x, y.y, y.z, y.w};
         }
-        if (k_out) reinterpret_cast<u32x4_a4*>(k_out)[w] = u32x4_a4{x.x, x.y, x.z, x.w};
-        if (v_out) reinterpret_cast<u32x4_a4*>(v_out)[w] = u32x4_a4{y.x, y.y, y.z, y.w};
     }
 }
 
@@ -127,31 +157,46 @@ void paged_upload_kernel(PagedPieces p) {
     }
 }
 
-// x [seq, heads, HD] -> [heads, seq, HD], normed and rotated.
+// x [seq, heads, HD] -> [heads, seq, HD], normed and rotated; the rows of a workgroup as for the append.
 template <int HD>
 __global__ __launch_bounds__(256)
-void norm_rope_kernel(const float* x, float* out, int seq, int heads, int start_pos, const float* w, float eps, Rotary r) {
+void norm_rope_kernel(const float* x, float* out, int seq, int heads, int tokens, int start_pos, const float* w, float eps, Rotary rotary) {
     constexpr int LANES = HD / 8, ROWS = 256 / LANES;
-    __shared__ float2 turn[HD / 2];
-    const int t = blockIdx.x, sub = threadIdx.x / LANES, d0 = 8 * (threadIdx.x % LANES);
-    for (int i = threadIdx.x; i < r.rot / 2; i += 256) turn[i] = rotary_turn(start_pos + t, r, i);
+    __shared__ float2 turn[TURN_TOKENS][HD / 2];
+    const int t0 = blockIdx.x * tokens, n = min(tokens, seq - t0), rows = heads * n;
+    const int sub = threadIdx.x / LANES, d0 = 8 * (threadIdx.x % LANES), step = gridDim.y * ROWS;
+    const auto from = [&](int r) { return x + ((size_t)(t0 + r % n) * heads + r / n) * HD; };
+    int r = blockIdx.y * ROWS + sub;
+    TurnRow<HD> y, next;
+    if (r < rows) y.load(from(r), d0);
+    turn_table<HD>(turn, start_pos + t0, n, rotary);
     __syncthreads();
-    for (int h = blockIdx.y * ROWS + sub; h < heads; h += gridDim.y * ROWS) {
-        float y[8];
-        norm_turn8<HD>(x + ((size_t)t * heads + h) * HD, d0, w, eps, r, turn, y);
-        float4* o = reinterpret_cast<float4*>(out + ((size_t)h * seq + t) * HD + d0);
-        o[0] = make_float4(y[0], y[1], y[2], y[3]);
-        o[1] = make_float4(y[4], y[5], y[6], y[7]);
+    for (; r < rows; r += step) {
+        if (r + step < rows) next.load(from(r + step), d0);
+        y.turn(from(r), d0, w, eps, rotary, turn[r % n]);
+        float4* o = reinterpret_cast<float4*>(out + ((size_t)(r / n) * seq + t0 + r % n) * HD + d0);
+        o[0] = make_float4(y.x[0], y.x[1], y.x[2], y.x[3]);
+        o[1] = make_float4(y.x[4], y.x[5], y.x[6], y.x[7]);
+        y = next;
     }
+}
+
+// Workgroups for `groups` groups of at most `passes` passes each: enough to fill the card, with at most all of a group's.
+unsigned shares(size_t groups, size_t passes) {
+    const size_t want = (TURN_WORKGROUPS + groups - 1) / groups;
+    return (unsigned)(want < 1 ? 1 : want < passes ? want : passes);
 }
 
 }  // namespace
 
 hipError_t paged_append_launch(const PagedAppend& a, bool f16, size_t hd, hipStream_t s) {
-    const unsigned rows = (unsigned)(256 / (hd / 8)), heads = (unsigned)(a.n_q + 2 * a.n_kv), per = (heads + rows - 1) / rows;
-    // (a captured call goes round its tokens)
-    const dim3 g(a.n_tokens < 0 ? 256u : (unsigned)a.n_tokens, per);
-    #define BARQ_APPEND(H, D) if (f16 == H && hd == D) hipLaunchKernelGGL((paged_append_kernel<H, D>), g, dim3(256), 0, s, a);
+    const bool captured = a.n_tokens < 0;   // (a captured call goes round the groups)
+    const size_t groups = captured ? 256 : (size_t)a.n_groups, most = captured || a.n_tokens > a.n_groups ? TURN_TOKENS : 1;
+    const size_t rows = 256 / (hd / 8), heads = (size_t)a.n_q + a.n_kv;
+    const unsigned per = shares(groups, (heads * most + rows - 1) / rows);
+    const unsigned per_v = shares(groups, ((size_t)a.n_kv * (f16 ? 2 : 4) * hd + 255) / 256);
+    const dim3 g((unsigned)groups, per + per_v);
+    #define BARQ_APPEND(H, D) if (f16 == H && hd == D) hipLaunchKernelGGL((paged_append_kernel<H, D>), g, dim3(256), 0, s, a, (int)per, (int)per_v);
     BARQ_APPEND(true, 64) BARQ_APPEND(true, 128) BARQ_APPEND(true, 256)
     BARQ_APPEND(false, 64) BARQ_APPEND(false, 128) BARQ_APPEND(false, 256)
     #undef BARQ_APPEND
@@ -159,8 +204,9 @@ hipError_t paged_append_launch(const PagedAppend& a, bool f16, size_t hd, hipStr
 }
 
 hipError_t paged_read_launch(const PagedAppend& a, bool f16, size_t hd, void* k_out, void* v_out, hipStream_t s) {
-    const size_t n = (size_t)(a.n_tokens < 0 ? 256 : a.n_tokens) * a.n_kv * (hd / (f16 ? 8 : 4));
-    const dim3 g((unsigned)((n + 255) / 256 < 4096 ? (n + 255) / 256 : 4096));
+    const bool captured = a.n_tokens < 0;
+    const size_t groups = captured ? 256 : (size_t)a.n_groups, most = captured || a.n_tokens > a.n_groups ? TURN_TOKENS : 1;
+    const dim3 g((unsigned)groups, shares(groups, (most * a.n_kv * (hd / (f16 ? 8 : 4)) + 255) / 256));
     uint8_t *k = static_cast<uint8_t*>(k_out), *v = static_cast<uint8_t*>(v_out);
     #define BARQ_READ(H, D) if (f16 == H && hd == D) hipLaunchKernelGGL((paged_read_kernel<H, D>), g, dim3(256), 0, s, a, k, v);
     BARQ_READ(true, 64) BARQ_READ(true, 128) BARQ_READ(true, 256)
@@ -179,11 +225,15 @@ hipError_t paged_upload_launch(const PagedPieces& p, hipStream_t s) {
 
 hipError_t norm_rope_launch(const float* x, float* out, size_t seq, size_t heads, size_t hd, size_t start_pos,
                             const float* w, float eps, const Rotary& r, hipStream_t s) {
-    const unsigned rows = (unsigned)(256 / (hd / 8)), per = (unsigned)((heads + rows - 1) / rows);
-    const dim3 g((unsigned)seq, per < 65535u ? per : 65535u);
-    if (hd == 64) hipLaunchKernelGGL(norm_rope_kernel<64>, g, dim3(256), 0, s, x, out, (int)seq, (int)heads, (int)start_pos, w, eps, r);
-    if (hd == 128) hipLaunchKernelGGL(norm_rope_kernel<128>, g, dim3(256), 0, s, x, out, (int)seq, (int)heads, (int)start_pos, w, eps, r);
-    if (hd == 256) hipLaunchKernelGGL(norm_rope_kernel<256>, g, dim3(256), 0, s, x, out, (int)seq, (int)heads, (int)start_pos, w, eps, r);
+    // tokens of a workgroup: 16, fewer while that leaves the card empty
+    size_t tokens = TURN_TOKENS;
+    while (tokens > 1 && (seq + tokens - 1) / tokens < 64) tokens /= 2;
+    const size_t groups = (seq + tokens - 1) / tokens, rows = 256 / (hd / 8);
+    const dim3 g((unsigned)groups, shares(groups, (heads * tokens + rows - 1) / rows));
+    #define BARQ_TURN(D) \
+        if (hd == D) hipLaunchKernelGGL(norm_rope_kernel<D>, g, dim3(256), 0, s, x, out, (int)seq, (int)heads, (int)tokens, (int)start_pos, w, eps, r);
+    BARQ_TURN(64) BARQ_TURN(128) BARQ_TURN(256)
+    #undef BARQ_TURN
     return hipGetLastError();
 }
 

@@ -93,6 +93,20 @@ inline PagedFault paged_check(const PagedLimits& lim, size_t n_seqs, const int32
     return PagedFault::none;
 }
 
+// The most groups of new tokens.
+inline size_t paged_max_groups(size_t max_seqs, size_t max_tokens) { return std::min(max_tokens, max_tokens / PAGE_BLOCK + 2 * max_seqs); }
+
+// A sequence's new tokens, the batch's t0 .. on, cut where a block ends.
+inline PagedGroup* paged_groups(int32_t t0, int32_t q_len, int32_t kv_len, const int32_t* ids, int log_page, PagedGroup* g) {
+    for (int32_t j = kv_len - q_len; j < kv_len;) {
+        const int32_t n = std::min(PAGE_BLOCK - j % PAGE_BLOCK, kv_len - j), id = ids[j >> log_page];
+        *g++ = {t0, n, id < 0 ? -1 : (id << log_page) + (j & ((1 << log_page) - 1)), j};
+        t0 += n;
+        j += n;
+    }
+    return g;
+}
+
 // The most items and merges that a plan of these limits has.
 inline size_t paged_max_tiles(size_t max_seqs, size_t max_tokens, size_t G) { return (max_tokens * G + 15) / 16 + max_seqs; }
 
@@ -119,6 +133,7 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
     for (const PagedSeq& s : seqs) {
         const int64_t rows = s.q_len * sh.G, past = s.kv_len - s.q_len;
         const bool many = rows >= sh.many_from;
+        // (all tiles of a sequence by one kernel, the last and smaller one too)
         const int64_t tile = many ? 128 : std::min<int64_t>(rows <= 16 ? 16 : 32, sh.few_rows), unit = many ? sh.many_step : sh.few_step;
         for (int64_t r = 0; r < rows; r += tile) {
             PagedItem it{};
@@ -134,6 +149,7 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
             it.b = (int32_t)low;
             it.v1 = (int32_t)(it.a + (end + unit - 1) / unit - low);
             it.part = -1;
+            it.tile = (int32_t)tile;
             steps[many] += it.v1;
             (many ? p.many : p.few).push_back(it);
         }
@@ -167,12 +183,12 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
             items.swap(cut);
         }
         // the longest first: the last workgroups to start are short ones
-        std::stable_sort(items.begin(), items.end(), [kind](const PagedItem& x, const PagedItem& y) {
-            if (!kind && (x.rows <= 16) != (y.rows <= 16)) return x.rows <= 16;
+        std::stable_sort(items.begin(), items.end(), [](const PagedItem& x, const PagedItem& y) {
+            if (x.tile != y.tile) return x.tile < y.tile;
             return x.v1 - x.v0 > y.v1 - y.v0;
         });
     }
-    p.few16 = (int)(std::find_if(p.few.begin(), p.few.end(), [](const PagedItem& x) { return x.rows > 16; }) - p.few.begin());
+    p.few16 = (int)(std::find_if(p.few.begin(), p.few.end(), [](const PagedItem& x) { return x.tile > 16; }) - p.few.begin());
 }
 
 }  // namespace barq

@@ -20,52 +20,76 @@ __device__ __forceinline__ float2 rotary_turn(int pos, const Rotary& r, int i) {
     return make_float2(cs * r.magnitude, sn * r.magnitude);
 }
 
-// The lane's eight dims d0 .. d0 + 7 of a head: x (a row at `row`, 16-byte aligned), by HD / 8 neighbouring lanes,
-// normed where w is not null, rotated where r.rot is not zero.  turn: cos and sin of pair i at turn[i].
+// The lane's eight dims d0 .. d0 + 7 of a head (a row of HD / 8 neighbouring lanes, 16-byte aligned): loaded, then
+// normed where w is not null and rotated where r.rot is not zero, with cos and sin of pair i at turn[i].
 template <int HD>
-__device__ __forceinline__ void norm_turn8(const float* __restrict__ row, int d0, const float* __restrict__ w, float eps,
-                                           const Rotary& r, const float2* turn, float (&y)[8]) {
+struct TurnRow {
     float x[8];
-    #pragma unroll
-    for (int u = 0; u < 2; u++) {
-        const float4 v = *reinterpret_cast<const float4*>(row + d0 + 4 * u);
-        x[4 * u] = v.x, x[4 * u + 1] = v.y, x[4 * u + 2] = v.z, x[4 * u + 3] = v.w;
-    }
-    float f = 1.0f;
-    if (w) {   // (the same order whatever the grid: a row's sum is its lanes')
-        float ss = 0.0f;
+    __device__ __forceinline__ void load(const float* __restrict__ row, int d0) {
         #pragma unroll
-        for (int e = 0; e < 8; e++) ss = __builtin_fmaf(x[e], x[e], ss);
-        ss = group_sum<HD / 8>(ss);
-        f = 1.0f / sqrtf(ss / (float)HD + fmaxf(eps, 1.1920929e-7f));
-        #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = (x[e] * f) * w[d0 + e];
-    }
-    #pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = x[e];
-    if (d0 >= r.rot) return;
-    if (r.layout == ROPE_INTERLEAVED) {
-        #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            if (d0 + e >= r.rot) break;
-            const float2 t = turn[(d0 + e) / 2];
-            y[e] = x[e] * t.x - x[e + 1] * t.y;
-            y[e + 1] = x[e] * t.y + x[e + 1] * t.x;
-        }
-    } else {
-        const int half = r.rot / 2;
-        #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int d = d0 + e;
-            if (d >= r.rot) break;
-            const bool low = d < half;
-            const int other = low ? d + half : d - half;
-            float z = row[other];
-            if (w) z = (z * f) * w[other];
-            const float2 t = turn[low ? d : other];
-            y[e] = low ? x[e] * t.x - z * t.y : z * t.y + x[e] * t.x;
+        for (int u = 0; u < 2; u++) {
+            const float4 v = *reinterpret_cast<const float4*>(row + d0 + 4 * u);
+            x[4 * u] = v.x, x[4 * u + 1] = v.y, x[4 * u + 2] = v.z, x[4 * u + 3] = v.w;
         }
     }
+    __device__ __forceinline__ void turn(const float* __restrict__ row, int d0, const float* __restrict__ w, float eps, const Rotary& r,
+                                         const float2* turn) {
+        float f = 1.0f;
+        if (w) {   // (the sum in the same order whatever the grid)
+            float ss = 0.0f;
+            #pragma unroll
+            for (int e = 0; e < 8; e++) ss = __builtin_fmaf(x[e], x[e], ss);
+            ss = group_sum<HD / 8>(ss);
+            f = 1.0f / sqrtf(ss / (float)HD + fmaxf(eps, 1.1920929e-7f));
+            #pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = (x[e] * f) * w[d0 + e];
+        }
+        if (r.layout == ROPE_INTERLEAVED) {
+            #pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                if (d0 + e < r.rot) {
+                    const float2 t = turn[(d0 + e) / 2];
+                    const float a = x[e] * t.x - x[e + 1] * t.y, b = x[e] * t.y + x[e + 1] * t.x;
+                    x[e] = a;
+                    x[e + 1] = b;
+                }
+            }
+        } else {
+            // the pairs' other halves: whole lanes of the row, or read once more
+            const int half = r.rot / 2, to = d0 < half ? half : -half;
+            float z[8];
+            if (half % 8 == 0) {
+                const int lane = (threadIdx.x & 63) + (d0 < r.rot ? to / 8 : 0);
+                #pragma unroll
+                for (int e = 0; e < 8; e++) z[e] = __shfl(x[e], lane);
+            } else {
+                #pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int d = d0 + e, other = d < half ? d + half : d - half;
+                    z[e] = d < r.rot ? row[other] : 0.0f;
+                    if (w && d < r.rot) z[e] = (z[e] * f) * w[other];
+                }
+            }
+            #pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int d = d0 + e;
+                if (d < r.rot) {
+                    const bool low = d < half;
+                    const float2 t = turn[low ? d : d - half];
+                    x[e] = low ? x[e] * t.x - z[e] * t.y : z[e] * t.y + x[e] * t.x;
+                }
+            }
+        }
+    }
+};
+
+constexpr int TURN_TOKENS = 16;   // tokens of a workgroup
+
+// cos and sin of tokens pos .. pos + n - 1: turn[token][HD / 2]
+template <int HD>
+__device__ __forceinline__ void turn_table(float2 (*turn)[HD / 2], int pos, int n, const Rotary& r) {
+    const int half = r.rot / 2;
+    for (int u = threadIdx.x; u < n * half; u += 256) turn[u / half][u % half] = rotary_turn(pos + u / half, r, u % half);
 }
 
 }  // namespace barq

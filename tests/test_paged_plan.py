@@ -41,12 +41,25 @@ static int plan() {
     paged_plan(sh, seqs, p);
     printf("%d %d %zu %d %zu %zu %zu\n", sh.few_step, sh.many_step, sh.part_rows, p.few16, p.few.size(), p.many.size(), p.merges.size());
     for (auto* v : {&p.few, &p.many})
-        for (auto& i : *v) printf("%d %d %d %d %d %d %d %d %d %d\n", i.q0, i.past, i.kv_len, i.row0, i.rows, i.a, i.b, i.v0, i.v1, i.part);
+        for (auto& i : *v) printf("%d %d %d %d %d %d %d %d %d %d %d\n", i.q0, i.past, i.kv_len, i.row0, i.rows, i.a, i.b, i.v0, i.v1, i.part, i.tile);
     for (auto& m : p.merges) printf("%d %d %d %d %d\n", m.q0, m.row0, m.rows, m.part, m.n_split);
     printf("%zu %zu\n", paged_max_tiles(n, max_tokens, sh.G), (size_t)(2 * (sh.few_target + sh.many_target)));
     return 0;
 }
-int main(int, char** v) { return strcmp(v[1], "check") ? plan() : check(); }
+static int groups() {
+    int t0, q, kv, log_page;
+    size_t n;
+    if (scanf("%d %d %d %d %zu", &t0, &q, &kv, &log_page, &n) != 5) return 1;
+    std::vector<int32_t> ids(n);
+    for (auto& x : ids) if (scanf("%d", &x) != 1) return 1;
+    std::vector<PagedGroup> g(paged_max_groups(1, q) + 1);
+    const PagedGroup* end = paged_groups(t0, q, kv, ids.data(), log_page, g.data());
+    for (const PagedGroup* p = g.data(); p < end; p++) printf("%d %d %d %d\n", p->t0, p->n, p->row, p->pos);
+    return 0;
+}
+int main(int, char** v) {
+    if (!strcmp(v[1], "groups")) return groups();
+    return strcmp(v[1], "check") ? plan() : check(); }
 """
 
 
@@ -90,6 +103,19 @@ def test_what_a_step_is_refused_for(program, q, kv, pages, fault, word):
     assert int(got) == fault and word in msg, out
 
 
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("q,kv", [(1, 1), (1, 16), (1, 17), (0, 5), (16, 16), (16, 40), (33, 64), (100, 259), (2, 33), (31, 47)])
+def test_tokens_in_groups_of_a_block(program, page, q, kv):
+    rng = random.Random(q + kv)
+    ids = rng.sample(range(40), -(-kv // page))
+    ids[rng.randrange(len(ids))] = -1
+    lines = [list(map(int, l.split())) for l in program("groups", 7, q, kv, page.bit_length() - 1, len(ids), *ids).splitlines()]
+    got = [(t + i, row + i if row >= 0 else -1, pos + i) for t, n, row, pos in lines for i in range(n)]
+    want = [(7 + i, ids[p // page] * page + p % page if ids[p // page] >= 0 else -1, p) for i, p in enumerate(range(kv - q, kv))]
+    assert got == want and len(lines) <= min(q, q // 16 + 2)
+    assert all(pos // 16 == (pos + n - 1) // 16 for _, n, _, pos in lines)
+
+
 def cover(program, G, n_kv, window, n_sink, f16, hd, seqs):
     tokens = max(sum(q for q, _ in seqs), 1)
     lines = [list(map(int, l.split())) for l in program(
@@ -99,12 +125,12 @@ def cover(program, G, n_kv, window, n_sink, f16, hd, seqs):
     merges = lines[1 + n_few + n_many:1 + n_few + n_many + n_merges]
     tiles, extra = lines[-1]
     assert n_merges <= tiles and max(n_few, n_many) <= tiles + extra   # what batch_create has room for
-    assert all((i[4] <= 16) == (k < few16) for k, i in enumerate(few))
+    assert all(i[10] == (16 if k < few16 else 32) for k, i in enumerate(few)) and all(i[10] == 128 for i in many)
     starts = [sum(q for q, _ in seqs[:s]) for s in range(len(seqs))]
     seen, parts, states = {}, {}, set()
-    for items, step, most in ((few, few_step, 32), (many, many_step, 128)):
-        for q0, past, kv, row0, rows, a, b, v0, v1, part in items:
-            assert 0 < rows <= most and v0 < v1
+    for items, step in ((few, few_step), (many, many_step)):
+        for q0, past, kv, row0, rows, a, b, v0, v1, part, tile in items:
+            assert 0 < rows <= tile and v0 < v1
             s = max(i for i, q in enumerate(starts) if q == q0 and seqs[i][0])
             assert (seqs[s][1], seqs[s][1] - seqs[s][0]) == (kv, past)
             steps = [v if v < a else v - a + b for v in range(v0, v1)]
