@@ -27,6 +27,13 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <bool H>
 __device__ __forceinline__ int tile_pos(int r, int h) { return H ? 16 * (r / 8) + 8 * h + r % 8 : 8 * (r / 4) + 4 * h + r % 4; }
 
+template <bool H>
+__device__ __forceinline__ u32x4v finite(u32x4v v) {
+    #pragma unroll
+    for (int e = 0; e < 4; e++) v[e] &= ~(H ? f16_bad(v[e]) : f32_bad(v[e]));
+    return v;
+}
+
 template <bool H, int HD>
 __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2)
 void paged_many_kernel(PagedAttn a, int count) {
@@ -87,6 +94,7 @@ void paged_many_kernel(PagedAttn a, int count) {
         // the wave's rows
         const int row0 = it.row0 + 32 * wave, end = it.row0 + it.rows, mine = min(row0 + i, end - 1), tok = mine / a.G;
         const int pos = it.past + tok, p_first = it.past + min(row0, end - 1) / a.G, p_last = it.past + min(row0 + 31, end - 1) / a.G;
+        const int all_first = it.past + it.row0 / a.G, all_last = it.past + (end - 1) / a.G;
         u32x4v qh[NC], ql[H ? NC : 1];
         float back = 1.0f;
         {
@@ -135,9 +143,61 @@ void paged_many_kernel(PagedAttn a, int count) {
             }
             const int base = base_of(j), have = has_now;
             has_now = has_next;
+            uint8_t *kt = lds + (size_t)(j & 1) * 2 * NB * BLOCK, *vt = kt + NB * BLOCK;
+            const auto sees = [&](int x) { return ((have >> (x / 16)) & 1) && sight.sees(pos, base + x); };
+            if (have != (1 << NB) - 1 || !sight.all(base, STEP, all_first, all_last)) {
+                // some row of the workgroup does not see all of the step: what is not finite in V becomes zero, after it
+                // has been put as NaN into the dims of the rows that see it (all waves find the same)
+                uint32_t any = 0;
+                for (int u = lane; u < NB * BLOCK / 16; u += 64) {
+                    const u32x4v x = reinterpret_cast<const u32x4v*>(vt)[u];
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) any |= H ? f16_bad(x[e]) : f32_bad(x[e]);
+                }
+                if (__any(any != 0)) {
+                    uint32_t seen = 0;   // bit 16 t + r
+                    #pragma unroll
+                    for (int b = 0; b < 16 * T; b++) seen |= sees(32 * (b / 16) + tile_pos<H>(b % 16, h)) ? 1u << b : 0u;
+                    #pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        f32x16 n = {};   // such places that a row sees
+                        #pragma unroll
+                        for (int t = 0; t < T; t++) {
+                            if constexpr (H) {
+                                #pragma unroll
+                                for (int u = 0; u < 2; u++) {
+                                    u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16), one;
+                                    #pragma unroll
+                                    for (int e = 0; e < 4; e++) {
+                                        const uint32_t two = seen >> (16 * t + 8 * u + 2 * e);
+                                        v[e] = f16_bad(v[e]) & 0x3C003C00u;
+                                        one[e] = (two & 1 ? 0x3C00u : 0u) | (two & 2 ? 0x3C000000u : 0u);
+                                    }
+                                    n = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, v), __builtin_bit_cast(h8v, one), n, 0, 0, 0);
+                                }
+                            } else {
+                                #pragma unroll
+                                for (int q = 0; q < 4; q++) {
+                                    const u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + q / 2) * BLOCK + ((2 * (q & 1) + h) * HD + 32 * d + i) * 16);
+                                    #pragma unroll
+                                    for (int e = 0; e < 4; e++)
+                                        n = __builtin_amdgcn_mfma_f32_32x32x2f32(f32_bad(v[e]) ? 1.0f : 0.0f, (seen >> (16 * t + 4 * q + e)) & 1 ? 1.0f : 0.0f, n, 0, 0, 0);
+                                }
+                            }
+                        }
+                        #pragma unroll
+                        for (int r = 0; r < 16; r++) o[d][r] = n[r] > 0.0f ? NAN : o[d][r];
+                    }
+                    __syncthreads();
+                    for (int u = threadIdx.x; u < NB * BLOCK / 16; u += 64 * NW) {
+                        u32x4v* x = reinterpret_cast<u32x4v*>(vt) + u;
+                        *x = finite<H>(*x);
+                    }
+                    __syncthreads();
+                }
+            }
             // no row of the wave, or nothing that one sees (first tokens end where the window's steps begin)
             if (row0 >= end || base > p_last || (a.window && base >= a.n_sink && base + STEP - 1 <= p_first - a.window)) continue;
-            const uint8_t *kt = lds + (size_t)(j & 1) * 2 * NB * BLOCK, *vt = kt + NB * BLOCK;
             const bool whole = have == (1 << NB) - 1 && sight.all(base, STEP, p_first, p_last);
             float s[T][16];
             #pragma unroll
@@ -160,26 +220,11 @@ void paged_many_kernel(PagedAttn a, int count) {
                 #pragma unroll
                 for (int r = 0; r < 16; r++) s[t][r] = H ? __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) : hi[r];
             }
-            uint32_t seen = 0xFFFFFFFFu;   // bit 16 t + r
-            bool bad = false;
             if (!whole) {
-                seen = 0;
                 #pragma unroll
                 for (int t = 0; t < T; t++)
                     #pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int x = 32 * t + tile_pos<H>(r, h);
-                        const bool see = ((have >> (x / 16)) & 1) && sight.sees(pos, base + x);
-                        seen |= see ? 1u << (16 * t + r) : 0u;
-                        s[t][r] = see ? s[t][r] : -INFINITY;
-                    }
-                uint32_t any = 0;
-                for (int u = lane; u < NB * BLOCK / 16; u += 64) {
-                    const u32x4v x = reinterpret_cast<const u32x4v*>(vt)[u];
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) any |= H ? f16_bad(x[e]) : f32_bad(x[e]);
-                }
-                bad = __any(any != 0);
+                    for (int r = 0; r < 16; r++) s[t][r] = sees(32 * t + tile_pos<H>(r, h)) ? s[t][r] : -INFINITY;
             }
             float top = s[0][0];
             #pragma unroll
@@ -210,72 +255,29 @@ void paged_many_kernel(PagedAttn a, int count) {
                 }
             }
             l = __builtin_fmaf(l, alpha, sum);
-            if (!bad) {
+            #pragma unroll
+            for (int d = 0; d < ND; d++) {
+                f32x16 y = {};
                 #pragma unroll
-                for (int d = 0; d < ND; d++) {
-                    f32x16 y = {};
-                    #pragma unroll
-                    for (int t = 0; t < T; t++) {
-                        if constexpr (H) {
+                for (int t = 0; t < T; t++) {
+                    if constexpr (H) {
+                        #pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const h8v v = *reinterpret_cast<const h8v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16);
+                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(h8v, pl[t][u]), y, 0, 0, 0);
+                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(h8v, ph[t][u]), y, 0, 0, 0);
+                        }
+                    } else {
+                        #pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const f32x4 x = *reinterpret_cast<const f32x4*>(vt + (2 * t + q / 2) * BLOCK + ((2 * (q & 1) + h) * HD + 32 * d + i) * 16);
                             #pragma unroll
-                            for (int u = 0; u < 2; u++) {
-                                const h8v v = *reinterpret_cast<const h8v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16);
-                                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(h8v, pl[t][u]), y, 0, 0, 0);
-                                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(h8v, ph[t][u]), y, 0, 0, 0);
-                            }
-                        } else {
-                            #pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                const f32x4 v = *reinterpret_cast<const f32x4*>(vt + (2 * t + q / 2) * BLOCK + ((2 * (q & 1) + h) * HD + 32 * d + i) * 16);
-                                #pragma unroll
-                                for (int e = 0; e < 4; e++) y = __builtin_amdgcn_mfma_f32_32x32x2f32(v[e], s[t][4 * q + e], y, 0, 0, 0);
-                            }
+                            for (int e = 0; e < 4; e++) y = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], s[t][4 * q + e], y, 0, 0, 0);
                         }
                     }
-                    #pragma unroll
-                    for (int r = 0; r < 16; r++) o[d][r] = __builtin_fmaf(o[d][r], alpha, y[r]);
                 }
-            } else {
-                // the same with what is not finite as zero, and the number of such places that a row sees
-                for (int d = 0; d < ND; d++) {
-                    f32x16 y = {}, n = {};
-                    #pragma unroll
-                    for (int t = 0; t < T; t++) {
-                        if constexpr (H) {
-                            #pragma unroll
-                            for (int u = 0; u < 2; u++) {
-                                u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16), is, one;
-                                #pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const uint32_t b = f16_bad(v[e]), two = seen >> (16 * t + 8 * u + 2 * e);
-                                    v[e] &= ~b;
-                                    is[e] = b & 0x3C003C00u;
-                                    one[e] = (two & 1 ? 0x3C00u : 0u) | (two & 2 ? 0x3C000000u : 0u);
-                                }
-                                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, is), __builtin_bit_cast(h8v, one), n, 0, 0, 0);
-                                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, v), __builtin_bit_cast(h8v, pl[t][u]), y, 0, 0, 0);
-                                y = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, v), __builtin_bit_cast(h8v, ph[t][u]), y, 0, 0, 0);
-                            }
-                        } else {
-                            #pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                const u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + q / 2) * BLOCK + ((2 * (q & 1) + h) * HD + 32 * d + i) * 16);
-                                #pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const uint32_t b = f32_bad(v[e]), z = v[e] & ~b;
-                                    n = __builtin_amdgcn_mfma_f32_32x32x2f32(b ? 1.0f : 0.0f, (seen >> (16 * t + 4 * q + e)) & 1 ? 1.0f : 0.0f, n, 0, 0, 0);
-                                    y = __builtin_amdgcn_mfma_f32_32x32x2f32(__builtin_bit_cast(float, z), s[t][4 * q + e], y, 0, 0, 0);
-                                }
-                            }
-                        }
-                    }
-                    #pragma unroll
-                    for (int dd = 0; dd < ND; dd++)
-                        if (dd == d) {
-                            #pragma unroll
-                            for (int r = 0; r < 16; r++) o[dd][r] = n[r] > 0.0f ? NAN : __builtin_fmaf(o[dd][r], alpha, y[r]);
-                        }
-                }
+                #pragma unroll
+                for (int r = 0; r < 16; r++) o[d][r] = __builtin_fmaf(o[d][r], alpha, y[r]);
             }
         }
         const float sum = swap32_add(l, l);
