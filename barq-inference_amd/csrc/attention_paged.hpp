@@ -52,7 +52,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedItem* p) {
 struct PagedSight {
     int window, n_sink;
     __device__ __forceinline__ bool sees(int row_pos, int j) const {
-        return j <= row_pos && (!window || j > row_pos - window || j < n_sink);
+        return (j <= row_pos) & ((window == 0) | (j > row_pos - window) | (j < n_sink));   // (no branches)
     }
     // all positions base .. base + n - 1 by all rows at positions first .. last
     __device__ __forceinline__ bool all(int base, int n, int first, int last) const {

@@ -15,6 +15,9 @@ namespace {
 
 constexpr int NW = 4;   // waves
 
+// sched_barrier: vector and scalar arithmetic may move across, loads and matrix products stay where they are
+#define BARQ_ONLY_ALU_CROSSES 0x0006
+
 __device__ __forceinline__ float halves_max(float v) {
     auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
     return fmaxf(__builtin_bit_cast(float, (int)b[0]), __builtin_bit_cast(float, (int)b[1]));
@@ -26,6 +29,16 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 // the MFMA stands for position 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4), in f32 the MFMA's own row 8 (r / 4) + 4 h + r % 4.
 template <bool H>
 __device__ __forceinline__ int tile_pos(int r, int h) { return H ? 16 * (r / 8) + 8 * h + r % 8 : 8 * (r / 4) + 4 * h + r % 4; }
+
+// Two weights as f16 hi (cut, one instruction for both) + lo (of what that leaves, to the nearest).
+__device__ __forceinline__ void split_weights(float x0, float x1, float minus_one, uint32_t& hi, uint32_t& lo) {
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    asm("" : "+v"(hi));
+    const h2v h = __builtin_bit_cast(h2v, hi);
+    const float r0 = __builtin_fmaf((float)h[0], minus_one, x0), r1 = __builtin_fmaf((float)h[1], minus_one, x1);
+    const h2v r = {(_Float16)r0, (_Float16)r1};
+    lo = __builtin_bit_cast(uint32_t, r);
+}
 
 template <bool H>
 __device__ __forceinline__ u32x4v finite(u32x4v v) {
@@ -144,7 +157,7 @@ void paged_many_kernel(PagedAttn a, int count) {
             const int base = base_of(j), have = has_now;
             has_now = has_next;
             uint8_t *kt = lds + (size_t)(j & 1) * 2 * NB * BLOCK, *vt = kt + NB * BLOCK;
-            const auto sees = [&](int x) { return ((have >> (x / 16)) & 1) && sight.sees(pos, base + x); };
+            const auto sees = [&](int x) { return (((have >> (x / 16)) & 1) != 0) & sight.sees(pos, base + x); };
             if (have != (1 << NB) - 1 || !sight.all(base, STEP, all_first, all_last)) {
                 // some row of the workgroup does not see all of the step: what is not finite in V becomes zero, after it
                 // has been put as NaN into the dims of the rows that see it (all waves find the same)
@@ -199,26 +212,41 @@ void paged_many_kernel(PagedAttn a, int count) {
             // no row of the wave, or nothing that one sees (first tokens end where the window's steps begin)
             if (row0 >= end || base > p_last || (a.window && base >= a.n_sink && base + STEP - 1 <= p_first - a.window)) continue;
             const bool whole = have == (1 << NB) - 1 && sight.all(base, STEP, p_first, p_last);
+            // scores: the next four pieces of K are fetched while the products of these run
+            constexpr int GC = NC / 4;
             float s[T][16];
-            #pragma unroll
-            for (int t = 0; t < T; t++) {
-                f32x16 hi = {}, lo = {};
-                const int slot = H ? 8 * ((i >> 2) & 1) + 4 * ((i >> 3) & 1) + (i & 3) : i & 15;
+            u32x4v kf[2][4];
+            const auto keys = [&](int n, u32x4v (&k)[4]) __attribute__((always_inline)) {
+                const int t = n / GC, slot = H ? 8 * ((i >> 2) & 1) + 4 * ((i >> 3) & 1) + (i & 3) : i & 15;
                 const uint8_t* kb = kt + (2 * t + (i >> 4)) * BLOCK + slot * 16 + h * 256;
                 #pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    const u32x4v k = *reinterpret_cast<const u32x4v*>(kb + c * 512);
+                for (int u = 0; u < 4; u++) k[u] = *reinterpret_cast<const u32x4v*>(kb + (n % GC * 4 + u) * 512);
+            };
+            keys(0, kf[0]);
+            f32x16 hi, lo;
+            #pragma unroll
+            for (int n = 0; n < T * GC; n++) {
+                if (n + 1 < T * GC) keys(n + 1, kf[(n + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(BARQ_ONLY_ALU_CROSSES);
+                if (n % GC == 0) hi = lo = f32x16{};
+                #pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int c = n % GC * 4 + u;
                     if constexpr (H) {
-                        lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, k), __builtin_bit_cast(h8v, ql[c]), lo, 0, 0, 0);
-                        hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, k), __builtin_bit_cast(h8v, qh[c]), hi, 0, 0, 0);
+                        const h8v k = __builtin_bit_cast(h8v, kf[n & 1][u]);
+                        lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(h8v, ql[c]), lo, 0, 0, 0);
+                        hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(h8v, qh[c]), hi, 0, 0, 0);
                     } else {
-                        const f32x4 x = __builtin_bit_cast(f32x4, k), y = __builtin_bit_cast(f32x4, qh[c]);
+                        const f32x4 x = __builtin_bit_cast(f32x4, kf[n & 1][u]), y = __builtin_bit_cast(f32x4, qh[c]);
                         #pragma unroll
                         for (int e = 0; e < 4; e++) hi = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], hi, 0, 0, 0);
                     }
                 }
-                #pragma unroll
-                for (int r = 0; r < 16; r++) s[t][r] = H ? __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) : hi[r];
+                __builtin_amdgcn_sched_barrier(BARQ_ONLY_ALU_CROSSES);
+                if (n % GC == GC - 1) {
+                    #pragma unroll
+                    for (int r = 0; r < 16; r++) s[n / GC][r] = H ? __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) : hi[r];
+                }
             }
             if (!whole) {
                 #pragma unroll
@@ -248,37 +276,57 @@ void paged_many_kernel(PagedAttn a, int count) {
                     #pragma unroll
                     for (int r = 0; r < 16; r += 2) {
                         uint32_t x, y;
-                        split_f16(s[t][r], s[t][r + 1], minus_one, x, y);
+                        split_weights(s[t][r], s[t][r + 1], minus_one, x, y);
                         ph[t][r / 8][r % 8 / 2] = x;
                         pl[t][r / 8][r % 8 / 2] = y;
                     }
                 }
             }
             l = __builtin_fmaf(l, alpha, sum);
+            // O: the next 32 dims' pieces of V likewise; the weights' small parts first, so that fewer sums are cut at y's size
+            constexpr int PIECES = H ? 2 * T : 4 * T;
+            u32x4v vf[2][PIECES];
+            const auto values = [&](int d, u32x4v (&v)[PIECES]) __attribute__((always_inline)) {
+                #pragma unroll
+                for (int u = 0; u < PIECES; u++)
+                    v[u] = *reinterpret_cast<const u32x4v*>(vt + (H ? u : u / 2) * BLOCK + ((H ? h : 2 * (u & 1) + h) * HD + 32 * d + i) * 16);
+            };
+            values(0, vf[0]);
+            f32x16 y[2];
+            const auto join = [&](int d, int r) __attribute__((always_inline)) { o[d][r] = __builtin_fmaf(o[d][r], alpha, y[d & 1][r]); };
             #pragma unroll
             for (int d = 0; d < ND; d++) {
-                f32x16 y = {};
-                #pragma unroll
-                for (int t = 0; t < T; t++) {
-                    if constexpr (H) {
-                        #pragma unroll
-                        for (int u = 0; u < 2; u++) {
-                            const h8v v = *reinterpret_cast<const h8v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16);
-                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(h8v, pl[t][u]), y, 0, 0, 0);
-                            y = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(h8v, ph[t][u]), y, 0, 0, 0);
-                        }
-                    } else {
-                        #pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const f32x4 x = *reinterpret_cast<const f32x4*>(vt + (2 * t + q / 2) * BLOCK + ((2 * (q & 1) + h) * HD + 32 * d + i) * 16);
+                if (d + 1 < ND) values(d + 1, vf[(d + 1) & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                y[d & 1] = f32x16{};
+                if constexpr (H) {
+                    #pragma unroll
+                    for (int u = 0; u < 2 * PIECES; u++) {
+                        const int at = u % PIECES;
+                        const u32x4v w = u < PIECES ? pl[at / 2][at & 1] : ph[at / 2][at & 1];
+                        y[d & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, vf[d & 1][at]), __builtin_bit_cast(h8v, w), y[d & 1], 0, 0, 0);
+                        // (the dims before these join in the products' shadow)
+                        if (d) {
                             #pragma unroll
-                            for (int e = 0; e < 4; e++) y = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], s[t][4 * q + e], y, 0, 0, 0);
+                            for (int r = u * 16 / (2 * PIECES); r < (u + 1) * 16 / (2 * PIECES); r++) join(d - 1, r);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else {
+                    #pragma unroll
+                    for (int u = 0; u < PIECES; u++) {
+                        const f32x4 x = __builtin_bit_cast(f32x4, vf[d & 1][u]);
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) y[d & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], s[u / 4][4 * (u % 4) + e], y[d & 1], 0, 0, 0);
+                        if (d) {
+                            #pragma unroll
+                            for (int r = u * 16 / PIECES; r < (u + 1) * 16 / PIECES; r++) join(d - 1, r);
                         }
                     }
                 }
-                #pragma unroll
-                for (int r = 0; r < 16; r++) o[d][r] = __builtin_fmaf(o[d][r], alpha, y[r]);
             }
+            #pragma unroll
+            for (int r = 0; r < 16; r++) join(ND - 1, r);
         }
         const float sum = swap32_add(l, l);
         if (row0 + i < end) {

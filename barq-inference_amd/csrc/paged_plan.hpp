@@ -22,7 +22,7 @@ struct PagedShape {
     int few_step = 32, many_step = 64;   // positions of a kernel's step
     int few_rows = 32;            // rows of the kernel for few's larger tiles
     int64_t many_from = 65;       // rows from which a sequence's tiles are the large ones
-    int64_t few_target = 1024, many_target = 512;   // workgroups that fill the card
+    int64_t few_target = 512, many_target = 512;    // workgroups that the card holds at once
     int64_t few_least = 4, many_least = 4;          // steps that a split has at least
     size_t part_rows = 0;         // partial states there is room for, for each kv head
 };
@@ -116,6 +116,7 @@ inline void paged_shape_for(PagedShape& sh, bool f16, size_t hd) {
     sh.many_step = f16 ? 64 : 32;
     sh.many_from = 65;
     sh.few_rows = hd == 256 ? 16 : 32;   // (two tiles of 256 dims do not fit the registers)
+    sh.few_target = hd == 256 ? 256 : 512;   // (one workgroup a CU, or two)
     sh.many_target = hd == 256 ? 256 : 512;
 }
 
@@ -161,7 +162,18 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
         const int64_t target = std::max<int64_t>((kind ? sh.many_target : sh.few_target) / sh.n_kv, 1);
         const int64_t least = kind ? sh.many_least : sh.few_least;
         if (!items.empty() && (int64_t)items.size() < target) {
-            const int64_t each = std::max((steps[kind] + target - 1) / target, least);
+            // steps of a split: the fewest (at least `least`) with which the splits all find room at once
+            int64_t each = std::max((steps[kind] + target - 1) / target, least);
+            const auto splits = [&](int64_t e) {
+                int64_t n = 0;
+                for (const PagedItem& it : items) n += (it.v1 + e - 1) / e;
+                return n;
+            };
+            for (int64_t n; (n = splits(each)) > target;) {
+                const int64_t more = each * n / target;   // (about as many splits too many as steps too few)
+                if (n == (int64_t)items.size()) break;
+                each = std::max(each + 1, std::min(more, each + each / 8));
+            }
             std::vector<PagedItem> cut;
             for (const PagedItem& it : items) {
                 int64_t n = std::max<int64_t>((it.v1 + each - 1) / each, 1);
