@@ -39,24 +39,30 @@ struct Step {
 
 template <bool H, int HD>
 struct Query {
-    static constexpr int NC = H ? HD / 32 : HD / 16;
+    static constexpr int NC = H ? HD / 32 : HD / 16, E = H ? 8 : 4;
     u32x4v hi[NC], lo[H ? NC : 1];   // f32: the values in hi
     float back;
-    __device__ __forceinline__ void load(const float* row, float scale, int g) {
-        if constexpr (H) {
-            float x[NC][8], m = 0.0f;
+    // fetched first, split when the keys and values are on their way
+    __device__ __forceinline__ static void fetch(const float* row, int g, float (&x)[NC][E]) {
+        #pragma unroll
+        for (int c = 0; c < NC; c++)
             #pragma unroll
-            for (int c = 0; c < NC; c++)
-                #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    const float4 y = *reinterpret_cast<const float4*>(row + 8 * (4 * c + g) + 4 * u);
-                    const float w[4] = {y.x, y.y, y.z, y.w};
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        x[c][4 * u + e] = w[e] * scale;
-                        m = fmaxf(m, __builtin_fabsf(x[c][4 * u + e]));
-                    }
-                }
+            for (int u = 0; u < E / 4; u++) {
+                const float4 y = *reinterpret_cast<const float4*>(row + E * (4 * c + g) + 4 * u);
+                x[c][4 * u] = y.x, x[c][4 * u + 1] = y.y, x[c][4 * u + 2] = y.z, x[c][4 * u + 3] = y.w;
+            }
+    }
+    __device__ __forceinline__ void split(float (&x)[NC][E], float scale) {
+        float m = 0.0f;
+        #pragma unroll
+        for (int c = 0; c < NC; c++)
+            #pragma unroll
+            for (int e = 0; e < E; e++) {
+                x[c][e] *= scale;
+                m = fmaxf(m, __builtin_fabsf(x[c][e]));
+            }
+        back = 1.0f;
+        if constexpr (H) {
             const float up = paged_row_scale(groups_max(m), back);
             #pragma unroll
             for (int c = 0; c < NC; c++)
@@ -68,14 +74,10 @@ struct Query {
                     lo[c][u] = l;
                 }
         } else {
-            back = 1.0f;
             #pragma unroll
-            for (int c = 0; c < NC; c++) {
-                const float4 y = *reinterpret_cast<const float4*>(row + 4 * (4 * c + g));
-                const float w[4] = {y.x * scale, y.y * scale, y.z * scale, y.w * scale};
+            for (int c = 0; c < NC; c++)
                 #pragma unroll
-                for (int u = 0; u < 4; u++) hi[c][u] = __builtin_bit_cast(uint32_t, w[u]);
-            }
+                for (int u = 0; u < 4; u++) hi[c][u] = __builtin_bit_cast(uint32_t, x[c][u]);
         }
     }
 };
@@ -160,14 +162,6 @@ void paged_few_kernel(PagedAttn a, int first, int count) {
     for (int w = blockIdx.x; w < count * a.n_kv; w += gridDim.x) {
         const int hk = w % a.n_kv;
         const PagedItem it = paged_item(&a.few[first + w / a.n_kv]);
-        Query<H, HD> q[NT];
-        int pos[NT];
-        #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int r = it.row0 + min(16 * n + i, it.rows - 1), tok = r / a.G, head = hk * a.G + r % a.G;
-            pos[n] = it.past + tok;
-            q[n].load(a.q + ((size_t)head * n_tokens + it.q0 + tok) * HD, a.scale, g);
-        }
         const int p_first = it.past + it.row0 / a.G, p_last = it.past + (it.row0 + it.rows - 1) / a.G;
         float m[NT], l[NT];
         f32x4 o[NT][NV];
@@ -221,8 +215,19 @@ void paged_few_kernel(PagedAttn a, int first, int count) {
             }
         };
         if (steps > 0) fetch_ids(0);
+        Query<H, HD> q[NT];
+        float raw[NT][Query<H, HD>::NC][E];
+        int pos[NT];
+        #pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int r = it.row0 + min(16 * n + i, it.rows - 1), tok = r / a.G, head = hk * a.G + r % a.G;
+            pos[n] = it.past + tok;
+            Query<H, HD>::fetch(a.q + ((size_t)head * n_tokens + it.q0 + tok) * HD, g, raw[n]);
+        }
         load(0, true);
         load(0, false);
+        #pragma unroll
+        for (int n = 0; n < NT; n++) q[n].split(raw[n], a.scale);
         for (int j = 0; j < steps; j++) {
             const int base = base_of(j), have = k_pages;
             const bool whole = have == (H ? 3 : 1) && sight.all(base, STEP, p_first, p_last);
