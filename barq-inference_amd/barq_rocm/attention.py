@@ -47,9 +47,10 @@ def apply_rope(be: Backend, x, seq_len, n_heads, head_dim, start_pos, rope_freq_
     return out
 
 
-def transpose_heads(be: Backend, x, seq_len, n_heads, head_dim, mem=L.MEM_DEVICE, sync=True):
+def transpose_heads(be: Backend, x, seq_len, n_heads, head_dim, mem=L.MEM_DEVICE, sync=True, out=None):
     """transpose_heads (transformer.rs:598-611)."""
-    out = _empty((n_heads, seq_len, head_dim), x, mem)
+    if out is None:
+        out = _empty((n_heads, seq_len, head_dim), x, mem)
     L.check(be._lib.barq_rocm_transpose_heads(be.h, _ptr(x), seq_len, n_heads, head_dim, _ptr(out), mem))
     if sync and mem == L.MEM_DEVICE:
         be.sync()

@@ -137,3 +137,69 @@ class PagedBatch:
         if sync and mem == L.MEM_DEVICE:
             self.be.sync()
         return out
+
+
+class Sequence:
+    """A sequence of a paged cache: its length and its page ids (-1: given back)."""
+
+    def __init__(self):
+        self.length, self.pages = 0, []
+
+
+class Pages:
+    """Which pages of a cache are free, and how many sequences have each."""
+
+    def __init__(self, n_pages: int, page_size: int):
+        self.page_size = page_size
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._users = [0] * n_pages
+
+    def free(self) -> int:
+        return len(self._free)
+
+    def grow(self, seq: Sequence, n_tokens: int):
+        """n_tokens more positions.  Fails without changing anything when the pages run out."""
+        need = -(-(seq.length + n_tokens) // self.page_size) - len(seq.pages)
+        if need > len(self._free):
+            raise L.BarqError(L.E_ALLOC, f"pages: {need} more are needed, {len(self._free)} are free")
+        for _ in range(need):
+            p = self._free.pop()
+            self._users[p] = 1
+            seq.pages.append(p)
+        seq.length += n_tokens
+
+    def shrink(self, seq: Sequence, length: int, n_pages: int | None = None):
+        """Back to `length` positions."""
+        n = -(-length // self.page_size) if n_pages is None else n_pages
+        while len(seq.pages) > n:
+            self._release(seq.pages.pop())
+        seq.length = length
+
+    def fork(self, seq: Sequence) -> Sequence:
+        """A sequence over the same whole pages: its length is theirs, and what it adds goes to pages of its own."""
+        new = Sequence()
+        new.length = seq.length // self.page_size * self.page_size
+        new.pages = seq.pages[:seq.length // self.page_size]
+        for p in new.pages:
+            if p >= 0:
+                self._users[p] += 1
+        return new
+
+    def drop_behind(self, seq: Sequence, window: int, n_sink: int = 0):
+        """Give back the pages that no query to come sees."""
+        first = -(-n_sink // self.page_size)
+        for i in range(first, max(seq.length - window + 1, 0) // self.page_size):
+            if seq.pages[i] >= 0:
+                self._release(seq.pages[i])
+                seq.pages[i] = -1
+
+    def close(self, seq: Sequence):
+        """The end of the sequence: its pages are free again."""
+        self.shrink(seq, 0)
+
+    def _release(self, p: int):
+        if p < 0:
+            return
+        self._users[p] -= 1
+        if self._users[p] == 0:
+            self._free.append(p)

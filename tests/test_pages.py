@@ -1,0 +1,146 @@
+"""Handing out the pages of a paged cache (barq_rocm.paged.Pages), and the
+rotary frequencies for long contexts: host code, no GPU."""
+import math
+import random
+
+import numpy as np
+import pytest
+
+from barq_rocm import _lib as L
+from barq_rocm import attention as A
+from barq_rocm.paged import Pages, Sequence
+
+
+def test_growing_and_closing():
+    p, a, b = Pages(5, 16), Sequence(), Sequence()
+    p.grow(a, 16)
+    p.grow(b, 17)
+    p.grow(a, 1)
+    assert (len(a.pages), len(b.pages), p.free()) == (2, 2, 1)
+    with pytest.raises(L.BarqError) as e:
+        p.grow(b, 32)
+    assert e.value.code == L.E_ALLOC and (b.length, len(b.pages), p.free()) == (17, 2, 1)
+    p.grow(b, 15)
+    assert p.free() == 1
+    p.close(a)
+    assert (a.length, a.pages, p.free()) == (0, [], 3)
+    p.grow(b, 33)
+    assert p.free() == 0 and sorted(b.pages) == list(range(5)) and len(set(b.pages)) == 5
+
+
+def test_a_fork_shares_whole_pages():
+    p, a = Pages(6, 16), Sequence()
+    p.grow(a, 40)
+    b = p.fork(a)
+    assert (b.length, b.pages) == (32, a.pages[:2])
+    p.grow(b, 5)
+    assert b.pages[2] not in a.pages and p.free() == 2
+    p.close(a)
+    assert p.free() == 3   # the shared ones stay b's
+    p.close(b)
+    assert p.free() == 6
+
+
+@pytest.mark.parametrize("window,n_sink", [(1, 0), (16, 0), (20, 1), (33, 16), (100, 17)])
+def test_what_is_behind_the_window_is_given_back(window, n_sink):
+    p, s = Pages(20, 16), Sequence()
+    for n in (50, 1, 1, 70, 1, 100):
+        p.grow(s, n)
+        p.drop_behind(s, window, n_sink)
+        # the next query is at s.length: it sees s.length - window + 1 .. on, and the first n_sink
+        for i, page in enumerate(s.pages):
+            seen = (i + 1) * 16 > s.length - window + 1 or i * 16 < n_sink
+            assert (page >= 0) == seen
+        held = [x for x in s.pages if x >= 0]
+        assert len(held) == len(set(held)) and p.free() == 20 - len(held)
+
+
+def test_drawn_sessions_lose_no_page():
+    rng = random.Random(2)
+    p, seqs = Pages(30, 16), []
+    for _ in range(2000):
+        what = rng.random()
+        if what < 0.3 and len(seqs) < 12:
+            seqs.append(p.fork(rng.choice(seqs)) if seqs and rng.random() < 0.5 else Sequence())
+        elif seqs and what < 0.8:
+            try:
+                p.grow(rng.choice(seqs), rng.randint(0, 40))
+            except L.BarqError:
+                pass
+        elif seqs and what < 0.9:
+            p.drop_behind(rng.choice(seqs), rng.randint(1, 30), rng.choice([0, 4, 20]))
+        elif seqs:
+            p.close(seqs.pop(rng.randrange(len(seqs))))
+        held = {x for s in seqs for x in s.pages if x >= 0}
+        assert p.free() == 30 - len(held)
+    for s in seqs:
+        p.close(s)
+    assert p.free() == 30
+
+
+def frequencies(scaling, rot, base, factor=1.0, trained=0.0, fast=32.0, slow=1.0):
+    plain = base ** (-2.0 * np.arange(rot // 2) / rot)
+    if scaling == L.ROPE_LINEAR:
+        return plain / factor, 1.0
+    if scaling == L.ROPE_NTK:
+        return (base * factor ** (rot / (rot - 2))) ** (-2.0 * np.arange(rot // 2) / rot), 1.0
+    if scaling == L.ROPE_YARN:
+        turns = trained * plain / (2 * math.pi)
+        keep = np.clip((turns - slow) / (fast - slow), 0, 1)
+        return plain * keep + plain / factor * (1 - keep), 0.1 * math.log(factor) + 1
+    return plain, 1.0
+
+
+@pytest.mark.parametrize("scaling,args", [(L.ROPE_PLAIN, ()), (L.ROPE_LINEAR, (4.0,)), (L.ROPE_NTK, (8.0,)), (L.ROPE_YARN, (16.0, 4096.0)),
+                                          (L.ROPE_YARN, (1.0, 4096.0)), (L.ROPE_YARN, (40.0, 8192.0, 20.0, 0.0))])
+@pytest.mark.parametrize("rot,base", [(128, 10000.0), (64, 500000.0), (22, 1e6), (4, 100.0)])
+def test_rope_frequencies(scaling, args, rot, base):
+    want, magnitude = frequencies(scaling, rot, base, *args)
+    f, m = A.rope_frequencies(scaling, rot, base, *args)
+    # computed in 64 bits and rounded once: half a step, and one more of 2^-50 for pow
+    assert f.dtype == np.float32 and np.all(np.abs(f - want) <= want * 2.0 ** -24 * (1 + 1e-6))
+    assert abs(m - magnitude) <= magnitude * 2.0 ** -24
+    if scaling == L.ROPE_NTK:   # the fastest pair stays, the slowest is slowed down by the whole factor
+        plain = frequencies(L.ROPE_PLAIN, rot, base)[0]
+        assert f[0] == 1 and f[-1] == pytest.approx(plain[-1] / args[0], rel=1e-6)
+
+
+def test_rope_frequencies_refused():
+    for code, args in ((L.E_DIM, (L.ROPE_PLAIN, 3, 1e4)), (L.E_DIM, (L.ROPE_PLAIN, 0, 1e4)), (L.E_UNSUPPORTED, (4, 64, 1e4)),
+                       (L.E_UNSUPPORTED, (-1, 64, 1e4)), (L.E_INVALID, (L.ROPE_PLAIN, 64, 0.0)), (L.E_INVALID, (L.ROPE_PLAIN, 64, math.nan)),
+                       (L.E_INVALID, (L.ROPE_LINEAR, 64, 1e4, 0.5)), (L.E_INVALID, (L.ROPE_NTK, 64, 1e4, math.inf)), (L.E_DIM, (L.ROPE_NTK, 2, 1e4, 2.0)),
+                       (L.E_INVALID, (L.ROPE_YARN, 64, 1e4, 2.0)), (L.E_INVALID, (L.ROPE_YARN, 64, 1e4, 2.0, 4096.0, 1.0, 1.0))):
+        with pytest.raises(L.BarqError) as e:
+            A.rope_frequencies(*args)
+        assert e.value.code == code, args
+    lib = L.lib()
+    assert lib.barq_rocm_rope_frequencies(0, 64, 1e4, 1.0, 0.0, 32.0, 1.0, None, None) == L.E_INVALID
+
+
+def test_refusals_before_any_device():
+    """What the paged calls refuse without a handle."""
+    import ctypes
+    lib, out = L.lib(), ctypes.c_void_p()
+    create = lib.barq_rocm_paged_cache_create
+    assert create(None, 4, 16, 1, 2, 64, L.F16, None) == L.E_INVALID
+    assert create(None, 4, 16, 1, 2, 64, L.Q4_0, ctypes.byref(out)) == L.E_UNSUPPORTED
+    assert create(None, 4, 16, 1, 2, 80, L.F16, ctypes.byref(out)) == L.E_UNSUPPORTED
+    for pages, size in ((4, 8), (4, 48), (4, 1 << 17), (0, 16), (1 << 31, 16)):
+        assert create(None, pages, size, 1, 2, 64, L.F16, ctypes.byref(out)) == L.E_DIM
+    assert create(None, 4, 16, 1, 2, 64, L.F16, ctypes.byref(out)) == L.E_INVALID   # the null handle
+    assert lib.barq_rocm_paged_batch_create(None, None, 4, 1, 1, 1, 0, 0, ctypes.byref(out)) == L.E_INVALID
+    assert lib.barq_rocm_paged_batch_set(None, None, 0, None, None, None, 0) == L.E_INVALID
+    assert lib.barq_rocm_paged_attention(None, None, 0, None, L.F32, None, L.MEM_DEVICE) == L.E_INVALID
+    assert lib.barq_rocm_paged_attention(None, None, 0, None, L.F32, None, 7) == L.E_INVALID
+    assert lib.barq_rocm_paged_append(None, None, 0, None, None, None, None, None, None, 0.0, None, L.MEM_DEVICE) == L.E_INVALID
+    assert lib.barq_rocm_paged_read(None, None, 0, None, None, L.MEM_DEVICE) == L.E_INVALID
+    assert lib.barq_rocm_paged_cache_destroy(None) == L.OK and lib.barq_rocm_paged_batch_destroy(None) == L.OK
+    norm = lib.barq_rocm_norm_rope
+    assert norm(None, None, 1, 1, 96, 0, None, 0.0, None, None, L.MEM_DEVICE) == L.E_UNSUPPORTED
+    assert norm(None, None, 1, 1, 64, 0, None, 0.0, None, None, L.MEM_DEVICE) == L.E_INVALID
+    for r, code in ((L.RotaryArg(7, 0, 1.0, 1.0, 16), L.E_DIM), (L.RotaryArg(66, 0, 1.0, 1.0, 16), L.E_DIM),
+                    (L.RotaryArg(8, 2, 1.0, 1.0, 16), L.E_INVALID), (L.RotaryArg(8, 0, 1.0, 1.0, None), L.E_INVALID)):
+        assert norm(None, 16, 1, 1, 64, 0, None, 0.0, ctypes.byref(r), 16, L.MEM_DEVICE) == code
+    assert norm(None, 16, 2, 1, 64, 0x7ffffffe, None, 0.0, None, 16, L.MEM_DEVICE) == L.E_DIM
+    assert norm(None, 16, 2, 1 << 40, 64, 0, None, 0.0, None, 16, L.MEM_DEVICE) == L.E_DIM
+    assert norm(None, None, 0, 1, 64, 0, None, 0.0, None, None, L.MEM_DEVICE) == L.OK
