@@ -14,13 +14,20 @@ from .attention import _empty
 from .backend import Backend, _ptr
 
 
+_F32 = set()   # the array libraries' float32
+
+
 def _rows(who, x, heads_dim, n_tokens):
     """n_tokens rows of f32, side by side in memory."""
-    size = x.size if isinstance(x, np.ndarray) else x.numel()
-    flat = x.flags.c_contiguous if isinstance(x, np.ndarray) else x.is_contiguous()
+    host = isinstance(x, np.ndarray)
+    size = x.size if host else x.numel()
     if size != n_tokens * heads_dim:
         raise L.BarqError(L.E_DIM, f"{who}: {size} values, {n_tokens} tokens of {heads_dim} are wanted")
-    if not flat or not str(x.dtype).endswith("float32"):
+    if x.dtype not in _F32:
+        if not str(x.dtype).endswith("float32"):
+            raise L.BarqError(L.E_INVALID, f"{who}: rows must be contiguous float32")
+        _F32.add(x.dtype)
+    if not (x.flags.c_contiguous if host else x.is_contiguous()):
         raise L.BarqError(L.E_INVALID, f"{who}: rows must be contiguous float32")
 
 
@@ -98,11 +105,14 @@ class PagedBatch:
         head (with k_norm) and rotated (with rotary); returns q [n_tokens,
         n_head*head_dim] likewise, as [n_head, n_tokens, head_dim], or None."""
         c, t = self.cache, self.n_tokens
-        for name, x, heads in (("q", q, self.n_head), ("k", k, c.n_head_kv), ("v", v, c.n_head_kv)):
-            if x is not None:
-                _rows(f"paged_append: {name}", x, heads * c.head_dim, t)
-        if q is not None and q_out is None:
-            q_out = _empty((self.n_head, t, c.head_dim), q, mem)
+        if q is not None:
+            _rows("paged_append: q", q, self.n_head * c.head_dim, t)
+            if q_out is None:
+                q_out = _empty((self.n_head, t, c.head_dim), q, mem)
+        if k is not None:
+            _rows("paged_append: k", k, c.n_head_kv * c.head_dim, t)
+        if v is not None:
+            _rows("paged_append: v", v, c.n_head_kv * c.head_dim, t)
         L.check(self.be._lib.barq_rocm_paged_append(self.be.h, self.b, layer, _ptr(q), _ptr(q_out), _ptr(k), _ptr(v), _ptr(q_norm),
                                                     _ptr(k_norm), eps, ctypes.byref(rotary.arg) if rotary is not None else None,
                                                     mem))
@@ -117,8 +127,8 @@ class PagedBatch:
             k, v = np.empty(shape, dtype), np.empty(shape, dtype)
         else:
             import torch
-            dev = torch.device("cuda", self.be.device)
-            k, v = (torch.empty(shape, dtype=getattr(torch, dtype), device=dev) for _ in "kv")
+            dtype, dev = torch.float16 if c.type == L.F16 else torch.float32, f"cuda:{self.be.device}"
+            k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
         L.check(self.be._lib.barq_rocm_paged_read(self.be.h, self.b, layer, _ptr(k), _ptr(v), mem))
         if sync and mem == L.MEM_DEVICE:
             self.be.sync()

@@ -88,21 +88,28 @@ __device__ __forceinline__ void scores(const Step<H, HD>& st, const Query<H, HD>
     constexpr int KT = Step<H, HD>::KT, NC = Step<H, HD>::NC;
     #pragma unroll
     for (int t = 0; t < KT; t++) {
-        f32x4 hi = {}, lo = {};
-        #pragma unroll
-        for (int c = 0; c < NC; c++) {
-            if constexpr (H) {
+        if constexpr (H) {
+            f32x4 hi = {}, lo = {};
+            #pragma unroll
+            for (int c = 0; c < NC; c++) {
                 const h8v k = __builtin_bit_cast(h8v, st.k[t][c]);
                 lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(h8v, q.lo[c]), lo, 0, 0, 0);
                 hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, __builtin_bit_cast(h8v, q.hi[c]), hi, 0, 0, 0);
-            } else {
+            }
+            #pragma unroll
+            for (int r = 0; r < 4; r++) s[4 * t + r] = __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) * q.back;
+        } else {
+            // four sums side by side: none waits for another, and each is cut a quarter as often
+            f32x4 part[4] = {};
+            #pragma unroll
+            for (int c = 0; c < NC; c++) {
                 const f32x4 k = __builtin_bit_cast(f32x4, st.k[t][c]), x = __builtin_bit_cast(f32x4, q.hi[c]);
                 #pragma unroll
-                for (int e = 0; e < 4; e++) hi = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], x[e], hi, 0, 0, 0);
+                for (int e = 0; e < 4; e++) part[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], x[e], part[e], 0, 0, 0);
             }
+            #pragma unroll
+            for (int r = 0; r < 4; r++) s[4 * t + r] = (part[0][r] + part[1][r]) + (part[2][r] + part[3][r]);
         }
-        #pragma unroll
-        for (int r = 0; r < 4; r++) s[4 * t + r] = H ? __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) * q.back : hi[r];
     }
 }
 

@@ -239,13 +239,16 @@ void paged_many_kernel(PagedAttn a, int count) {
                     } else {
                         const f32x4 x = __builtin_bit_cast(f32x4, kf[n & 1][u]), y = __builtin_bit_cast(f32x4, qh[c]);
                         #pragma unroll
-                        for (int e = 0; e < 4; e++) hi = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], hi, 0, 0, 0);
+                        for (int e = 0; e < 4; e += 2) {
+                            hi = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], hi, 0, 0, 0);
+                            lo = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e + 1], y[e + 1], lo, 0, 0, 0);
+                        }
                     }
                 }
                 __builtin_amdgcn_sched_barrier(BARQ_ONLY_ALU_CROSSES);
                 if (n % GC == GC - 1) {
                     #pragma unroll
-                    for (int r = 0; r < 16; r++) s[n / GC][r] = H ? __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) : hi[r];
+                    for (int r = 0; r < 16; r++) s[n / GC][r] = H ? __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) : hi[r] + lo[r];
                 }
             }
             if (!whole) {
