@@ -142,6 +142,14 @@ void paged_many_kernel(PagedAttn a, int count) {
                 }
             }
         }
+        if constexpr (H && HD == 256) {
+            // (256 registers of a wave take only products' operands and results: the queries)
+            #pragma unroll
+            for (int c = 0; c < NC; c++) {
+                asm("" : "+a"(qh[c]));
+                asm("" : "+a"(ql[c]));
+            }
+        }
         float m = -INFINITY, l = 0.0f;
         f32x16 o[ND];
         #pragma unroll
@@ -209,18 +217,16 @@ void paged_many_kernel(PagedAttn a, int count) {
                     __syncthreads();
                 }
             }
-            // no row of the wave, or nothing that one sees (first tokens end where the window's steps begin)
-            if (row0 >= end || base > p_last || (a.window && base >= a.n_sink && base + STEP - 1 <= p_first - a.window)) continue;
             const bool whole = have == (1 << NB) - 1 && sight.all(base, STEP, p_first, p_last);
-            // scores: the next four pieces of K are fetched while the products of these run
-            constexpr int GC = NC / 4;
+            // scores: the next pieces of K are fetched while the products of these run
+            constexpr int KG = HD == 256 ? 2 : 4, GC = NC / KG;   // (four at a time do not fit the registers of 256 dims)
             float s[T][16];
-            u32x4v kf[2][4];
-            const auto keys = [&](int n, u32x4v (&k)[4]) __attribute__((always_inline)) {
+            u32x4v kf[2][KG];
+            const auto keys = [&](int n, u32x4v (&k)[KG]) __attribute__((always_inline)) {
                 const int t = n / GC, slot = H ? 8 * ((i >> 2) & 1) + 4 * ((i >> 3) & 1) + (i & 3) : i & 15;
                 const uint8_t* kb = kt + (2 * t + (i >> 4)) * BLOCK + slot * 16 + h * 256;
                 #pragma unroll
-                for (int u = 0; u < 4; u++) k[u] = *reinterpret_cast<const u32x4v*>(kb + (n % GC * 4 + u) * 512);
+                for (int u = 0; u < KG; u++) k[u] = *reinterpret_cast<const u32x4v*>(kb + (n % GC * KG + u) * 512);
             };
             keys(0, kf[0]);
             f32x16 hi, lo;
@@ -230,8 +236,8 @@ void paged_many_kernel(PagedAttn a, int count) {
                 __builtin_amdgcn_sched_barrier(BARQ_ONLY_ALU_CROSSES);
                 if (n % GC == 0) hi = lo = f32x16{};
                 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const int c = n % GC * 4 + u;
+                for (int u = 0; u < KG; u++) {
+                    const int c = n % GC * KG + u;
                     if constexpr (H) {
                         const h8v k = __builtin_bit_cast(h8v, kf[n & 1][u]);
                         lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(h8v, ql[c]), lo, 0, 0, 0);
@@ -301,13 +307,12 @@ void paged_many_kernel(PagedAttn a, int count) {
             for (int d = 0; d < ND; d++) {
                 if (d + 1 < ND) values(d + 1, vf[(d + 1) & 1]);
                 __builtin_amdgcn_sched_barrier(0);
-                y[d & 1] = f32x16{};
                 if constexpr (H) {
                     #pragma unroll
                     for (int u = 0; u < 2 * PIECES; u++) {
                         const int at = u % PIECES;
                         const u32x4v w = u < PIECES ? pl[at / 2][at & 1] : ph[at / 2][at & 1];
-                        y[d & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, vf[d & 1][at]), __builtin_bit_cast(h8v, w), y[d & 1], 0, 0, 0);
+                        y[d & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, vf[d & 1][at]), __builtin_bit_cast(h8v, w), u ? y[d & 1] : f32x16{}, 0, 0, 0);
                         // (the dims before these join in the products' shadow)
                         if (d) {
                             #pragma unroll
@@ -320,7 +325,7 @@ void paged_many_kernel(PagedAttn a, int count) {
                     for (int u = 0; u < PIECES; u++) {
                         const f32x4 x = __builtin_bit_cast(f32x4, vf[d & 1][u]);
                         #pragma unroll
-                        for (int e = 0; e < 4; e++) y[d & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], s[u / 4][4 * (u % 4) + e], y[d & 1], 0, 0, 0);
+                        for (int e = 0; e < 4; e++) y[d & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], s[u / 4][4 * (u % 4) + e], u || e ? y[d & 1] : f32x16{}, 0, 0, 0);
                         if (d) {
                             #pragma unroll
                             for (int r = u * 16 / PIECES; r < (u + 1) * 16 / PIECES; r++) join(d - 1, r);
