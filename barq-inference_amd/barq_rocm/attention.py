@@ -36,6 +36,24 @@ def _check_mass(who, n_head_kv, *arrays):
             raise L.BarqError(L.E_INVALID, f"{who}: mass must be contiguous float32")
 
 
+_F32 = set()   # the array libraries' float32
+
+
+def _check_f32(who, what, t, n):
+    """n float32 values, side by side in memory (a raw address or nothing is taken as it is)."""
+    if t is None or isinstance(t, int):
+        return
+    host = isinstance(t, np.ndarray)
+    if (t.size if host else t.numel()) != n:
+        raise L.BarqError(L.E_DIM, f"{who}: {what} has {t.size if host else t.numel()} values, {n} are wanted")
+    if t.dtype not in _F32:
+        if not str(t.dtype).endswith("float32"):
+            raise L.BarqError(L.E_INVALID, f"{who}: {what} must be contiguous float32")
+        _F32.add(t.dtype)
+    if not (t.flags.c_contiguous if host else t.is_contiguous()):
+        raise L.BarqError(L.E_INVALID, f"{who}: {what} must be contiguous float32")
+
+
 def apply_rope(be: Backend, x, seq_len, n_heads, head_dim, start_pos, rope_freq_scale, rope_inv_freq, layout,
                mem=L.MEM_DEVICE, sync=True):
     """apply_rope (transformer.rs:514-562): x [seq, n_heads*head_dim] -> [n_heads, seq, head_dim]."""
@@ -92,6 +110,8 @@ def norm_rope(be: Backend, x, seq_len, n_heads, head_dim, start_pos, rotary=None
     [seq, n_heads*head_dim] -> [n_heads, seq, head_dim]."""
     if out is None:
         out = _empty((n_heads, seq_len, head_dim), x, mem)
+    for what, t, n in (("x", x, seq_len * n_heads * head_dim), ("norm", norm, head_dim), ("out", out, seq_len * n_heads * head_dim)):
+        _check_f32("norm_rope", what, t, n)
     L.check(be._lib.barq_rocm_norm_rope(be.h, _ptr(x), seq_len, n_heads, head_dim, start_pos, _ptr(norm), eps,
                                         ctypes.byref(rotary.arg) if rotary is not None else None, _ptr(out), mem))
     if sync and mem == L.MEM_DEVICE:

@@ -10,25 +10,8 @@ import ctypes
 import numpy as np
 
 from . import _lib as L
-from .attention import _empty
+from .attention import _check_f32, _empty
 from .backend import Backend, _ptr
-
-
-_F32 = set()   # the array libraries' float32
-
-
-def _rows(who, x, heads_dim, n_tokens):
-    """n_tokens rows of f32, side by side in memory."""
-    host = isinstance(x, np.ndarray)
-    size = x.size if host else x.numel()
-    if size != n_tokens * heads_dim:
-        raise L.BarqError(L.E_DIM, f"{who}: {size} values, {n_tokens} tokens of {heads_dim} are wanted")
-    if x.dtype not in _F32:
-        if not str(x.dtype).endswith("float32"):
-            raise L.BarqError(L.E_INVALID, f"{who}: rows must be contiguous float32")
-        _F32.add(x.dtype)
-    if not (x.flags.c_contiguous if host else x.is_contiguous()):
-        raise L.BarqError(L.E_INVALID, f"{who}: rows must be contiguous float32")
 
 
 class PagedCache:
@@ -105,14 +88,18 @@ class PagedBatch:
         head (with k_norm) and rotated (with rotary); returns q [n_tokens,
         n_head*head_dim] likewise, as [n_head, n_tokens, head_dim], or None."""
         c, t = self.cache, self.n_tokens
+        hd = c.head_dim
+        nq, nk, who = t * self.n_head * hd, t * c.n_head_kv * hd, "paged_append"
         if q is not None:
-            _rows("paged_append: q", q, self.n_head * c.head_dim, t)
+            _check_f32(who, "q", q, nq)
             if q_out is None:
-                q_out = _empty((self.n_head, t, c.head_dim), q, mem)
-        if k is not None:
-            _rows("paged_append: k", k, c.n_head_kv * c.head_dim, t)
-        if v is not None:
-            _rows("paged_append: v", v, c.n_head_kv * c.head_dim, t)
+                q_out = _empty((self.n_head, t, hd), q, mem)
+            else:
+                _check_f32(who, "q_out", q_out, nq)
+            _check_f32(who, "q_norm", q_norm, hd)
+        _check_f32(who, "k", k, nk)
+        _check_f32(who, "v", v, nk)
+        _check_f32(who, "k_norm", k_norm, hd)
         L.check(self.be._lib.barq_rocm_paged_append(self.be.h, self.b, layer, _ptr(q), _ptr(q_out), _ptr(k), _ptr(v), _ptr(q_norm),
                                                     _ptr(k_norm), eps, ctypes.byref(rotary.arg) if rotary is not None else None,
                                                     mem))
@@ -139,7 +126,12 @@ class PagedBatch:
         out_type Q8_K the rows' blocks, uint8 [n_tokens, n_head*head_dim/256 * 292]."""
         c, t = self.cache, self.n_tokens
         width = self.n_head * c.head_dim
-        _rows("paged_attention: q", q, width, t)
+        _check_f32("paged_attention", "q", q, t * width)
+        if out is not None and not isinstance(out, int):
+            if out_type == L.F32:
+                _check_f32("paged_attention", "out", out, t * width)
+            elif (out.nbytes if isinstance(out, np.ndarray) else out.numel() * out.element_size()) != t * (width // 256 * 292):
+                raise L.BarqError(L.E_DIM, f"paged_attention: out must have {t} rows of {width // 256 * 292} bytes")
         if out is None:
             out = (_empty((t, self.n_head, c.head_dim), q, mem) if out_type == L.F32
                    else _empty((t, width // 256 * 292), q, mem, dtype="uint8"))

@@ -272,13 +272,13 @@ void paged_few_kernel(PagedAttn a, int first, int count) {
                 #pragma unroll
                 for (int e = 1; e < NP; e++) top = fmaxf(top, s[n][e]);
                 top = fmaxf(m[n], groups_max(top));
-                const float ref = top == -INFINITY ? 0.0f : top, shift = H ? ref - 15.0f : ref;
+                const float ref = top == -INFINITY ? 0.0f : top;
                 alpha[n] = paged_exp2(m[n] - ref);
                 m[n] = top;
                 float sum = 0.0f;
                 #pragma unroll
                 for (int e = 0; e < NP; e++) {
-                    s[n][e] = paged_exp2(s[n][e] - shift);
+                    s[n][e] = paged_exp2(H ? (s[n][e] - ref) + 15.0f : s[n][e] - ref);   // (in this order: at most 15 whatever the scores)
                     sum += s[n][e];
                 }
                 l[n] = __builtin_fmaf(l[n], alpha[n], sum);

@@ -1,5 +1,6 @@
 // What the kernels of attention over a paged cache share (attention_paged.hip:
-// few rows of a sequence, attention_paged_many.hip: many).
+// few rows of a sequence; many: attention_paged_many.hip over f16 rows,
+// attention_paged_f32.hip over f32 ones).
 //
 // Row r of a sequence and kv head (new token r / G at position p, query head r % G):
 //   s_j = (q . K[j]) / sqrt(HD)   for j <= p and, with a window, j > p - window or j < first tokens, j's page there
@@ -14,12 +15,13 @@
 // f16 values whose products have sums of their own: an element is off by 2^-23
 // of itself down to 2^-29 of the row's largest, by 2^-52 of the largest below that.
 // A weight exp2(s - max + 15), at most 2^15, is split into two f16 values likewise
-// but joined in one sum: it is off by 2^-23 of itself down to 2^-17 of the row's
+// but joined in one sum: it is off by 2^-22 of itself down to 2^-17 of the row's
 // largest weight, by 2^-40 of the largest below that.  That is half of the matrix rate for results
 // that one f16 value a weight would have at 2^-12.  The MFMA's f32 sums are not rounded to
 // nearest, so each step's start from zero and join O in one fma.
-// Over an f32 cache all products are the f32 MFMA's, an eighth of the rate
-// of split f16 with three products but with nothing to bound.
+// Over an f32 cache few rows take the f32 MFMA (they are bound by the reading all the
+// same), many rows six products of bf16 parts: within 2^-23 of |x y| whatever the values (those beyond
+// 3.38e38 read as NaN, for bf16 rounds them to infinity).
 //
 // V in unseen places: a weight of zero keeps finite values out, not NaN.  Steps
 // that some row does not see all of replace what is not finite by zero, and put

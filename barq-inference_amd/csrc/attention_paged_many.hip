@@ -1,10 +1,10 @@
-// Attention over a paged KV cache for sequences with many rows (new tokens x the
-// query heads of a kv head): prompts and their chunks.  attention_paged.hpp has the
-// formulas and numerics.
+// Attention over a paged KV cache of f16 rows for sequences with many rows (new tokens
+// x the query heads of a kv head): prompts and their chunks.  attention_paged.hpp has
+// the formulas and numerics, attention_paged_f32.hip the kernel for f32 rows.
 //
 // Bound by the matrix products: two of f16 for each of an f32 result's.  A workgroup
-// is four waves of 32 rows each, the queries in registers; a step's K and V (64 positions in
-// f16, 32 in f32) come by direct loads into one of two LDS buffers while the other is
+// is four waves of 32 rows each, the queries in registers; a step's K and V (64
+// positions) come by direct loads into one of two LDS buffers while the other is
 // computed on.  The pages' blocks are the MFMA operands' layout already, so they
 // are copied as they lie and read without bank conflicts: wave w fetches block w.
 #include "attention_paged.hpp"
@@ -25,10 +25,9 @@ __device__ __forceinline__ float halves_max(float v) {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// Register r of a lane of half h is position base + at(r, h) of a tile of 32: in f16 16 (r / 8) + 8 h + r % 8 (row i of
-// the MFMA stands for position 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4), in f32 the MFMA's own row 8 (r / 4) + 4 h + r % 4.
-template <bool H>
-__device__ __forceinline__ int tile_pos(int r, int h) { return H ? 16 * (r / 8) + 8 * h + r % 8 : 8 * (r / 4) + 4 * h + r % 4; }
+// Register r of a lane of half h is this position of a tile of 32: row i of the MFMA stands for position 16 (i / 16) +
+// 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4, so that a half's eight positions of a block are one piece of V.
+__device__ __forceinline__ int tile_pos(int r, int h) { return 16 * (r / 8) + 8 * h + r % 8; }
 
 // Two weights as f16 hi (cut, one instruction for both) + lo (of what that leaves, to the nearest).
 __device__ __forceinline__ void split_weights(float x0, float x1, float minus_one, uint32_t& hi, uint32_t& lo) {
@@ -40,18 +39,17 @@ __device__ __forceinline__ void split_weights(float x0, float x1, float minus_on
     lo = __builtin_bit_cast(uint32_t, r);
 }
 
-template <bool H>
 __device__ __forceinline__ u32x4v finite(u32x4v v) {
     #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] &= ~(H ? f16_bad(v[e]) : f32_bad(v[e]));
+    for (int e = 0; e < 4; e++) v[e] &= ~f16_bad(v[e]);
     return v;
 }
 
-template <bool H, int HD>
+template <int HD>
 __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2)
 void paged_many_kernel(PagedAttn a, int count) {
-    constexpr int STEP = H ? 64 : 32, T = STEP / 32, NB = STEP / PAGE_BLOCK, NC = H ? HD / 16 : HD / 8, ND = HD / 32;
-    constexpr int BLOCK = PAGE_BLOCK * HD * (H ? 2 : 4);   // bytes
+    constexpr int STEP = 64, T = STEP / 32, NB = STEP / PAGE_BLOCK, NC = HD / 16, ND = HD / 32;
+    constexpr int BLOCK = PAGE_BLOCK * HD * 2;   // bytes
     extern __shared__ __align__(16) uint8_t lds[];         // [2][K, V][NB][BLOCK]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
     int n_tokens = a.n_tokens;
@@ -82,21 +80,19 @@ void paged_many_kernel(PagedAttn a, int count) {
                 for (int b = 0; b < NB; b++) {
                     const int p = at + 16 * b < it.kv_len ? table[(at + 16 * b) >> a.log_page] : -1;
                     has |= p >= 0 ? 1 << b : 0;
-                    if (b == (wave & (NB - 1))) id = p;
+                    if (b == wave) id = p;
                 }
             }
         };
         const auto fetch = [&](int j, int has_all) {
-            // f16: K and V of block `wave`; f32, of two blocks a step: K by waves 0 and 1, V by the others
-            const int blk = wave & (NB - 1), p = __builtin_amdgcn_readlane(id, j & 63), at = base_of(j) + 16 * blk;
+            const int p = __builtin_amdgcn_readlane(id, j & 63), at = base_of(j) + 16 * wave;
             const size_t off = ((size_t)max(p, 0) * a.n_kv + hk) * page_bytes + (size_t)((at & ((1 << a.log_page) - 1)) >> 4) * BLOCK;
             #pragma unroll
             for (int kv = 0; kv < 2; kv++) {
-                if (!H && kv != wave / 2) continue;
-                i32x4v r = make_rsrc4((kv ? a.v : a.k) + off, (has_all >> blk) & 1 ? BLOCK : 0);   // (no page: zeros)
+                i32x4v r = make_rsrc4((kv ? a.v : a.k) + off, (has_all >> wave) & 1 ? BLOCK : 0);   // (no page: zeros)
                 #pragma unroll
                 for (int e = 0; e < 4; e++) r[e] = __builtin_amdgcn_readfirstlane(r[e]);
-                const uint32_t to = lds0 + (((j & 1) * 2 + kv) * NB + blk) * BLOCK;
+                const uint32_t to = lds0 + (((j & 1) * 2 + kv) * NB + wave) * BLOCK;
                 #pragma unroll
                 for (int u = 0; u < BLOCK / 1024; u++) lds_load16_at(r, to + 1024 * u, lane * 16, 1024 * u);
             }
@@ -108,41 +104,31 @@ void paged_many_kernel(PagedAttn a, int count) {
         const int row0 = it.row0 + 32 * wave, end = it.row0 + it.rows, mine = min(row0 + i, end - 1), tok = mine / a.G;
         const int pos = it.past + tok, p_first = it.past + min(row0, end - 1) / a.G, p_last = it.past + min(row0 + 31, end - 1) / a.G;
         const int all_first = it.past + it.row0 / a.G, all_last = it.past + (end - 1) / a.G;
-        u32x4v qh[NC], ql[H ? NC : 1];
+        u32x4v qh[NC], ql[NC];
         float back = 1.0f;
         {
             const float* row = a.q + ((size_t)(hk * a.G + mine % a.G) * n_tokens + it.q0 + tok) * HD;
-            if constexpr (H) {
-                float m = 0.0f;
-                #pragma unroll
-                for (int c = 0; c < 2 * NC; c++) {
-                    const float4 y = *reinterpret_cast<const float4*>(row + 16 * (c / 2) + 8 * h + 4 * (c & 1));
-                    m = fmaxf(fmaxf(fmaxf(m, __builtin_fabsf(y.x * a.scale)), fmaxf(__builtin_fabsf(y.y * a.scale), __builtin_fabsf(y.z * a.scale))),
-                              __builtin_fabsf(y.w * a.scale));
-                }
-                const float up = paged_row_scale(halves_max(m), back);
-                #pragma unroll
-                for (int c = 0; c < NC; c++)
-                    #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const float4 y = *reinterpret_cast<const float4*>(row + 16 * c + 8 * h + 4 * u);
-                        uint32_t x0, y0, x1, y1;
-                        paged_split(y.x * a.scale * up, y.y * a.scale * up, x0, y0);
-                        paged_split(y.z * a.scale * up, y.w * a.scale * up, x1, y1);
-                        qh[c][2 * u] = x0, qh[c][2 * u + 1] = x1;
-                        ql[c][2 * u] = y0, ql[c][2 * u + 1] = y1;
-                    }
-            } else {
-                #pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    const float4 y = *reinterpret_cast<const float4*>(row + 8 * c + 4 * h);
-                    const float x[4] = {y.x * a.scale, y.y * a.scale, y.z * a.scale, y.w * a.scale};
-                    #pragma unroll
-                    for (int u = 0; u < 4; u++) qh[c][u] = __builtin_bit_cast(uint32_t, x[u]);
-                }
+            float m = 0.0f;
+            #pragma unroll
+            for (int c = 0; c < 2 * NC; c++) {
+                const float4 y = *reinterpret_cast<const float4*>(row + 16 * (c / 2) + 8 * h + 4 * (c & 1));
+                m = fmaxf(fmaxf(fmaxf(m, __builtin_fabsf(y.x * a.scale)), fmaxf(__builtin_fabsf(y.y * a.scale), __builtin_fabsf(y.z * a.scale))),
+                          __builtin_fabsf(y.w * a.scale));
             }
+            const float up = paged_row_scale(halves_max(m), back);
+            #pragma unroll
+            for (int c = 0; c < NC; c++)
+                #pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const float4 y = *reinterpret_cast<const float4*>(row + 16 * c + 8 * h + 4 * u);
+                    uint32_t x0, y0, x1, y1;
+                    paged_split(y.x * a.scale * up, y.y * a.scale * up, x0, y0);
+                    paged_split(y.z * a.scale * up, y.w * a.scale * up, x1, y1);
+                    qh[c][2 * u] = x0, qh[c][2 * u + 1] = x1;
+                    ql[c][2 * u] = y0, ql[c][2 * u + 1] = y1;
+                }
         }
-        if constexpr (H && HD == 256) {
+        if constexpr (HD == 256) {
             // (256 registers of a wave take only products' operands and results: the queries)
             #pragma unroll
             for (int c = 0; c < NC; c++) {
@@ -173,37 +159,27 @@ void paged_many_kernel(PagedAttn a, int count) {
                 for (int u = lane; u < NB * BLOCK / 16; u += 64) {
                     const u32x4v x = reinterpret_cast<const u32x4v*>(vt)[u];
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) any |= H ? f16_bad(x[e]) : f32_bad(x[e]);
+                    for (int e = 0; e < 4; e++) any |= f16_bad(x[e]);
                 }
                 if (__any(any != 0)) {
                     uint32_t seen = 0;   // bit 16 t + r
                     #pragma unroll
-                    for (int b = 0; b < 16 * T; b++) seen |= sees(32 * (b / 16) + tile_pos<H>(b % 16, h)) ? 1u << b : 0u;
+                    for (int b = 0; b < 16 * T; b++) seen |= sees(32 * (b / 16) + tile_pos(b % 16, h)) ? 1u << b : 0u;
                     #pragma unroll
                     for (int d = 0; d < ND; d++) {
                         f32x16 n = {};   // such places that a row sees
                         #pragma unroll
                         for (int t = 0; t < T; t++) {
-                            if constexpr (H) {
+                            #pragma unroll
+                            for (int u = 0; u < 2; u++) {
+                                u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16), one;
                                 #pragma unroll
-                                for (int u = 0; u < 2; u++) {
-                                    u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16), one;
-                                    #pragma unroll
-                                    for (int e = 0; e < 4; e++) {
-                                        const uint32_t two = seen >> (16 * t + 8 * u + 2 * e);
-                                        v[e] = f16_bad(v[e]) & 0x3C003C00u;
-                                        one[e] = (two & 1 ? 0x3C00u : 0u) | (two & 2 ? 0x3C000000u : 0u);
-                                    }
-                                    n = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, v), __builtin_bit_cast(h8v, one), n, 0, 0, 0);
+                                for (int e = 0; e < 4; e++) {
+                                    const uint32_t two = seen >> (16 * t + 8 * u + 2 * e);
+                                    v[e] = f16_bad(v[e]) & 0x3C003C00u;
+                                    one[e] = (two & 1 ? 0x3C00u : 0u) | (two & 2 ? 0x3C000000u : 0u);
                                 }
-                            } else {
-                                #pragma unroll
-                                for (int q = 0; q < 4; q++) {
-                                    const u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + q / 2) * BLOCK + ((2 * (q & 1) + h) * HD + 32 * d + i) * 16);
-                                    #pragma unroll
-                                    for (int e = 0; e < 4; e++)
-                                        n = __builtin_amdgcn_mfma_f32_32x32x2f32(f32_bad(v[e]) ? 1.0f : 0.0f, (seen >> (16 * t + 4 * q + e)) & 1 ? 1.0f : 0.0f, n, 0, 0, 0);
-                                }
+                                n = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, v), __builtin_bit_cast(h8v, one), n, 0, 0, 0);
                             }
                         }
                         #pragma unroll
@@ -212,7 +188,7 @@ void paged_many_kernel(PagedAttn a, int count) {
                     __syncthreads();
                     for (int u = threadIdx.x; u < NB * BLOCK / 16; u += 64 * NW) {
                         u32x4v* x = reinterpret_cast<u32x4v*>(vt) + u;
-                        *x = finite<H>(*x);
+                        *x = finite(*x);
                     }
                     __syncthreads();
                 }
@@ -223,7 +199,7 @@ void paged_many_kernel(PagedAttn a, int count) {
             float s[T][16];
             u32x4v kf[2][KG];
             const auto keys = [&](int n, u32x4v (&k)[KG]) __attribute__((always_inline)) {
-                const int t = n / GC, slot = H ? 8 * ((i >> 2) & 1) + 4 * ((i >> 3) & 1) + (i & 3) : i & 15;
+                const int t = n / GC, slot = 8 * ((i >> 2) & 1) + 4 * ((i >> 3) & 1) + (i & 3);
                 const uint8_t* kb = kt + (2 * t + (i >> 4)) * BLOCK + slot * 16 + h * 256;
                 #pragma unroll
                 for (int u = 0; u < KG; u++) k[u] = *reinterpret_cast<const u32x4v*>(kb + (n % GC * KG + u) * 512);
@@ -238,30 +214,21 @@ void paged_many_kernel(PagedAttn a, int count) {
                 #pragma unroll
                 for (int u = 0; u < KG; u++) {
                     const int c = n % GC * KG + u;
-                    if constexpr (H) {
-                        const h8v k = __builtin_bit_cast(h8v, kf[n & 1][u]);
-                        lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(h8v, ql[c]), lo, 0, 0, 0);
-                        hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(h8v, qh[c]), hi, 0, 0, 0);
-                    } else {
-                        const f32x4 x = __builtin_bit_cast(f32x4, kf[n & 1][u]), y = __builtin_bit_cast(f32x4, qh[c]);
-                        #pragma unroll
-                        for (int e = 0; e < 4; e += 2) {
-                            hi = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], hi, 0, 0, 0);
-                            lo = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e + 1], y[e + 1], lo, 0, 0, 0);
-                        }
-                    }
+                    const h8v k = __builtin_bit_cast(h8v, kf[n & 1][u]);
+                    lo = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(h8v, ql[c]), lo, 0, 0, 0);
+                    hi = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(h8v, qh[c]), hi, 0, 0, 0);
                 }
                 __builtin_amdgcn_sched_barrier(BARQ_ONLY_ALU_CROSSES);
                 if (n % GC == GC - 1) {
                     #pragma unroll
-                    for (int r = 0; r < 16; r++) s[n / GC][r] = H ? __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]) : hi[r] + lo[r];
+                    for (int r = 0; r < 16; r++) s[n / GC][r] = __builtin_fmaf(lo[r], 1.0f / 2048, hi[r]);
                 }
             }
             if (!whole) {
                 #pragma unroll
                 for (int t = 0; t < T; t++)
                     #pragma unroll
-                    for (int r = 0; r < 16; r++) s[t][r] = sees(32 * t + tile_pos<H>(r, h)) ? s[t][r] : -INFINITY;
+                    for (int r = 0; r < 16; r++) s[t][r] = sees(32 * t + tile_pos(r, h)) ? s[t][r] : -INFINITY;
             }
             float top = s[0][0];
             #pragma unroll
@@ -269,36 +236,42 @@ void paged_many_kernel(PagedAttn a, int count) {
                 #pragma unroll
                 for (int r = 0; r < 16; r++) top = fmaxf(top, s[t][r]);
             top = fmaxf(m, halves_max(top) * back);
-            const float ref = top == -INFINITY ? 0.0f : top, shift = H ? 15.0f - ref : -ref;
-            const float alpha = paged_exp2(m - ref);
+            const float ref = top == -INFINITY ? 0.0f : top, alpha = paged_exp2(m - ref);
             m = top;
+            // exponents s * back - ref + 15 in one fma, unless 15 - ref would round by more than 2^-4
+            float mul = back, shift = 15.0f - ref;
+            if (__any(__builtin_fabsf(ref) > 1048576.0f)) {
+                #pragma unroll
+                for (int t = 0; t < T; t++)
+                    #pragma unroll
+                    for (int r = 0; r < 16; r++) s[t][r] = s[t][r] * back - ref;
+                mul = 1.0f, shift = 15.0f;
+            }
             float sum = 0.0f;
-            u32x4v ph[T][2], pl[T][2];   // f16
+            u32x4v ph[T][2], pl[T][2];
             #pragma unroll
             for (int t = 0; t < T; t++) {
                 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    s[t][r] = paged_exp2(__builtin_fmaf(s[t][r], back, shift));
+                    s[t][r] = paged_exp2(__builtin_fmaf(s[t][r], mul, shift));
                     sum += s[t][r];
                 }
-                if constexpr (H) {
-                    #pragma unroll
-                    for (int r = 0; r < 16; r += 2) {
-                        uint32_t x, y;
-                        split_weights(s[t][r], s[t][r + 1], minus_one, x, y);
-                        ph[t][r / 8][r % 8 / 2] = x;
-                        pl[t][r / 8][r % 8 / 2] = y;
-                    }
+                #pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    uint32_t x, y;
+                    split_weights(s[t][r], s[t][r + 1], minus_one, x, y);
+                    ph[t][r / 8][r % 8 / 2] = x;
+                    pl[t][r / 8][r % 8 / 2] = y;
                 }
             }
             l = __builtin_fmaf(l, alpha, sum);
             // O: the next 32 dims' pieces of V likewise; the weights' small parts first, so that fewer sums are cut at y's size
-            constexpr int PIECES = H ? 2 * T : 4 * T;
+            constexpr int PIECES = 2 * T;
             u32x4v vf[2][PIECES];
             const auto values = [&](int d, u32x4v (&v)[PIECES]) __attribute__((always_inline)) {
                 #pragma unroll
                 for (int u = 0; u < PIECES; u++)
-                    v[u] = *reinterpret_cast<const u32x4v*>(vt + (H ? u : u / 2) * BLOCK + ((H ? h : 2 * (u & 1) + h) * HD + 32 * d + i) * 16);
+                    v[u] = *reinterpret_cast<const u32x4v*>(vt + u * BLOCK + (h * HD + 32 * d + i) * 16);
             };
             values(0, vf[0]);
             f32x16 y[2];
@@ -307,30 +280,17 @@ void paged_many_kernel(PagedAttn a, int count) {
             for (int d = 0; d < ND; d++) {
                 if (d + 1 < ND) values(d + 1, vf[(d + 1) & 1]);
                 __builtin_amdgcn_sched_barrier(0);
-                if constexpr (H) {
-                    #pragma unroll
-                    for (int u = 0; u < 2 * PIECES; u++) {
-                        const int at = u % PIECES;
-                        const u32x4v w = u < PIECES ? pl[at / 2][at & 1] : ph[at / 2][at & 1];
-                        y[d & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, vf[d & 1][at]), __builtin_bit_cast(h8v, w), u ? y[d & 1] : f32x16{}, 0, 0, 0);
-                        // (the dims before these join in the products' shadow)
-                        if (d) {
-                            #pragma unroll
-                            for (int r = u * 16 / (2 * PIECES); r < (u + 1) * 16 / (2 * PIECES); r++) join(d - 1, r);
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                } else {
-                    #pragma unroll
-                    for (int u = 0; u < PIECES; u++) {
-                        const f32x4 x = __builtin_bit_cast(f32x4, vf[d & 1][u]);
+                #pragma unroll
+                for (int u = 0; u < 2 * PIECES; u++) {
+                    const int at = u % PIECES;
+                    const u32x4v w = u < PIECES ? pl[at / 2][at & 1] : ph[at / 2][at & 1];
+                    y[d & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, vf[d & 1][at]), __builtin_bit_cast(h8v, w), u ? y[d & 1] : f32x16{}, 0, 0, 0);
+                    // (the dims before these join in the products' shadow)
+                    if (d) {
                         #pragma unroll
-                        for (int e = 0; e < 4; e++) y[d & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], s[u / 4][4 * (u % 4) + e], u || e ? y[d & 1] : f32x16{}, 0, 0, 0);
-                        if (d) {
-                            #pragma unroll
-                            for (int r = u * 16 / PIECES; r < (u + 1) * 16 / PIECES; r++) join(d - 1, r);
-                        }
+                        for (int r = u * 16 / (2 * PIECES); r < (u + 1) * 16 / (2 * PIECES); r++) join(d - 1, r);
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             #pragma unroll
@@ -359,23 +319,23 @@ void paged_many_kernel(PagedAttn a, int count) {
     }
 }
 
-template <bool H, int HD>
+template <int HD>
 hipError_t launch(const PagedAttn& a, hipStream_t s) {
-    constexpr unsigned bytes = 2 * 2 * (H ? 64 : 32) * HD * (H ? 2 : 4);
+    constexpr unsigned bytes = 2 * 2 * 64 * HD * 2;
     if (bytes > 65536) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_many_kernel<H, HD>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&paged_many_kernel<HD>), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (e != hipSuccess) return e;
     }
     const dim3 g(a.n_tokens < 0 ? 1024u : (unsigned)a.n_many * (unsigned)a.n_kv);
-    hipLaunchKernelGGL((paged_many_kernel<H, HD>), g, dim3(64 * NW), bytes, s, a, a.n_many);
+    hipLaunchKernelGGL(paged_many_kernel<HD>, g, dim3(64 * NW), bytes, s, a, a.n_many);
     return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t paged_many_launch(const PagedAttn& a, bool f16, int hd, hipStream_t s) {
-    if (f16) return hd == 64 ? launch<true, 64>(a, s) : hd == 128 ? launch<true, 128>(a, s) : launch<true, 256>(a, s);
-    return hd == 64 ? launch<false, 64>(a, s) : hd == 128 ? launch<false, 128>(a, s) : launch<false, 256>(a, s);
+    if (!f16) return paged_many_f32_launch(a, hd, s);
+    return hd == 64 ? launch<64>(a, s) : hd == 128 ? launch<128>(a, s) : launch<256>(a, s);
 }
 
 }  // namespace barq

@@ -343,5 +343,6 @@ struct PagedAttn {
 };
 hipError_t paged_attention_launch(const PagedAttn& a, bool f16, int hd, hipStream_t s);
 hipError_t paged_many_launch(const PagedAttn& a, bool f16, int hd, hipStream_t s);   // its items of many rows (attention_paged_many.hip)
+hipError_t paged_many_f32_launch(const PagedAttn& a, int hd, hipStream_t s);        // of f32 rows (attention_paged_f32.hip)
 
 }  // namespace barq

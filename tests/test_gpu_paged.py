@@ -297,6 +297,25 @@ def test_sizes_of_the_values(be, type_, rows, q_size, k_size, v_size):
 
 
 @pytest.mark.parametrize("type_", [B.F16, B.F32])
+@pytest.mark.parametrize("rows", [1, 24, 150])
+@pytest.mark.parametrize("log_size", [10, 19, 21, 23, 25, 30, 60])
+def test_scores_of_every_size(be, type_, rows, log_size):
+    """Scores of about 2^log_size, the largest one three times: those positions share all of the weight."""
+    n, hd, rng = 200 + rows, 64, np.random.default_rng(log_size)
+    k, v = np.zeros((n, 1, hd), F32), rng.standard_normal((n, 1, hd)).astype(F32)
+    k[:, 0, 0] = rng.choice([0.5, 0.25, -1.0, 0.0], n)
+    top = [3, 77, 190]
+    k[top, 0, 0] = 1
+    c = Case(be, type_, 2, 1, hd, 16, [(rows, n)], k=k, v=v)
+    c.q[:] = 0
+    c.q[..., 0] = F32(1.37 * 2.0 ** log_size)
+    want = np.broadcast_to(c.vc[top].mean(0), (rows, 2, hd))   # (the others' weight: e^(-2^log_size / 16) at most)
+    got = c.batch.attention(c.layer, dev(c.q)).cpu().numpy()
+    # three equal weights, each f16 part of them exact or off by 2^-23; sums and division 2^-21
+    assert_within(got, want, 2.0 ** -20 * np.abs(c.vc[top]).mean(0) + np.zeros_like(want) + 2.0 ** -36 + (np.exp(-2.0 ** log_size / 16) * 4))
+
+
+@pytest.mark.parametrize("type_", [B.F16, B.F32])
 def test_rows_in_q8_k_blocks(be, type_):
     import torch
     for seqs in ([(1, 300)], [(70, 200), (1, 40), (3, 3)]):
@@ -548,7 +567,13 @@ def test_refusals(be):
     refused(L.E_INVALID, b.append, 0, k.half(), k)
     refused(L.E_INVALID, b.attention, 2, q)
     refused(L.E_DIM, b.attention, 0, q[:2])
-    refused(L.E_UNSUPPORTED, b.attention, 0, q, out_type=B.Q8_0, out=q)
+    refused(L.E_UNSUPPORTED, b.attention, 0, q, out_type=B.Q8_0, out=torch.empty(2 * 292, dtype=torch.uint8, device="cuda"))
+    refused(L.E_DIM, b.attention, 0, q, out=q[:2])
+    refused(L.E_DIM, b.attention, 0, q, out_type=B.Q8_K, out=q)
+    refused(L.E_DIM, b.append, 0, k, k, q=q, q_out=q[:3])
+    refused(L.E_DIM, b.append, 0, k, k, k_norm=k[0, 0, :63])
+    refused(L.E_DIM, A.norm_rope, be, k, 3, 2, 64, 0)
+    refused(L.E_DIM, A.norm_rope, be, k, 2, 2, 64, 0, norm=k[0, 0, :32])
     refused(L.E_DIM, P.PagedBatch(P.PagedCache(be, 1, 16, 1, 1, 64), 2, 1, 1, 1).attention, 0, q[:2, :0], out_type=B.Q8_K)
     for rot, code in ((3, L.E_DIM), (66, L.E_DIM)):
         r = A.Rotary(dev(freqs(rot)), rot)
@@ -556,7 +581,7 @@ def test_refusals(be):
         refused(code, A.norm_rope, be, k, 2, 2, 64, 0, r)
     refused(L.E_INVALID, b.append, 0, k, k, rotary=A.Rotary(dev(freqs(64)), 64, layout=2))
     refused(L.E_DIM, A.Rotary, dev(freqs(64)), 32)
-    refused(L.E_UNSUPPORTED, A.norm_rope, be, k, 2, 2, 32, 0)
+    refused(L.E_UNSUPPORTED, A.norm_rope, be, k[..., :32].contiguous(), 2, 2, 32, 0)
     refused(L.E_DIM, A.norm_rope, be, k, 2, 2, 64, 0x7fffffff)
     x = torch.zeros(300, device="cuda")[1:257]
     refused(L.E_INVALID, A.norm_rope, be, x, 2, 2, 64, 0)
