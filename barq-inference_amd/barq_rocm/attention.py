@@ -19,9 +19,14 @@ ROPE_INTERLEAVED = L.ROPE_INTERLEAVED
 ROPE_SPLIT_HALF = L.ROPE_SPLIT_HALF
 
 
+_F32 = set()   # the array libraries' float32, as _check_f32 meets them
+
+
 def _empty(shape, like, mem, dtype="float32"):
     if mem == L.MEM_HOST:
         return np.empty(shape, dtype=np.dtype(dtype))
+    if dtype == "float32" and like.dtype in _F32:
+        return like.new_empty(shape)   # (half a microsecond less than by its names)
     import torch
     return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
 
@@ -34,9 +39,6 @@ def _check_mass(who, n_head_kv, *arrays):
         flat = m.flags.c_contiguous if isinstance(m, np.ndarray) else m.is_contiguous()
         if not flat or not str(m.dtype).endswith("float32"):
             raise L.BarqError(L.E_INVALID, f"{who}: mass must be contiguous float32")
-
-
-_F32 = set()   # the array libraries' float32
 
 
 def _check_f32(who, what, t, n):
@@ -85,6 +87,7 @@ class Rotary:
             raise L.BarqError(L.E_DIM, f"Rotary: inv_freq must be {rot_dim // 2} float32 values")
         self.inv_freq = inv_freq   # (kept alive: the argument below has its address)
         self.arg = L.RotaryArg(rot_dim, layout, freq_scale, magnitude, _ptr(inv_freq) or None)
+        self.ref = ctypes.byref(self.arg)
 
     @classmethod
     def scaled(cls, rot_dim, base, layout=ROPE_INTERLEAVED, scaling=L.ROPE_PLAIN, factor=1.0, trained=0.0, fast=32.0, slow=1.0,
@@ -108,12 +111,16 @@ def norm_rope(be: Backend, x, seq_len, n_heads, head_dim, start_pos, rotary=None
               sync=True, out=None):
     """RMSNorm of each head (with norm) and the rotation, in one pass: x
     [seq, n_heads*head_dim] -> [n_heads, seq, head_dim]."""
+    n = seq_len * n_heads * head_dim
+    _check_f32("norm_rope", "x", x, n)
+    if norm is not None:
+        _check_f32("norm_rope", "norm", norm, head_dim)
     if out is None:
         out = _empty((n_heads, seq_len, head_dim), x, mem)
-    for what, t, n in (("x", x, seq_len * n_heads * head_dim), ("norm", norm, head_dim), ("out", out, seq_len * n_heads * head_dim)):
-        _check_f32("norm_rope", what, t, n)
+    else:
+        _check_f32("norm_rope", "out", out, n)
     L.check(be._lib.barq_rocm_norm_rope(be.h, _ptr(x), seq_len, n_heads, head_dim, start_pos, _ptr(norm), eps,
-                                        ctypes.byref(rotary.arg) if rotary is not None else None, _ptr(out), mem))
+                                        None if rotary is None else rotary.ref, _ptr(out), mem))
     if sync and mem == L.MEM_DEVICE:
         be.sync()
     return out

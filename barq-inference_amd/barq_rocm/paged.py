@@ -96,12 +96,14 @@ class PagedBatch:
                 q_out = _empty((self.n_head, t, hd), q, mem)
             else:
                 _check_f32(who, "q_out", q_out, nq)
-            _check_f32(who, "q_norm", q_norm, hd)
+            if q_norm is not None:
+                _check_f32(who, "q_norm", q_norm, hd)
         _check_f32(who, "k", k, nk)
         _check_f32(who, "v", v, nk)
-        _check_f32(who, "k_norm", k_norm, hd)
+        if k_norm is not None:
+            _check_f32(who, "k_norm", k_norm, hd)
         L.check(self.be._lib.barq_rocm_paged_append(self.be.h, self.b, layer, _ptr(q), _ptr(q_out), _ptr(k), _ptr(v), _ptr(q_norm),
-                                                    _ptr(k_norm), eps, ctypes.byref(rotary.arg) if rotary is not None else None,
+                                                    _ptr(k_norm), eps, None if rotary is None else rotary.ref,
                                                     mem))
         return q_out
 
