@@ -147,38 +147,31 @@ struct Weights {
     }
 };
 
-// NT tiles of 16 rows.
-template <bool H, int HD, int NT>
-__global__ __launch_bounds__(64 * NW, HD == 256 || NT == 2 ? 1 : 2)
-void paged_few_kernel(PagedAttn a, int first, int count) {
+template <bool H, int HD>
+__global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2)
+void paged_few_kernel(PagedAttn a, int count) {
     constexpr int STEP = H ? 32 : 16, E = H ? 8 : 4, KT = H ? 2 : 1, NV = HD / 16, NP = 4 * KT;
     constexpr int ROW = HD + 4;   // floats of a row in LDS: 16-byte pieces, the four groups in other banks
     constexpr size_t BLOCK = (size_t)PAGE_BLOCK * HD * (H ? 2 : 4);
     __shared__ __align__(16) float o_s[NW][16][ROW];
-    __shared__ float m_s[NW][16 * NT], l_s[NW][16 * NT];
+    __shared__ float m_s[NW][16], l_s[NW][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
     int n_tokens = a.n_tokens;
     if (n_tokens < 0) {
         n_tokens = a.counts->n_tokens;
-        first = NT == 1 ? 0 : a.counts->few16;
-        count = (NT == 1 ? a.counts->few16 : a.counts->few) - first;
+        count = a.counts->few;
     }
     const float minus_one = f16_minus_one();
     const PagedSight sight = {a.window, a.n_sink};
     const size_t page_bytes = BLOCK << (a.log_page - 4);   // of one kv head
     for (int w = blockIdx.x; w < count * a.n_kv; w += gridDim.x) {
         const int hk = w % a.n_kv;
-        const PagedItem it = paged_item(&a.few[first + w / a.n_kv]);
+        const PagedItem it = paged_item(&a.few[w / a.n_kv]);
         const int p_first = it.past + it.row0 / a.G, p_last = it.past + (it.row0 + it.rows - 1) / a.G;
-        float m[NT], l[NT];
-        f32x4 o[NT][NV];
+        float m = -INFINITY, l = 0.0f;
+        f32x4 o[NV];
         #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            m[n] = -INFINITY;
-            l[n] = 0.0f;
-            #pragma unroll
-            for (int d = 0; d < NV; d++) o[n][d] = f32x4{};
-        }
+        for (int d = 0; d < NV; d++) o[d] = f32x4{};
         const int32_t* table = a.table + it.table;
         const int steps = (it.v1 - it.v0 - wave + NW - 1) / NW;   // this wave's (none: 0 or less)
         const auto base_of = [&](int j) {
@@ -222,153 +215,122 @@ void paged_few_kernel(PagedAttn a, int first, int count) {
             }
         };
         if (steps > 0) fetch_ids(0);
-        Query<H, HD> q[NT];
-        float raw[NT][Query<H, HD>::NC][E];
-        int pos[NT];
-        #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int r = it.row0 + min(16 * n + i, it.rows - 1), tok = r / a.G, head = hk * a.G + r % a.G;
-            pos[n] = it.past + tok;
-            Query<H, HD>::fetch(a.q + ((size_t)head * n_tokens + it.q0 + tok) * HD, g, raw[n]);
-        }
+        Query<H, HD> q;
+        float raw[Query<H, HD>::NC][E];
+        const int mine = it.row0 + min(i, it.rows - 1), tok = mine / a.G, pos = it.past + tok;
+        Query<H, HD>::fetch(a.q + ((size_t)(hk * a.G + mine % a.G) * n_tokens + it.q0 + tok) * HD, g, raw);
         load(0, true);
         load(0, false);
-        #pragma unroll
-        for (int n = 0; n < NT; n++) q[n].split(raw[n], a.scale);
+        q.split(raw, a.scale);
         for (int j = 0; j < steps; j++) {
             const int base = base_of(j), have = k_pages;
             const bool whole = have == (H ? 3 : 1) && sight.all(base, STEP, p_first, p_last);
-            float s[NT][NP];
-            #pragma unroll
-            for (int n = 0; n < NT; n++) scores<H, HD>(st, q[n], s[n]);
-            if (((j + 1) & 63) == 0) fetch_ids(j + 1);
-            load(j + 1, true);
-            uint32_t seen[NT];   // bit e: the lane's row sees the lane's position e
-            bool bad = false;
+            uint32_t seen = 0;   // bit e: the lane's row sees the lane's position e
             if (!whole) {
                 const bool here = H && g >= 2 ? have & 2 : have & 1;   // (a group's positions lie in one block)
                 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    seen[n] = 0;
-                    #pragma unroll
-                    for (int e = 0; e < NP; e++) {
-                        const bool see = here && sight.sees(pos[n], base + E * g + e);
-                        seen[n] |= see ? 1u << e : 0u;
-                        s[n][e] = see ? s[n][e] : -INFINITY;
-                    }
-                }
+                for (int e = 0; e < NP; e++) seen |= (here & sight.sees(pos, base + E * g + e)) ? 1u << e : 0u;
                 uint32_t any = 0;
                 #pragma unroll
                 for (int d = 0; d < NV; d++)
                     #pragma unroll
                     for (int u = 0; u < 4; u++) any |= H ? f16_bad(st.v[d][u]) : f32_bad(st.v[d][u]);
-                bad = __any(any != 0);
-            }
-            float alpha[NT];
-            Weights<H> p[NT];
-            #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float top = s[n][0];
-                #pragma unroll
-                for (int e = 1; e < NP; e++) top = fmaxf(top, s[n][e]);
-                top = fmaxf(m[n], groups_max(top));
-                const float ref = top == -INFINITY ? 0.0f : top;
-                alpha[n] = paged_exp2(m[n] - ref);
-                m[n] = top;
-                float sum = 0.0f;
-                #pragma unroll
-                for (int e = 0; e < NP; e++) {
-                    s[n][e] = paged_exp2(H ? (s[n][e] - ref) + 15.0f : s[n][e] - ref);   // (in this order: at most 15 whatever the scores)
-                    sum += s[n][e];
-                }
-                l[n] = __builtin_fmaf(l[n], alpha[n], sum);
-                p[n].set(s[n], minus_one);
-            }
-            if (!bad) {
-                #pragma unroll
-                for (int d = 0; d < NV; d++)
-                    #pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        const f32x4 y = p[n].times(st.v[d]);
-                        #pragma unroll
-                        for (int r = 0; r < 4; r++) o[n][d][r] = __builtin_fmaf(o[n][d][r], alpha[n], y[r]);
-                    }
-            } else {
-                #pragma unroll
-                for (int n = 0; n < NT; n++) {
+                if (__any(any != 0)) {   // NaN where a row sees what is not finite, and zero in its place
                     Weights<H> ones;
                     float z[NP];
                     #pragma unroll
-                    for (int e = 0; e < NP; e++) z[e] = (seen[n] >> e) & 1 ? 1.0f : 0.0f;
+                    for (int e = 0; e < NP; e++) z[e] = (seen >> e) & 1 ? 1.0f : 0.0f;
                     ones.set(z, minus_one);
                     #pragma unroll
                     for (int d = 0; d < NV; d++) {
-                        u32x4v v = st.v[d], is;
+                        u32x4v is;
                         #pragma unroll
                         for (int u = 0; u < 4; u++) {
-                            const uint32_t b = H ? f16_bad(v[u]) : f32_bad(v[u]);
-                            v[u] &= ~b;
+                            const uint32_t b = H ? f16_bad(st.v[d][u]) : f32_bad(st.v[d][u]);
                             is[u] = b & (H ? 0x3C003C00u : 0x3F800000u);
+                            st.v[d][u] &= ~b;
                         }
-                        const f32x4 y = p[n].times(v), nan = ones.times(is);
+                        const f32x4 nan = ones.times(is);
                         #pragma unroll
-                        for (int r = 0; r < 4; r++) o[n][d][r] = nan[r] > 0.0f ? NAN : __builtin_fmaf(o[n][d][r], alpha[n], y[r]);
+                        for (int r = 0; r < 4; r++) o[d][r] = nan[r] > 0.0f ? NAN : o[d][r];
                     }
                 }
+            }
+            float s[NP];
+            scores<H, HD>(st, q, s);
+            if (((j + 1) & 63) == 0) fetch_ids(j + 1);
+            load(j + 1, true);
+            if (!whole) {
+                #pragma unroll
+                for (int e = 0; e < NP; e++) s[e] = (seen >> e) & 1 ? s[e] : -INFINITY;
+            }
+            float top = s[0];
+            #pragma unroll
+            for (int e = 1; e < NP; e++) top = fmaxf(top, s[e]);
+            top = fmaxf(m, groups_max(top));
+            const float ref = top == -INFINITY ? 0.0f : top, alpha = paged_exp2(m - ref);
+            m = top;
+            float sum = 0.0f;
+            #pragma unroll
+            for (int e = 0; e < NP; e++) {
+                s[e] = paged_exp2(H ? (s[e] - ref) + 15.0f : s[e] - ref);   // (in this order: at most 15 whatever the scores)
+                sum += s[e];
+            }
+            l = __builtin_fmaf(l, alpha, sum);
+            Weights<H> p;
+            p.set(s, minus_one);
+            #pragma unroll
+            for (int d = 0; d < NV; d++) {
+                const f32x4 y = p.times(st.v[d]);
+                #pragma unroll
+                for (int r = 0; r < 4; r++) o[d][r] = __builtin_fmaf(o[d][r], alpha, y[r]);
             }
             load(j + 1, false);
         }
         // the four waves' states, joined
-        #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            l[n] = groups_sum(l[n]);
-            if (g == 0) {
-                m_s[wave][16 * n + i] = m[n];
-                l_s[wave][16 * n + i] = l[n];
-            }
+        l = groups_sum(l);
+        if (g == 0) {
+            m_s[wave][i] = m;
+            l_s[wave][i] = l;
         }
         __syncthreads();
-        #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            const int at = 16 * n + i;
-            float top = m_s[0][at];
+        {
+            float top = m_s[0][i];
             #pragma unroll
-            for (int u = 1; u < NW; u++) top = fmaxf(top, m_s[u][at]);
-            const float mine = m[n] == -INFINITY ? 1.0f : paged_exp2(m[n] - top);   // (1: o is zero, or NaN and stays it)
+            for (int u = 1; u < NW; u++) top = fmaxf(top, m_s[u][i]);
+            const float f = m == -INFINITY ? 1.0f : paged_exp2(m - top);   // (1: o is zero, or NaN and stays it)
             #pragma unroll
             for (int d = 0; d < NV; d++) {
                 f32x4 y;
                 #pragma unroll
-                for (int r = 0; r < 4; r++) y[r] = o[n][d][r] * mine;
+                for (int r = 0; r < 4; r++) y[r] = o[d][r] * f;
                 *reinterpret_cast<f32x4*>(&o_s[wave][i][16 * d + 4 * g]) = y;
             }
-            __syncthreads();
-            for (int u = threadIdx.x; u < 16 * (HD / 4); u += 64 * NW) {
-                const int row = u / (HD / 4), d = 4 * (u % (HD / 4)), r = 16 * n + row;
-                if (r < it.rows) {
-                    float t = m_s[0][r];
-                    #pragma unroll
-                    for (int x = 1; x < NW; x++) t = fmaxf(t, m_s[x][r]);
-                    float sum = 0.0f;
-                    #pragma unroll
-                    for (int x = 0; x < NW; x++) sum = __builtin_fmaf(l_s[x][r], m_s[x][r] == -INFINITY ? 1.0f : paged_exp2(m_s[x][r] - t), sum);
-                    f32x4 y = *reinterpret_cast<const f32x4*>(&o_s[0][row][d]);
-                    #pragma unroll
-                    for (int x = 1; x < NW; x++) y += *reinterpret_cast<const f32x4*>(&o_s[x][row][d]);
-                    if (it.part < 0) {
-                        const int rr = it.row0 + r, tok = it.q0 + rr / a.G, head = hk * a.G + rr % a.G;
-                        float* out = a.out + ((size_t)tok * a.n_head + head) * HD + d;
-                        #pragma unroll
-                        for (int e = 0; e < 4; e++) out[e] = sum == 0.0f ? 0.0f : y[e] / sum;
-                    } else {
-                        const size_t row_at = (size_t)hk * a.part_rows + it.part + r;
-                        *reinterpret_cast<f32x4*>(a.part + row_at * HD + d) = y;
-                        if (d == 0) a.stat[row_at] = make_float2(t, sum);
-                    }
-                }
-            }
-            __syncthreads();
         }
+        __syncthreads();
+        for (int u = threadIdx.x; u < it.rows * (HD / 4); u += 64 * NW) {
+            const int r = u / (HD / 4), d = 4 * (u % (HD / 4));
+            float top = m_s[0][r];
+            #pragma unroll
+            for (int x = 1; x < NW; x++) top = fmaxf(top, m_s[x][r]);
+            float sum = 0.0f;
+            #pragma unroll
+            for (int x = 0; x < NW; x++) sum = __builtin_fmaf(l_s[x][r], m_s[x][r] == -INFINITY ? 1.0f : paged_exp2(m_s[x][r] - top), sum);
+            f32x4 y = *reinterpret_cast<const f32x4*>(&o_s[0][r][d]);
+            #pragma unroll
+            for (int x = 1; x < NW; x++) y += *reinterpret_cast<const f32x4*>(&o_s[x][r][d]);
+            if (it.part < 0) {
+                const int rr = it.row0 + r;
+                float* out = a.out + ((size_t)(it.q0 + rr / a.G) * a.n_head + hk * a.G + rr % a.G) * HD + d;
+                #pragma unroll
+                for (int e = 0; e < 4; e++) out[e] = sum == 0.0f ? 0.0f : y[e] / sum;
+            } else {
+                const size_t at = (size_t)hk * a.part_rows + it.part + r;
+                *reinterpret_cast<f32x4*>(a.part + at * HD + d) = y;
+                if (d == 0) a.stat[at] = make_float2(top, sum);
+            }
+        }
+        __syncthreads();   // (a next item's states go where this one's are read from)
     }
 }
 
@@ -467,16 +429,13 @@ hipError_t paged_attention_launch(const PagedAttn& a, bool f16, int hd, hipStrea
     // A captured call replays with other counts: its grids are fixed, their workgroups go round the items.
     const bool captured = a.n_tokens < 0;
     const auto grid = [&](int n) { return dim3(captured ? 1024u : (unsigned)n * (unsigned)a.n_kv); };
-    const int few32 = a.n_few - a.n_few16;
-    #define BARQ_FEW(H, D)                                                                                                      \
-        if (f16 == H && hd == D) {                                                                                              \
-            if (captured || a.n_few16) hipLaunchKernelGGL((paged_few_kernel<H, D, 1>), grid(a.n_few16), dim3(256), 0, s, a, 0, a.n_few16); \
-            if constexpr (D != 256)                                                                                            \
-                if (captured || few32) hipLaunchKernelGGL((paged_few_kernel<H, D, 2>), grid(few32), dim3(256), 0, s, a, a.n_few16, few32);    \
-        }
-    BARQ_FEW(true, 64) BARQ_FEW(true, 128) BARQ_FEW(true, 256)
-    BARQ_FEW(false, 64) BARQ_FEW(false, 128) BARQ_FEW(false, 256)
-    #undef BARQ_FEW
+    if (captured || a.n_few) {
+        #define BARQ_FEW(H, D) \
+            if (f16 == H && hd == D) hipLaunchKernelGGL((paged_few_kernel<H, D>), grid(a.n_few), dim3(64 * NW), 0, s, a, a.n_few);
+        BARQ_FEW(true, 64) BARQ_FEW(true, 128) BARQ_FEW(true, 256)
+        BARQ_FEW(false, 64) BARQ_FEW(false, 128) BARQ_FEW(false, 256)
+        #undef BARQ_FEW
+    }
     if (captured || a.n_many) {
         const hipError_t e = paged_many_launch(a, f16, hd, s);
         if (e != hipSuccess) return e;

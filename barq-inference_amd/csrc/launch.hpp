@@ -332,7 +332,7 @@ struct PagedAttn {
     const PagedMerge* merges;
     const PagedCounts* counts;
     int n_tokens;          // -1: counts has them (a captured call)
-    int n_few16, n_few, n_many, n_merges;
+    int n_few, n_many, n_merges;
     int merge_span;        // workgroups of a merge
     int n_head, n_kv, G, log_page;
     int window, n_sink;

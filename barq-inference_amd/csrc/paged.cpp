@@ -384,7 +384,6 @@ int barq_rocm_paged_batch_set(barq_rocm_handle* h, barq_rocm_paged_batch* b, siz
     for (size_t s = 0; s < n_seqs; s++)
         if (q_len[s]) counts.groups += (kv_len[s] - 1) / barq::PAGE_BLOCK - (kv_len[s] - q_len[s]) / barq::PAGE_BLOCK + 1;
     counts.few = (int32_t)plan.few.size();
-    counts.few16 = plan.few16;
     counts.many = (int32_t)plan.many.size();
     counts.merges = (int32_t)plan.merges.size();
     const auto piece = [&](size_t to, size_t bytes) {
@@ -583,7 +582,6 @@ int barq_rocm_paged_attention(barq_rocm_handle* h, barq_rocm_paged_batch* b, siz
     x.merges = reinterpret_cast<const barq::PagedMerge*>(b->mem + b->merges_at);
     x.counts = b->dev_counts();
     x.n_tokens = captured ? -1 : (int)t;
-    x.n_few16 = b->plan.few16;
     x.n_few = (int)b->plan.few.size();
     x.n_many = (int)b->plan.many.size();
     x.n_merges = (int)b->plan.merges.size();

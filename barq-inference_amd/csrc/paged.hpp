@@ -37,8 +37,7 @@ struct PagedItem {
                      // tokens that stay visible, then the window
     int32_t v0, v1;  // this item's steps
     int32_t part;    // its first row among the partial states, -1: it writes the output itself
-    int32_t tile;    // rows of its tile's kernel: 16, 32, 128
-    int32_t pad[4];
+    int32_t pad[5];
 };
 static_assert(sizeof(PagedItem) == 64, "items are fetched as 64 bytes");
 
@@ -51,9 +50,8 @@ static_assert(sizeof(PagedMerge) == 32, "");
 // What a replayed graph reads anew (a call outside a capture passes it along).
 struct PagedCounts {
     int32_t n_tokens, few, many, merges;
-    int32_t few16;   // items of `few` in tiles of 16 rows: the first ones
     int32_t groups;
-    int32_t pad[10];
+    int32_t pad[11];
 };
 static_assert(sizeof(PagedCounts) == 64, "");
 

@@ -1,11 +1,17 @@
 // How a step's attention over a paged cache is cut into workgroups (host).
 //
 // A sequence's rows (new tokens x query heads of a kv head) are cut into tiles of
-// 16, 32 (the kernel for few rows) or 128 (for many); a tile's rows see the key
+// 16 (the kernel for few rows) or 128 (for many); a tile's rows see the key
 // positions [0, first tokens) and [window's start, last row's position], counted
 // in the kernel's steps.  Where there are fewer tiles than the card has room for,
-// the tiles' steps are split, evenly over all of them, so that the longest
-// workgroup is about the mean one; what the splits leave is merged.
+// the tiles' steps are split, evenly over all of them, as far as all workgroups
+// find room at once; what the splits leave is merged.
+//
+// Which kernel: a tile of 16 rows reads the keys for itself alone, one of 128 is
+// slow to begin and to end.  One sequence of 32 query heads on 8, 128 dims, 4000 positions
+// before, f16, few / many us: 100 rows 18.1 / 24.7, 128 17.7 / 25.2, 192 22.0 / 29.3, 256 23.7 / 30.0; eight such
+// sequences: 100 rows 59.4 / 72.1, 200 106 / 82.5; f32: 128 rows 35.9 / 35.4, 256 58.5 / 48.7.  Where the kernel for many
+// runs anyway it takes middling sequences along: eight of 112 to 200 rows 82.5 us, the smaller ones in a launch of their own 107.
 #pragma once
 #include <algorithm>
 #include <cstdint>
@@ -16,12 +22,15 @@
 
 namespace barq {
 
+constexpr int64_t PAGED_FEW_ROWS = 16, PAGED_MANY_ROWS = 128;   // of a tile
+
 struct PagedShape {
     int G = 1, n_kv = 1;          // query heads of a kv head, kv heads
     int64_t window = 0, n_sink = 0;
     int few_step = 32, many_step = 64;   // positions of a kernel's step
-    int few_rows = 32;            // rows of the kernel for few's larger tiles
-    int64_t many_from = 65;       // rows from which a sequence's tiles are the large ones
+    // rows from which a sequence's tiles are the large ones: many_from, or alone_from if the smaller tiles of all sequences
+    // below that take at most alone_tiles workgroups; beside_from where another sequence has that many
+    int64_t many_from = 129, alone_from = 257, alone_tiles = 256, beside_from = 65;
     int64_t few_target = 512, many_target = 512;    // workgroups that the card holds at once
     int64_t few_least = 4, many_least = 4;          // steps that a split has at least
     size_t part_rows = 0;         // partial states there is room for, for each kv head
@@ -34,7 +43,6 @@ struct PagedSeq {
 struct PagedPlan {
     std::vector<PagedItem> few, many;
     std::vector<PagedMerge> merges;
-    int few16 = 0;
 };
 
 struct PagedLimits {
@@ -110,13 +118,13 @@ inline PagedGroup* paged_groups(int32_t t0, int32_t q_len, int32_t kv_len, const
 // The most items and merges that a plan of these limits has.
 inline size_t paged_max_tiles(size_t max_seqs, size_t max_tokens, size_t G) { return (max_tokens * G + 15) / 16 + max_seqs; }
 
-// The kernels' steps for a type and head_dim, and from how many rows the one for many is taken.
+// The kernels' steps and numbers of workgroups for a type and head_dim.
 inline void paged_shape_for(PagedShape& sh, bool f16, size_t hd) {
     sh.few_step = f16 ? 32 : 16;
     sh.many_step = f16 ? 64 : 32;
-    sh.many_from = 65;
-    sh.few_rows = hd == 256 ? 16 : 32;   // (two tiles of 256 dims do not fit the registers)
-    sh.few_target = hd == 256 ? 256 : 512;   // (one workgroup a CU, or two)
+    if (!f16) sh.alone_from = sh.many_from;
+    // by the kernels' registers: one, two, three workgroups a CU
+    sh.few_target = hd == 256 ? 256 : hd == 128 ? 512 : 768;
     sh.many_target = hd == 256 ? 256 : 512;
 }
 
@@ -130,12 +138,17 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
     p.few.clear();
     p.many.clear();
     p.merges.clear();
-    int64_t steps[2] = {0, 0}, q0 = 0;
+    int64_t steps[2] = {0, 0}, q0 = 0, small = 0, longest = 0;
+    for (const PagedSeq& s : seqs) {
+        longest = std::max(longest, s.q_len * sh.G);
+        if (s.q_len * sh.G < sh.alone_from) small += (s.q_len * sh.G + PAGED_FEW_ROWS - 1) / PAGED_FEW_ROWS;
+    }
+    int64_t many_from = small * sh.n_kv <= sh.alone_tiles ? sh.alone_from : sh.many_from;
+    if (longest >= many_from) many_from = sh.beside_from;
     for (const PagedSeq& s : seqs) {
         const int64_t rows = s.q_len * sh.G, past = s.kv_len - s.q_len;
-        const bool many = rows >= sh.many_from;
-        // (all tiles of a sequence by one kernel, the last and smaller one too)
-        const int64_t tile = many ? 128 : std::min<int64_t>(rows <= 16 ? 16 : 32, sh.few_rows), unit = many ? sh.many_step : sh.few_step;
+        const bool many = rows >= many_from;
+        const int64_t tile = many ? PAGED_MANY_ROWS : PAGED_FEW_ROWS, unit = many ? sh.many_step : sh.few_step;
         for (int64_t r = 0; r < rows; r += tile) {
             PagedItem it{};
             it.q0 = (int32_t)q0;
@@ -150,7 +163,6 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
             it.b = (int32_t)low;
             it.v1 = (int32_t)(it.a + (end + unit - 1) / unit - low);
             it.part = -1;
-            it.tile = (int32_t)tile;
             steps[many] += it.v1;
             (many ? p.many : p.few).push_back(it);
         }
@@ -196,11 +208,9 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
         }
         // the longest first: the last workgroups to start are short ones
         std::stable_sort(items.begin(), items.end(), [](const PagedItem& x, const PagedItem& y) {
-            if (x.tile != y.tile) return x.tile < y.tile;
             return x.v1 - x.v0 > y.v1 - y.v0;
         });
     }
-    p.few16 = (int)(std::find_if(p.few.begin(), p.few.end(), [](const PagedItem& x) { return x.tile > 16; }) - p.few.begin());
 }
 
 }  // namespace barq

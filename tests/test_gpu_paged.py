@@ -209,7 +209,7 @@ def test_tokens_without_a_page(be):
 
 LENS = [
     [(1, 1)], [(1, 31)], [(1, 32)], [(1, 33)], [(1, 1000)], [(3, 3)], [(17, 200)], [(33, 33)], [(40, 300)], [(130, 130)],
-    [(200, 517)], [(1, 5), (1, 400), (1, 64), (1, 129)], [(0, 50), (5, 77), (1, 1), (0, 0), (64, 150), (2, 258)],
+    [(200, 517)], [(300, 300)], [(1, 5), (1, 400), (1, 64), (1, 129)], [(0, 50), (5, 77), (1, 1), (0, 0), (64, 150), (2, 258)],
 ]
 
 
@@ -276,7 +276,7 @@ def test_nan_and_infinity_in_the_cache(be, type_, hd, rows, before):
 
 
 @pytest.mark.parametrize("type_", [B.F16, B.F32])
-@pytest.mark.parametrize("rows", [1, 24, 100])
+@pytest.mark.parametrize("rows", [1, 24, 150])
 @pytest.mark.parametrize("q_size,k_size,v_size", [(1e-30, 1, 1), (1e4, 1, 1), (1, 300, 1), (30, 30, 6e4), (1, 1e-6, 1e-6), (0, 1, 1),
                                                   (1e30, 1e-20, 1)])
 def test_sizes_of_the_values(be, type_, rows, q_size, k_size, v_size):
@@ -344,7 +344,7 @@ def test_a_long_cache(be, type_):
     b.set([n], [n], table)
     torch.cuda.synchronize()
     b.append(0, k, v)
-    for rows in (1, 3, 70):
+    for rows in (1, 3, 140):
         q = torch.randn(2, rows, hd, device="cuda", generator=g)
         torch.cuda.synchronize()
         b.set([rows], [n], table)

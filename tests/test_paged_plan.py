@@ -39,9 +39,9 @@ static int plan() {
     for (auto& s : seqs) if (scanf("%" SCNd64 " %" SCNd64, &s.q_len, &s.kv_len) != 2) return 1;
     PagedPlan p;
     paged_plan(sh, seqs, p);
-    printf("%d %d %zu %d %zu %zu %zu\n", sh.few_step, sh.many_step, sh.part_rows, p.few16, p.few.size(), p.many.size(), p.merges.size());
+    printf("%d %d %zu %zu %zu %zu\n", sh.few_step, sh.many_step, sh.part_rows, p.few.size(), p.many.size(), p.merges.size());
     for (auto* v : {&p.few, &p.many})
-        for (auto& i : *v) printf("%d %d %d %d %d %d %d %d %d %d %d\n", i.q0, i.past, i.kv_len, i.row0, i.rows, i.a, i.b, i.v0, i.v1, i.part, i.tile);
+        for (auto& i : *v) printf("%d %d %d %d %d %d %d %d %d %d\n", i.q0, i.past, i.kv_len, i.row0, i.rows, i.a, i.b, i.v0, i.v1, i.part);
     for (auto& m : p.merges) printf("%d %d %d %d %d\n", m.q0, m.row0, m.rows, m.part, m.n_split);
     printf("%zu %zu\n", paged_max_tiles(n, max_tokens, sh.G), (size_t)(2 * (sh.few_target + sh.many_target)));
     return 0;
@@ -120,16 +120,15 @@ def cover(program, G, n_kv, window, n_sink, f16, hd, seqs):
     tokens = max(sum(q for q, _ in seqs), 1)
     lines = [list(map(int, l.split())) for l in program(
         "plan", G, n_kv, window, n_sink, int(f16), hd, tokens, len(seqs), *(x for s in seqs for x in s)).splitlines()]
-    few_step, many_step, part_rows, few16, n_few, n_many, n_merges = lines[0]
+    few_step, many_step, part_rows, n_few, n_many, n_merges = lines[0]
     few, many = lines[1:1 + n_few], lines[1 + n_few:1 + n_few + n_many]
     merges = lines[1 + n_few + n_many:1 + n_few + n_many + n_merges]
     tiles, extra = lines[-1]
     assert n_merges <= tiles and max(n_few, n_many) <= tiles + extra   # what batch_create has room for
-    assert all(i[10] == (16 if k < few16 else 32) for k, i in enumerate(few)) and all(i[10] == 128 for i in many)
     starts = [sum(q for q, _ in seqs[:s]) for s in range(len(seqs))]
     seen, parts, states = {}, {}, set()
-    for items, step in ((few, few_step), (many, many_step)):
-        for q0, past, kv, row0, rows, a, b, v0, v1, part, tile in items:
+    for items, step, tile in ((few, few_step, 16), (many, many_step, 128)):
+        for q0, past, kv, row0, rows, a, b, v0, v1, part in items:
             assert 0 < rows <= tile and v0 < v1
             s = max(i for i, q in enumerate(starts) if q == q0 and seqs[i][0])
             assert (seqs[s][1], seqs[s][1] - seqs[s][0]) == (kv, past)
