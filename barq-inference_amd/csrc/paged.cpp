@@ -325,7 +325,8 @@ int barq_rocm_paged_batch_create(barq_rocm_handle* h, barq_rocm_paged_cache* c, 
     b->part_at = a.add(p.n_head_kv * b->part_rows * p.head_dim * sizeof(float));
     hipError_t e = hipMalloc(&b->mem, a.used);
     // (no sequences yet)
-    if (e == hipSuccess) e = hipMemset(b->mem, 0, sizeof(barq::PagedCounts));
+    if (e == hipSuccess) e = hipMemset(b->mem + b->counts_at, 0, sizeof(barq::PagedCounts));
+    if (e == hipSuccess) e = hipStreamSynchronize(nullptr);   // (before a set() on another stream)
     for (Stage& s : b->stage)
         if (e == hipSuccess) e = hipEventCreateWithFlags(&s.done, hipEventDisableTiming);
     if (e != hipSuccess) {

@@ -550,8 +550,9 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
  * a stream that is being captured.  Calls captured in a graph replay with
  * whatever batch_set gave since, so n_tokens may change within the batch's limits
  * (q, out and the other buffers are then those of that many tokens;
- * rows behind them are left as they are).  A batch has its own scratch memory: calls on one batch must be ordered by the caller,
- * calls on different batches need not be.  A cache's memory lives until the
+ * rows behind them are left as they are).  A batch has its own scratch memory, partial states of the attention for the
+ * most part (at most 64 MiB with 128 dims, 128 MiB with 256; less for few tokens): calls on one batch must
+ * be ordered by the caller, calls on different batches need not be.  A cache's memory lives until the
  * cache and all its batches are destroyed. */
 typedef struct barq_rocm_paged_cache barq_rocm_paged_cache;
 typedef struct barq_rocm_paged_batch barq_rocm_paged_batch;
@@ -609,7 +610,9 @@ int barq_rocm_rope_frequencies(int scaling, size_t rot_dim, double base, double 
  * (out_type BARQ_TYPE_F32), or its rows as Q8_K blocks (BARQ_TYPE_Q8_K: n_head * head_dim a
  * multiple of 256; the bytes barq_rocm_quantize_act writes for them).  A query that sees no position
  * gives zeros.  Softmax statistics and sums are f32.  Over an f16 cache a query element counts to 2^-23 of itself or 2^-52 of
- * its row's largest, a weight to 2^-23 of itself or 2^-40 of its row's largest, whichever is more.
+ * its row's largest, a weight to 2^-22 of itself or 2^-40 of its row's largest, whichever is more.  Over an
+ * f32 cache products count to 2^-23 of themselves; of sequences with more than 64 rows (new tokens x n_head /
+ * n_head_kv), q, K and V beyond 3.38e38 may count as NaN.
  * Device buffers: q, q_out, k, v, x and norm_rope's out 16-byte aligned, the others 4-byte. */
 int barq_rocm_norm_rope(barq_rocm_handle* h, const float* x, size_t seq_len, size_t n_heads, size_t head_dim,
                         size_t start_pos, const float* norm, float eps, const barq_rocm_rotary* rotary, float* out,
