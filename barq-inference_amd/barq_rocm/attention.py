@@ -85,6 +85,7 @@ class Rotary:
     def __init__(self, inv_freq, rot_dim, layout=ROPE_INTERLEAVED, freq_scale=1.0, magnitude=1.0):
         if tuple(inv_freq.shape) != (rot_dim // 2,) or not str(inv_freq.dtype).endswith("float32"):
             raise L.BarqError(L.E_DIM, f"Rotary: inv_freq must be {rot_dim // 2} float32 values")
+        _check_f32("Rotary", "inv_freq", inv_freq, rot_dim // 2)
         self.inv_freq = inv_freq   # (kept alive: the argument below has its address)
         self.arg = L.RotaryArg(rot_dim, layout, freq_scale, magnitude, _ptr(inv_freq) or None)
         self.ref = ctypes.byref(self.arg)

@@ -39,6 +39,7 @@ backend's stream; torch only allocates the activation buffers.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import numpy as np
@@ -227,8 +228,9 @@ class DeviceLlama:
         out = []
         for m in "qk":
             w = self.get(f"blk.{il}.attn_{m}_norm.weight")
-            if w is not None and w[1] * w[2] != self.cfg.head_dim:
-                raise NotImplementedError(f"blk.{il}.attn_{m}_norm.weight: {w[1] * w[2]} values, not one for each dim of a head")
+            if w is not None and (w[0] != L.F32 or w[1] * w[2] != self.cfg.head_dim):
+                raise NotImplementedError(f"blk.{il}.attn_{m}_norm.weight: {w[1] * w[2]} values of type {w[0]}, not an f32 one for each dim "
+                                          "of a head")
             out.append(None if w is None else w[3])
         return out
 
@@ -310,31 +312,42 @@ class PagedLlama(DeviceLlama):
     def step(self, news, trace=None):
         """news: (paged.Sequence, its new tokens: a list or array of ids) for each sequence.
         -> logits [sequences with new tokens, n_vocab] (device f32) of their last tokens.  The
-        sequences grow by their tokens; pages behind the window are given back."""
+        sequences grow by their tokens (a step that fails leaves them as they were); pages behind the
+        window are given back.  The logits' buffer is the next step's too."""
         import torch
         c = self.cfg
         q_lens = [len(t) for _, t in news]
-        before = [(seq, seq.length, len(seq.pages)) for seq, _ in news]
+        before = [(seq, seq.length) for seq, _ in news]
         try:
             for seq, t in news:
                 self.pages.grow(seq, len(t))
             self.batch.set(q_lens, [s.length for s, _ in news], [s.pages for s, _ in news])
+            ids = np.concatenate([np.asarray(t, np.int32) for _, t in news]) if news else np.empty(0, np.int32)
+            if len(ids) == 0:
+                return torch.empty((0, self.n_vocab), dtype=torch.float32, device="cuda")
+            last = np.cumsum(q_lens)[np.asarray(q_lens) > 0].astype(np.int32) - 1
+            with torch.cuda.stream(torch.cuda.ExternalStream(self.be.stream())):
+                both = torch.from_numpy(np.concatenate([ids, last])).cuda()
+            self.last = None if len(last) == len(ids) else both[len(ids):]
+            logits = self.forward_hidden(self.embed(both[:len(ids)]), 0, trace)
         except Exception:
-            for seq, length, n in reversed(before):   # nothing has been computed: the sequences are as they were
-                self.pages.shrink(seq, length, n)
+            for seq, length in before:   # (what a layer has written lies behind their ends)
+                self.pages.shrink(seq, length)
             raise
-        ids = np.concatenate([np.asarray(t, np.int32) for _, t in news]) if news else np.empty(0, np.int32)
-        if len(ids) == 0:
-            return torch.empty((0, self.n_vocab), dtype=torch.float32, device="cuda")
-        last = np.cumsum(q_lens)[np.asarray(q_lens) > 0].astype(np.int32) - 1
-        with torch.cuda.stream(torch.cuda.ExternalStream(self.be.stream())):
-            both = torch.from_numpy(np.concatenate([ids, last])).cuda()
-        self.last = None if len(last) == len(ids) else both[len(ids):]
-        logits = self.forward_hidden(self.embed(both[:len(ids)]), 0, trace)
         if c.window:
             for seq, _ in news:
                 self.pages.drop_behind(seq, c.window, c.n_sink)
         return logits
+
+    def _buf(self, key, shape, dtype="float32"):
+        """A part of one buffer for each use, of a step's most rows: steps have any number of them."""
+        import torch
+        name, n = key if isinstance(key, tuple) else (key, 1)
+        size = math.prod(shape)
+        if name not in self._bufs:
+            most = self.batch.max_seqs if name in ("xq_out", "logits", "last_res", "last_ff") else self.batch.max_tokens
+            self._bufs[name] = torch.empty(size // n * most, dtype=getattr(torch, dtype), device="cuda")
+        return self._bufs[name][:size].view(shape)
 
     def _attend(self, il, xq, seq, start_pos, qr, aq):
         q, k, v = self._project(il, xq, seq)

@@ -144,14 +144,16 @@ class PagedBatch:
 
 
 class Sequence:
-    """A sequence of a paged cache: its length and its page ids (-1: given back)."""
+    """A sequence of a paged cache: its length and its page ids (-1: given back).
+    gone: between these two lengths the next query would miss positions that were given back."""
 
     def __init__(self):
-        self.length, self.pages = 0, []
+        self.length, self.pages, self.gone = 0, [], (0, 0)
 
 
 class Pages:
-    """Which pages of a cache are free, and how many sequences have each."""
+    """Which pages of a cache are free, and how many sequences have each.  A page that
+    is not full belongs to one sequence."""
 
     def __init__(self, n_pages: int, page_size: int):
         self.page_size = page_size
@@ -163,6 +165,8 @@ class Pages:
 
     def grow(self, seq: Sequence, n_tokens: int):
         """n_tokens more positions.  Fails without changing anything when the pages run out."""
+        if n_tokens < 0:
+            raise L.BarqError(L.E_DIM, f"pages: {n_tokens} tokens")
         need = -(-(seq.length + n_tokens) // self.page_size) - len(seq.pages)
         if need > len(self._free):
             raise L.BarqError(L.E_ALLOC, f"pages: {need} more are needed, {len(self._free)} are free")
@@ -172,18 +176,29 @@ class Pages:
             seq.pages.append(p)
         seq.length += n_tokens
 
-    def shrink(self, seq: Sequence, length: int, n_pages: int | None = None):
-        """Back to `length` positions."""
-        n = -(-length // self.page_size) if n_pages is None else n_pages
+    def shrink(self, seq: Sequence, length: int):
+        """Back to `length` positions (drafted tokens that were not taken).  Refused where the next token would go to a page
+        that other sequences have, or would miss positions that were given back."""
+        if not 0 <= length <= seq.length:
+            raise L.BarqError(L.E_DIM, f"pages: from {seq.length} back to {length} positions")
+        self._check_window(seq, length)
+        n = -(-length // self.page_size)
+        if length % self.page_size and length < seq.length and self._users[seq.pages[n - 1]] > 1:
+            raise L.BarqError(L.E_INVALID, f"pages: position {length} is on a page that other sequences have")
         while len(seq.pages) > n:
             self._release(seq.pages.pop())
         seq.length = length
+        if length <= seq.gone[0]:
+            seq.gone = (0, 0)
 
     def fork(self, seq: Sequence) -> Sequence:
         """A sequence over the same whole pages: its length is theirs, and what it adds goes to pages of its own."""
         new = Sequence()
-        new.length = seq.length // self.page_size * self.page_size
-        new.pages = seq.pages[:seq.length // self.page_size]
+        n = seq.length // self.page_size
+        self._check_window(seq, n * self.page_size)
+        new.length, new.pages = n * self.page_size, seq.pages[:n]
+        if new.length > seq.gone[0]:
+            new.gone = seq.gone
         for p in new.pages:
             if p >= 0:
                 self._users[p] += 1
@@ -196,10 +211,18 @@ class Pages:
             if seq.pages[i] >= 0:
                 self._release(seq.pages[i])
                 seq.pages[i] = -1
+                start, end = seq.gone
+                seq.gone = (min(start, i * self.page_size) if end else i * self.page_size,
+                            max(end, (i + 1) * self.page_size + window - 1))
 
     def close(self, seq: Sequence):
         """The end of the sequence: its pages are free again."""
         self.shrink(seq, 0)
+
+    def _check_window(self, seq: Sequence, length: int):
+        if seq.gone[0] < length < seq.gone[1]:
+            raise L.BarqError(L.E_INVALID, f"pages: a query at position {length} would miss positions that were given back (one at "
+                                           f"{seq.gone[1]} does not)")
 
     def _release(self, p: int):
         if p < 0:

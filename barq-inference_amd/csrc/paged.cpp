@@ -21,6 +21,7 @@ using namespace barq_api;
 namespace {
 
 constexpr size_t INT_MOST = 0x7fffffff;
+constexpr size_t GRID_MOST = (1u << 24) - 1;   // workgroups of 256: a launch has fewer than 2^32 threads
 
 struct Pool {
     int device = 0, type = BARQ_TYPE_F16, log_page = 0;
@@ -186,7 +187,7 @@ int barq_rocm_norm_rope(barq_rocm_handle* h, const float* x, size_t seq_len, siz
     BARQ_CHECK(check_rotary(rotary, head_dim, who));
     if (seq_len == 0 || n_heads == 0) return ok();
     if (!x || !out) return fail(BARQ_E_INVALID, "%s: null buffer", who);
-    if (seq_len > INT_MOST || start_pos > INT_MOST - seq_len || n_heads > INT_MOST / head_dim || n_heads * head_dim > (SIZE_MAX / 16) / seq_len)
+    if (seq_len > GRID_MOST || start_pos > INT_MOST - seq_len || n_heads > INT_MOST / head_dim || n_heads * head_dim > (SIZE_MAX / 16) / seq_len)
         return fail(BARQ_E_DIM, "%s: %zu rows from position %zu, %zu heads", who, seq_len, start_pos, n_heads);
     if (mem == BARQ_MEM_DEVICE && !(aligned(x, 16) && aligned(out, 16) && aligned(norm, 4) && (!rotary || aligned(rotary->inv_freq, 4))))
         return fail(BARQ_E_INVALID, "%s: x and out must be 16-byte aligned, norm and inv_freq 4-byte", who);
@@ -285,7 +286,8 @@ int barq_rocm_paged_batch_create(barq_rocm_handle* h, barq_rocm_paged_cache* c, 
     if (max_seqs == 0 || max_tokens == 0 || max_pages == 0)
         return fail(BARQ_E_DIM, "%s: max_seqs, max_tokens and max_pages must be positive", who);
     if (n_head > INT_MOST / p.head_dim || max_tokens > INT_MOST / n_head || max_seqs > INT_MOST / n_head ||
-        max_seqs > INT_MOST / max_pages || window > INT_MOST || n_sink > INT_MOST)
+        max_seqs > INT_MOST / max_pages || window > INT_MOST || n_sink > INT_MOST ||
+        max_tokens * n_head / 16 + 4 * max_seqs * p.n_head_kv > GRID_MOST)   // (tiles of rows; groups of new tokens, twice)
         return fail(BARQ_E_DIM, "%s: %zu sequences, %zu tokens, %zu pages, %zu heads, window %zu, %zu first tokens", who, max_seqs,
                     max_tokens, max_pages, n_head, window, n_sink);
     DeviceGuard g(h);

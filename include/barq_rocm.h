@@ -552,7 +552,8 @@ int barq_rocm_attention_mass(barq_rocm_handle* h, const float* q, const barq_roc
  * (q, out and the other buffers are then those of that many tokens;
  * rows behind them are left as they are).  A batch has its own scratch memory, partial states of the attention for the
  * most part (at most 64 MiB with 128 dims, 128 MiB with 256; less for few tokens): calls on one batch must
- * be ordered by the caller, calls on different batches need not be.  A cache's memory lives until the
+ * be ordered by the caller, calls on different batches need not be.  max_tokens * n_head / 16 + 4 * max_seqs * n_head_kv
+ * stays below 2^24.  A cache's memory lives until the
  * cache and all its batches are destroyed. */
 typedef struct barq_rocm_paged_cache barq_rocm_paged_cache;
 typedef struct barq_rocm_paged_batch barq_rocm_paged_batch;
@@ -597,7 +598,7 @@ int barq_rocm_rope_frequencies(int scaling, size_t rot_dim, double base, double 
 
 /* norm_rope = RMSNorm of every head (norm [head_dim] or NULL: none; eps as in
  * barq_rocm_rms_norm) and the rotation, in one pass: x [seq_len, n_heads *
- * head_dim] -> out [n_heads, seq_len, head_dim], which must not overlap.  For models with
+ * head_dim] -> out [n_heads, seq_len, head_dim], which must not overlap; seq_len < 2^24.  For models with
  * norms of their queries and keys whose session has a cache of its own.
  * paged_append = the same on q (into q_out [n_head, n_tokens, head_dim]; both NULL: no q)
  * and k, then k and v (projections [n_tokens, n_head_kv * head_dim]) into the

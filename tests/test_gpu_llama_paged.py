@@ -150,6 +150,44 @@ def test_a_step_that_does_not_fit_changes_nothing(be, weights):
     assert m.step([]).shape == (0, N_VOCAB) and m.step([(a, [])]).shape == (0, N_VOCAB)
 
 
+def test_a_step_that_fails_on_its_way_changes_nothing(be, weights):
+    c, there = CONFIGS["plain"], table(weights, "plain")
+    full = PagedLlama(be, c, there, P.PagedCache(be, 6, 16, 2, c.n_head_kv, c.head_dim), 2, 40, 4)
+    lame = PagedLlama(be, c, lambda name: None if name == "blk.1.ffn_up.weight" else there(name), full.cache, 2, 40, 4, pages=full.pages)
+    a, b = P.Sequence(), P.Sequence()
+    news = [(a, ids(20, 1)), (b, ids(3, 2))], [(a, ids(13, 3)), (b, ids(14, 4))]
+    full.step(news[0])
+    was = [(s.length, list(s.pages)) for s in (a, b)] + [full.pages.free()]
+    with pytest.raises(KeyError):
+        lame.step(news[1])
+    assert [(s.length, s.pages) for s in (a, b)] + [full.pages.free()] == was
+
+    def logits(step):
+        x = full.step(step)
+        be.sync()
+        return x.cpu().numpy()
+    got = logits(news[1])
+    again = [P.Sequence(), P.Sequence()]
+    full.pages.close(a)
+    full.pages.close(b)
+    for new in news:
+        want = logits([(s, t) for s, (_, t) in zip(again, new)])
+    assert np.array_equal(got, want)   # what the failed step has written is overwritten
+
+
+def test_buffers_do_not_grow_with_the_steps(be, weights):
+    c = CONFIGS["plain"]
+    m = PagedLlama(be, c, table(weights, "plain"), P.PagedCache(be, 24, 16, 2, c.n_head_kv, c.head_dim), 4, 40, 16)
+    seqs, where = [P.Sequence() for _ in range(4)], None
+    for n in (1, 2, 3, 7, 1, 8, 9, 4):
+        m.step([(s, ids(n, i)) for i, s in enumerate(seqs)])
+        m.step([(seqs[0], ids(1, 9))])
+        now = {k: (b.data_ptr(), b.numel()) for k, b in m._bufs.items()}
+        assert where is None or {k: now[k] for k in where} == where
+        where = now
+    assert len(where) <= 16
+
+
 def test_windows_are_for_pages(be, weights):
     c = CONFIGS["window"]
     with pytest.raises(NotImplementedError):

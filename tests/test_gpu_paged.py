@@ -545,7 +545,8 @@ def test_refusals(be):
         refused(code, P.PagedCache, be, *args[:5], type=args[5])
     c = P.PagedCache(be, 4, 16, 2, 2, 64)
     for args, code in (((3, 1, 8, 4), L.E_DIM), ((0, 1, 8, 4), L.E_DIM), ((4, 0, 8, 4), L.E_DIM), ((4, 1, 0, 4), L.E_DIM), ((4, 1, 8, 0), L.E_DIM),
-                       ((4, 1, 1 << 40, 4), L.E_DIM), ((4, 1 << 20, 8, 1 << 20), L.E_DIM)):
+                       ((4, 1, 1 << 40, 4), L.E_DIM), ((4, 1 << 20, 8, 1 << 20), L.E_DIM),
+                       ((4, 1 << 22, 8, 1), L.E_DIM), ((4, 1, 1 << 26, 1), L.E_DIM)):
         refused(code, P.PagedBatch, c, *args)
     b = P.PagedBatch(c, 4, 2, 8, 3)
     b.set([2], [20], [[1, 3]])

@@ -55,18 +55,85 @@ def test_what_is_behind_the_window_is_given_back(window, n_sink):
         assert len(held) == len(set(held)) and p.free() == 20 - len(held)
 
 
+def test_back_into_a_shared_page_is_refused():
+    p, a = Pages(6, 16), Sequence()
+    p.grow(a, 40)
+    b = p.fork(a)
+    p.shrink(a, 33)   # a page of its own
+    with pytest.raises(L.BarqError) as e:
+        p.shrink(a, 20)   # what it would add next is b's prefix
+    assert e.value.code == L.E_INVALID and (a.length, len(a.pages), p.free()) == (33, 3, 3)
+    p.shrink(a, 32)
+    p.shrink(a, 16)
+    p.shrink(b, 32)
+    with pytest.raises(L.BarqError):
+        p.shrink(a, 9)
+    p.shrink(b, 17)   # the second page is b's alone by now
+    p.close(b)
+    p.shrink(a, 9)
+    assert (a.length, len(a.pages), p.free()) == (9, 1, 5)
+    for length in (-1, 10):
+        with pytest.raises(L.BarqError) as e:
+            p.shrink(a, length)
+        assert e.value.code == L.E_DIM and a.length == 9
+    with pytest.raises(L.BarqError) as e:
+        p.grow(a, -1)
+    assert e.value.code == L.E_DIM and a.length == 9
+
+
+@pytest.mark.parametrize("window,n_sink", [(1, 0), (5, 0), (16, 0), (20, 1), (33, 16), (70, 17)])
+def test_back_to_where_the_window_is_gone_is_refused(window, n_sink):
+    rng = random.Random(window)
+    for _ in range(300):
+        p, s = Pages(20, 16), Sequence()
+        for n in (rng.randint(0, 120), rng.randint(1, 40)):
+            p.grow(s, n)
+            if rng.random() < 0.8:
+                p.drop_behind(s, window, n_sink)
+
+        def there(length):
+            """The query at `length` sees no position that is given back, nor goes to one."""
+            return all(s.pages[j // 16] >= 0 for j in range(-(-length // 16) * 16) if j > length - window or j < n_sink)
+        for what in (p.shrink, p.fork):
+            length = rng.randint(0, s.length) if what == p.shrink else s.length // 16 * 16
+            try:
+                fine, was = there(length), (s.length, list(s.pages))
+                got = what(s, length) if what == p.shrink else what(s)
+            except L.BarqError as e:
+                # (a window of one position needs nothing before the first of a page: refused all the same)
+                assert e.code == L.E_INVALID and (not fine or window == 1) and was == (s.length, s.pages)
+                continue
+            assert fine
+            t = s if what == p.shrink else got
+            assert t.length == length
+            # what it then grows to and gives back stays consistent
+            p.grow(t, 3)
+            p.drop_behind(t, window, n_sink)
+        p.close(s)
+        assert s.gone == (0, 0)
+
+
 def test_drawn_sessions_lose_no_page():
     rng = random.Random(2)
     p, seqs = Pages(30, 16), []
     for _ in range(2000):
         what = rng.random()
         if what < 0.3 and len(seqs) < 12:
-            seqs.append(p.fork(rng.choice(seqs)) if seqs and rng.random() < 0.5 else Sequence())
+            try:
+                seqs.append(p.fork(rng.choice(seqs)) if seqs and rng.random() < 0.5 else Sequence())
+            except L.BarqError as e:   # (behind the window)
+                assert e.code == L.E_INVALID
         elif seqs and what < 0.8:
             try:
                 p.grow(rng.choice(seqs), rng.randint(0, 40))
             except L.BarqError:
                 pass
+        elif seqs and what < 0.85:
+            s = rng.choice(seqs)
+            try:
+                p.shrink(s, rng.randint(0, s.length))
+            except L.BarqError as e:
+                assert e.code == L.E_INVALID
         elif seqs and what < 0.9:
             p.drop_behind(rng.choice(seqs), rng.randint(1, 30), rng.choice([0, 4, 20]))
         elif seqs:
@@ -142,5 +209,6 @@ def test_refusals_before_any_device():
                     (L.RotaryArg(8, 2, 1.0, 1.0, 16), L.E_INVALID), (L.RotaryArg(8, 0, 1.0, 1.0, None), L.E_INVALID)):
         assert norm(None, 16, 1, 1, 64, 0, None, 0.0, ctypes.byref(r), 16, L.MEM_DEVICE) == code
     assert norm(None, 16, 2, 1, 64, 0x7ffffffe, None, 0.0, None, 16, L.MEM_DEVICE) == L.E_DIM
+    assert norm(None, 16, 1 << 24, 1, 64, 0, None, 0.0, None, 16, L.MEM_DEVICE) == L.E_DIM
     assert norm(None, 16, 2, 1 << 40, 64, 0, None, 0.0, None, 16, L.MEM_DEVICE) == L.E_DIM
     assert norm(None, None, 0, 1, 64, 0, None, 0.0, None, None, L.MEM_DEVICE) == L.OK
