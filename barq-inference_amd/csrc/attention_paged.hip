@@ -234,14 +234,13 @@ void paged_few_kernel(PagedAttn a, int count) {
             uint32_t seen = 0;   // bit e: the lane's row sees the lane's position e
             if (!whole) {
                 const bool here = H && g >= 2 ? have & 2 : have & 1;   // (a group's positions lie in one block)
-                #pragma unroll
-                for (int e = 0; e < NP; e++) seen |= (here & sight.sees(pos, base + E * g + e)) ? 1u << e : 0u;
+                seen = here ? (uint32_t)sight.mask(pos, base + E * g) : 0u;
                 uint32_t any = 0;
                 #pragma unroll
                 for (int d = 0; d < NV; d++)
                     #pragma unroll
-                    for (int u = 0; u < 4; u++) any |= H ? f16_bad(st.v[d][u]) : f32_bad(st.v[d][u]);
-                if (__any(any != 0)) {   // NaN where a row sees what is not finite, and zero in its place
+                    for (int u = 0; u < 4; u++) any |= H ? f16_bad_mark(st.v[d][u]) : f32_bad_mark(st.v[d][u]);
+                if (__any((any & (H ? 0x80008000u : 0x80000000u)) != 0)) {   // NaN where a row sees what is not finite, and zero in its place
                     Weights<H> ones;
                     float z[NP];
                     #pragma unroll
@@ -268,7 +267,7 @@ void paged_few_kernel(PagedAttn a, int count) {
             load(j + 1, true);
             if (!whole) {
                 #pragma unroll
-                for (int e = 0; e < NP; e++) s[e] = (seen >> e) & 1 ? s[e] : -INFINITY;
+                for (int e = 0; e < NP; e++) s[e] = seen_or_none(s[e], bit_as_mask(seen, e));
             }
             float top = s[0];
             #pragma unroll

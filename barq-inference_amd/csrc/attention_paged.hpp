@@ -53,8 +53,12 @@ __device__ __forceinline__ PagedItem paged_item(const PagedItem* p) {
 // What a row sees.
 struct PagedSight {
     int window, n_sink;
-    __device__ __forceinline__ bool sees(int row_pos, int j) const {
-        return (j <= row_pos) & ((window == 0) | (j > row_pos - window) | (j < n_sink));   // (no branches)
+    // bit x, below 64: the row at row_pos sees position base + x (windows are at most 2^31 - 4096)
+    __device__ __forceinline__ uint64_t mask(int row_pos, int base) const {
+        const auto below = [](int n) { return n > 0 ? ~0ull >> (64 - min(n, 64)) : 0ull; };
+        uint64_t m = below(row_pos - base + 1);
+        if (window) m &= ~below(row_pos - base - window + 1) | below(n_sink - base);
+        return m;
     }
     // all positions base .. base + n - 1 by all rows at positions first .. last
     __device__ __forceinline__ bool all(int base, int n, int first, int last) const {
@@ -79,6 +83,15 @@ __device__ __forceinline__ void paged_split(float x0, float x1, uint32_t& hi, ui
     lo = __builtin_bit_cast(uint32_t, l);
 }
 
+// x where `keep` is all ones, -infinity where it is zero
+__device__ __forceinline__ float seen_or_none(float x, int keep) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(int, x) & keep) | (0xFF800000 & ~keep));
+}
+__device__ __forceinline__ int bit_as_mask(uint32_t bits, int i) { return (int)(bits << (31 - i)) >> 31; }
+
+// Bit 15 of an f16 half that is not finite, bit 31 of the other or of an f32; other bits say nothing.
+__device__ __forceinline__ uint32_t f16_bad_mark(uint32_t x) { return (x & 0x7C007C00u) + 0x04000400u; }
+__device__ __forceinline__ uint32_t f32_bad_mark(uint32_t x) { return (x & 0x7F800000u) + 0x00800000u; }
 // The f16 halves of a dword that are not finite, as 0xFFFF each.
 __device__ __forceinline__ uint32_t f16_bad(uint32_t x) {
     return ((((x & 0x7C007C00u) + 0x04000400u) >> 15) & 0x00010001u) * 0xFFFFu;

@@ -136,8 +136,14 @@ void paged_many_f32_kernel(PagedAttn a, int count) {
             wait_vmcnt<0>();
             __syncthreads();   // the step is there for all waves, and none still reads the parts of the one before
             const int base = base_of(j), have = has_now;
-            const auto sees = [&](int x) { return (((have >> (x / 16)) & 1) != 0) & sight.sees(pos, base + x); };
-            // Where some row of the workgroup does not see all of the step, what is not finite in V becomes zero, after it has
+            // bit 8 (r / 4) + r % 4: the lane's row sees its register r
+            const auto seen_by = [&]() __attribute__((always_inline)) {
+                uint32_t m = (uint32_t)sight.mask(pos, base);
+                #pragma unroll
+                for (int b = 0; b < NB; b++) m &= (have >> b) & 1 ? ~0u : ~(0xFFFFu << (16 * b));
+                return m >> (4 * h);
+            };
+            // Where some row of the workgroup does not see all of the step: what is not finite in V becomes zero, after it has
             // been put as NaN into the dims of the rows that see it.
             const bool edge = have != (1 << NB) - 1 || !sight.all(base, STEP, all_first, all_last);
             if (edge) {
@@ -145,9 +151,10 @@ void paged_many_f32_kernel(PagedAttn a, int count) {
                 for (int u = lane; u < RAW / 16; u += 64) {
                     const u32x4v x = reinterpret_cast<const u32x4v*>(raw_v)[u];
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) any |= f32_bad(x[e]);
+                    for (int e = 0; e < 4; e++) any |= f32_bad_mark(x[e]);
                 }
-                if (__any(any != 0)) {
+                if (__any((any >> 31) != 0)) {
+                    const uint32_t seen = seen_by();
                     #pragma unroll
                     for (int d = 0; d < ND; d++) {
                         f32x16 n = {};   // such places that a row sees
@@ -156,7 +163,7 @@ void paged_many_f32_kernel(PagedAttn a, int count) {
                             const u32x4v v = *reinterpret_cast<const u32x4v*>(raw_v + (g / 2) * BLOCK + ((2 * (g & 1) + h) * HD + 32 * d + i) * 16);
                             #pragma unroll
                             for (int e = 0; e < 4; e++)
-                                n = __builtin_amdgcn_mfma_f32_32x32x2f32(f32_bad(v[e]) ? 1.0f : 0.0f, sees(8 * g + 4 * h + e) ? 1.0f : 0.0f, n, 0, 0, 0);
+                                n = __builtin_amdgcn_mfma_f32_32x32x2f32(f32_bad(v[e]) ? 1.0f : 0.0f, (seen >> (8 * g + e)) & 1 ? 1.0f : 0.0f, n, 0, 0, 0);
                         }
                         #pragma unroll
                         for (int r = 0; r < 16; r++) o[d][r] = n[r] > 0.0f ? NAN : o[d][r];
@@ -214,8 +221,9 @@ void paged_many_f32_kernel(PagedAttn a, int count) {
             }
             has_now = has_next;
             if (have != (1 << NB) - 1 || !sight.all(base, STEP, p_first, p_last)) {
+                const uint32_t seen = seen_by();
                 #pragma unroll
-                for (int r = 0; r < 16; r++) s[r] = sees(8 * (r / 4) + 4 * h + r % 4) ? s[r] : -INFINITY;
+                for (int r = 0; r < 16; r++) s[r] = seen_or_none(s[r], bit_as_mask(seen, 8 * (r / 4) + r % 4));
             }
             float top = s[0];
             #pragma unroll

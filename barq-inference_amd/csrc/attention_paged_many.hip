@@ -7,18 +7,20 @@
 // positions) come by direct loads into one of two LDS buffers while the other is
 // computed on.  The pages' blocks are the MFMA operands' layout already, so they
 // are copied as they lie and read without bank conflicts: wave w fetches block w.
-// 2048 tokens of 32 heads of 128 dims after 6000 positions: 446 us, 529 TFLOP/s counted once, 1058 of f16
-// products; an 8192^3 f16 product has 1158 on this card, which holds its clock near 2.0 GHz under either.
-// The matrix unit is busy for 49 % of the cycles and the vector unit for about 42 %: 350 vector instructions
-// beside a wave's 64 products of a step.  64 dims have half the products for the same softmax and are bound by that
-// (4000 tokens that see 1024 back: 89 us, 334 TFLOP/s).  256 dims take 476 registers, one wave a SIMD.
+// 2048 tokens of 32 heads of 128 dims after 6000 positions: 442 to 472 us by card, 533 to 500 TFLOP/s counted once, twice
+// that of f16 products.  The card's power holds that down, not a wait: a loop of nothing but these products reaches 2570
+// TFLOP/s on equal operands, 1670 on random ones, 1190 with 8 fmas beside each (a step has 320 vector instructions
+// for 64 products); an 8192^3 f16 product has 1158.  So what counts is instructions left out: O in scalars (as
+// vectors they are copied once a step), what a row sees as bits (a step at a window's edge takes a third fewer): together
+// 464 -> 454 here, 102 -> 96 for 4000 tokens of 64 dims that see 1024 back (half the products for the same softmax), 96 -> 91
+// for attention_mixed's 256 dims (446 registers, one wave a SIMD).
 #include "attention_paged.hpp"
 
 namespace barq {
 
 namespace {
 
-constexpr int NW = 4;   // waves
+constexpr int NW = 4;   // waves, of which each fetches a block of a step's four
 
 // sched_barrier: vector and scalar arithmetic may move across, loads and matrix products stay where they are
 #define BARQ_ONLY_ALU_CROSSES 0x0006
@@ -30,9 +32,8 @@ __device__ __forceinline__ float halves_max(float v) {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// Register r of a lane of half h is this position of a tile of 32: row i of the MFMA stands for position 16 (i / 16) +
-// 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4, so that a half's eight positions of a block are one piece of V.
-__device__ __forceinline__ int tile_pos(int r, int h) { return 16 * (r / 8) + 8 * h + r % 8; }
+// Register r of a lane of half h is position 16 (r / 8) + 8 h + r % 8 of a tile of 32: row i of the MFMA stands for
+// position 16 (i / 16) + 8 (i / 4 % 2) + 4 (i / 8 % 2) + i % 4, so that a half's eight positions of a block are one piece of V.
 
 // Two weights as f16 hi (cut, one instruction for both) + lo (of what that leaves, to the nearest).
 __device__ __forceinline__ void split_weights(float x0, float x1, float minus_one, uint32_t& hi, uint32_t& lo) {
@@ -56,6 +57,7 @@ void paged_many_kernel(PagedAttn a, int count) {
     constexpr int STEP = 64, T = STEP / 32, NB = STEP / PAGE_BLOCK, NC = HD / 16, ND = HD / 32;
     constexpr int BLOCK = PAGE_BLOCK * HD * 2;   // bytes
     extern __shared__ __align__(16) uint8_t lds[];         // [2][K, V][NB][BLOCK]
+    __shared__ int bad_s[2][NW];                           // whether a step's block of V has what is not finite
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
     int n_tokens = a.n_tokens;
     if (n_tokens < 0) {
@@ -142,34 +144,51 @@ void paged_many_kernel(PagedAttn a, int count) {
             }
         }
         float m = -INFINITY, l = 0.0f;
-        f32x16 o[ND];
+        float o[ND][16];
         #pragma unroll
-        for (int d = 0; d < ND; d++) o[d] = f32x16{};
+        for (int d = 0; d < ND; d++)
+            #pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
         for (int j = 0; j < steps; j++) {
+            const int base = base_of(j), have = has_now;
+            uint8_t *kt = lds + (size_t)(j & 1) * 2 * NB * BLOCK, *vt = kt + NB * BLOCK;
+            const bool edge = have != (1 << NB) - 1 || !sight.all(base, STEP, all_first, all_last);
             wait_vmcnt<0>();
+            asm volatile("" ::: "memory");
+            if (edge) {   // (each wave looks through the block that it fetched)
+                uint32_t any = 0;
+                #pragma unroll
+                for (int u = 0; u < BLOCK / 1024; u++) {
+                    const u32x4v x = reinterpret_cast<const u32x4v*>(vt + wave * BLOCK)[64 * u + lane];
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) any |= f16_bad_mark(x[e]);
+                }
+                const bool found = __any((any & 0x80008000u) != 0);
+                if (lane == 0) bad_s[j & 1][wave] = found;
+            }
             __syncthreads();   // the step is there for all waves, and none still reads the other buffer
             if (j + 1 < steps) {
                 if (((j + 1) & 63) == 0) fetch_ids(j + 1);
                 has_next = __builtin_amdgcn_readlane(has, (j + 1) & 63);
                 fetch(j + 1, has_next);
             }
-            const int base = base_of(j), have = has_now;
             has_now = has_next;
-            uint8_t *kt = lds + (size_t)(j & 1) * 2 * NB * BLOCK, *vt = kt + NB * BLOCK;
-            const auto sees = [&](int x) { return (((have >> (x / 16)) & 1) != 0) & sight.sees(pos, base + x); };
-            if (have != (1 << NB) - 1 || !sight.all(base, STEP, all_first, all_last)) {
+            // bit 16 (r / 8) + r % 8 of word t: the lane's row sees its register r of tile t
+            const bool whole = have == (1 << NB) - 1 && sight.all(base, STEP, p_first, p_last);
+            uint32_t seen[T];
+            if (!whole) {
+                uint64_t m = sight.mask(pos, base);
+                #pragma unroll
+                for (int b = 0; b < NB; b++) m &= (have >> b) & 1 ? ~0ull : ~(0xFFFFull << (16 * b));
+                m >>= 8 * h;
+                seen[0] = (uint32_t)m;
+                seen[1] = (uint32_t)(m >> 32);
+            }
+            if (edge) {
                 // some row of the workgroup does not see all of the step: what is not finite in V becomes zero, after it
                 // has been put as NaN into the dims of the rows that see it (all waves find the same)
-                uint32_t any = 0;
-                for (int u = lane; u < NB * BLOCK / 16; u += 64) {
-                    const u32x4v x = reinterpret_cast<const u32x4v*>(vt)[u];
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) any |= f16_bad(x[e]);
-                }
-                if (__any(any != 0)) {
-                    uint32_t seen = 0;   // bit 16 t + r
-                    #pragma unroll
-                    for (int b = 0; b < 16 * T; b++) seen |= sees(32 * (b / 16) + tile_pos(b % 16, h)) ? 1u << b : 0u;
+                if (bad_s[j & 1][0] | bad_s[j & 1][1] | bad_s[j & 1][2] | bad_s[j & 1][3]) {
+                    if (whole) seen[0] = seen[1] = ~0u;
                     #pragma unroll
                     for (int d = 0; d < ND; d++) {
                         f32x16 n = {};   // such places that a row sees
@@ -180,7 +199,7 @@ void paged_many_kernel(PagedAttn a, int count) {
                                 u32x4v v = *reinterpret_cast<const u32x4v*>(vt + (2 * t + u) * BLOCK + (h * HD + 32 * d + i) * 16), one;
                                 #pragma unroll
                                 for (int e = 0; e < 4; e++) {
-                                    const uint32_t two = seen >> (16 * t + 8 * u + 2 * e);
+                                    const uint32_t two = seen[t] >> (16 * u + 2 * e);
                                     v[e] = f16_bad(v[e]) & 0x3C003C00u;
                                     one[e] = (two & 1 ? 0x3C00u : 0u) | (two & 2 ? 0x3C000000u : 0u);
                                 }
@@ -198,7 +217,6 @@ void paged_many_kernel(PagedAttn a, int count) {
                     __syncthreads();
                 }
             }
-            const bool whole = have == (1 << NB) - 1 && sight.all(base, STEP, p_first, p_last);
             // scores: the next pieces of K are fetched while the products of these run
             constexpr int KG = HD == 256 ? 2 : 4, GC = NC / KG;   // (four at a time do not fit the registers of 256 dims)
             float s[T][16];
@@ -233,7 +251,7 @@ void paged_many_kernel(PagedAttn a, int count) {
                 #pragma unroll
                 for (int t = 0; t < T; t++)
                     #pragma unroll
-                    for (int r = 0; r < 16; r++) s[t][r] = sees(32 * t + tile_pos(r, h)) ? s[t][r] : -INFINITY;
+                    for (int r = 0; r < 16; r++) s[t][r] = seen_or_none(s[t][r], bit_as_mask(seen[t], 16 * (r / 8) + r % 8));
             }
             float top = s[0][0];
             #pragma unroll

@@ -600,7 +600,7 @@ int barq_rocm_paged_attention(barq_rocm_handle* h, barq_rocm_paged_batch* b, siz
     x.n_kv = (int)p.n_head_kv;
     x.G = b->shape.G;
     x.log_page = p.log_page;
-    x.window = (int)b->window;
+    x.window = (int)std::min<size_t>(b->window, 0x7ffff000);   // (no position is beyond that)
     x.n_sink = (int)b->n_sink;
     x.scale = (float)(M_LOG2E / std::sqrt((double)p.head_dim));
     x.part = reinterpret_cast<float*>(b->mem + b->part_at);
