@@ -276,6 +276,34 @@ def test_nan_and_infinity_in_the_cache(be, type_, hd, rows, before):
 
 
 @pytest.mark.parametrize("type_", [B.F16, B.F32])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("window,n_sink", [(1, 0), (17, 2), (64, 16), (90, 70)])
+@pytest.mark.parametrize("rows,before", [(1, 299), (7, 200), (200, 150)])
+def test_nan_and_infinity_beside_a_window(be, type_, hd, window, n_sink, rows, before):
+    n = rows + before
+    rng = np.random.default_rng(rows + hd)
+    k, v = (rng.standard_normal((n, 2, hd)).astype(F32) for _ in "kv")
+    for x in (k, v):
+        for value in (np.nan, np.inf, -np.inf):
+            for head in range(2):
+                x[rng.integers(n), head, rng.integers(hd)] = value
+    c = Case(be, type_, 8, 2, hd, 32, [(rows, n)], window, n_sink, k=k, v=v, gone=[(0, 2)])
+    want, off = c.want()
+    assert_within(c.batch.attention(c.layer, dev(c.q)).cpu().numpy(), want, off)
+
+
+@pytest.mark.parametrize("type_", [B.F16, B.F32])
+@pytest.mark.parametrize("rows", [1, 24, 150])
+def test_windows_longer_than_everything(be, type_, rows):
+    c = Case(be, type_, 8, 2, 64, 16, [(rows, rows + 333), (0, 5), (1, 1)])
+    want = c.batch.attention(c.layer, dev(c.q)).cpu().numpy()
+    for window, n_sink in ((rows + 333, 0), (1000, 1000), (2 ** 31 - 4096, 0), (2 ** 31 - 4095, 7), (2 ** 31 - 1, 2 ** 31 - 1), (1, 2 ** 31 - 1)):
+        b = P.PagedBatch(c.cache, 8, 3, rows + 1, c.table.shape[1], window, n_sink)
+        b.set(c.new, c.lens, c.table)
+        assert np.array_equal(b.attention(c.layer, dev(c.q)).cpu().numpy(), want), (window, n_sink)
+
+
+@pytest.mark.parametrize("type_", [B.F16, B.F32])
 @pytest.mark.parametrize("rows", [1, 24, 150])
 @pytest.mark.parametrize("q_size,k_size,v_size", [(1e-30, 1, 1), (1e4, 1, 1), (1, 300, 1), (30, 30, 6e4), (1, 1e-6, 1e-6), (0, 1, 1),
                                                   (1e30, 1e-20, 1)])
