@@ -3,8 +3,8 @@
 // one tensor by itself.
 //
 // Bound by the bytes: q is read and written in f32, K and V read in f32 and written
-// in the cache's type: 2048 tokens of 32 + 8 heads of 128 dims, 92 MB, in 20.2 us (4.6 TB/s of a copy's 5.2 beyond the
-// last-level cache), 17.7 of them without the launch.  A workgroup has up to 16 tokens of one block and some of their
+// in the cache's type: 2048 tokens of 32 + 8 heads of 128 dims, 92 MB, in 19.7 us (4.7 TB/s of a copy's 5.2 beyond the
+// last-level cache), 17.2 of them without the launch.  A workgroup has up to 16 tokens of one block and some of their
 // heads: HD / 8 lanes a row of q or K, the next rows in flight while these are rotated; of
 // V eight tokens (four in f32) of a dim a lane, which are 16 bytes there.  The pairs' cos and
 // sin (64-bit angles) are formed once for a workgroup's tokens, while its first rows come.
@@ -35,27 +35,32 @@ __device__ __forceinline__ size_t block_of(int row, int hk, int n_kv, int log_pa
     return (((page * n_kv + hk) << (log_page - 4)) + (slot >> 4)) * (PAGE_BLOCK * HD * (H ? 2 : 4));
 }
 
-// The workgroups' rows: of a group of n tokens, 2^s at most, row r is token r % 2^s (if there is one) of head r / 2^s; workgroup
-// y of `per` has rows y * ROWS + sub + k * per * ROWS.
+// The workgroups' rows: of a group of n tokens (or a quarter of them), 2^s at most, row r is token r % 2^s (if there is one) of
+// head r / 2^s; the workgroups of the same tokens take ROWS of them each in turn.
 __device__ __forceinline__ int log_tokens(int n) { return n < 2 ? 0 : 32 - __builtin_clz(n - 1); }
 
 template <bool H, int HD>
 __global__ __launch_bounds__(256)
-void paged_append_kernel(PagedAppend a, int per, int per_v) {
+void paged_append_kernel(PagedAppend a, int per, int per_v, int parts) {
     constexpr int LANES = HD / 8, ROWS = 256 / LANES;
     __shared__ __align__(16) float2 turn[TURN_TOKENS][HD / 2];
     const int n_tokens = a.n_tokens < 0 ? a.counts->n_tokens : a.n_tokens, n_groups = a.n_tokens < 0 ? a.counts->groups : a.n_groups;
     const int sub = threadIdx.x / LANES, d0 = 8 * (threadIdx.x % LANES), heads = a.n_q + a.n_kv;
     for (int w = blockIdx.x; w < n_groups; w += gridDim.x) {
-        const PagedGroup gr = a.groups[w];
+        PagedGroup gr = a.groups[w];
         if ((int)blockIdx.y < per) {
+            if (parts > 1) {   // these tokens of the group
+                const int t = TURN_TOKENS / parts * (blockIdx.y % parts);
+                gr.t0 += t, gr.pos += t, gr.n = min(gr.n - t, TURN_TOKENS / parts), gr.row += gr.row < 0 ? 0 : t;
+                if (gr.n <= 0) continue;
+            }
             const int log_n = log_tokens(gr.n), mask = (1 << log_n) - 1, rows = heads << log_n;
             const auto from = [&](int r) {   // (a token that is not there: the last one)
                 const int head = r >> log_n, t = gr.t0 + min(r & mask, gr.n - 1);
                 return head < a.n_q ? a.q + ((size_t)t * a.n_q + head) * HD : a.k + ((size_t)t * a.n_kv + head - a.n_q) * HD;
             };
-            const int step = per * ROWS;
-            int r = blockIdx.y * ROWS + sub;
+            const int step = per / parts * ROWS;
+            int r = blockIdx.y / parts * ROWS + sub;
             TurnRow<HD> ahead[TURN_AHEAD];
             #pragma unroll
             for (int k = 0; k < TURN_AHEAD; k++)
@@ -214,10 +219,14 @@ hipError_t paged_append_launch(const PagedAppend& a, bool f16, size_t hd, hipStr
     const bool captured = a.n_tokens < 0;   // (a captured call goes round the groups)
     const size_t groups = captured ? 256 : (size_t)a.n_groups, most = captured || a.n_tokens > a.n_groups ? TURN_TOKENS : 1;
     const size_t rows = 256 / (hd / 8), heads = (size_t)a.n_q + a.n_kv;
-    const unsigned per = shares(groups, (heads * most + rows - 1) / rows);
+    // whole groups' tokens in quarters: a token's cos and sin are formed by fewer workgroups, K is still written 64 bytes at a
+    // time (append and read of 2048 tokens of 16 + 2 heads of 256 dims 24.5 -> 22.4 us, of 32 + 8 of 128 27.6 -> 27.0, of
+    // 4000 of 8 + 8 32.5 -> 33.2)
+    const int parts = !captured && 8 * groups <= (size_t)a.n_tokens ? 4 : 1;
+    const unsigned per = (shares(groups, (heads * most + rows - 1) / rows) + parts - 1) / parts * parts;
     const unsigned per_v = shares(groups, ((size_t)a.n_kv * (f16 ? 2 : 4) * hd + 255) / 256);
     const dim3 g((unsigned)groups, per + per_v);
-    #define BARQ_APPEND(H, D) if (f16 == H && hd == D) hipLaunchKernelGGL((paged_append_kernel<H, D>), g, dim3(256), 0, s, a, (int)per, (int)per_v);
+    #define BARQ_APPEND(H, D) if (f16 == H && hd == D) hipLaunchKernelGGL((paged_append_kernel<H, D>), g, dim3(256), 0, s, a, (int)per, (int)per_v, parts);
     BARQ_APPEND(true, 64) BARQ_APPEND(true, 128) BARQ_APPEND(true, 256)
     BARQ_APPEND(false, 64) BARQ_APPEND(false, 128) BARQ_APPEND(false, 256)
     #undef BARQ_APPEND
@@ -246,9 +255,11 @@ hipError_t paged_upload_launch(const PagedPieces& p, hipStream_t s) {
 
 hipError_t norm_rope_launch(const float* x, float* out, size_t seq, size_t heads, size_t hd, size_t start_pos,
                             const float* w, float eps, const Rotary& r, hipStream_t s) {
-    // tokens of a workgroup: 16, fewer while that leaves the card empty
+    // tokens of a workgroup: 16, fewer while there are few of those, so that several workgroups form the same cos and sin only
+    // where one token's heads are many (2048 tokens of 32 heads of 128 dims 13.7 us, 15.5 with 16 tokens each; 4000 of 64
+    // dims 14.4 and 13.9)
     size_t tokens = TURN_TOKENS;
-    while (tokens > 1 && (seq + tokens - 1) / tokens < 64) tokens /= 2;
+    while (tokens > 1 && (seq + tokens - 1) / tokens < TURN_WORKGROUPS / 2) tokens /= 2;
     const size_t groups = (seq + tokens - 1) / tokens, rows = 256 / (hd / 8);
     const dim3 g((unsigned)groups, shares(groups, (heads * tokens + rows - 1) / rows));
     #define BARQ_TURN(D) \
