@@ -19,13 +19,19 @@ ROPE_INTERLEAVED = L.ROPE_INTERLEAVED
 ROPE_SPLIT_HALF = L.ROPE_SPLIT_HALF
 
 
-_F32 = set()   # the array libraries' float32, as _check_f32 meets them
+_TENSOR = _FLOAT = None   # torch's tensor and float32, once one has come
+
+
+def _know_torch():
+    global _TENSOR, _FLOAT
+    import torch
+    _TENSOR, _FLOAT = torch.Tensor, torch.float32
 
 
 def _empty(shape, like, mem, dtype="float32"):
     if mem == L.MEM_HOST:
         return np.empty(shape, dtype=np.dtype(dtype))
-    if dtype == "float32" and like.dtype in _F32:
+    if dtype == "float32" and like.__class__ is _TENSOR and like.dtype is _FLOAT:
         return like.new_empty(shape)   # (half a microsecond less than by its names)
     import torch
     return torch.empty(shape, dtype=getattr(torch, dtype), device=like.device)
@@ -41,19 +47,20 @@ def _check_mass(who, n_head_kv, *arrays):
             raise L.BarqError(L.E_INVALID, f"{who}: mass must be contiguous float32")
 
 
-def _check_f32(who, what, t, n):
-    """n float32 values, side by side in memory (a raw address or nothing is taken as it is)."""
+def _f32_at(who, what, t, n):
+    """Address of n float32 values, side by side in memory (a raw address or nothing is taken as it is)."""
+    if t.__class__ is _TENSOR and t.dtype is _FLOAT and t.numel() == n and t.is_contiguous():
+        return t.data_ptr()   # (the usual case first: a call for one token is bound by the host)
     if t is None or isinstance(t, int):
-        return
+        return t
     host = isinstance(t, np.ndarray)
     if (t.size if host else t.numel()) != n:
         raise L.BarqError(L.E_DIM, f"{who}: {what} has {t.size if host else t.numel()} values, {n} are wanted")
-    if t.dtype not in _F32:
-        if not str(t.dtype).endswith("float32"):
-            raise L.BarqError(L.E_INVALID, f"{who}: {what} must be contiguous float32")
-        _F32.add(t.dtype)
-    if not (t.flags.c_contiguous if host else t.is_contiguous()):
+    if not str(t.dtype).endswith("float32") or not (t.flags.c_contiguous if host else t.is_contiguous()):
         raise L.BarqError(L.E_INVALID, f"{who}: {what} must be contiguous float32")
+    if not host:
+        _know_torch()
+    return _ptr(t)
 
 
 def apply_rope(be: Backend, x, seq_len, n_heads, head_dim, start_pos, rope_freq_scale, rope_inv_freq, layout,
@@ -85,9 +92,9 @@ class Rotary:
     def __init__(self, inv_freq, rot_dim, layout=ROPE_INTERLEAVED, freq_scale=1.0, magnitude=1.0):
         if tuple(inv_freq.shape) != (rot_dim // 2,) or not str(inv_freq.dtype).endswith("float32"):
             raise L.BarqError(L.E_DIM, f"Rotary: inv_freq must be {rot_dim // 2} float32 values")
-        _check_f32("Rotary", "inv_freq", inv_freq, rot_dim // 2)
+        at = _f32_at("Rotary", "inv_freq", inv_freq, rot_dim // 2)
         self.inv_freq = inv_freq   # (kept alive: the argument below has its address)
-        self.arg = L.RotaryArg(rot_dim, layout, freq_scale, magnitude, _ptr(inv_freq) or None)
+        self.arg = L.RotaryArg(rot_dim, layout, freq_scale, magnitude, at or None)
         self.ref = ctypes.byref(self.arg)
 
     @classmethod
@@ -113,15 +120,13 @@ def norm_rope(be: Backend, x, seq_len, n_heads, head_dim, start_pos, rotary=None
     """RMSNorm of each head (with norm) and the rotation, in one pass: x
     [seq, n_heads*head_dim] -> [n_heads, seq, head_dim]."""
     n = seq_len * n_heads * head_dim
-    _check_f32("norm_rope", "x", x, n)
-    if norm is not None:
-        _check_f32("norm_rope", "norm", norm, head_dim)
+    at, norm_at = _f32_at("norm_rope", "x", x, n), _f32_at("norm_rope", "norm", norm, head_dim)
     if out is None:
         out = _empty((n_heads, seq_len, head_dim), x, mem)
-    else:
-        _check_f32("norm_rope", "out", out, n)
-    L.check(be._lib.barq_rocm_norm_rope(be.h, _ptr(x), seq_len, n_heads, head_dim, start_pos, _ptr(norm), eps,
-                                        None if rotary is None else rotary.ref, _ptr(out), mem))
+    rc = be._lib.barq_rocm_norm_rope(be.h, at, seq_len, n_heads, head_dim, start_pos, norm_at, eps,
+                                     None if rotary is None else rotary.ref, _f32_at("norm_rope", "out", out, n), mem)
+    if rc:
+        L.check(rc)
     if sync and mem == L.MEM_DEVICE:
         be.sync()
     return out

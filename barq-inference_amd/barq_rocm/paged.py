@@ -10,7 +10,7 @@ import ctypes
 import numpy as np
 
 from . import _lib as L
-from .attention import _check_f32, _empty
+from .attention import _empty, _f32_at
 from .backend import Backend, _ptr
 
 
@@ -27,6 +27,14 @@ class PagedCache:
         self.c = c
         self.n_pages, self.page_size, self.n_layers, self.n_head_kv, self.head_dim, self.type = (
             n_pages, page_size, n_layers, n_head_kv, head_dim, type)
+        self._like = None
+
+    def like(self):
+        """A torch tensor of the cache's type on its device."""
+        if self._like is None:
+            import torch
+            self._like = torch.empty(0, dtype=torch.float16 if self.type == L.F16 else torch.float32, device=f"cuda:{self.be.device}")
+        return self._like
 
     def close(self):
         if self.c:
@@ -90,35 +98,31 @@ class PagedBatch:
         c, t = self.cache, self.n_tokens
         hd = c.head_dim
         nq, nk, who = t * self.n_head * hd, t * c.n_head_kv * hd, "paged_append"
-        if q is not None:
-            _check_f32(who, "q", q, nq)
-            if q_out is None:
-                q_out = _empty((self.n_head, t, hd), q, mem)
-            else:
-                _check_f32(who, "q_out", q_out, nq)
-            if q_norm is not None:
-                _check_f32(who, "q_norm", q_norm, hd)
-        _check_f32(who, "k", k, nk)
-        _check_f32(who, "v", v, nk)
-        if k_norm is not None:
-            _check_f32(who, "k_norm", k_norm, hd)
-        L.check(self.be._lib.barq_rocm_paged_append(self.be.h, self.b, layer, _ptr(q), _ptr(q_out), _ptr(k), _ptr(v), _ptr(q_norm),
-                                                    _ptr(k_norm), eps, None if rotary is None else rotary.ref,
-                                                    mem))
+        if q is not None and q_out is None:
+            q_out = _empty((self.n_head, t, hd), q, mem)
+        rc = self.be._lib.barq_rocm_paged_append(
+            self.be.h, self.b, layer, _f32_at(who, "q", q, nq), _f32_at(who, "q_out", q_out, nq), _f32_at(who, "k", k, nk),
+            _f32_at(who, "v", v, nk), _f32_at(who, "q_norm", q_norm, hd), _f32_at(who, "k_norm", k_norm, hd), eps,
+            None if rotary is None else rotary.ref, mem)
+        if rc:
+            L.check(rc)
         return q_out
 
     def read(self, layer, mem=L.MEM_DEVICE, sync=True):
         """The tokens' rows as the cache holds them: (k, v), each [n_tokens,
         n_head_kv, head_dim] float16 or float32."""
         c = self.cache
-        shape, dtype = (self.n_tokens, c.n_head_kv, c.head_dim), "float16" if c.type == L.F16 else "float32"
+        shape = self.n_tokens, c.n_head_kv, c.head_dim
         if mem == L.MEM_HOST:
+            dtype = "float16" if c.type == L.F16 else "float32"
             k, v = np.empty(shape, dtype), np.empty(shape, dtype)
+            rc = self.be._lib.barq_rocm_paged_read(self.be.h, self.b, layer, _ptr(k), _ptr(v), mem)
         else:
-            import torch
-            dtype, dev = torch.float16 if c.type == L.F16 else torch.float32, f"cuda:{self.be.device}"
-            k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
-        L.check(self.be._lib.barq_rocm_paged_read(self.be.h, self.b, layer, _ptr(k), _ptr(v), mem))
+            like = c.like()
+            k, v = like.new_empty(shape), like.new_empty(shape)
+            rc = self.be._lib.barq_rocm_paged_read(self.be.h, self.b, layer, k.data_ptr(), v.data_ptr(), mem)
+        if rc:
+            L.check(rc)
         if sync and mem == L.MEM_DEVICE:
             self.be.sync()
         return k, v
@@ -128,16 +132,18 @@ class PagedBatch:
         out_type Q8_K the rows' blocks, uint8 [n_tokens, n_head*head_dim/256 * 292]."""
         c, t = self.cache, self.n_tokens
         width = self.n_head * c.head_dim
-        _check_f32("paged_attention", "q", q, t * width)
+        at = _f32_at("paged_attention", "q", q, t * width)
         if out is not None and not isinstance(out, int):
             if out_type == L.F32:
-                _check_f32("paged_attention", "out", out, t * width)
+                _f32_at("paged_attention", "out", out, t * width)
             elif (out.nbytes if isinstance(out, np.ndarray) else out.numel() * out.element_size()) != t * (width // 256 * 292):
                 raise L.BarqError(L.E_DIM, f"paged_attention: out must have {t} rows of {width // 256 * 292} bytes")
         if out is None:
             out = (_empty((t, self.n_head, c.head_dim), q, mem) if out_type == L.F32
                    else _empty((t, width // 256 * 292), q, mem, dtype="uint8"))
-        L.check(self.be._lib.barq_rocm_paged_attention(self.be.h, self.b, layer, _ptr(q), out_type, _ptr(out), mem))
+        rc = self.be._lib.barq_rocm_paged_attention(self.be.h, self.b, layer, at, out_type, _ptr(out), mem)
+        if rc:
+            L.check(rc)
         if sync and mem == L.MEM_DEVICE:
             self.be.sync()
         return out
