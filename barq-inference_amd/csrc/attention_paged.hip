@@ -3,7 +3,8 @@
 // has the formulas and numerics.
 //
 // Bound by the reading of K and V: 32 sequences of up to 8000 positions (8 kv heads of
-// 128 dims, f16), 556 MB, in 104 us, 5.3 TB/s; a 1 GiB copy has 5.2 here.  A workgroup is four
+// 128 dims, f16), 556 MB, in 96 us with the merge, 5.8 TB/s; loads alone, on the same pages and as many workgroups, have 6.5
+// that pass the caches by and 5.9 otherwise.  A workgroup is four
 // waves, each with key steps of its own (every fourth of the item's), so nothing is shared
 // and nothing waits before the end: the pages' layout is the MFMA operands', 16 bytes a
 // lane straight into registers.  A step is 32 positions in f16, 16 in f32: 16 KiB of K and V
@@ -153,7 +154,8 @@ struct Weights {
     }
 };
 
-template <bool H, int HD>
+// ONCE: keys and values that nothing reads again soon pass the caches by.
+template <bool H, int HD, bool ONCE>
 __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2)
 void paged_few_kernel(PagedAttn a, int count) {
     constexpr int STEP = H ? 32 : 16, E = H ? 8 : 4, KT = H ? 2 : 1, NV = HD / 16, NP = 4 * KT;
@@ -170,9 +172,9 @@ void paged_few_kernel(PagedAttn a, int count) {
     const float minus_one = f16_minus_one();
     const PagedSight sight = {a.window, a.n_sink};
     const size_t page_bytes = BLOCK << (a.log_page - 4);   // of one kv head
-    for (int w = blockIdx.x; w < count * a.n_kv; w += gridDim.x) {
+    for (int w = blockIdx.x, at = w / a.n_kv; w < count * a.n_kv;) {
         const int hk = w % a.n_kv;
-        const PagedItem it = paged_item(&a.few[w / a.n_kv]);
+        const PagedItem it = paged_item(&a.few[at]);
         const int p_first = it.past + it.row0 / a.G, p_last = it.past + (it.row0 + it.rows - 1) / a.G;
         float m = -INFINITY, l = 0.0f;
         f32x4 o[NV];
@@ -201,6 +203,9 @@ void paged_few_kernel(PagedAttn a, int count) {
         // One set of registers: K's are free once the scores are there, V's after P V, and take the next step's at once.
         Step<H, HD> st;
         int k_pages = 0;   // bit 0, 1: the first 16 positions of the step in K's registers have a page, the others
+        const auto fetch = [](const uint8_t* p) __attribute__((always_inline)) {
+            return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const u32x4v*>(p)) : *reinterpret_cast<const u32x4v*>(p);
+        };
         const auto load = [&](int j, bool keys) __attribute__((always_inline)) {
             if (j >= steps) return;
             const int at = base_of(j), p0 = __builtin_amdgcn_readlane(id0, j & 63), p1 = H ? __builtin_amdgcn_readlane(id1, j & 63) : -1;
@@ -212,12 +217,12 @@ void paged_few_kernel(PagedAttn a, int count) {
                 for (int t = 0; t < KT; t++) {
                     const int slot = H ? (8 * (i >> 2) + 4 * t + (i & 3)) & 15 : i;
                     #pragma unroll
-                    for (int c = 0; c < Step<H, HD>::NC; c++) st.k[t][c] = *reinterpret_cast<const u32x4v*>(b + ((4 * c + g) * 16 + slot) * 16);
+                    for (int c = 0; c < Step<H, HD>::NC; c++) st.k[t][c] = fetch(b + ((4 * c + g) * 16 + slot) * 16);
                 }
             } else {
                 const uint8_t* b = H && g >= 2 ? b1 : b0;
                 #pragma unroll
-                for (int d = 0; d < NV; d++) st.v[d] = *reinterpret_cast<const u32x4v*>(b + ((H ? g & 1 : g) * HD + 16 * d + i) * 16);
+                for (int d = 0; d < NV; d++) st.v[d] = fetch(b + ((H ? g & 1 : g) * HD + 16 * d + i) * 16);
             }
         };
         if (steps > 0) fetch_ids(0);
@@ -336,6 +341,11 @@ void paged_few_kernel(PagedAttn a, int count) {
             }
         }
         __syncthreads();   // (a next item's states go where this one's are read from)
+        at = it.next;
+        if (at < 0) {
+            w += gridDim.x;
+            at = w / a.n_kv;
+        }
     }
 }
 
@@ -436,10 +446,13 @@ hipError_t paged_attention_launch(const PagedAttn& a, bool f16, int hd, hipStrea
     const bool captured = a.n_tokens < 0;
     const auto grid = [&](int n) { return dim3(captured ? 1024u : (unsigned)n * (unsigned)a.n_kv); };
     if (captured || a.n_few) {
-        #define BARQ_FEW(H, D) \
-            if (f16 == H && hd == D) hipLaunchKernelGGL((paged_few_kernel<H, D>), grid(a.n_few), dim3(64 * NW), 0, s, a, a.n_few);
-        BARQ_FEW(true, 64) BARQ_FEW(true, 128) BARQ_FEW(true, 256)
-        BARQ_FEW(false, 64) BARQ_FEW(false, 128) BARQ_FEW(false, 256)
+        #define BARQ_FEW(H, D, O) \
+            if (f16 == H && hd == D && a.once == O) \
+                hipLaunchKernelGGL((paged_few_kernel<H, D, O>), grid(a.n_few), dim3(64 * NW), 0, s, a, a.n_few);
+        BARQ_FEW(true, 64, false) BARQ_FEW(true, 128, false) BARQ_FEW(true, 256, false)
+        BARQ_FEW(false, 64, false) BARQ_FEW(false, 128, false) BARQ_FEW(false, 256, false)
+        BARQ_FEW(true, 64, true) BARQ_FEW(true, 128, true) BARQ_FEW(true, 256, true)
+        BARQ_FEW(false, 64, true) BARQ_FEW(false, 128, true) BARQ_FEW(false, 256, true)
         #undef BARQ_FEW
     }
     if (captured || a.n_many) {

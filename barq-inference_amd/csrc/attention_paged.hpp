@@ -46,7 +46,7 @@ __device__ __forceinline__ PagedItem paged_item(const PagedItem* p) {
     const int* from = reinterpret_cast<const int*>(p);
     int* to = reinterpret_cast<int*>(&it);
     #pragma unroll
-    for (int i = 0; i < 11; i++) to[i] = __builtin_amdgcn_readfirstlane(from[i]);
+    for (int i = 0; i < 12; i++) to[i] = __builtin_amdgcn_readfirstlane(from[i]);
     return it;
 }
 

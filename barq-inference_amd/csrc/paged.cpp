@@ -386,7 +386,7 @@ int barq_rocm_paged_batch_set(barq_rocm_handle* h, barq_rocm_paged_batch* b, siz
     counts.n_tokens = (int32_t)tokens;
     for (size_t s = 0; s < n_seqs; s++)
         if (q_len[s]) counts.groups += (kv_len[s] - 1) / barq::PAGE_BLOCK - (kv_len[s] - q_len[s]) / barq::PAGE_BLOCK + 1;
-    counts.few = (int32_t)plan.few.size();
+    counts.few = (int32_t)plan.n_few;
     counts.many = (int32_t)plan.many.size();
     counts.merges = (int32_t)plan.merges.size();
     const auto piece = [&](size_t to, size_t bytes) {
@@ -585,7 +585,8 @@ int barq_rocm_paged_attention(barq_rocm_handle* h, barq_rocm_paged_batch* b, siz
     x.merges = reinterpret_cast<const barq::PagedMerge*>(b->mem + b->merges_at);
     x.counts = b->dev_counts();
     x.n_tokens = captured ? -1 : (int)t;
-    x.n_few = (int)b->plan.few.size();
+    x.n_few = (int)b->plan.n_few;
+    x.once = b->plan.once;   // (a hint: a captured call keeps the one of its capture)
     x.n_many = (int)b->plan.many.size();
     x.n_merges = (int)b->plan.merges.size();
     x.merge_span = 128;

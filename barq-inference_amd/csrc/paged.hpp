@@ -37,7 +37,8 @@ struct PagedItem {
                      // tokens that stay visible, then the window
     int32_t v0, v1;  // this item's steps
     int32_t part;    // its first row among the partial states, -1: it writes the output itself
-    int32_t pad[5];
+    int32_t next;    // the item that the same workgroup takes after this one, -1: none (few rows)
+    int32_t pad[4];
 };
 static_assert(sizeof(PagedItem) == 64, "items are fetched as 64 bytes");
 

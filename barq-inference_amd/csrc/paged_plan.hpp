@@ -33,6 +33,11 @@ struct PagedShape {
     int64_t many_from = 129, alone_from = 257, alone_tiles = 256, beside_from = 65;
     int64_t few_target = 512, many_target = 512;    // workgroups that the card holds at once
     int64_t few_least = 4, many_least = 4;          // steps that a split has at least
+    int64_t few_start = 4;        // steps that an item's beginning and end take the time of (2 and 8 measured 1 to 2 % worse)
+    int64_t step_bytes = 16384;   // of K and V in a step of few rows
+    // bytes of K and V that few rows read from which they pass the caches by: 16 sequences' 256 / 192 / 160 / 128 / 96 MB
+    // take 49.9 / 40.0 / 35.2 / 29.3 / 27.0 us so, 53.0 / 42.0 / 36.5 / 27.2 / 22.2 otherwise (the same pages again and again)
+    int64_t once_from = 160 << 20;
     size_t part_rows = 0;         // partial states there is room for, for each kv head
 };
 
@@ -43,6 +48,8 @@ struct PagedSeq {
 struct PagedPlan {
     std::vector<PagedItem> few, many;
     std::vector<PagedMerge> merges;
+    size_t n_few = 0;             // workgroups for few rows: items 0 .. n_few - 1, and what follows each of them
+    bool once = false;            // whether few rows' keys and values are read as passing by
 };
 
 struct PagedLimits {
@@ -123,6 +130,7 @@ inline void paged_shape_for(PagedShape& sh, bool f16, size_t hd) {
     sh.few_step = f16 ? 32 : 16;
     sh.many_step = f16 ? 64 : 32;
     if (!f16) sh.alone_from = sh.many_from;
+    sh.step_bytes = 128 * (int64_t)hd;
     // by the kernels' registers: one, two, three workgroups a CU
     sh.few_target = hd == 256 ? 256 : hd == 128 ? 512 : 768;
     sh.many_target = hd == 256 ? 256 : 512;
@@ -134,11 +142,64 @@ inline size_t paged_part_rows(const PagedShape& sh, size_t max_tokens) {
     return std::min(max_tokens * sh.G * splits, std::max<size_t>(131072 / sh.n_kv, 256));
 }
 
+// Cuts tiles into shares of equal time for `slots` workgroups, one after another through the tiles, so that a workgroup may end
+// one tile and begin the next; an item takes its steps' time and `start` besides.  cut: the workgroups' first items, n of
+// them, then what they go on with; part is the tile's number.  false: no better than `worst`, the longest time without that.
+// Where each tile is cut by itself up to half of the slots may stay empty: 33 / 40 / 48 sequences of 3000, 3000 and 1500
+// positions (8 kv heads, 128 dims, 64 slots) 99 / 104 / 66 us, with shares 73 / 86 / 64.  Tiles that read the same keys are
+// not cut so: side by side one reads them for the others too (eight sequences of 25 tokens 60 us, with shares 99).
+inline bool paged_shares(const std::vector<PagedItem>& tiles, int64_t steps, int64_t slots, int64_t least, int64_t start, int64_t worst,
+                         std::vector<PagedItem>& cut, size_t& n) {
+    std::vector<PagedItem> row;   // the shares one behind the other
+    std::vector<char> first;      // whether an item begins one
+    int64_t share = std::max((steps + start * ((int64_t)tiles.size() + slots) + slots - 1) / slots, start + least);
+    for (bool fits = false; !fits; share += std::max<int64_t>(share / 32, 1)) {
+        if (share * 16 > worst * 15) return false;   // (a sixteenth at least, or it is not worth it)
+        row.clear();
+        first.clear();
+        n = 0;
+        int64_t left = 0;   // of the share
+        for (size_t t = 0; t < tiles.size(); t++) {
+            const int64_t end = tiles[t].v1;
+            for (int64_t v = 0; v < end;) {
+                first.push_back(left < start + least);
+                if (first.back()) {
+                    left = share;
+                    n++;
+                }
+                int64_t take = std::min(end - v, left - start);
+                if (take < end - v) {
+                    take -= take % least;   // (the waves' steps alike)
+                    if (end - v - take < least) take = end - v;
+                }
+                row.push_back(tiles[t]);
+                row.back().v0 = (int32_t)v;
+                row.back().v1 = (int32_t)(v + take);
+                row.back().part = (int32_t)t;
+                v += take;
+                left -= take + start;
+            }
+        }
+        fits = (int64_t)n <= slots;
+    }
+    cut.resize(row.size());
+    size_t head = 0, rest = n, last = 0;
+    for (size_t i = 0; i < row.size(); i++) {
+        const size_t at = first[i] ? head++ : rest++;
+        cut[at] = row[i];
+        if (!first[i]) cut[last].next = (int32_t)at;
+        last = at;
+    }
+    return true;
+}
+
 inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, PagedPlan& p) {
     p.few.clear();
     p.many.clear();
     p.merges.clear();
+    p.n_few = 0;
     int64_t steps[2] = {0, 0}, q0 = 0, small = 0, longest = 0;
+    bool apart = true;   // no two tiles of few rows read the same keys and values
     for (const PagedSeq& s : seqs) {
         longest = std::max(longest, s.q_len * sh.G);
         if (s.q_len * sh.G < sh.alone_from) small += (s.q_len * sh.G + PAGED_FEW_ROWS - 1) / PAGED_FEW_ROWS;
@@ -163,11 +224,14 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
             it.b = (int32_t)low;
             it.v1 = (int32_t)(it.a + (end + unit - 1) / unit - low);
             it.part = -1;
+            it.next = -1;
+            apart &= many || rows <= tile;
             steps[many] += it.v1;
             (many ? p.many : p.few).push_back(it);
         }
         q0 += s.q_len;
     }
+    p.once = apart && steps[0] * sh.n_kv * sh.step_bytes >= sh.once_from;
     size_t part = 0;
     for (int kind = 0; kind < 2; kind++) {
         std::vector<PagedItem>& items = kind ? p.many : p.few;
@@ -187,6 +251,35 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
                 each = std::max(each + 1, std::min(more, each + each / 8));
             }
             std::vector<PagedItem> cut;
+            int64_t longest = 0;
+            for (const PagedItem& it : items) {
+                const int64_t n = (it.v1 + each - 1) / each;
+                longest = std::max(longest, (it.v1 + n - 1) / n);
+            }
+            if (!kind && apart && paged_shares(items, steps[0], target, least, sh.few_start, longest + sh.few_start, cut, p.n_few)) {
+                std::vector<int32_t> n(items.size(), 0);
+                size_t rows = 0;
+                for (const PagedItem& c : cut) n[c.part]++;
+                for (size_t t = 0; t < items.size(); t++) rows += n[t] > 1 ? (size_t)n[t] * items[t].rows : 0;
+                if (rows <= sh.part_rows) {
+                    std::vector<int32_t> at(items.size(), -1);
+                    for (size_t t = 0; t < items.size(); t++) {
+                        if (n[t] < 2) continue;
+                        const PagedItem& it = items[t];
+                        p.merges.push_back({it.q0, it.row0, it.rows, (int32_t)part, n[t], {0, 0, 0}});
+                        at[t] = (int32_t)part;
+                        part += (size_t)n[t] * it.rows;
+                    }
+                    for (PagedItem& c : cut) {
+                        int32_t& to = at[c.part];
+                        c.part = to;
+                        if (to >= 0) to += c.rows;
+                    }
+                    items.swap(cut);
+                    continue;
+                }
+                cut.clear();
+            }
             for (const PagedItem& it : items) {
                 int64_t n = std::max<int64_t>((it.v1 + each - 1) / each, 1);
                 n = std::min<int64_t>(n, (int64_t)((sh.part_rows - part) / (size_t)it.rows));
@@ -210,6 +303,7 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
         std::stable_sort(items.begin(), items.end(), [](const PagedItem& x, const PagedItem& y) {
             return x.v1 - x.v0 > y.v1 - y.v0;
         });
+        if (!kind) p.n_few = items.size();
     }
 }
 

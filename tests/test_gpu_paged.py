@@ -359,6 +359,69 @@ def test_rows_in_q8_k_blocks(be, type_):
         assert np.array_equal(host[0], rows.cpu().numpy()) and np.array_equal(host[1], want.cpu().numpy())
 
 
+# 64 kv heads leave 4 to 12 workgroups a head, fewer than these lengths fill evenly: some end one sequence and begin the next
+UNEVEN = [[(1, n) for n in (700, 650, 600, 720, 690)], [(1, 40), (1, 900), (2, 33), (0, 300), (1, 1), (1, 820), (1, 760)],
+          [(1, 900 + 17 * i) for i in range(8)], [(1, 1500), (1, 1500), (1, 1500)]]
+
+
+@pytest.mark.parametrize("type_", [B.F16, B.F32])
+@pytest.mark.parametrize("hd,window,n_sink", [(64, 0, 0), (128, 0, 0), (256, 0, 0), (128, 500, 40)])
+@pytest.mark.parametrize("seqs", UNEVEN, ids=lambda s: "+".join(f"{q}of{n}" for q, n in s))
+def test_workgroups_that_go_on_with_another_sequence(be, type_, hd, window, n_sink, seqs):
+    c = Case(be, type_, 64, 64, hd, 32, seqs, window, n_sink, layers=1)
+    want, off = c.want()
+    assert_within(c.batch.attention(c.layer, dev(c.q)).cpu().numpy(), want, off)
+
+
+@pytest.mark.parametrize("type_", [B.F16, B.F32])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_more_than_the_caches_keep(be, type_, hd):
+    """Over 160 MB of K and V, which are then read past the caches."""
+    n = (200 << 20) // (64 * hd * (4 if type_ == B.F16 else 8)) // 3
+    c = Case(be, type_, 64, 64, hd, 64, [(1, n), (1, n - 77), (0, 9), (1, n + 30)], layers=1)
+    got = c.batch.attention(c.layer, dev(c.q)).cpu().numpy()
+    want, off = c.want()
+    assert_within(got, want, off)
+
+
+def test_replays_with_other_workgroups(be):
+    """A captured call goes round whatever shares the latest set() made."""
+    import torch
+    c = Case(be, B.F16, 64, 64, 64, 32, UNEVEN[2], layers=1)
+    q = dev(c.q)
+    tables = [(c.new, c.lens), ([1] + [0] * 7, [300] * 8), ([1] * 8, [30] * 7 + [1019]), ([0] * 8, c.lens), ([1, 1, 1] + [0] * 5, [300] * 8)]
+    out = torch.empty(8 * 64 * 64, device="cuda")
+
+    def call():
+        L.check(be._lib.barq_rocm_paged_attention(be.h, c.batch.b, 0, q.data_ptr(), L.F32, out.data_ptr(), L.MEM_DEVICE))
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda.set_stream(stream)
+    be.set_stream(stream.cuda_stream)
+    try:
+        want = []
+        for new, lens in tables:
+            c.batch.set(new, lens, c.table)
+            out.fill_(-7.0)
+            call()
+            torch.cuda.synchronize()
+            want.append(out.clone())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            call()
+        other = torch.randn(1 << 20, device="cuda")
+        for i in (0, 1, 2, 0, 3, 4, 0, 2):
+            c.batch.set(*tables[i], c.table)
+            out.fill_(-7.0)
+            other.mul_(1.0001)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[i]), i
+    finally:
+        torch.cuda.set_stream(torch.cuda.default_stream())
+        be.set_stream(None)
+
+
 @pytest.mark.parametrize("type_", [B.F16, B.F32])
 def test_a_long_cache(be, type_):
     """100000 positions, a few of which matter."""

@@ -40,6 +40,9 @@ static int plan() {
     PagedPlan p;
     paged_plan(sh, seqs, p);
     printf("%d %d %zu %zu %zu %zu\n", sh.few_step, sh.many_step, sh.part_rows, p.few.size(), p.many.size(), p.merges.size());
+    printf("%zu %d", p.n_few, (int)p.once);
+    for (auto& i : p.few) printf(" %d", i.next);
+    printf("\n");
     for (auto* v : {&p.few, &p.many})
         for (auto& i : *v) printf("%d %d %d %d %d %d %d %d %d %d\n", i.q0, i.past, i.kv_len, i.row0, i.rows, i.a, i.b, i.v0, i.v1, i.part);
     for (auto& m : p.merges) printf("%d %d %d %d %d\n", m.q0, m.row0, m.rows, m.part, m.n_split);
@@ -121,8 +124,18 @@ def cover(program, G, n_kv, window, n_sink, f16, hd, seqs):
     lines = [list(map(int, l.split())) for l in program(
         "plan", G, n_kv, window, n_sink, int(f16), hd, tokens, len(seqs), *(x for s in seqs for x in s)).splitlines()]
     few_step, many_step, part_rows, n_few, n_many, n_merges = lines[0]
+    n_groups, once, *nexts = lines.pop(1)
     few, many = lines[1:1 + n_few], lines[1 + n_few:1 + n_few + n_many]
     merges = lines[1 + n_few + n_many:1 + n_few + n_many + n_merges]
+    # every item of few rows belongs to one workgroup, and its chain ends
+    taken = []
+    for i in range(n_groups):
+        while i >= 0:
+            taken.append(i)
+            i = nexts[i]
+    assert sorted(taken) == list(range(n_few))
+    q_of = {sum(q for q, _ in seqs[:s]): q for s, (q, _) in enumerate(seqs) if q}
+    assert once == (sum(i[8] - i[7] for i in few) * n_kv * 128 * hd >= 160 << 20 and all(q_of[i[0]] * G <= 16 for i in few))
     tiles, extra = lines[-1]
     assert n_merges <= tiles and max(n_few, n_many) <= tiles + extra   # what batch_create has room for
     starts = [sum(q for q, _ in seqs[:s]) for s in range(len(seqs))]
@@ -166,6 +179,32 @@ def test_every_row_sees_its_positions_once(program, seqs, window, n_sink):
     G, n_kv = rng.choice([(1, 8), (4, 8), (7, 2), (20, 1), (2, 64)])
     for f16, hd in ((True, 128), (False, 64), (True, 256)):
         cover(program, G, n_kv, window, n_sink, f16, hd, seqs)
+
+
+@pytest.mark.parametrize("lens", [(700, 650, 600, 720, 690), tuple(900 + 17 * i for i in range(8)), (1500,) * 3])
+def test_shares_go_on_from_one_sequence_to_the_next(program, lens):
+    """Some workgroup has two sequences, all have about the same work, and tiles that read the same keys are not cut so."""
+    goes_on = 0
+    for hd, slots in ((64, 12), (128, 8), (256, 4)):
+        for new in (1, 17):
+            cover(program, 1, 64, 0, 0, True, hd, [(new, n) for n in lens])
+            out = program("plan", 1, 64, 0, 0, 1, hd, new * len(lens), len(lens), *(x for n in lens for x in (new, n))).splitlines()
+            n_few, (groups, _, *nexts) = int(out[0].split()[3]), map(int, out[1].split())
+            items = [list(map(int, l.split())) for l in out[2:2 + n_few]]
+            if new == 17:
+                assert groups == n_few
+            elif groups < n_few:
+                goes_on += 1
+                assert groups <= slots
+                load = []
+                for i in range(groups):
+                    load.append(0)
+                    while i >= 0:
+                        load[-1] += items[i][8] - items[i][7] + 4
+                        i = nexts[i]
+                # a share and what a tile's end adds to it, less than four steps; the last may be short
+                assert max(load) <= min(load[:-1]) + 11 + max(load) / 16
+    assert goes_on
 
 
 def test_drawn_steps(program):
