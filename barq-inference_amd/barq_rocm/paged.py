@@ -94,7 +94,8 @@ class PagedBatch:
     def append(self, layer, k, v, q=None, rotary=None, q_norm=None, k_norm=None, eps=1e-5, q_out=None, mem=L.MEM_DEVICE):
         """k, v [n_tokens, n_head_kv*head_dim] into the layer's pages, k normed by
         head (with k_norm) and rotated (with rotary); returns q [n_tokens,
-        n_head*head_dim] likewise, as [n_head, n_tokens, head_dim], or None."""
+        n_head*head_dim] likewise, as [n_head, n_tokens, head_dim], or None.  Enqueued on
+        the backend's stream and not waited for."""
         c, t = self.cache, self.n_tokens
         hd = c.head_dim
         nq, nk, who = t * self.n_head * hd, t * c.n_head_kv * hd, "paged_append"

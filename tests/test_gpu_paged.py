@@ -60,6 +60,7 @@ class Case:
         self.layer = layers - 1
         if self.total:
             self.fill.append(self.layer, dev(self.k), dev(self.v))
+            be.sync()   # (before torch gives their memory to the next tensor)
         self.batch = P.PagedBatch(self.cache, heads, len(seqs), max(sum(self.new), 1), self.table.shape[1], window, n_sink)
         self.batch.set(self.new, self.lens, self.table)
         f16 = type_ == B.F16
@@ -139,6 +140,7 @@ def test_append(be, type_, hd, rot, half, norm, scale, magnitude, start, page, h
     old = rng.standard_normal((2, pages * page, kv, hd)).astype(np.float16).astype(F32)
     for layer in range(2):
         whole.append(layer, dev(old[0]), dev(old[1]))
+        be.sync()
     b.set(new, lens, table)
     q, k, v = (rng.standard_normal((t, n, hd)).astype(F32) for n in (heads, kv, kv))
     wq, wk = ((1 + 0.3 * rng.standard_normal(hd)).astype(F32) for _ in "qk") if norm else (None, None)
@@ -197,6 +199,7 @@ def test_tokens_without_a_page(be):
     b.set([40], [40], [[1, -1, 0]])
     r = A.Rotary(dev(freqs(64)), 64)
     qo = b.append(0, dev(k), dev(v), q=dev(q), rotary=r)
+    be.sync()
     assert_within(qo.cpu().numpy(), norm_turn(q, np.arange(40), freqs(64), 64, False).transpose(1, 0, 2),
                   turn_bound(q, None, 0, 64, False, 1).transpose(1, 0, 2))
     kr, vr = (x.cpu().numpy() for x in b.read(0))
@@ -495,9 +498,11 @@ def test_a_shared_prefix(be):
     k, v = (rng.standard_normal((32, 1, 64)).astype(F32) for _ in "kv")
     b.set([32], [32], [[5, 2]])
     b.append(0, dev(k), dev(v))
+    be.sync()
     k2, v2 = (rng.standard_normal((9, 1, 64)).astype(F32) for _ in "kv")
     b.set([4, 5], [36, 37], [[5, 2, 0], [5, 2, 3]])
     b.append(0, dev(k2), dev(v2))
+    be.sync()
     q = rng.standard_normal((2, 9, 64)).astype(F32)
     seqs = [(m, np.concatenate([k, k2[a:a + m]]).astype(np.float64), np.concatenate([v, v2[a:a + m]]).astype(np.float64), None)
             for m, a in ((4, 0), (5, 4))]
