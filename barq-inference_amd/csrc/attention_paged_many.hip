@@ -218,7 +218,7 @@ void paged_many_kernel(PagedAttn a, int count) {
                 }
             }
             // scores: the next pieces of K are fetched while the products of these run
-            constexpr int KG = HD == 256 ? 2 : 4, GC = NC / KG;   // (four at a time do not fit the registers of 256 dims)
+            constexpr int KG = 4, GC = NC / KG;
             float s[T][16];
             u32x4v kf[2][KG];
             const auto keys = [&](int n, u32x4v (&k)[KG]) __attribute__((always_inline)) {
