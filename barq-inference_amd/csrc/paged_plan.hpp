@@ -4,8 +4,9 @@
 // 16 (the kernel for few rows) or 128 (for many); a tile's rows see the key
 // positions [0, first tokens) and [window's start, last row's position], counted
 // in the kernel's steps.  Where there are fewer tiles than the card has room for,
-// the tiles' steps are split, evenly over all of them, as far as all workgroups
-// find room at once; what the splits leave is merged.
+// the tiles' steps are split, each tile by itself and as far as all workgroups
+// find room at once, or (few rows of different sequences) into even shares through
+// all of them; what the splits leave is merged.
 //
 // Which kernel: a tile of 16 rows reads the keys for itself alone, one of 128 is
 // slow to begin and to end.  One sequence of 32 query heads on 8, 128 dims, 4000 positions
