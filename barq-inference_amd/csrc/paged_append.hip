@@ -39,7 +39,7 @@ __device__ __forceinline__ size_t block_of(int row, int hk, int n_kv, int log_pa
 // head r / 2^s; the workgroups of the same tokens take ROWS of them each in turn.
 __device__ __forceinline__ int log_tokens(int n) { return n < 2 ? 0 : 32 - __builtin_clz(n - 1); }
 
-template <bool H, int HD>
+template <bool H, int HD, bool ODD>
 __global__ __launch_bounds__(256)
 void paged_append_kernel(PagedAppend a, int per, int per_v, int parts) {
     constexpr int LANES = HD / 8, ROWS = 256 / LANES;
@@ -61,7 +61,7 @@ void paged_append_kernel(PagedAppend a, int per, int per_v, int parts) {
             };
             const int step = per / parts * ROWS;
             int r = blockIdx.y / parts * ROWS + sub;
-            TurnRow<HD> ahead[TURN_AHEAD];
+            TurnRow<HD, ODD> ahead[TURN_AHEAD];
             #pragma unroll
             for (int k = 0; k < TURN_AHEAD; k++)
                 if (r + k * step < rows) ahead[k].load(from(r + k * step), d0);
@@ -72,10 +72,10 @@ void paged_append_kernel(PagedAppend a, int per, int per_v, int parts) {
                 #pragma unroll
                 for (int k = 0; k < TURN_AHEAD; k++, r += step) {
                     if (r >= rows) break;
-                    TurnRow<HD> x = ahead[k];
+                    TurnRow<HD, ODD> x = ahead[k];
                     if (r + TURN_AHEAD * step < rows) ahead[k].load(from(r + TURN_AHEAD * step), d0);
                     const int head = r >> log_n, t = r & mask;
-                    x.turn(from(r), d0, head < a.n_q ? a.q_norm : a.k_norm, a.eps, a.rotary, turn[min(t, gr.n - 1)]);
+                    x.turn(d0, head < a.n_q ? a.q_norm : a.k_norm, a.eps, a.rotary, turn[min(t, gr.n - 1)]);
                     if (t >= gr.n) {
                     } else if (head < a.n_q) {
                         float4* out = reinterpret_cast<float4*>(a.q_out + ((size_t)head * n_tokens + gr.t0 + t) * HD + d0);
@@ -175,7 +175,7 @@ void paged_upload_kernel(PagedPieces p) {
 }
 
 // x [seq, heads, HD] -> [heads, seq, HD], normed and rotated; the rows of a workgroup as for the append.
-template <int HD>
+template <int HD, bool ODD>
 __global__ __launch_bounds__(256)
 void norm_rope_kernel(const float* x, float* out, int seq, int heads, int tokens, int start_pos, const float* w, float eps, Rotary rotary) {
     constexpr int LANES = HD / 8, ROWS = 256 / LANES;
@@ -184,7 +184,7 @@ void norm_rope_kernel(const float* x, float* out, int seq, int heads, int tokens
     const int sub = threadIdx.x / LANES, d0 = 8 * (threadIdx.x % LANES), step = gridDim.y * ROWS;
     const auto from = [&](int r) { return x + ((size_t)(t0 + min(r & mask, n - 1)) * heads + (r >> log_n)) * HD; };
     int r = blockIdx.y * ROWS + sub;
-    TurnRow<HD> ahead[TURN_AHEAD];
+    TurnRow<HD, ODD> ahead[TURN_AHEAD];
     #pragma unroll
     for (int k = 0; k < TURN_AHEAD; k++)
         if (r + k * step < rows) ahead[k].load(from(r + k * step), d0);
@@ -194,10 +194,10 @@ void norm_rope_kernel(const float* x, float* out, int seq, int heads, int tokens
         #pragma unroll
         for (int k = 0; k < TURN_AHEAD; k++, r += step) {
             if (r >= rows) break;
-            TurnRow<HD> y = ahead[k];
+            TurnRow<HD, ODD> y = ahead[k];
             if (r + TURN_AHEAD * step < rows) ahead[k].load(from(r + TURN_AHEAD * step), d0);
             const int t = r & mask;
-            y.turn(from(r), d0, w, eps, rotary, turn[min(t, n - 1)]);
+            y.turn(d0, w, eps, rotary, turn[min(t, n - 1)]);
             if (t < n) {
                 float4* o = reinterpret_cast<float4*>(out + ((size_t)(r >> log_n) * seq + t0 + t) * HD + d0);
                 o[0] = make_float4(y.x[0], y.x[1], y.x[2], y.x[3]);
@@ -226,9 +226,14 @@ hipError_t paged_append_launch(const PagedAppend& a, bool f16, size_t hd, hipStr
     const unsigned per = (shares(groups, (heads * most + rows - 1) / rows) + parts - 1) / parts * parts;
     const unsigned per_v = shares(groups, ((size_t)a.n_kv * (f16 ? 2 : 4) * hd + 255) / 256);
     const dim3 g((unsigned)groups, per + per_v);
-    #define BARQ_APPEND(H, D) if (f16 == H && hd == D) hipLaunchKernelGGL((paged_append_kernel<H, D>), g, dim3(256), 0, s, a, (int)per, (int)per_v, parts);
-    BARQ_APPEND(true, 64) BARQ_APPEND(true, 128) BARQ_APPEND(true, 256)
-    BARQ_APPEND(false, 64) BARQ_APPEND(false, 128) BARQ_APPEND(false, 256)
+    const bool odd = rotary_odd(a.rotary);
+    #define BARQ_APPEND(H, D, O) \
+        if (f16 == H && hd == D && odd == O) \
+            hipLaunchKernelGGL((paged_append_kernel<H, D, O>), g, dim3(256), 0, s, a, (int)per, (int)per_v, parts);
+    BARQ_APPEND(true, 64, false) BARQ_APPEND(true, 128, false) BARQ_APPEND(true, 256, false)
+    BARQ_APPEND(false, 64, false) BARQ_APPEND(false, 128, false) BARQ_APPEND(false, 256, false)
+    BARQ_APPEND(true, 64, true) BARQ_APPEND(true, 128, true) BARQ_APPEND(true, 256, true)
+    BARQ_APPEND(false, 64, true) BARQ_APPEND(false, 128, true) BARQ_APPEND(false, 256, true)
     #undef BARQ_APPEND
     return hipGetLastError();
 }
@@ -262,9 +267,11 @@ hipError_t norm_rope_launch(const float* x, float* out, size_t seq, size_t heads
     while (tokens > 1 && (seq + tokens - 1) / tokens < TURN_WORKGROUPS / 2) tokens /= 2;
     const size_t groups = (seq + tokens - 1) / tokens, rows = 256 / (hd / 8);
     const dim3 g((unsigned)groups, shares(groups, (heads * tokens + rows - 1) / rows));
-    #define BARQ_TURN(D) \
-        if (hd == D) hipLaunchKernelGGL(norm_rope_kernel<D>, g, dim3(256), 0, s, x, out, (int)seq, (int)heads, (int)tokens, (int)start_pos, w, eps, r);
-    BARQ_TURN(64) BARQ_TURN(128) BARQ_TURN(256)
+    const bool odd = rotary_odd(r);
+    #define BARQ_TURN(D, O) \
+        if (hd == D && odd == O) hipLaunchKernelGGL((norm_rope_kernel<D, O>), g, dim3(256), 0, s, x, out, (int)seq, (int)heads, (int)tokens, (int)start_pos, w, eps, r);
+    BARQ_TURN(64, false) BARQ_TURN(128, false) BARQ_TURN(256, false)
+    BARQ_TURN(64, true) BARQ_TURN(128, true) BARQ_TURN(256, true)
     #undef BARQ_TURN
     return hipGetLastError();
 }

@@ -96,6 +96,12 @@ ROT = [  # hd, rot, half, norm, freq_scale, magnitude, start
     (256, 64, False, False, 1.0, 1.0, 9),
     (128, 2, True, True, 1.0, 1.0, 5),
     (64, 0, True, True, 1.0, 1.0, 3),
+    # halves that end within a lane's eight dims
+    (64, 62, True, True, 1.0, 1.0, 500),
+    (128, 126, True, False, 1.0, 1.1, 20000),
+    (256, 130, True, True, 0.5, 1.0, 12345),
+    (128, 10, True, True, 1.0, 1.0, 70),
+    (256, 232, True, False, 1.0, 1.0, 33),
 ]
 
 
