@@ -20,12 +20,12 @@
 // that one f16 value a weight would have at 2^-12.  The MFMA's f32 sums are not rounded to
 // nearest, so each step's start from zero and join O in one fma.
 // Over an f32 cache few rows take the f32 MFMA (they are bound by the reading all the
-// same), many rows six products of bf16 parts: within 2^-23 of |x y| whatever the values (those beyond
-// 3.38e38 read as NaN, for bf16 rounds them to infinity).
+// same), many rows six products of bf16 parts: within 2^-23 of |x y| whatever the values (those from
+// 3.3961e38 on read as NaN where they are seen, for bf16 rounds them to infinity).
 //
 // V in unseen places: a weight of zero keeps finite values out, not NaN.  Steps
-// that some row does not see all of replace what is not finite by zero, and put
-// NaN where a row does see one.
+// that some row does not see all of replace what is not finite (or has bf16 parts that
+// are not) by zero, and put NaN where a row does see one.
 #pragma once
 #include "common.hpp"
 #include "f16_split.hpp"

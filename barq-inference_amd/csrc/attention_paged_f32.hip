@@ -46,6 +46,10 @@ __device__ __forceinline__ void split3(const float (&x)[8], u32x4v (&p)[PARTS]) 
         for (int k = 0; k < PARTS; k++) p[k][u] = w[k];
     }
 }
+// What split3 makes infinite or NaN: NaN, infinities, and finite values that round to bf16's infinity.  As a mark in bit 31
+// (other bits say nothing), as a mask.
+__device__ __forceinline__ uint32_t wild_mark(uint32_t x) { return (x & 0x7FFFFFFFu) + 0x00808000u; }
+__device__ __forceinline__ uint32_t wild(uint32_t x) { return (x & 0x7FFFFFFFu) >= 0x7F7F8000u ? 0xFFFFFFFFu : 0u; }
 __device__ __forceinline__ f32x16 product(u32x4v a, u32x4v b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
 }
@@ -143,15 +147,15 @@ void paged_many_f32_kernel(PagedAttn a, int count) {
                 for (int b = 0; b < NB; b++) m &= (have >> b) & 1 ? ~0u : ~(0xFFFFu << (16 * b));
                 return m >> (4 * h);
             };
-            // Where some row of the workgroup does not see all of the step: what is not finite in V becomes zero, after it has
-            // been put as NaN into the dims of the rows that see it.
+            // Where some row of the workgroup does not see all of the step: what has no finite parts in V becomes zero, after it
+            // has been put as NaN into the dims of the rows that see it (a weight of zero times infinity is not zero).
             const bool edge = have != (1 << NB) - 1 || !sight.all(base, STEP, all_first, all_last);
             if (edge) {
                 uint32_t any = 0;
                 for (int u = lane; u < RAW / 16; u += 64) {
                     const u32x4v x = reinterpret_cast<const u32x4v*>(raw_v)[u];
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) any |= f32_bad_mark(x[e]);
+                    for (int e = 0; e < 4; e++) any |= wild_mark(x[e]);
                 }
                 if (__any((any >> 31) != 0)) {
                     const uint32_t seen = seen_by();
@@ -163,7 +167,7 @@ void paged_many_f32_kernel(PagedAttn a, int count) {
                             const u32x4v v = *reinterpret_cast<const u32x4v*>(raw_v + (g / 2) * BLOCK + ((2 * (g & 1) + h) * HD + 32 * d + i) * 16);
                             #pragma unroll
                             for (int e = 0; e < 4; e++)
-                                n = __builtin_amdgcn_mfma_f32_32x32x2f32(f32_bad(v[e]) ? 1.0f : 0.0f, (seen >> (8 * g + e)) & 1 ? 1.0f : 0.0f, n, 0, 0, 0);
+                                n = __builtin_amdgcn_mfma_f32_32x32x2f32(wild(v[e]) ? 1.0f : 0.0f, (seen >> (8 * g + e)) & 1 ? 1.0f : 0.0f, n, 0, 0, 0);
                         }
                         #pragma unroll
                         for (int r = 0; r < 16; r++) o[d][r] = n[r] > 0.0f ? NAN : o[d][r];
@@ -187,7 +191,7 @@ void paged_many_f32_kernel(PagedAttn a, int count) {
                 u32x4v y0 = *reinterpret_cast<const u32x4v*>(from), y1 = *reinterpret_cast<const u32x4v*>(from + 2 * HD * 16);
                 if (edge) {
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) y0[e] &= ~f32_bad(y0[e]), y1[e] &= ~f32_bad(y1[e]);
+                    for (int e = 0; e < 4; e++) y0[e] &= ~wild(y0[e]), y1[e] &= ~wild(y1[e]);
                 }
                 const f32x4 x0 = __builtin_bit_cast(f32x4, y0), x1 = __builtin_bit_cast(f32x4, y1);
                 const float y[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
