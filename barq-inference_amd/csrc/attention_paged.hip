@@ -181,6 +181,7 @@ void paged_few_kernel(PagedAttn a, int count) {
         #pragma unroll
         for (int d = 0; d < NV; d++) o[d] = f32x4{};
         const int32_t* table = a.table + it.table;
+        const float unit = paged_weight_unit(it.kv_len);
         const int steps = (it.v1 - it.v0 - wave + NW - 1) / NW;   // this wave's (none: 0 or less)
         const auto base_of = [&](int j) {
             const int v = it.v0 + wave + NW * j;
@@ -283,7 +284,7 @@ void paged_few_kernel(PagedAttn a, int count) {
             float sum = 0.0f;
             #pragma unroll
             for (int e = 0; e < NP; e++) {
-                s[e] = paged_exp2(H ? (s[e] - ref) + 15.0f : s[e] - ref);   // (in this order: at most 15 whatever the scores)
+                s[e] = H ? paged_exp2((s[e] - ref) + 15.0f) : paged_exp2(s[e] - ref) * unit;   // (in this order: at most 15 whatever the scores)
                 sum += s[e];
             }
             l = __builtin_fmaf(l, alpha, sum);

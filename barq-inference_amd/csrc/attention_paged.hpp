@@ -38,6 +38,11 @@ namespace barq {
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// What the weights over an f32 cache of n positions (1 or more) are multiplied by: below 1 / n, a power of two.  Their sum is then below
+// 1, so that no sum of weights times V, of a step, an item or a merge, is larger than the largest |V| (the division by the weights' sum
+// takes it out again, exactly); products below 2^-126 lose bits, of V below 2^-126 n.
+__device__ __forceinline__ float paged_weight_unit(int n) { return __builtin_bit_cast(float, (uint32_t)(95 + __builtin_clz(n)) << 23); }
+
 __device__ __forceinline__ float paged_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // An item, in scalar registers.

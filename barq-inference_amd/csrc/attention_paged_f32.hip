@@ -77,6 +77,7 @@ void paged_many_f32_kernel(PagedAttn a, int count) {
         const PagedItem it = paged_item(&a.many[w / a.n_kv]);
         const int32_t* table = a.table + it.table;
         const int steps = it.v1 - it.v0;
+        const float unit = paged_weight_unit(it.kv_len);
         const auto base_of = [&](int j) {
             const int v = it.v0 + j;
             return (v < it.a ? v : v - it.a + it.b) * STEP;
@@ -242,7 +243,7 @@ void paged_many_f32_kernel(PagedAttn a, int count) {
                 float y[8];
                 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    y[e] = paged_exp2(s[8 * u + e] - ref);
+                    y[e] = paged_exp2(s[8 * u + e] - ref) * unit;
                     sum += y[e];
                 }
                 split3(y, pw[u]);

@@ -612,7 +612,8 @@ int barq_rocm_rope_frequencies(int scaling, size_t rot_dim, double base, double 
  * multiple of 256; the bytes barq_rocm_quantize_act writes for them).  A query that sees no position
  * gives zeros.  Softmax statistics and sums are f32.  Over an f16 cache a query element counts to 2^-23 of itself or 2^-52 of
  * its row's largest, a weight to 2^-22 of itself or 2^-40 of its row's largest, whichever is more.  Over an
- * f32 cache products count to 2^-23 of themselves; of sequences with more than 64 rows (new tokens x n_head /
+ * f32 cache products count to 2^-23 of themselves (less where V is below 2^-126 kv_len) and no sum on the way is larger than the largest
+ * |V| that a query sees; of sequences with more than 64 rows (new tokens x n_head /
  * n_head_kv), q, K and V from 3.39e38 on may count as NaN for the queries that see them.
  * Device buffers: q, q_out, k, v, x and norm_rope's out 16-byte aligned, the others 4-byte. */
 int barq_rocm_norm_rope(barq_rocm_handle* h, const float* x, size_t seq_len, size_t n_heads, size_t head_dim,
