@@ -212,7 +212,11 @@ class Pages:
         return new
 
     def drop_behind(self, seq: Sequence, window: int, n_sink: int = 0):
-        """Give back the pages that no query to come sees."""
+        """Give back the pages that no query to come sees (window and n_sink as a batch has them; without a window, 0, none)."""
+        if window < 0 or n_sink < 0:
+            raise L.BarqError(L.E_DIM, f"pages: a window of {window} positions, {n_sink} first ones")
+        if window == 0:
+            return
         first = -(-n_sink // self.page_size)
         for i in range(first, max(seq.length - window + 1, 0) // self.page_size):
             if seq.pages[i] >= 0:

@@ -212,3 +212,27 @@ def test_refusals_before_any_device():
     assert norm(None, 16, 1 << 24, 1, 64, 0, None, 0.0, None, 16, L.MEM_DEVICE) == L.E_DIM
     assert norm(None, 16, 2, 1 << 40, 64, 0, None, 0.0, None, 16, L.MEM_DEVICE) == L.E_DIM
     assert norm(None, None, 0, 1, 64, 0, None, 0.0, None, None, L.MEM_DEVICE) == L.OK
+
+
+@pytest.mark.parametrize("length", [0, 1, 15, 16, 31, 40])
+@pytest.mark.parametrize("n_sink", [0, 1, 40])
+def test_without_a_window_nothing_is_given_back(length, n_sink):
+    """A window of 0 is none, as for a batch."""
+    p, s = Pages(8, 16), Sequence()
+    p.grow(s, length)
+    was = list(s.pages)
+    p.drop_behind(s, 0, n_sink)
+    assert s.pages == was and p.free() == 8 - len(was) and s.gone == (0, 0)
+    p.grow(s, 1)
+    p.shrink(s, 0)
+    assert p.free() == 8
+
+
+@pytest.mark.parametrize("window,n_sink", [(-1, 0), (-100, 4), (5, -1), (0, -1), (16, -40)])
+def test_windows_below_nothing_are_refused(window, n_sink):
+    p, s = Pages(8, 16), Sequence()
+    p.grow(s, 100)
+    was = list(s.pages)
+    with pytest.raises(L.BarqError) as e:
+        p.drop_behind(s, window, n_sink)
+    assert e.value.code == L.E_DIM and s.pages == was and p.free() == 1 and s.gone == (0, 0)
