@@ -47,9 +47,21 @@ def _check_mass(who, n_head_kv, *arrays):
             raise L.BarqError(L.E_INVALID, f"{who}: mass must be contiguous float32")
 
 
-def _f32_at(who, what, t, n):
-    """Address of n float32 values, side by side in memory (a raw address or nothing is taken as it is)."""
-    if t.__class__ is _TENSOR and t.dtype is _FLOAT and t.numel() == n and t.is_contiguous():
+def _place(be: Backend, mem):
+    """Where a call's buffers are: a device's number, -1 for host memory."""
+    return be.device if mem == L.MEM_DEVICE else -1
+
+
+def _check_place(who, what, t, place):
+    at = -1 if isinstance(t, np.ndarray) else t.get_device()
+    if at != place:
+        where = ["host memory" if x < 0 else f"device {x}" for x in (place, at)]
+        raise L.BarqError(L.E_INVALID, f"{who}: {what} must be in {where[0]}, it is in {where[1]}")
+
+
+def _f32_at(who, what, t, n, place):
+    """Address of n float32 values, side by side in the memory of `place` (a raw address or nothing is taken as it is)."""
+    if t.__class__ is _TENSOR and t.dtype is _FLOAT and t.numel() == n and t.get_device() == place and t.is_contiguous():
         return t.data_ptr()   # (the usual case first: a call for one token is bound by the host)
     if t is None or isinstance(t, int):
         return t
@@ -58,6 +70,7 @@ def _f32_at(who, what, t, n):
         raise L.BarqError(L.E_DIM, f"{who}: {what} has {t.size if host else t.numel()} values, {n} are wanted")
     if not str(t.dtype).endswith("float32") or not (t.flags.c_contiguous if host else t.is_contiguous()):
         raise L.BarqError(L.E_INVALID, f"{who}: {what} must be contiguous float32")
+    _check_place(who, what, t, place)
     if not host:
         _know_torch()
     return _ptr(t)
@@ -87,15 +100,22 @@ def transpose_heads(be: Backend, x, seq_len, n_heads, head_dim, mem=L.MEM_DEVICE
 class Rotary:
     """The rotation of a head's first rot_dim dims (barq_rocm_rotary): pair i
     turns by position * freq_scale * inv_freq[i].  inv_freq lives where the calls'
-    `mem` says."""
+    `mem` says (they refuse another one)."""
 
     def __init__(self, inv_freq, rot_dim, layout=ROPE_INTERLEAVED, freq_scale=1.0, magnitude=1.0):
         if tuple(inv_freq.shape) != (rot_dim // 2,) or not str(inv_freq.dtype).endswith("float32"):
             raise L.BarqError(L.E_DIM, f"Rotary: inv_freq must be {rot_dim // 2} float32 values")
-        at = _f32_at("Rotary", "inv_freq", inv_freq, rot_dim // 2)
+        self.place = -1 if isinstance(inv_freq, np.ndarray) else inv_freq.get_device()
+        at = _f32_at("Rotary", "inv_freq", inv_freq, rot_dim // 2, self.place)
         self.inv_freq = inv_freq   # (kept alive: the argument below has its address)
         self.arg = L.RotaryArg(rot_dim, layout, freq_scale, magnitude, at or None)
         self.ref = ctypes.byref(self.arg)
+
+    def ref_in(self, who, place):
+        """The argument for a call on buffers there."""
+        if self.place != place and self.arg.rot_dim:
+            _check_place(who, "inv_freq", self.inv_freq, place)
+        return self.ref
 
     @classmethod
     def scaled(cls, rot_dim, base, layout=ROPE_INTERLEAVED, scaling=L.ROPE_PLAIN, factor=1.0, trained=0.0, fast=32.0, slow=1.0,
@@ -119,12 +139,13 @@ def norm_rope(be: Backend, x, seq_len, n_heads, head_dim, start_pos, rotary=None
               sync=True, out=None):
     """RMSNorm of each head (with norm) and the rotation, in one pass: x
     [seq, n_heads*head_dim] -> [n_heads, seq, head_dim]."""
-    n = seq_len * n_heads * head_dim
-    at, norm_at = _f32_at("norm_rope", "x", x, n), _f32_at("norm_rope", "norm", norm, head_dim)
+    n, place = seq_len * n_heads * head_dim, _place(be, mem)
+    at, norm_at = _f32_at("norm_rope", "x", x, n, place), _f32_at("norm_rope", "norm", norm, head_dim, place)
     if out is None:
         out = _empty((n_heads, seq_len, head_dim), x, mem)
     rc = be._lib.barq_rocm_norm_rope(be.h, at, seq_len, n_heads, head_dim, start_pos, norm_at, eps,
-                                     None if rotary is None else rotary.ref, _f32_at("norm_rope", "out", out, n), mem)
+                                     None if rotary is None else rotary.ref_in("norm_rope", place),
+                                     _f32_at("norm_rope", "out", out, n, place), mem)
     if rc:
         L.check(rc)
     if sync and mem == L.MEM_DEVICE:

@@ -10,7 +10,7 @@ import ctypes
 import numpy as np
 
 from . import _lib as L
-from .attention import _empty, _f32_at
+from .attention import _check_place, _empty, _f32_at, _place
 from .backend import Backend, _ptr
 
 
@@ -98,13 +98,13 @@ class PagedBatch:
         the backend's stream and not waited for."""
         c, t = self.cache, self.n_tokens
         hd = c.head_dim
-        nq, nk, who = t * self.n_head * hd, t * c.n_head_kv * hd, "paged_append"
+        nq, nk, who, place = t * self.n_head * hd, t * c.n_head_kv * hd, "paged_append", _place(self.be, mem)
         if q is not None and q_out is None:
             q_out = _empty((self.n_head, t, hd), q, mem)
         rc = self.be._lib.barq_rocm_paged_append(
-            self.be.h, self.b, layer, _f32_at(who, "q", q, nq), _f32_at(who, "q_out", q_out, nq), _f32_at(who, "k", k, nk),
-            _f32_at(who, "v", v, nk), _f32_at(who, "q_norm", q_norm, hd), _f32_at(who, "k_norm", k_norm, hd), eps,
-            None if rotary is None else rotary.ref, mem)
+            self.be.h, self.b, layer, _f32_at(who, "q", q, nq, place), _f32_at(who, "q_out", q_out, nq, place),
+            _f32_at(who, "k", k, nk, place), _f32_at(who, "v", v, nk, place), _f32_at(who, "q_norm", q_norm, hd, place),
+            _f32_at(who, "k_norm", k_norm, hd, place), eps, None if rotary is None else rotary.ref_in(who, place), mem)
         if rc:
             L.check(rc)
         return q_out
@@ -132,13 +132,15 @@ class PagedBatch:
         """q [n_head, n_tokens, head_dim] -> [n_tokens, n_head, head_dim], or with
         out_type Q8_K the rows' blocks, uint8 [n_tokens, n_head*head_dim/256 * 292]."""
         c, t = self.cache, self.n_tokens
-        width = self.n_head * c.head_dim
-        at = _f32_at("paged_attention", "q", q, t * width)
+        width, place = self.n_head * c.head_dim, _place(self.be, mem)
+        at = _f32_at("paged_attention", "q", q, t * width, place)
         if out is not None and not isinstance(out, int):
             if out_type == L.F32:
-                _f32_at("paged_attention", "out", out, t * width)
+                _f32_at("paged_attention", "out", out, t * width, place)
             elif (out.nbytes if isinstance(out, np.ndarray) else out.numel() * out.element_size()) != t * (width // 256 * 292):
                 raise L.BarqError(L.E_DIM, f"paged_attention: out must have {t} rows of {width // 256 * 292} bytes")
+            else:
+                _check_place("paged_attention", "out", out, place)
         if out is None:
             out = (_empty((t, self.n_head, c.head_dim), q, mem) if out_type == L.F32
                    else _empty((t, width // 256 * 292), q, mem, dtype="uint8"))

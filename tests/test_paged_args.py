@@ -1,0 +1,81 @@
+"""What the Python side of the paged cache and norm_rope refuses before the
+library is called: host code, no GPU."""
+from types import SimpleNamespace
+
+import numpy as np
+import pytest
+import torch
+
+from barq_rocm import _lib as L
+from barq_rocm import attention as A
+from barq_rocm.paged import PagedBatch
+
+
+class NoCalls:
+    def __getattr__(self, name):
+        def call(*args):
+            raise AssertionError(f"{name} was called")
+        return call
+
+
+BE = SimpleNamespace(h=None, device=0, _lib=NoCalls(), sync=lambda: None)
+
+
+def batch(n_tokens=3, n_head=4, n_head_kv=2, head_dim=64):
+    b = PagedBatch.__new__(PagedBatch)
+    b.be, b.b, b.n_head, b.n_tokens = BE, None, n_head, n_tokens
+    b.cache = SimpleNamespace(n_head_kv=n_head_kv, head_dim=head_dim, type=L.F16)
+    return b
+
+
+def refused(code, f, *a, **k):
+    with pytest.raises(L.BarqError) as e:
+        f(*a, **k)
+    assert e.value.code == code, e.value
+
+
+HOST = [lambda *s: np.zeros(s, np.float32), lambda *s: torch.zeros(s)]
+
+
+@pytest.mark.parametrize("host", HOST, ids=["numpy", "torch"])
+def test_host_memory_in_device_calls(host):
+    """16 stands for an address on the device, which is taken as it is."""
+    b, kv, q, hd = batch(), host(3, 2, 64), host(3, 4, 64), host(64)
+    for args in (dict(k=kv, v=16), dict(k=16, v=kv), dict(k=16, v=16, q=q, q_out=16), dict(k=16, v=16, q=16, q_out=q),
+                 dict(k=16, v=16, q=16, q_out=16, q_norm=hd), dict(k=16, v=16, k_norm=hd),
+                 dict(k=16, v=16, rotary=A.Rotary(host(32), 64))):
+        refused(L.E_INVALID, b.append, 0, **args)
+    refused(L.E_INVALID, b.attention, 0, q)
+    refused(L.E_INVALID, b.attention, 0, 16, out=q)
+    for out in (np.zeros((3, 292), np.uint8), torch.zeros((3, 292), dtype=torch.uint8)):
+        refused(L.E_INVALID, b.attention, 0, 16, out_type=L.Q8_K, out=out)
+    for args in (dict(x=q, out=16), dict(x=16, out=q), dict(x=16, out=16, norm=hd), dict(x=16, out=16, rotary=A.Rotary(host(32), 64))):
+        x = args.pop("x")
+        refused(L.E_INVALID, A.norm_rope, BE, x, 3, 4, 64, 0, **args)
+
+
+@pytest.mark.parametrize("host", HOST, ids=["numpy", "torch"])
+def test_host_memory_in_host_calls(host):
+    """It gets as far as the library."""
+    b, kv, q, hd, r = batch(), host(3, 2, 64), host(3, 4, 64), host(64), A.Rotary(host(32), 64)
+    for f in (lambda: b.append(0, kv, kv, q=q, q_out=host(4, 3, 64), rotary=r, q_norm=hd, k_norm=hd, mem=L.MEM_HOST),
+              lambda: b.attention(0, q, out=host(3, 4, 64), mem=L.MEM_HOST),
+              lambda: A.norm_rope(BE, q, 3, 4, 64, 0, r, hd, mem=L.MEM_HOST, out=host(4, 3, 64))):
+        with pytest.raises(AssertionError, match="was called"):
+            f()
+
+
+@pytest.mark.gpu
+def test_device_memory_in_host_calls_and_on_other_devices():
+    b, kv, q, hd = batch(), torch.zeros(3, 2, 64, device="cuda"), torch.zeros(3, 4, 64, device="cuda"), torch.zeros(64, device="cuda")
+    h, r = np.zeros(1000, np.float32), A.Rotary(torch.zeros(32, device="cuda"), 64)
+    other = SimpleNamespace(h=None, device=1, _lib=NoCalls(), sync=lambda: None)
+    for be, mem, at in ((BE, L.MEM_HOST, h.ctypes.data), (other, L.MEM_DEVICE, 16)):
+        b.be = be
+        for args in (dict(k=kv, v=at), dict(k=at, v=kv), dict(k=at, v=at, q=q, q_out=at), dict(k=at, v=at, q=at, q_out=q),
+                     dict(k=at, v=at, k_norm=hd), dict(k=at, v=at, rotary=r)):
+            refused(L.E_INVALID, b.append, 0, mem=mem, **args)
+        refused(L.E_INVALID, b.attention, 0, q, mem=mem)
+        refused(L.E_INVALID, b.attention, 0, at, out=q, mem=mem)
+        refused(L.E_INVALID, A.norm_rope, be, q, 3, 4, 64, 0, mem=mem)
+        refused(L.E_INVALID, A.norm_rope, be, at, 3, 4, 64, 0, rotary=r, out=at, mem=mem)
