@@ -91,7 +91,8 @@ def transpose_heads(be: Backend, x, seq_len, n_heads, head_dim, mem=L.MEM_DEVICE
     """transpose_heads (transformer.rs:598-611)."""
     if out is None:
         out = _empty((n_heads, seq_len, head_dim), x, mem)
-    L.check(be._lib.barq_rocm_transpose_heads(be.h, _ptr(x), seq_len, n_heads, head_dim, _ptr(out), mem))
+    at = _f32_at("transpose_heads", "out", out, seq_len * n_heads * head_dim, _place(be, mem))
+    L.check(be._lib.barq_rocm_transpose_heads(be.h, _ptr(x), seq_len, n_heads, head_dim, at, mem))
     if sync and mem == L.MEM_DEVICE:
         be.sync()
     return out

@@ -139,6 +139,8 @@ class PagedBatch:
                 _f32_at("paged_attention", "out", out, t * width, place)
             elif (out.nbytes if isinstance(out, np.ndarray) else out.numel() * out.element_size()) != t * (width // 256 * 292):
                 raise L.BarqError(L.E_DIM, f"paged_attention: out must have {t} rows of {width // 256 * 292} bytes")
+            elif not (out.flags.c_contiguous if isinstance(out, np.ndarray) else out.is_contiguous()):
+                raise L.BarqError(L.E_INVALID, "paged_attention: out must be contiguous")
             else:
                 _check_place("paged_attention", "out", out, place)
         if out is None:

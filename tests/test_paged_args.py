@@ -79,3 +79,23 @@ def test_device_memory_in_host_calls_and_on_other_devices():
         refused(L.E_INVALID, b.attention, 0, at, out=q, mem=mem)
         refused(L.E_INVALID, A.norm_rope, be, q, 3, 4, 64, 0, mem=mem)
         refused(L.E_INVALID, A.norm_rope, be, at, 3, 4, 64, 0, rotary=r, out=at, mem=mem)
+
+
+def test_outputs_that_are_not_side_by_side():
+    """Their bytes are as many as the call writes, in more memory or in less."""
+    b = batch()
+    b.be = SimpleNamespace(h=None, device=-1, _lib=NoCalls(), sync=lambda: None)   # (so that memory here is what the call wants)
+    for out in (torch.zeros((3, 584), dtype=torch.uint8)[:, ::2], torch.zeros((1, 292), dtype=torch.uint8).expand(3, 292),
+                np.zeros((3, 584), np.uint8)[:, ::2], np.broadcast_to(np.zeros((1, 292), np.uint8), (3, 292))):
+        for mem in (L.MEM_DEVICE, L.MEM_HOST):
+            refused(L.E_INVALID, b.attention, 0, 16, out_type=L.Q8_K, out=out, mem=mem)
+
+
+@pytest.mark.parametrize("host", HOST, ids=["numpy", "torch"])
+def test_outputs_of_transpose_heads(host):
+    for out, code in ((host(4, 3, 63), L.E_DIM), (host(5, 3, 64), L.E_DIM), (host(4, 3, 128)[..., ::2], L.E_INVALID),
+                      (host(4, 3, 64).astype("float64") if isinstance(host(1), np.ndarray) else host(4, 3, 64).double(), L.E_INVALID)):
+        refused(code, A.transpose_heads, BE, host(3, 4, 64), 3, 4, 64, mem=L.MEM_HOST, out=out)
+    refused(L.E_INVALID, A.transpose_heads, BE, 16, 3, 4, 64, out=host(4, 3, 64))
+    with pytest.raises(AssertionError, match="was called"):
+        A.transpose_heads(BE, host(3, 4, 64), 3, 4, 64, mem=L.MEM_HOST, out=host(4, 3, 64))
