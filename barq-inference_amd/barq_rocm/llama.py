@@ -322,7 +322,7 @@ class PagedLlama(DeviceLlama):
             for seq, t in news:
                 self.pages.grow(seq, len(t))
             self.batch.set(q_lens, [s.length for s, _ in news], [s.pages for s, _ in news])
-            ids = np.concatenate([np.asarray(t, np.int32) for _, t in news]) if news else np.empty(0, np.int32)
+            ids = P._int32("PagedLlama.step", "token ids", np.concatenate([np.asarray(t) for _, t in news]) if news else [])
             if len(ids) == 0:
                 return torch.empty((0, self.n_vocab), dtype=torch.float32, device="cuda")
             last = np.cumsum(q_lens)[np.asarray(q_lens) > 0].astype(np.int32) - 1

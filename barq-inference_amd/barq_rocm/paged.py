@@ -14,6 +14,21 @@ from .attention import _check_place, _empty, _f32_at, _place
 from .backend import Backend, _ptr
 
 
+def _int32(who, what, a):
+    """Numbers as int32, side by side; refused where that would make others of them."""
+    x = np.asarray(a)
+    if x.dtype == np.int32:
+        return np.ascontiguousarray(x)
+    try:
+        with np.errstate(invalid="ignore"):
+            y = np.ascontiguousarray(x, dtype=np.int32)
+    except OverflowError:
+        y = None
+    if y is None or not (x == y).all():
+        raise L.BarqError(L.E_INVALID, f"{who}: {what} must be whole numbers of 32 bits")
+    return y
+
+
 class PagedCache:
     """n_pages pages of page_size positions for each layer and kv head; type
     F16 or F32."""
@@ -77,15 +92,15 @@ class PagedBatch:
     def set(self, q_lens, kv_lens, pages):
         """q_lens, kv_lens: one number a sequence; pages: [sequences, pages]
         int32 (or a list of lists of ids), -1 where there is none."""
-        q = np.ascontiguousarray(q_lens, dtype=np.int32)
-        kv = np.ascontiguousarray(kv_lens, dtype=np.int32)
+        who = "paged_batch_set"
+        q, kv = _int32(who, "q_lens", q_lens), _int32(who, "kv_lens", kv_lens)
         if not isinstance(pages, np.ndarray):
-            width = max((len(p) for p in pages), default=0)
-            table = np.full((len(pages), width), -1, np.int32)
-            for row, ids in zip(table, pages):
-                row[:len(ids)] = ids
+            n = np.array([len(p) for p in pages], np.int64)
+            table = np.full((len(n), n.max(initial=0)), -1, np.int32)
+            if table.size:
+                table[np.arange(table.shape[1]) < n[:, None]] = _int32(who, "pages", np.concatenate([np.asarray(p) for p in pages]))
             pages = table
-        pages = np.ascontiguousarray(pages, dtype=np.int32)
+        pages = _int32(who, "pages", pages)
         if q.ndim != 1 or q.shape != kv.shape or pages.ndim != 2 or len(pages) != len(q):
             raise L.BarqError(L.E_DIM, f"paged_batch_set: q_lens {q.shape}, kv_lens {kv.shape}, pages {pages.shape}")
         L.check(self.be._lib.barq_rocm_paged_batch_set(self.be.h, self.b, len(q), _ptr(q), _ptr(kv), _ptr(pages), pages.shape[1]))

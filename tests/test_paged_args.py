@@ -1,5 +1,6 @@
 """What the Python side of the paged cache and norm_rope refuses before the
 library is called: host code, no GPU."""
+import ctypes
 from types import SimpleNamespace
 
 import numpy as np
@@ -99,3 +100,46 @@ def test_outputs_of_transpose_heads(host):
     refused(L.E_INVALID, A.transpose_heads, BE, 16, 3, 4, 64, out=host(4, 3, 64))
     with pytest.raises(AssertionError, match="was called"):
         A.transpose_heads(BE, host(3, 4, 64), 3, 4, 64, mem=L.MEM_HOST, out=host(4, 3, 64))
+
+
+@pytest.mark.parametrize("arrays", [
+    (np.array([2 ** 32 + 1]), [20], [[1, 2]]), ([1], np.array([2 ** 32 + 20]), [[1, 2]]), ([1], [20], np.array([[1, 2 ** 32 + 2]])),
+    ([1], [20], [np.array([1, 2 ** 32 + 2])]), ([1], [20], [[1, 2 ** 32 + 2]]), ([1], [20], [[1, 2 ** 64]]), ([2 ** 31], [20], [[1, 2]]), ([1], [20], np.array([[1, 2 ** 31]], np.uint32)),
+    ([1.5], [20], [[1, 2]]), ([1], [20], np.array([[1, 2.25]])), ([1], [float("nan")], [[1, 2]]), ([1], [20], [[1, 2.5]])])
+def test_numbers_that_are_no_int32(arrays):
+    """They were taken for others: 2^32 + 2 for 2, 1.5 for 1."""
+    b = batch()
+    refused(L.E_INVALID, b.set, *arrays)
+    assert b.n_tokens == 3
+
+
+def test_numbers_of_other_types():
+    """What is an int32 in value gets as far as the library, as that."""
+    b, got = batch(), []
+
+    class Takes:
+        @staticmethod
+        def barq_rocm_paged_batch_set(h, batch, n, q, kv, pages, stride):
+            at = [np.ctypeslib.as_array((ctypes.c_int32 * k).from_address(p)).tolist() for p, k in ((q, n), (kv, n), (pages, n * stride)) if k]
+            got.append((n, stride, at))
+            return 0
+    b.be = SimpleNamespace(h=None, device=0, _lib=Takes, sync=lambda: None)
+    for t in (np.int32, np.int64, np.uint8, np.float64):
+        b.set(np.array([1, 3], t), np.array([4, 20], t), np.array([[5, 7], [9, 3]], t))
+        assert got.pop() == (2, 2, [[1, 3], [4, 20], [5, 7, 9, 3]]) and b.n_tokens == 4
+    b.set([1, 3], (4, 20), [[5], np.array([9, -1])])
+    assert got.pop() == (2, 2, [[1, 3], [4, 20], [5, -1, 9, -1]])
+    b.set([], [], [])
+    assert got.pop() == (0, 0, []) and b.n_tokens == 0
+
+
+def test_token_ids_that_are_no_int32():
+    """A step fails with them, and its sequences are as before."""
+    from barq_rocm.llama import PagedLlama
+    from barq_rocm.paged import Pages, Sequence
+    m, s = PagedLlama.__new__(PagedLlama), Sequence()
+    m.be, m.cfg, m.pages = BE, SimpleNamespace(window=0, n_sink=0), Pages(4, 16)
+    m.batch = SimpleNamespace(set=lambda *a: None)
+    for ids in (np.array([5, 2 ** 32 + 5]), [1.5], np.array([2 ** 31]), [2 ** 32 + 5]):
+        refused(L.E_INVALID, m.step, [(s, [1, 2]), (s, ids)])
+        assert s.length == 0 and m.pages.free() == 4
