@@ -194,3 +194,20 @@ def test_windows_are_for_pages(be, weights):
         DeviceLlama(be, c, table(weights, "window"), A.KVCache(be, 64, 2, c.n_head_kv, c.head_dim))
     with pytest.raises(B.BarqError):
         PagedLlama(be, c, table(weights, "window"), P.PagedCache(be, 4, 16, 3, c.n_head_kv, c.head_dim), 1, 8, 4)
+
+
+def test_a_model_without_head_norms_is_not_asked_for_them_again(be, weights):
+    """A lookup in every layer of every token costs the host more than a launch saves."""
+    import torch
+    for name, asked in (("plain", 0), ("norms", 4)):
+        c, names, find = CONFIGS[name], [], table(weights, name)
+
+        def get(n):
+            names.append(n)
+            return find(n)
+        m = DeviceLlama(be, c, get, A.KVCache(be, 8, 2, c.n_head_kv, c.head_dim))
+        names.clear()
+        for pos in range(2):
+            m.forward(torch.tensor([pos], dtype=torch.int32, device="cuda"), pos)
+        be.sync()
+        assert sum("_norm.weight" in n and ".attn_q" in n or ".attn_k_norm" in n for n in names) == 2 * asked
