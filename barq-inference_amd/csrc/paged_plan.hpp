@@ -137,10 +137,11 @@ inline void paged_shape_for(PagedShape& sh, bool f16, size_t hd) {
     sh.many_target = hd == 256 ? 256 : 512;
 }
 
-// Partial states to have room for (of each kv head): 64 MiB of them with 128 dims at most.
+// Partial states to have room for (of each kv head): 64 MiB of them with 128 dims at most.  (So many kv heads that a tile's states find no
+// room are as many workgroups, and nothing is split.)
 inline size_t paged_part_rows(const PagedShape& sh, size_t max_tokens) {
     const size_t splits = 2 * (size_t)std::max(sh.few_target, sh.many_target) / sh.n_kv + 2;
-    return std::min(max_tokens * sh.G * splits, std::max<size_t>(131072 / sh.n_kv, 256));
+    return std::min(max_tokens * sh.G * splits, (size_t)131072 / sh.n_kv);
 }
 
 // Cuts tiles into shares of equal time for `slots` workgroups, one after another through the tiles, so that a workgroup may end

@@ -217,3 +217,13 @@ def test_drawn_steps(program):
         w = rng.choice([0, 0, rng.randint(1, 2000)])
         cover(program, rng.choice([1, 2, 4, 7, 20]), rng.choice([1, 2, 8, 32]), w, rng.choice([0, 4, 300]) if w else 0,
               rng.random() < 0.7, rng.choice([64, 128, 256]), seqs)
+
+
+@pytest.mark.parametrize("n_kv", [1, 8, 100, 512, 513, 700, 5000, 65535])
+def test_partial_states_have_a_bound(program, n_kv):
+    """64 MiB with 128 dims, whatever the number of kv heads."""
+    for hd in (64, 128, 256):
+        for seqs in ([(1, 5000)], [(40, 900), (1, 3)], [(300, 3000)]):
+            out = program("plan", 2, n_kv, 0, 0, 1, hd, 1000, len(seqs), *(x for s in seqs for x in s)).splitlines()
+            assert int(out[0].split()[2]) * n_kv * hd * 4 <= (64 << 20) * hd // 128
+            cover(program, 2, n_kv, 0, 0, True, hd, seqs)
