@@ -15,13 +15,15 @@
 // f16 values whose products have sums of their own: an element is off by 2^-23
 // of itself down to 2^-29 of the row's largest, by 2^-52 of the largest below that.
 // A weight exp2(s - max + 15), at most 2^15, is split into two f16 values likewise
-// but joined in one sum: it is off by 2^-22 of itself down to 2^-17 of the row's
-// largest weight, by 2^-40 of the largest below that.  That is half of the matrix rate for results
+// but joined in one sum: the split is off by 2^-22 of it (many rows, which cut the first part: 2^-21) down to 2^-17 of the
+// row's largest weight, by 2^-40 of the largest below that; an exponent of 8 to 16 is rounded by 2^-21, which is
+// 2^-21.5 of the weight, and exp2 by 2^-23: 2^-20 in all.  That is half of the matrix rate for results
 // that one f16 value a weight would have at 2^-12.  The MFMA's f32 sums are not rounded to
 // nearest, so each step's start from zero and join O in one fma.
 // Over an f32 cache few rows take the f32 MFMA (they are bound by the reading all the
-// same), many rows six products of bf16 parts: within 2^-23 of |x y| whatever the values (those from
-// 3.3961e38 on read as NaN where they are seen, for bf16 rounds them to infinity).
+// same), many rows six products of bf16 parts: within 2^-23 of |x y| for values from 2^-110 on (those from
+// 3.3961e38 on read as NaN where they are seen, for bf16 rounds them to infinity).  Weights are at most 1 / kv_len there
+// (paged_weight_unit).
 //
 // V in unseen places: a weight of zero keeps finite values out, not NaN.  Steps
 // that some row does not see all of replace what is not finite (or has bf16 parts that

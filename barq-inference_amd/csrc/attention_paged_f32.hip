@@ -2,13 +2,13 @@
 // and their chunks.  attention_paged.hpp has the formulas and numerics.
 //
 // Bound by the matrix products: six of bf16 for each f32 product.  An f32 value is
-// exactly the sum of three bf16 values (8 bits each, any exponent), so that the three largest
-// products of two values' parts and the three next are within 2^-23 of |x y|, whatever the values' sizes;
+// exactly the sum of three bf16 values (8 bits each, f32's exponents: below 2^-110 the last has fewer bits), so that the three
+// largest products of two values' parts and the three next are within 2^-23 of |x y|;
 // the sums of the five smaller ones are kept apart from the largest's, so that the MFMA's cuts count
 // a few times only.  That is 2.7 times the rate of the f32 MFMA.  A workgroup is four waves of 32 rows,
 // the queries' parts in registers; a step's 32 positions come by direct loads into LDS as they lie, the waves share
 // their conversion into the operands' layout there, and the next step is fetched while this one is computed on.
-// A 2048-token prompt of 32 heads on 8, 128 dims: 264 to 273 us, 130 TFLOP/s counted once (on the f32 MFMA 397, which
+// A 2048-token prompt of 32 heads on 8, 128 dims: 259 to 273 us by card, 130 TFLOP/s counted once (on the f32 MFMA 397, which
 // reaches 154 in an 8192^3 product).
 #include "attention_paged.hpp"
 

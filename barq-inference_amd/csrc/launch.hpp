@@ -334,7 +334,7 @@ struct PagedAttn {
     int n_tokens;          // -1: counts has them (a captured call)
     int n_few, n_many, n_merges;
     int merge_span;        // workgroups of a merge
-    bool once;             // few rows: nothing reads their keys and values again soon
+    bool once;             // few rows: their keys and values pass the caches by
     int n_head, n_kv, G, log_page;
     int window, n_sink;
     float scale;           // log2(e) / sqrt(hd)

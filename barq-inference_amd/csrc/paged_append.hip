@@ -3,8 +3,8 @@
 // one tensor by itself.
 //
 // Bound by the bytes: q is read and written in f32, K and V read in f32 and written
-// in the cache's type: 2048 tokens of 32 + 8 heads of 128 dims, 92 MB, in 19.7 us (4.7 TB/s of a copy's 5.2 beyond the
-// last-level cache), 17.2 of them without the launch.  A workgroup has up to 16 tokens of one block and some of their
+// in the cache's type: 2048 tokens of 32 + 8 heads of 128 dims, 92 MB, in 19.7 us (4.7 TB/s; a copy has 8.0 within the
+// last-level cache's size, as here, 5.2 beyond it), 17.2 of them without the launch.  A workgroup has up to 16 tokens of one block and some of their
 // heads: HD / 8 lanes a row of q or K, the next rows in flight while these are rotated; of
 // V eight tokens (four in f32) of a dim a lane, which are 16 bytes there.  The pairs' cos and
 // sin (64-bit angles) are formed once for a workgroup's tokens, while its first rows come.

@@ -13,6 +13,7 @@
 // before, f16, few / many us: 100 rows 18.1 / 24.7, 128 17.7 / 25.2, 192 22.0 / 29.3, 256 23.7 / 30.0; eight such
 // sequences: 100 rows 59.4 / 72.1, 200 106 / 82.5; f32: 128 rows 35.9 / 35.4, 256 58.5 / 48.7.  Where the kernel for many
 // runs anyway it takes middling sequences along: eight of 112 to 200 rows 82.5 us, the smaller ones in a launch of their own 107.
+// 64 and 256 dims take the same numbers; they were not measured there.
 #pragma once
 #include <algorithm>
 #include <cstdint>
@@ -37,7 +38,9 @@ struct PagedShape {
     int64_t few_start = 4;        // steps that an item's beginning and end take the time of (2 and 8 measured 1 to 2 % worse)
     int64_t step_bytes = 16384;   // of K and V in a step of few rows
     // bytes of K and V that few rows read from which they pass the caches by: 16 sequences' 256 / 192 / 160 / 128 / 96 MB
-    // take 49.9 / 40.0 / 35.2 / 29.3 / 27.0 us so, 53.0 / 42.0 / 36.5 / 27.2 / 22.2 otherwise (the same pages again and again)
+    // take 49.9 / 40.0 / 35.2 / 29.3 / 27.0 us so, 53.0 / 42.0 / 36.5 / 27.2 / 22.2 otherwise (the same pages again and again:
+    // what a model's other layers leave of them in the caches was not measured).  Counted by lengths: a page that sequences share
+    // counts for each, 16 / 32 / 64 sequences of 4000 positions on the same pages take 23.6 / 38.8 / 64.1 us so, 21.9 / 32.5 / 53.9 otherwise
     int64_t once_from = 160 << 20;
     size_t part_rows = 0;         // partial states there is room for, for each kv head
 };
@@ -132,7 +135,7 @@ inline void paged_shape_for(PagedShape& sh, bool f16, size_t hd) {
     sh.many_step = f16 ? 64 : 32;
     if (!f16) sh.alone_from = sh.many_from;
     sh.step_bytes = 128 * (int64_t)hd;
-    // by the kernels' registers: one, two, three workgroups a CU
+    // by the kernels' registers: one, two, three workgroups a CU (f32 rows of 64 dims have room for four, not used)
     sh.few_target = hd == 256 ? 256 : hd == 128 ? 512 : 768;
     sh.many_target = hd == 256 ? 256 : 512;
 }
@@ -201,7 +204,7 @@ inline void paged_plan(const PagedShape& sh, const std::vector<PagedSeq>& seqs, 
     p.merges.clear();
     p.n_few = 0;
     int64_t steps[2] = {0, 0}, q0 = 0, small = 0, longest = 0;
-    bool apart = true;   // no two tiles of few rows read the same keys and values
+    bool apart = true;   // no two tiles of few rows are of one sequence (sequences may share pages)
     for (const PagedSeq& s : seqs) {
         longest = std::max(longest, s.q_len * sh.G);
         if (s.q_len * sh.G < sh.alone_from) small += (s.q_len * sh.G + PAGED_FEW_ROWS - 1) / PAGED_FEW_ROWS;

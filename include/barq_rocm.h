@@ -600,7 +600,7 @@ int barq_rocm_rope_frequencies(int scaling, size_t rot_dim, double base, double 
  * barq_rocm_rms_norm) and the rotation, in one pass: x [seq_len, n_heads *
  * head_dim] -> out [n_heads, seq_len, head_dim], which must not overlap; seq_len < 2^24.  For models with
  * norms of their queries and keys whose session has a cache of its own.
- * paged_append = the same on q (into q_out [n_head, n_tokens, head_dim]; both NULL: no q)
+ * paged_append = the same on q (into q_out [n_head, n_tokens, head_dim], which must not overlap q; both NULL: no q)
  * and k, then k and v (projections [n_tokens, n_head_kv * head_dim]) into the
  * layer's pages.  A token's position is its place in its sequence.
  * paged_read = the rows that the cache holds of the batch's tokens, in its type:
@@ -611,7 +611,8 @@ int barq_rocm_rope_frequencies(int scaling, size_t rot_dim, double base, double 
  * (out_type BARQ_TYPE_F32), or its rows as Q8_K blocks (BARQ_TYPE_Q8_K: n_head * head_dim a
  * multiple of 256; the bytes barq_rocm_quantize_act writes for them).  A query that sees no position
  * gives zeros.  Softmax statistics and sums are f32.  Over an f16 cache a query element counts to 2^-23 of itself or 2^-52 of
- * its row's largest, a weight to 2^-22 of itself or 2^-40 of its row's largest, whichever is more.  Over an
+ * its row's largest, a weight to 2^-20 of itself (the rounding of its exponent, exp2 and its split; what its score is off by comes
+ * to that) or 2^-40 of its row's largest, whichever is more.  Over an
  * f32 cache products count to 2^-23 of themselves (less where V is below 2^-126 kv_len) and no sum on the way is larger than the largest
  * |V| that a query sees; of sequences with more than 64 rows (new tokens x n_head /
  * n_head_kv), q, K and V from 3.39e38 on may count as NaN for the queries that see them.
