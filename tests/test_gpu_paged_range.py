@@ -1,11 +1,12 @@
 """Attention over a paged cache at the ends of f32's range: finite values of
-every size where no query looks, and averages of values near the largest."""
+every size where no query looks, and averages of values near the largest; and
+numbers of heads, pages and positions at the ends of theirs."""
 import numpy as np
 import pytest
 
 import barq_rocm as B
 from barq_rocm import paged as P
-from paged_ref import assert_within
+from paged_ref import assert_within, attention, cache_values
 from test_gpu_paged import Case, dev
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +72,47 @@ def test_averages_of_small_values(be, rows):
     c = Case(be, B.F32, 4, 1, 64, 32, [(rows, n)], k=F32(0.1) * k, v=v * F32(2.0 ** -90))
     want, off = c.want()
     assert_within(c.batch.attention(c.layer, dev(c.q)).cpu().numpy(), want, off)
+
+
+@pytest.mark.parametrize("type_", [B.F16, B.F32])
+@pytest.mark.parametrize("heads,kv,hd,page,seqs,window,n_sink", [
+    (200, 1, 64, 16, [(1, 500), (2, 90)], 0, 0),          # a token's rows over several tiles, of either kernel
+    (256, 2, 128, 32, [(1, 333), (3, 3)], 40, 5),
+    (600, 600, 64, 16, [(1, 700), (5, 60)], 0, 0),        # more kv heads than workgroups: nothing is split
+    (1100, 550, 64, 16, [(70, 130)], 30, 2),
+    (8, 2, 64, 65536, [(1, 700), (90, 200)], 0, 0),       # one page
+    (6, 2, 256, 4096, [(1, 4097), (0, 3), (33, 5000)], 1000, 64)])
+def test_heads_and_pages_of_every_number(be, type_, heads, kv, hd, page, seqs, window, n_sink):
+    c = Case(be, type_, heads, kv, hd, page, seqs, window, n_sink, layers=1)
+    want, off = c.want()
+    assert_within(c.batch.attention(c.layer, dev(c.q)).cpu().numpy(), want, off)
+
+
+@pytest.mark.parametrize("type_", [B.F16, B.F32])
+def test_a_pool_beyond_32_bits(be, type_):
+    """More than 2^32 bytes of K in a layer, and the second layer behind it: rows at both ends."""
+    import torch
+    hd, kv, page = 256, 8, 64
+    pages = (1 << 32) // (kv * hd * page * (2 if type_ == B.F16 else 4)) + 9
+    c = P.PagedCache(be, pages, page, 2, kv, hd, type=type_)
+    b = P.PagedBatch(c, kv, 2, 400, 4)
+    rng = np.random.default_rng(3)
+    table = np.array([[0, pages - 1, 1, pages - 2], [pages - 3, 2, pages - 4, 3]], np.int32)
+    k, v = (rng.standard_normal((2, 400, kv, hd)).astype(F32) for _ in "kv")
+    b.set([200, 200], [200, 200], table)
+    for layer in range(2):
+        x, y = dev(k[layer]), dev(v[layer])
+        b.append(layer, x, y)
+        be.sync()
+    for layer in range(2):
+        kk, vv = (cache_values(x[layer], type_ == B.F16) for x in (k, v))
+        for got, held in zip(b.read(layer), (kk, vv)):
+            assert np.array_equal(got.cpu().numpy().astype(np.float64), held)
+    for new in (1, 100):
+        b.set([new, new], [200, 200], table)
+        q = rng.standard_normal((kv, 2 * new, hd)).astype(F32)
+        for layer in range(2):
+            kk, vv = (cache_values(x[layer], type_ == B.F16) for x in (k, v))
+            want, off = attention(q, [(new, kk[:200], vv[:200], None), (new, kk[200:], vv[200:], None)])
+            assert_within(b.attention(layer, dev(q)).cpu().numpy(), want, off)
+    torch.cuda.synchronize()
